@@ -43,6 +43,8 @@ extern "C" {
 #define SN_CAP_SUNNY        (1u << 7)  /* sn_abi_sunny_* whole-model handle */
 #define SN_CAP_BATCH        (1u << 8)  /* batched steps + state export/import */
 #define SN_CAP_RECUR_BWD    (1u << 9)  /* sn_abi_recur_bwd */
+#define SN_CAP_TRAIN        (1u << 10) /* sn_abi_layer_norm, _bwd, sn_abi_adamw_step */
+#define SN_CAP_SAMPLE       (1u << 11) /* sn_abi_sample */
 
 /* Status codes (reference sn_abi.h:41-46, docs/ABI.md:55-68) */
 #define SN_OK              0
@@ -216,6 +218,75 @@ sn_status   sn_abi_rwkv7_prefill_batch(SnAbiRwkv7* m, const int32_t* tokens, int
 /* S (B,L,NH,HS,HS), shift (B,L,2,D) */
 sn_status   sn_abi_rwkv7_get_state(SnAbiRwkv7* m, int32_t B, float* S, float* shift);
 int32_t     sn_abi_rwkv7_dims(const SnAbiRwkv7* m, int32_t* dims8); /* vocab,D,HS,NH,F,L,q4,group */
+
+/* ----------------------------------------------------- enqueue-only operators
+ * No counterpart in the reference's native code (it leaves these to torch and
+ * numpy). Unlike the calls above, they take device memory only (all of one
+ * GPU, which need not be the calling thread's current one; host memory is
+ * refused with SN_E_INVAL), enqueue on `cuda_stream` (NULL = legacy default
+ * stream) and return without synchronising, whatever set_stream / set_async
+ * say. They hold no state and no memory of their own between calls, so they
+ * may be captured into a CUDA graph and used from several threads and
+ * streams; calls that share arrays are the caller's to order. */
+#define SN_F32   0
+#define SN_BF16  1
+#define SN_F16   2
+
+/* Layer norm of `rows` rows of D values: y = (x - mean) * rstd * w + b, the
+ * variance biased, rstd = 1 / sqrt(var + eps). x has rows at a stride of ldx
+ * elements, y is contiguous; both are of `dtype`. w, b (D) are of `wdtype`:
+ * SN_F32 or `dtype`; either may be NULL (1, 0). mean, rstd (rows) fp32 are
+ * what the backward pass needs and may be NULL. Sums are fp32. */
+sn_status sn_abi_layer_norm(const void* x, int64_t ldx, const void* w, const void* b, void* y,
+                            float* mean, float* rstd, int32_t dtype, int32_t wdtype,
+                            int64_t rows, int32_t D, float eps, void* cuda_stream);
+/* Its gradients: dx (rows, D) contiguous, of `dtype`; dw, db (D) of `wdtype`,
+ * overwritten; each may be NULL. The same input gives the same bits. ws: at
+ * least sn_abi_layer_norm_bwd_ws bytes (asked with the arrays' GPU current)
+ * when dw or db is wanted, free again when the work enqueued here is done. */
+int64_t   sn_abi_layer_norm_bwd_ws(int64_t rows, int32_t D, int32_t dtype);
+sn_status sn_abi_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                                const void* w, const float* mean, const float* rstd, void* dx,
+                                void* dw, void* db, void* ws, int64_t ws_bytes, int32_t dtype,
+                                int32_t wdtype, int64_t rows, int32_t D, void* cuda_stream);
+
+/* One AdamW step of `count` tensors: lists (in host memory) of the device
+ * addresses of parameters (`dtype`), gradients (`grad_dtype`) and states, and
+ * of the tensors' sizes. Per value, in fp32:
+ *   m = m*b1 + g*(1-b1);  v = v*b2 + g*g*(1-b2);
+ *   p = p*(1 - lr*wd) - m / (sqrt(v) / sqrt(1-b2^step) + eps) * lr / (1-b1^step)
+ * state_bits 32: avg, sq are m, v in fp32. state_bits 8: avg, sq are e4m3
+ * codes of m and sqrt(v), avg_scale, sq_scale lists of fp32 arrays with one
+ * scale for each 256 values of a tensor (value = code * scale; a new scale is
+ * the block's largest magnitude / 448; sqrt(v) > 0 keeps a code > 0). step
+ * counts from 1; step_dev and lr_dev, where not NULL, are read from the GPU
+ * when the kernel runs (a replayed graph sees new values). No tensor may
+ * appear twice or overlap another. */
+sn_status sn_abi_adamw_step(int32_t count, void* const* params, const void* const* grads,
+                            void* const* avg, void* const* sq, float* const* avg_scale,
+                            float* const* sq_scale, const int64_t* sizes, int32_t dtype,
+                            int32_t grad_dtype, int32_t state_bits, int64_t step,
+                            const int64_t* step_dev, double lr, const double* lr_dev,
+                            double beta1, double beta2, double eps, double weight_decay,
+                            void* cuda_stream);
+
+/* The next token of each of B rows of V logits (rows `ld` elements apart),
+ * drawn with given uniform numbers u in [0, 1) (B; fp64 where u_f64, else
+ * fp32): the rule of the reference's sample_logits (serve.py:30-57) and min-p.
+ * temperature, top_k, top_p, min_p: arrays of B on the GPU, or NULL and the
+ * one value beside them. temperature <= 0 takes the lowest id of the largest
+ * logit. Otherwise weights exp((x - max) / temperature); 0 < top_k < V keeps
+ * the ids with a logit of at least the k-th largest; 0 < top_p < 1 keeps of
+ * those, in descending order and equal ones by id, each whose predecessors
+ * weigh less than top_p of them all; min_p keeps the weights of at least
+ * min_p; the token is the first id whose weight and those of the ids before
+ * it exceed u times the kept weight. NaN counts as -infinity; a row of
+ * nothing else gives -1; a largest logit of +infinity is taken itself. */
+sn_status sn_abi_sample(const void* logits, int64_t ld, int32_t dtype, const void* u,
+                        int32_t u_f64, const double* temperature, double temperature0,
+                        const int32_t* top_k, int32_t top_k0, const double* top_p,
+                        double top_p0, const double* min_p, double min_p0, int32_t B,
+                        int32_t V, int32_t* tokens, void* cuda_stream);
 
 #ifdef __cplusplus
 }

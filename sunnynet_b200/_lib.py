@@ -13,6 +13,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libsunnynet_cuda.so"
 
 V, I32, U32, P = ctypes.c_void_p, ctypes.c_int32, ctypes.c_uint32, ctypes.c_char_p
 CI = ctypes.c_int
+I64, F32, F64 = ctypes.c_int64, ctypes.c_float, ctypes.c_double
 
 # name -> (restype, argtypes); every symbol declared in include/*.h
 SIGNATURES = {
@@ -72,6 +73,14 @@ SIGNATURES = {
     "sn_abi_rwkv7_prefill_batch": (I32, [V, V, I32, I32, V]),
     "sn_abi_rwkv7_get_state": (I32, [V, I32, V, V]),
     "sn_abi_rwkv7_dims": (I32, [V, V]),
+    # sn_abi.h, enqueue-only operators
+    "sn_abi_layer_norm": (I32, [V, I64, V, V, V, V, V, I32, I32, I64, I32, F32, V]),
+    "sn_abi_layer_norm_bwd_ws": (I64, [I64, I32, I32]),
+    "sn_abi_layer_norm_bwd": (I32, [V, I64, V, I64, V, V, V, V, V, V, V, I64, I32, I32, I64, I32,
+                                    V]),
+    "sn_abi_adamw_step": (I32, [I32, V, V, V, V, V, V, V, I32, I32, I32, I64, V, F64, V, F64, F64,
+                                F64, F64, V]),
+    "sn_abi_sample": (I32, [V, I64, I32, V, I32, V, F64, V, I32, V, F64, V, F64, I32, I32, V, V]),
     # recur.h
     "sn_set_threads": (None, [CI]),
     "sn_threads": (CI, []),
@@ -171,6 +180,14 @@ def profile_report() -> dict:
 def check(rc: int, what: str = "") -> None:
     if rc != 0:
         raise SnError(int(rc), f"{what}: {last_error()}")
+
+
+def dtype_code(t) -> int:
+    """SN_F32 / SN_BF16 / SN_F16 of a torch dtype (sn_abi.h)."""
+    code = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}.get(str(t))
+    if code is None:
+        raise TypeError(f"float32, bfloat16 or float16 wanted, not {t}")
+    return code
 
 
 def ptr(x):

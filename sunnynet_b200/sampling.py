@@ -1,0 +1,68 @@
+"""The draw of the next token on the GPU: the reference's sample_logits
+(serve.py:30-57) and min-p for a batch of rows, from given uniform numbers.
+
+``serve.BatchEngine`` draws with it; a decode loop of its own calls ``sample``
+on the logits that ``SunnyBatch.step`` or ``Rwkv7Batch.step`` left on the GPU.
+"""
+from __future__ import annotations
+
+import math
+
+from ._lib import check, dtype_code
+from .runtime import load_runtime
+
+__all__ = ["sample"]
+
+
+def _setting(name, v, B, device, dtype):
+    """(address or None, one value, what keeps the address alive)."""
+    import torch
+    if not isinstance(v, torch.Tensor):
+        return None, v, None
+    if tuple(v.shape) != (B,) or v.device != device:
+        raise ValueError(f"sample: {name} is one number or {B} of them on {device}")
+    v = v.to(dtype).contiguous()
+    return v.data_ptr(), 0, v
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+    """Tokens (B,) int32 drawn from logits (B, V) (float32, bfloat16 or
+    float16, on a GPU; rows may lie at a stride) with uniform numbers u (B,) in
+    [0, 1) (float32 or float64).
+
+    temperature, top_k, top_p, min_p: a number for all rows, or a tensor (B,)
+    on the logits' GPU (float64, top_k int32; others are converted by a kernel
+    each). temperature <= 0 takes the lowest id of the largest logit. top_k of
+    0 (or >= V), top_p of 1 and min_p of 0 keep every id; ids as likely as the
+    k-th stay. A row without a logit above -inf gives -1. Only enqueues, on
+    torch's current stream of that GPU."""
+    import torch
+    if logits.dim() != 2 or not logits.is_cuda:
+        raise ValueError("sample: logits (B, V) on a GPU are wanted")
+    B, V = logits.shape
+    if V == 0:
+        raise ValueError("sample: no logits to draw from")
+    if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V:
+        raise ValueError("sample: the logits of a row must lie side by side")
+    dev = logits.device
+    if tuple(u.shape) != (B,) or u.device != dev or \
+            u.dtype not in (torch.float32, torch.float64):
+        raise ValueError(f"sample: u has {B} numbers of float32 or float64 on {dev}")
+    if out is None:
+        out = torch.empty(B, dtype=torch.int32, device=dev)
+    elif tuple(out.shape) != (B,) or out.dtype != torch.int32 or out.device != dev or \
+            not out.is_contiguous():
+        raise ValueError(f"sample: out has {B} contiguous int32 values on {dev}")
+    u = u.contiguous()
+    t, t0, keep_t = _setting("temperature", temperature, B, dev, torch.float64)
+    k, k0, keep_k = _setting("top_k", top_k, B, dev, torch.int32)
+    p, p0, keep_p = _setting("top_p", top_p, B, dev, torch.float64)
+    q, q0, keep_q = _setting("min_p", min_p, B, dev, torch.float64)
+    if not math.isfinite(t0) or not math.isfinite(p0) or not q0 <= 1:
+        raise ValueError("sample: temperature and top_p are finite, min_p is at most 1")
+    check(load_runtime().sn_abi_sample(
+        logits.data_ptr(), max(logits.stride(0), V), dtype_code(logits.dtype), u.data_ptr(),
+        int(u.dtype == torch.float64), t, float(t0), k, max(0, min(int(k0), 0x7fffffff)), p,
+        float(p0), q, float(q0), B, V, out.data_ptr(), torch.cuda.current_stream(dev).cuda_stream),
+        "sample")
+    return out
