@@ -18,21 +18,37 @@
 // depends on no scheduling, and differs from the rule in real numbers only
 // where u meets a border to about 2^-40.
 //
-// A row is read from HBM once, by a cluster of 1 to 8 CTAs that each keep a
-// slice of it in shared memory as order-preserving 32-bit keys. Neither top-k
-// nor top-p sorts: both look for one border key, the largest with "count (or
-// weight) of the larger keys < target <= that plus its own". A histogram over
-// 512 bins between the row's largest logit and the point where weights vanish
-// gives the border's bin; the bin's few keys are gathered and compared with
-// one another. A bin of more than kList keys is cut into 512 bins again, by
-// key, until it is small or holds a single key (at most five rounds). The
-// CTAs of a cluster read one another's histograms and lists through
-// distributed shared memory and come to the same border by themselves.
+// What bounds a batch of rows is not HBM but the instructions spent on a logit:
+// an exact weight takes about 40, 14 of them in 64 bits. So what can be kept is
+// narrowed first. A histogram over 512 bins, linear from the largest logit down,
+// counts the logits; for top-k the bins down to the k-th, for top-p those whose
+// count times the bin's least weight reaches p of the row's weight (estimated
+// from above in fp32) hold every id that can stay. The ids of those bins are
+// listed by id, and only they get exact weights. Top-p's target p * (weight of
+// all) needs the rest's weight too: it comes from the fp32 estimate with its
+// worst-case error; where the two ends of that error do not lead to the same
+// ids (a percent of the rows) the row's weight is summed exactly.
+//
+// Neither top-k nor top-p sorts: both look for one border key, the largest
+// with "count (or weight) of the larger keys < target <= that plus its own".
+// The first histogram leaves a range of keys for it; the range is cut into 512
+// bins by key, whose counts or weights give the border's bin, until a bin's
+// keys are kList or fewer, or one (at most five rounds); these are gathered and
+// compared with one another. A top-k row with at most kList listed ids, the
+// usual case, is finished by one CTA that compares all of them.
+//
+// A row belongs to a cluster of 1 to 8 CTAs. With few rows each CTA keeps a
+// slice of the row in shared memory, and the CTAs read one another's
+// histograms and lists through distributed shared memory. With rows enough
+// for every SM a row belongs to one CTA, which keeps no more than the list and
+// reads the row from L2 again: the cost of a CTA's fixed steps (scans,
+// searches) is then spread over the whole row.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <cmath>
+#include <cstddef>
 
 #include "caller.cuh"
 #include "ptx.cuh"
@@ -45,11 +61,29 @@ typedef unsigned long long u64;
 typedef unsigned int u32;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kBins = 512;     // two to a thread
+constexpr int kCut = 1024;     // bins of the first histogram, four to a thread
+constexpr int kBins = 512;     // of the others, two to a thread
 constexpr int kList = 256;     // keys resolved by comparing them all: one to a thread
+constexpr int kCand = 8192;    // logits a CTA that keeps no slice lists: 32 KB, four CTAs on an SM
+constexpr int kProbe = 4 * kThreads;  // first logits of a row, from which the bins take their place
+constexpr int kPow = 128;      // table of 2^(j/128)
 constexpr int kMaxCluster = 8;
-constexpr u32 kNothing = 0x007fffffu;  // key of -infinity (and of NaN)
-constexpr u32 kInfinite = 0xff800000u; // key of +infinity
+constexpr u32 kNothing = 0x007fffffu;  // key of -infinity
+
+// 2^(j/128) by the exponential series, computed by the compiler.
+struct PowTable {
+    double v[kPow];
+    constexpr PowTable() : v{} {
+        for (int j = 0; j < kPow; ++j) {
+            double x = j * 0.69314718055994530942 / kPow, e = 1.0;
+            for (int k = 24; k > 0; --k) e = 1.0 + e * x / k;
+            v[j] = e;
+        }
+    }
+};
+__device__ constexpr PowTable g_pow{};
+
+__device__ __forceinline__ double two_to(int n) { return __hiloint2double((1023 + n) << 20, 0); }
 
 struct Setting {  // one value, or one for each row
     const double* rows;
@@ -67,9 +101,8 @@ struct SampleArgs {
     int one_k, u_wide, V, slice, bits;
 };
 
-// Bits of x ordered like the numbers, -0 taken for 0 and NaN for -infinity.
+// Bits of x ordered like the numbers, -0 taken for 0.
 __device__ __forceinline__ u32 key_of(float x) {
-    if (!(x == x)) return kNothing;
     const u32 b = __float_as_uint(x + 0.0f);
     return b ^ ((u32)((int)b >> 31) | 0x80000000u);
 }
@@ -78,79 +111,141 @@ __device__ __forceinline__ float value_of(u32 k) {
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
-__device__ __forceinline__ u32 peer_u32(const u32* local, u32 rank) {
-    u32 v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(dsmem_addr(local, rank)) : "memory");
-    return v;
-}
-
-__device__ __forceinline__ void peer_store(u64* local, u32 rank, u64 v) {
-    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dsmem_addr(local, rank)), "l"(v)
-                 : "memory");
-}
-
 struct Shared {
-    double pow16[16];        // 2^(j/16)
-    u64 told[9][kMaxCluster];  // a value of each CTA, one line per exchange
+    double pow[kPow];           // 2^(j/128)
+    u64 told[14][kMaxCluster];  // a value of each CTA, one line per exchange
     u64 red[kWarps];
     u64 warp_sum[kWarps];
-    u32 lo[kBins], hi[kBins];  // a bin's count or weight, as two words
+    alignas(16) u32 count[kCut];  // of cut()
+    alignas(16) u32 lo[kBins], hi[kBins];  // a bin's count or weight, as two words, of border()
     u32 list[2][kList], listed[2];  // keys of the border's bin, of top-k and of top-p
-    u32 least, most;         // their range
-    u32 all[kList];          // every CTA's list
+    u32 least, most;           // their range
+    u32 all[kList];            // every CTA's list
     u64 weight[kList];
     u64 found[4];
+    u32 edge[2];
+};
+static_assert(offsetof(Shared, told) % 8 == 0 && offsetof(Shared, count) % 16 == 0 &&
+                  offsetof(Shared, lo) % 16 == 0 && offsetof(Shared, hi) % 16 == 0,
+              "vector loads of other CTAs' counters");
+
+// The CTAs of a row: a cluster, or (ONE) a CTA by itself.
+template <bool ONE>
+struct Team {
+    u32 rank, ctas;
+    __device__ Team() : rank(ONE ? 0 : cluster_rank()), ctas(ONE ? 1 : cluster_size()) {}
+    __device__ __forceinline__ void sync() const {
+        if (ONE || ctas == 1)
+            __syncthreads();
+        else
+            cluster_sync();
+    }
+    // Reads of another CTA's shared memory take several hundred cycles: the
+    // callers issue all of theirs before they use the first.
+    __device__ __forceinline__ u32 read(const u32* local, u32 from) const {
+        if (ONE) return *local;
+        u32 v;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(dsmem_addr(local, from)));
+        return v;
+    }
+    // N counters from each CTA, added up
+    template <int N>
+    __device__ __forceinline__ void add_up(const u32* local, u64 (&sum)[N]) const {
+        static_assert(N == 2 || N == 4, "a vector load each");
+        u32 v[ONE ? 1 : kMaxCluster][N];
+#pragma unroll
+        for (int c = 0; c < (ONE ? 1 : kMaxCluster); ++c) {
+            if (ONE) {
+                for (int j = 0; j < N; ++j) v[c][j] = local[j];
+            } else if (c < (int)ctas) {
+                const u32 at = dsmem_addr(local, c);
+                if constexpr (N == 4)
+                    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(v[c][0]), "=r"(v[c][1]), "=r"(v[c][2]), "=r"(v[c][3])
+                                 : "r"(at));
+                else
+                    asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];"
+                                 : "=r"(v[c][0]), "=r"(v[c][1])
+                                 : "r"(at));
+            } else {
+                for (int j = 0; j < N; ++j) v[c][j] = 0;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            sum[j] = 0;
+#pragma unroll
+            for (int c = 0; c < (ONE ? 1 : kMaxCluster); ++c) sum[j] += v[c][j];
+        }
+    }
+    // Thread i's place among the CTAs' lists, laid one behind the other: of
+    // which CTA (ctas: behind them all) and where in its list; count[c] long.
+    __device__ __forceinline__ u32 place(const u64* count, u32 i, u32* at) const {
+        u32 c = 0;
+        *at = i;
+#pragma unroll
+        for (int k = 0; k < (ONE ? 1 : kMaxCluster); ++k)
+            if (k < (int)ctas && c == (u32)k && *at >= (u32)count[k]) *at -= (u32)count[k], ++c;
+        return c;
+    }
+    // v into the place of *local in CTA `to`
+    __device__ __forceinline__ void store(u64* local, u32 to, u64 v) const {
+        if (ONE)
+            *local = v;
+        else
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(dsmem_addr(local, to)), "l"(v)
+                         : "memory");
+    }
+    // v of this CTA into every CTA's line, by the first threads
+    __device__ __forceinline__ void tell(u64* line, u64 v) const {
+        if (threadIdx.x < ctas) store(line + rank, threadIdx.x, v);
+    }
 };
 
 // One row's numbers, the same in every thread of the cluster.
 struct Row {
     double max, scale;  // w = 2^((x - max) * scale)
-    int shift;          // 52 - bits
-    float max_f, bin;   // linear bins: (max - x) * bin
+    double unit;        // 2^(52 - bits): a double near it ends at 2^-bits
+    float max_f, scale_f;
+    float ref, bin;     // linear bins: (ref - x) * bin
+    float cutoff;       // logits below weigh nothing
 };
 
-// 2^((x - max) * scale) * 2^bits, cut to a whole number. The fraction f of the
-// exponent in 16ths is left to the exponential series of f ln2 / 16 < 0.0434:
-// its eighth term is below 2^-51.
-__device__ __forceinline__ u64 weigh(const Row& r, const Shared& s, u32 key) {
-    const double d = ((double)value_of(key) - r.max) * r.scale;
-    if (!(d >= -64.0)) return 0;  // too far below, -infinity among them
-    const double n = floor(d * 16.0);
-    const double f = fma(n, -0.0625, d) * 0.69314718055994530942;
-    double e = 1.0 / 5040;
-    e = fma(e, f, 1.0 / 720);
-    e = fma(e, f, 1.0 / 120);
-    e = fma(e, f, 1.0 / 24);
-    e = fma(e, f, 1.0 / 6);
-    e = fma(e, f, 0.5);
+// 2^((x - max) * scale) * 2^bits to the nearest whole number. The exponent's
+// nearest 128th goes to the table, the rest |f| <= 2^-8 to the exponential
+// series of f ln2, whose fifth term is below 2^-49.
+__device__ __forceinline__ u64 weigh(const Row& r, const Shared& s, float x) {
+    constexpr double whole128 = 1.5 * 0x1p45;  // doubles near it are 128ths
+    constexpr double ln2 = 0.69314718055994530942;
+    const double below = (double)fmaxf(x, r.cutoff) - r.max;
+    const double near = fma(below, r.scale, whole128);
+    const double f = fma(below, r.scale, whole128 - near);
+    double e = ln2 * ln2 * ln2 * ln2 / 24;
+    e = fma(e, f, ln2 * ln2 * ln2 / 6);
+    e = fma(e, f, ln2 * ln2 / 2);
+    e = fma(e, f, ln2);
     e = fma(e, f, 1.0);
-    e = fma(e, f, 1.0);
-    const int i = (int)n;  // -1024 .. 0
-    const u64 v = (u64)__double_as_longlong(e * s.pow16[i & 15]);  // near [1, 2)
-    const u64 m = (v & 0xfffffffffffffull) | 0x10000000000000ull;
-    const int sh = r.shift + 1023 - (int)(v >> 52) - (i >> 4);
-    return sh < 64 ? m >> sh : 0;
+    const int i = __double2loint(near);  // 128ths, 0 down to -8320
+    e *= s.pow[i & (kPow - 1)];
+    e = __hiloint2double(__double2hiint(e) + ((i >> 7) << 20), __double2loint(e));
+    e += r.unit;
+    const u64 w = (u64)(__double_as_longlong(e) - __double_as_longlong(r.unit));
+    return x < r.cutoff ? 0 : w;
 }
 
+// Bin of x, its distance below ref to the nearest, the first and the last bin
+// taking what is beyond them: adding 2^23 leaves the rounded number in the low
+// bits.
 __device__ __forceinline__ int linear_bin(const Row& r, float x) {
-    return (int)fminf((r.max_f - x) * r.bin, (float)(kBins - 1));
+    const float v = __saturatef((r.ref - x) * (r.bin * (1.0f / (kCut - 1))));
+    return __float_as_int(fmaf(v, (float)(kCut - 1), 8388608.0f)) - 0x4b000000;
 }
 
-// A barrier over the CTAs of a row.
-__device__ __forceinline__ void row_sync(u32 ctas) {
-    if (ctas == 1)
-        __syncthreads();
-    else
-        cluster_sync();
-}
-
-__device__ __forceinline__ u64 warp_max(u64 v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const u64 w = __shfl_xor_sync(0xffffffffu, v, o);
-        v = w > v ? w : v;
-    }
-    return v;
+// 2^x to 2^-22 of itself.
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 __device__ __forceinline__ u64 warp_add(u64 v) {
@@ -179,34 +274,146 @@ __device__ __forceinline__ u64 block_upto(Shared& s, u64 v) {
     return v;
 }
 
+// Sum over the CTA's threads, the same in all.
+__device__ __forceinline__ u64 block_add(Shared& s, u64 v) {
+    v = warp_add(v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s.warp_sum[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) v += s.warp_sum[k];
+    return v;
+}
+
 template <typename T>
 __device__ __forceinline__ float number(T v);
 template <>
-__device__ __forceinline__ float number<float>(float v) { return v; }
+__device__ __forceinline__ float number<float>(float v) { return fmaxf(v, -INFINITY); }
 template <>
-__device__ __forceinline__ float number<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float number<__nv_bfloat16>(__nv_bfloat16 v) {
+    return fmaxf(__bfloat162float(v), -INFINITY);
+}
 template <>
-__device__ __forceinline__ float number<__half>(__half v) { return __half2float(v); }
+__device__ __forceinline__ float number<__half>(__half v) {
+    return fmaxf(__half2float(v), -INFINITY);
+}
 
-// A CTA's slice [first, first + n) of a row: its keys from shared memory, or
-// (rows too long for it) from the logits again.
-template <typename T, bool HELD>
-struct Slice {
+template <typename T, int P>
+struct alignas(sizeof(T) * P) Pack {
+    T v[P];
+};
+
+// A CTA's slice of a row in the caller's memory, from the 16-byte boundary at or
+// before its first logit: the `skip` places in front of that, those behind the
+// last and NaN read as -infinity.
+template <typename T>
+struct Far {
+    static constexpr int P = 16 / sizeof(T), U = 16 / P;  // logits of a pack, packs in flight
     const T* x;
-    const u32* held;
-    int n, first;
-    __device__ __forceinline__ u32 operator[](int i) const {
-        return HELD ? held[i] : key_of(number<T>(x[i]));
+    int n, skip;  // n: places, skipped ones among them
+    __device__ __forceinline__ float value(int i) const {
+        return i < skip ? -INFINITY : number<T>(x[i]);
+    }
+    __device__ __forceinline__ int id(int i) const { return i - skip; }
+    __device__ __forceinline__ int packs() const { return (n + P - 1) / P; }
+    __device__ __forceinline__ void load(int i, float (&v)[P]) const {
+        if (i * P >= skip && (i + 1) * P <= n) {
+            const Pack<T, P> p = reinterpret_cast<const Pack<T, P>*>(x)[i];
+#pragma unroll
+            for (int j = 0; j < P; ++j) v[j] = number<T>(p.v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < P; ++j) v[j] = i * P + j < n ? value(i * P + j) : -INFINITY;
+        }
     }
 };
 
-// What the border of top-k or top-p is.
-struct Border {
-    u32 key;
-    u64 ahead;  // count or weight of the larger keys
-    u64 ties;   // ids that have this key
-    u64 target;
+// The same in shared memory, in fp32 and whole packs.
+struct Near {
+    static constexpr int P = 4, U = 1;
+    const float* x;
+    int n, skip;
+    __device__ __forceinline__ float value(int i) const { return x[i]; }
+    __device__ __forceinline__ int id(int i) const { return i - skip; }
+    __device__ __forceinline__ int packs() const { return (n + 3) / 4; }
+    __device__ __forceinline__ void load(int i, float (&v)[4]) const {
+        const float4 f = reinterpret_cast<const float4*>(x)[i];
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    }
 };
+
+// Of a slice in shared memory: the places of what can stay, in order.
+struct NearListed {
+    static constexpr int P = 1, U = 4;
+    Near of;
+    const unsigned short* at;
+    int n;
+    __device__ __forceinline__ float value(int i) const { return of.x[at[i]]; }
+    __device__ __forceinline__ int id(int i) const { return of.id(at[i]); }
+    __device__ __forceinline__ int packs() const { return n; }
+    __device__ __forceinline__ void load(int i, float (&v)[1]) const { v[0] = value(i); }
+};
+
+// Of a whole row that is not kept: the logits of what can stay, in order of
+// id. Their ids are found again for the one that is drawn.
+struct FarListed {
+    static constexpr int P = 1, U = 4;
+    const float* x;
+    int n;
+    __device__ __forceinline__ float value(int i) const { return x[i]; }
+    __device__ __forceinline__ int id(int i) const { return i; }
+    __device__ __forceinline__ int packs() const { return n; }
+    __device__ __forceinline__ void load(int i, float (&v)[1]) const { v[0] = x[i]; }
+};
+
+// f(place, logit, position in its pack) for each of a slice, padding included,
+// in no order, but ascending within a thread.
+template <typename S, typename F>
+__device__ __forceinline__ void each(const S& x, F f) {
+    const int packs = x.packs();
+    for (int q = threadIdx.x; q < packs; q += S::U * kThreads) {
+        float v[S::U][S::P];
+#pragma unroll
+        for (int j = 0; j < S::U; ++j)
+            if (q + j * kThreads < packs) x.load(q + j * kThreads, v[j]);
+#pragma unroll
+        for (int j = 0; j < S::U; ++j) {
+            if (q + j * kThreads >= packs) break;
+#pragma unroll
+            for (int e = 0; e < S::P; ++e) f((q + j * kThreads) * S::P + e, v[j][e], e);
+        }
+    }
+}
+
+// f(logit, weight) for each of a slice; the weights of a pack, or of the packs
+// of one, are formed side by side (each is a chain of a dozen operations).
+template <typename S, typename F>
+__device__ __forceinline__ void each_weighed(const Row& r, const Shared& s, const S& x, F f) {
+    constexpr int P = S::P, U = P == 1 ? S::U : 1;
+    const int packs = x.packs();
+    for (int q = threadIdx.x; q < packs; q += U * kThreads) {
+        float v[U][P];
+        u64 w[U][P];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            if (q + j * kThreads < packs) {
+                x.load(q + j * kThreads, v[j]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < P; ++e) v[j][e] = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+#pragma unroll
+            for (int e = 0; e < P; ++e) w[j][e] = weigh(r, s, v[j][e]);
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+#pragma unroll
+            for (int e = 0; e < P; ++e) f(v[j][e], w[j][e]);
+    }
+}
 
 // The weight that top-p's ids have to reach: p of the whole, at least 1 (the
 // largest logit's id always stays).
@@ -215,50 +422,90 @@ __device__ __forceinline__ u64 share(double p, u64 whole) {
     return want < 1.0 ? 1 : want < (double)whole ? (u64)want : whole;
 }
 
+// Where a border key can be: [from, to]; keys above `to` lie ahead of it, and
+// number `ahead` (top-k); `keys`: how many it is among.
+struct Range {
+    u32 from, to;
+    u64 ahead;
+    u32 keys;
+};
+
+// What the border of top-k or top-p is.
+struct Border {
+    u32 key;
+    u64 ahead;  // count or weight of the larger keys
+    u64 ties;   // ids that have this key
+    u64 total, target;  // weight of what it is among, and top-p's target
+};
+
+// The weight of a row's ids that are not in hand, in units of the weights: at
+// least and at most. `below`: they are in hand, as keys below the range.
+struct Rest {
+    u64 least, most;
+    bool below;
+};
+
 // The border key: count (or, BY_WEIGHT, weight) of larger keys < target <=
-// that and its own. Candidates are keys >= floor; `few`: they are known to
-// be kList at most. BY_WEIGHT the target is p of all candidates' weight.
-template <bool BY_WEIGHT, typename S>
-__device__ Border border(Shared& s, const Row& r, const S& x, u32 floor_key, u32 top, u64 target,
-                         double p, bool few, u32 rank, u32 ctas) {
+// that and its own. The target of a weight is p of the weight of all keys >=
+// in.from and of the rest.
+template <bool BY_WEIGHT, bool ONE, typename S>
+__device__ Border border(Shared& s, const Row& r, const S& x, const Range& in, u64 target,
+                         double p, Rest rest, Team<ONE> t) {
     const int tid = threadIdx.x;
     u32* list = s.list[BY_WEIGHT];
-    u64(*told)[kMaxCluster] = s.told + (BY_WEIGHT ? 4 : 1);  // three lines
-    u32 from = floor_key, to = top;
-    u64 base = 0;
-    int shift = -1;  // -1: linear bins
+    // three lines; no call follows one of its kind without a barrier between
+    u64(*told)[kMaxCluster] = s.told + (BY_WEIGHT ? 4 : 1);
+    u32 from = in.from, to = in.to;
+    u64 base = BY_WEIGHT ? 0 : in.ahead;
+    int shift = max(0, 32 - __clz(to - from) - 9);  // (to - from) >> shift < 512
     int bin = -1;
-    for (;;) {
+    // few enough to gather at once: for a weight, only with nothing else to weigh
+    bool few = in.keys <= kList && (!BY_WEIGHT || (in.ahead == 0 && !rest.below));
+    u64 total = 0;
+    for (bool first = true;; first = false) {
         if (!few) {
             for (int b = tid; b < kBins; b += kThreads) s.lo[b] = s.hi[b] = 0;
             __syncthreads();
-            for (int i = tid; i < x.n; i += kThreads) {
-                const u32 k = x[i];
-                if (k < from || k > to) continue;
-                const int b = shift < 0 ? linear_bin(r, value_of(k)) : (int)((to - k) >> shift);
-                if (BY_WEIGHT) {
-                    const u64 w = weigh(r, s, k);
-                    const u32 a = (u32)w, old = atomicAdd(&s.lo[b], a);
+            u64 above = 0, below = 0;
+            if (BY_WEIGHT) {
+                each_weighed(r, s, x, [&](float f, u64 w) {
+                    const u32 k = key_of(f);
+                    above += first && k > to ? w : 0;
+                    below += first && k < from ? w : 0;
+                    if (k < from || k > to || w == 0) return;
+                    const u32 b = (to - k) >> shift, a = (u32)w, old = atomicAdd(&s.lo[b], a);
                     const u32 c = (u32)(w >> 32) + (old + a < old ? 1u : 0u);
                     if (c) atomicAdd(&s.hi[b], c);
-                } else {
-                    atomicAdd(&s.lo[b], 1u);
-                }
+                });
+            } else {
+                each(x, [&](int, float f, int) {
+                    const u32 k = key_of(f);
+                    if (k >= from && k <= to) atomicAdd(&s.lo[(to - k) >> shift], 1u);
+                });
             }
-            row_sync(ctas);
-            u64 v[2] = {0, 0};
-            for (u32 c = 0; c < ctas; ++c)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int b = 2 * tid + j;
-                    v[j] += (u64)peer_u32(&s.lo[b], c);
-                    if (BY_WEIGHT) v[j] += (u64)peer_u32(&s.hi[b], c) << 32;
+            if (BY_WEIGHT && first) {
+                t.tell(s.told[10], block_add(s, above));
+                if (rest.below) t.tell(s.told[11], block_add(s, below));
+            }
+            t.sync();
+            if (BY_WEIGHT && first)
+                for (u32 c = 0; c < t.ctas; ++c) {
+                    base += s.told[10][c];
+                    if (rest.below) total += s.told[11][c];
                 }
+            u64 v[2];
+            t.add_up(&s.lo[2 * tid], v);
+            if (BY_WEIGHT) {
+                u64 high[2];
+                t.add_up(&s.hi[2 * tid], high);
+                v[0] += high[0] << 32, v[1] += high[1] << 32;
+            }
             const u64 upto = block_upto(s, v[0] + v[1]);
             if (BY_WEIGHT && target == 0) {
                 if (tid == kThreads - 1) s.found[0] = upto;
                 __syncthreads();
-                target = share(p, s.found[0]);
+                total += base + s.found[0];
+                target = share(p, total + rest.least);
                 __syncthreads();
             }
             const u64 before = upto - v[0] - v[1];
@@ -275,72 +522,64 @@ __device__ Border border(Shared& s, const Row& r, const S& x, u32 floor_key, u32
         if (tid == 0) s.listed[BY_WEIGHT] = 0, s.least = 0xffffffffu, s.most = 0;
         __syncthreads();
         u32 least = 0xffffffffu, most = 0;
-        for (int i = tid; i < x.n; i += kThreads) {
-            const u32 k = x[i];
-            if (k < from || k > to) continue;
-            if (!few &&
-                (shift < 0 ? linear_bin(r, value_of(k)) : (int)((to - k) >> shift)) != bin)
-                continue;
+        each(x, [&](int, float f, int) {
+            const u32 k = key_of(f);
+            if (k < from || k > to || (!few && (int)((to - k) >> shift) != bin)) return;
             least = min(least, k);
             most = max(most, k);
             const u32 at = atomicAdd(&s.listed[BY_WEIGHT], 1u);
             if (at < kList) list[at] = k;
-        }
+        });
         least = __reduce_min_sync(0xffffffffu, least);
         most = __reduce_max_sync(0xffffffffu, most);
-        if ((tid & 31) == 0) {
+        if ((tid & 31) == 0 && least <= most) {
             atomicMin(&s.least, least);
             atomicMax(&s.most, most);
         }
         __syncthreads();
-        if (tid < (int)ctas) {
-            peer_store(&told[0][rank], tid, s.listed[BY_WEIGHT]);
-            peer_store(&told[1][rank], tid, s.least);
-            peer_store(&told[2][rank], tid, s.most);
-        }
-        row_sync(ctas);
+        t.tell(told[0], s.listed[BY_WEIGHT]);
+        t.tell(told[1], s.least);
+        t.tell(told[2], s.most);
+        t.sync();
         u64 count = 0;
-        for (u32 c = 0; c < ctas; ++c) {
+        least = 0xffffffffu, most = 0;
+        for (u32 c = 0; c < t.ctas; ++c) {
             count += told[0][c];
             least = min(least, (u32)told[1][c]);
             most = max(most, (u32)told[2][c]);
         }
-        from = __reduce_min_sync(0xffffffffu, least);
-        to = __reduce_max_sync(0xffffffffu, most);
+        from = least;
+        to = most;
         if (from == to) {  // one key, however often
-            if (BY_WEIGHT && target == 0) target = share(p, count * weigh(r, s, from));
-            return {from, base, count, target};
+            if (BY_WEIGHT && target == 0) {
+                total = count * weigh(r, s, value_of(from));
+                target = share(p, total + rest.least);
+            }
+            return {from, base, count, total, target};
         }
         if (count <= kList) {
-            u32 at = 0;
-            for (u32 c = 0; c < ctas; ++c) {
-                const u32 n = (u32)told[0][c];
-                for (u32 j = tid; j < n; j += kThreads) s.all[at + j] = peer_u32(&list[j], c);
-                at += n;
+            u32 at;
+            const u32 c = t.place(told[0], tid, &at);
+            const bool mine_in = c < t.ctas;
+            const u32 mine = mine_in ? t.read(&list[at], c) : 0;
+            const u64 w = BY_WEIGHT && mine_in ? weigh(r, s, value_of(mine)) : 0;
+            s.all[tid] = mine;  // no key behind the last
+            if (BY_WEIGHT) s.weight[tid] = w;
+            if (BY_WEIGHT && target == 0) {
+                total = block_add(s, w);
+                target = share(p, total + rest.least);
             }
             __syncthreads();
-            const bool in = tid < (int)count;
-            const u32 mine = in ? s.all[tid] : 0;
-            if (BY_WEIGHT) {
-                const u64 w = in ? weigh(r, s, mine) : 0;
-                s.weight[tid] = w;
-                if (target == 0) {  // p of the listed candidates
-                    const u64 upto = block_upto(s, w);
-                    if (tid == kThreads - 1) s.found[0] = upto;
-                    __syncthreads();
-                    target = share(p, s.found[0]);
-                }
-                __syncthreads();
-            }
-            if (in) {
-                u64 more = 0, own = 0, ties = 0;
-                for (int j = 0; j < (int)count; ++j) {
+            if (mine_in) {
+                u64 more = 0;
+                u32 ties = 0;
+#pragma unroll 8
+                for (int j = 0; j < (int)(count + 7) / 8 * 8; ++j) {
                     const u32 k = s.all[j];
-                    const u64 w = BY_WEIGHT ? s.weight[j] : 1;
-                    more += k > mine ? w : 0;
-                    own += k == mine ? w : 0;
+                    more += k > mine ? (BY_WEIGHT ? s.weight[j] : 1) : 0;
                     ties += k == mine;
                 }
+                const u64 own = ties * (BY_WEIGHT ? s.weight[tid] : 1);
                 if (base + more < target && target <= base + more + own) {  // all its ties say the same
                     s.found[1] = mine;
                     s.found[2] = base + more;
@@ -348,34 +587,40 @@ __device__ Border border(Shared& s, const Row& r, const S& x, u32 floor_key, u32
                 }
             }
             __syncthreads();
-            return {(u32)s.found[1], s.found[2], s.found[3], target};
+            return {(u32)s.found[1], s.found[2], s.found[3], total, target};
         }
-        const u32 span = to - from;
-        shift = max(0, 32 - __clz(span) - 9);  // span >> shift < 512
+        shift = max(0, 32 - __clz(to - from) - 9);
         few = false;
     }
 }
 
-// First id, by id, at which the running sum of measure(i, key) over the row
-// exceeds the target that aim(total) gives; -1 in CTAs that do not hold it.
-template <typename S, typename M, typename A>
-__device__ int first_beyond(Shared& s, const S& x, u64* told, u32 rank, u32 ctas, M measure,
-                            A aim) {
+// Index (in x) of the first id at which the running sum of measure(i, logit) over
+// the row exceeds the target that aim(total) gives; -1 in CTAs that do not
+// hold it.
+template <bool ONE, typename S, typename M, typename A>
+__device__ int first_beyond(Shared& s, const S& x, u64* told, Team<ONE> t, M measure, A aim) {
     const int tid = threadIdx.x, w = tid >> 5, lane = tid & 31;
-    const int part = (x.n + kThreads - 1) / kThreads * 32;  // a warp's run of ids
-    const int lo = min(w * part, x.n), hi = min(lo + part, x.n);
+    const int packs = x.packs(), part = (packs + kThreads - 1) / kThreads * 32;
+    const int lo = min(w * part, packs), hi = min(lo + part, packs);  // a warp's run
     u64 sum = 0;
-    for (int i = lo + lane; i < hi; i += 32) sum += measure(i, x[i]);
-    sum = warp_add(sum);
-    if (lane == 0) s.warp_sum[w] = sum;
-    __syncthreads();
-    u64 mine = 0;
-    for (int k = 0; k < kWarps; ++k) mine += s.warp_sum[k];
-    if (tid < (int)ctas) peer_store(told + rank, tid, mine);
-    row_sync(ctas);
+    for (int i = lo + lane; i < hi; i += 32 * S::U) {
+        float v[S::U][S::P];
+#pragma unroll
+        for (int j = 0; j < S::U; ++j)
+            if (i + 32 * j < hi) x.load(i + 32 * j, v[j]);
+#pragma unroll
+        for (int j = 0; j < S::U; ++j) {
+            if (i + 32 * j >= hi) break;
+#pragma unroll
+            for (int e = 0; e < S::P; ++e) sum += measure((i + 32 * j) * S::P + e, v[j][e]);
+        }
+    }
+    const u64 mine = block_add(s, sum);
+    t.tell(told, mine);
+    t.sync();
     u64 total = 0, before = 0;
-    for (u32 c = 0; c < ctas; ++c) {
-        if (c == rank) before = total;
+    for (u32 c = 0; c < t.ctas; ++c) {
+        if (c == t.rank) before = total;
         total += told[c];
     }
     const u64 target = aim(total);
@@ -383,19 +628,17 @@ __device__ int first_beyond(Shared& s, const S& x, u64* told, u32 rank, u32 ctas
     int k = 0;
     while (target >= before + s.warp_sum[k]) before += s.warp_sum[k++];
     // the run of warp k, a few ids to each thread
-    const int a = min(k * part, x.n), b = min(a + part, x.n);
+    const int a = min(k * part * S::P, x.n), b = min((k + 1) * part * S::P, x.n);
     const int n = (b - a + kThreads - 1) / kThreads;
     const int from = min(a + tid * n, b), to = min(from + n, b);
     sum = 0;
-    for (int i = from; i < to; ++i) sum += measure(i, x[i]);
-    u64 upto = before + block_upto(s, sum);
-    if (tid == 0) s.found[0] = ~0ull;
-    __syncthreads();
+    for (int i = from; i < to; ++i) sum += measure(i, x.value(i));
+    const u64 upto = before + block_upto(s, sum);
     if (target < upto && target >= upto - sum) {
         u64 at = upto - sum;
         int i = from;
         for (; i < to - 1; ++i) {
-            at += measure(i, x[i]);
+            at += measure(i, x.value(i));
             if (at > target) break;
         }
         s.found[0] = (u64)i;
@@ -404,147 +647,550 @@ __device__ int first_beyond(Shared& s, const S& x, u64* told, u32 rank, u32 ctas
     return (int)s.found[0];
 }
 
-template <typename T, bool HELD>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
-    extern __shared__ __align__(16) u32 held[];
-    __shared__ Shared s;
-    const int tid = threadIdx.x;
-    const u32 ctas = cluster_size(), rank = cluster_rank();
-    const int row = blockIdx.x / ctas;
-    Slice<T, HELD> x;
-    x.first = min((long long)rank * a.slice, (long long)a.V);
-    x.n = min(a.slice, a.V - x.first);
-    x.x = static_cast<const T*>(a.logits) + row * a.ld + x.first;
-    x.held = held;
-    if (tid < 16) s.pow16[tid] = exp2(tid / 16.0);
-
-    // keys, the largest with its lowest id, the smallest above -infinity
-    u64 best = 0;
-    u32 least = 0xffffffffu;
-    const auto take = [&](int i, float v) {
-        const u32 k = key_of(v);
-        if (HELD) held[i] = k;
-        const u64 c = (u64)k << 32 | (0xffffffffu - (u32)(x.first + i));
-        best = c > best ? c : best;
-        if (k > kNothing) least = min(least, k);
-    };
-    {
-        constexpr int P = 16 / sizeof(T), U = 4;
-        struct alignas(16) Pack {
-            T v[P];
-        };
-        const int head = min(x.n, (int)((16 - ((uintptr_t)x.x & 15)) % 16 / sizeof(T)));
-        const int packs = (x.n - head) / P;
-        const Pack* px = reinterpret_cast<const Pack*>(x.x + head);
-        for (int q = tid; q < packs; q += U * kThreads) {
-            Pack v[U];
-#pragma unroll
-            for (int j = 0; j < U; ++j)
-                if (q + j * kThreads < packs) v[j] = px[q + j * kThreads];
-#pragma unroll
-            for (int j = 0; j < U; ++j)
-                if (q + j * kThreads < packs)
-#pragma unroll
-                    for (int e = 0; e < P; ++e)
-                        take(head + (q + j * kThreads) * P + e, number<T>(v[j].v[e]));
-        }
-        for (int i = tid; i < head; i += kThreads) take(i, number<T>(x.x[i]));
-        for (int i = head + packs * P + tid; i < x.n; i += kThreads) take(i, number<T>(x.x[i]));
+// Key of the smallest number whose linear bin is `bin` or nearer, by the lanes
+// of a warp: it lies in (out, in], at first within 256 keys of the bin's edge in
+// real numbers where those ends say so, cut to a 32nd by each step. One above
+// the row's largest where that lies in a farther bin.
+__device__ u32 near_edge(const Row& r, int bin) {
+    const u32 lane = threadIdx.x & 31, top = key_of(r.max_f);
+    if (linear_bin(r, r.max_f) > bin) return top + 1;
+    const u32 guess = key_of(fminf(fmaxf(r.ref - (bin + 0.5f) / r.bin, -3e38f), r.max_f));
+    u32 out = guess - 256, in = min(guess + 256, top);
+    if (!(out > kNothing && out < in && linear_bin(r, value_of(out)) > bin)) out = kNothing;
+    if (linear_bin(r, value_of(in)) > bin) in = top;
+    while (in - out > 1) {
+        const u32 step = (in - out + 31) / 32;
+        const u32 at = min((u64)out + (u64)step * (lane + 1), (u64)in);
+        const u32 near = __ballot_sync(0xffffffffu, linear_bin(r, value_of(at)) <= bin);
+        const int f = __ffs(near) - 1;  // the last lane's is `in` itself
+        const u32 low = out;
+        out = f ? (u32)min((u64)low + (u64)step * f, (u64)in) : low;
+        in = (u32)min((u64)low + (u64)step * (f + 1), (u64)in);
     }
-    best = warp_max(best);
-    least = __reduce_min_sync(0xffffffffu, least);
-    if ((tid & 31) == 0) {
-        s.red[tid >> 5] = best;
-        s.warp_sum[tid >> 5] = least;
+    return in;
+}
+
+// Narrows where the border is, from the counts of the linear bins and, for
+// top-p, the estimate `sum` of the weight of all relative to ref's. Returns how
+// many ids lie in the range or above; 0: the bins lie in the wrong place.
+template <bool ONE>
+__device__ u32 cut(Shared& s, const Row& r, int V, int k, double p, int bits, Team<ONE> t,
+                   double sum, Range* range) {
+    constexpr int N = kCut / kThreads;
+    const int tid = threadIdx.x;
+    u64 whole[2] = {0, 0};
+    if (k <= 0) {
+        // 2^-12 is more than its terms' 2^-22, the roundings of exponents up to
+        // 200 (3 * 2^-24 * 200 * ln 2 < 2^-15) and those of sums of 2^10 terms
+        sum *= exp2(((double)r.ref - r.max) * r.scale);
+        if (!(sum >= 0.5 && sum < 2.0 * V)) return 0;  // ref is too far off
+        const double units = sum * two_to(bits);
+        whole[0] = (u64)(units * (1 - 0x1p-12));
+        whole[1] = (u64)(units * (1 + 0x1p-12));
+    }
+    u64 sums[N];
+    u32 n[N], own = 0;
+    t.add_up(&s.count[N * tid], sums);
+#pragma unroll
+    for (int j = 0; j < N; ++j) own += n[j] = (u32)sums[j];
+    u32 counted = (u32)block_upto(s, own) - own;  // before this thread's bins
+    if (tid == 0) s.found[0] = kCut, s.found[3] = 0;
+    __syncthreads();
+    // found: the border's bin or a farther one, ids up to it, ids in it; and
+    // how many nearest bins are surely ahead of the border
+    if (k > 0) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (counted < (u32)k && (u32)k <= counted + n[j]) {
+                s.found[0] = s.found[3] = N * tid + j;
+                s.found[1] = counted + n[j];
+                s.found[2] = n[j];
+            }
+            counted += n[j];
+        }
+    } else {  // the weight of a bin's ids is between those of its edges
+        const float step = (float)(r.scale / r.bin), unit_f = (float)two_to(bits);
+        const float d0 = (float)(((double)r.ref - r.max) * r.scale);  // bin 0's middle
+        u64 lo[N], hi[N], lo_upto = 0, hi_upto = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int b = N * tid + j;
+            const float slack = 0x1p-16f + 0x1p-21f * fabsf(d0);
+            const float far = fminf(d0 - (b + 0.5f) * step * (1 + 0x1p-18f), 0.0f);
+            const float near = b == 0 ? 0.0f : fminf(d0 - (b - 0.5f) * step * (1 - 0x1p-18f), 0.0f);
+            lo[j] = (u64)(n[j] * (unit_f * (1 - slack) * fast_exp2(far)));
+            hi[j] = (u64)(n[j] * (unit_f * (1 + slack) * fast_exp2(near))) + n[j];
+            lo_upto += lo[j];
+            hi_upto += hi[j];
+        }
+        lo_upto = block_upto(s, lo_upto) - lo_upto;
+        hi_upto = block_upto(s, hi_upto) - hi_upto;
+        const u64 sure = share(p, whole[1]), may = share(p, whole[0]);
+        u32 ahead = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            counted += n[j];
+            if (lo_upto < sure && sure <= lo_upto + lo[j]) {
+                s.found[0] = N * tid + j;
+                s.found[1] = counted;
+            }
+            lo_upto += lo[j];
+            hi_upto += hi[j];
+            ahead += hi_upto < may;  // bins up to which the row is lighter (the sums ascend)
+        }
+        ahead = (u32)block_add(s, ahead);
+        if (tid == 0) s.found[3] = ahead;
     }
     __syncthreads();
-    for (int k = 0; k < kWarps; ++k) {
-        best = s.red[k] > best ? s.red[k] : best;
-        least = min(least, (u32)s.warp_sum[k]);
+    // no bin, or the last, which has no far edge: every id can stay
+    const int bin = (int)s.found[0], ahead = (int)s.found[3];
+    const bool open = bin >= kCut - 2;
+    if (tid < 32) {
+        const u32 e = open ? kNothing : near_edge(r, bin);
+        if (tid == 0) s.edge[0] = e;
+    } else if (tid < 64) {
+        const u32 e = ahead > 0 ? near_edge(r, min(ahead, kCut - 1) - 1) - 1 : key_of(r.max_f);
+        if (tid == 32) s.edge[1] = e;
     }
-    if (tid < (int)ctas) {
-        peer_store(&s.told[0][rank], tid, best);
-        peer_store(&s.told[7][rank], tid, least);
-    }
-    row_sync(ctas);
-    for (u32 c = 0; c < ctas; ++c) {
-        best = s.told[0][c] > best ? s.told[0][c] : best;
-        least = min(least, (u32)s.told[7][c]);
-    }
+    __syncthreads();
+    range->from = s.edge[0];
+    range->to = s.edge[1];
+    range->ahead = k > 0 ? s.found[1] - s.found[2] : range->to < key_of(r.max_f);
+    const u32 all = open && k <= 0 ? (u32)V : (u32)s.found[1];
+    range->keys = k > 0 ? (u32)s.found[2] : all;
+    __syncthreads();
+    return all;
+}
 
-    const u32 top = (u32)(best >> 32);
-    const double T_ = a.temperature.at(row);
-    if (top <= kNothing || top >= kInfinite || !(T_ > 0.0)) {
-        // nothing to draw, or nothing but the largest (its lowest id)
-        if (rank == 0 && tid == 0)
-            a.out[row] = top <= kNothing ? -1 : (int)(0xffffffffu - (u32)best);
-        return;
+// Marks the places of a slice's logits >= least, a bit each in words of 32, then
+// gives put(position, place) for each in order; returns their number. REST: the
+// weight of the others is estimated and added to *rest.
+template <bool REST, typename S, typename F>
+__device__ int list(Shared& s, const Row& r, const S& x, float least, u32* marks, float* rest,
+                    F put) {
+    constexpr int U = 8;
+    const int tid = threadIdx.x, words = (x.n + 31) / 32;
+    for (int w0 = (tid >> 5) * U; w0 < words; w0 += kWarps * U) {
+        float v[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int i = (w0 + j) * 32 + (tid & 31);
+            v[j] = i < x.n ? x.value(i) : -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const u32 m = __ballot_sync(0xffffffffu, v[j] >= least);
+            if ((tid & 31) == j && w0 + j < words) marks[w0 + j] = m;
+        }
+        if (REST) {
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+                v[j] = v[j] >= least ? 0.0f : fast_exp2((v[j] - r.max_f) * r.scale_f);
+            *rest += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        }
     }
-    Row r;
-    r.max_f = value_of(top);
-    r.max = r.max_f;
-    r.scale = fmin(1.4426950408889634074 / T_, 1e300);
-    r.shift = 52 - a.bits;
-    // beyond 46 / log2(e) temperatures below the largest every weight is 0
-    const float range = fminf((float)fmin(32.0 * T_, 3e38), r.max_f - value_of(least));
-    r.bin = fminf(kBins / range, 3e38f);
+    __syncthreads();
+    // a few neighbouring words to each thread
+    const int each = (words + kThreads - 1) / kThreads;
+    const int lo = min(tid * each, words), hi = min(lo + each, words);
+    u32 mine = 0;
+    for (int w = lo; w < hi; ++w) mine += __popc(marks[w]);
+    const u32 upto = (u32)block_upto(s, mine);
+    if (tid == kThreads - 1) s.found[0] = upto;
+    u32 at = upto - mine;
+    for (int w = lo; w < hi; ++w)
+        for (u32 m = marks[w]; m; m &= m - 1) put(at++, w * 32 + __ffs(m) - 1);
+    __syncthreads();
+    return (int)s.found[0];
+}
 
-    const int k = a.top_k ? a.top_k[row] : a.one_k;
-    const double p = a.top_p.at(row);
-    u32 key = 0;              // kept: larger keys, and of the equal ones ids up to `last`
+// Place of the m-th marked, from 0, in the thread that finds it; -1 in others.
+__device__ __forceinline__ int marked_place(Shared& s, int n, const u32* marks, u32 m) {
+    const int words = (n + 31) / 32, each = (words + kThreads - 1) / kThreads;
+    const int lo = min((int)threadIdx.x * each, words), hi = min(lo + each, words);
+    u32 mine = 0;
+    for (int w = lo; w < hi; ++w) mine += __popc(marks[w]);
+    u32 at = (u32)block_upto(s, mine) - mine;
+    if (m < at || m >= at + mine) return -1;
+    for (int w = lo; w < hi; ++w)
+        for (u32 b = marks[w]; b; b &= b - 1)
+            if (at++ == m) return w * 32 + __ffs(b) - 1;
+    return -1;
+}
+
+struct Rule {
+    int k;              // 0: none
+    double p, u;        // p of 1: none
+    u64 w_floor;        // least weight
+    __device__ __forceinline__ u64 aim(u64 total) const {  // u of the kept weight
+        const double t = u * (double)total;
+        return !(t > 0.0) ? 0ull : t >= (double)total ? total - 1 : min((u64)t, total - 1);
+    }
+};
+
+// The draw among the listed ids of a top-k row, kList of the whole row at most,
+// by the CTA of rank 0: a thread for each id, which counts and weighs those
+// ahead of it. The lists are in order of id. Returns the id (first + x.id), -1
+// in other CTAs.
+template <bool ONE, typename L>
+__device__ int draw_few(Shared& s, const Row& r, const L& x, int first, const Rule& g,
+                        Team<ONE> t) {
+    const int tid = threadIdx.x;
+    // each CTA leaves its keys and ids where rank 0 reads them
+    for (int i = tid; i < x.n; i += kThreads) {
+        s.list[0][i] = key_of(x.value(i));
+        s.list[1][i] = (u32)(first + x.id(i));
+    }
+    if (tid == 0) t.store(&s.told[1][t.rank], 0, (u64)x.n);
+    t.sync();
+    if (t.rank == 0) {
+        u32 at, count = 0;
+        for (u32 c = 0; c < t.ctas; ++c) count += (u32)s.told[1][c];
+        const u32 c = t.place(s.told[1], tid, &at);
+        const bool in = c < t.ctas;
+        const u32 mine = in ? t.read(&s.list[0][at], c) : 0;
+        const u32 id = in ? t.read(&s.list[1][at], c) : 0;
+        const u64 w = in ? weigh(r, s, value_of(mine)) : 0;
+        s.all[tid] = mine;  // no key behind the last
+        s.weight[tid] = w;
+        __syncthreads();
+        int more = 0;   // larger ones
+        u64 ahead = 0;  // weight of the ids before this in descending order
+        if (in) {
+#pragma unroll 8
+            for (int j = 0; j < (int)(count + 7) / 8 * 8; ++j) {
+                const u32 k = s.all[j];
+                more += k > mine;
+                ahead += k > mine || (k == mine && j < tid) ? s.weight[j] : 0;
+            }
+        }
+        bool stays = in && more < g.k;
+        const u64 target = g.p < 1.0 ? share(g.p, block_add(s, stays ? w : 0)) : ~0ull;
+        stays = stays && ahead < target && w >= g.w_floor;
+        const u64 upto = block_upto(s, stays ? w : 0);
+        if (tid == kThreads - 1) s.found[1] = upto;
+        __syncthreads();
+        const u64 goal = g.aim(s.found[1]);
+        if (stays && goal < upto && goal >= upto - w) s.found[0] = id;
+    }
+    t.sync();  // no CTA ends while rank 0 may still read from it
+    return t.rank == 0 ? (int)s.found[0] : -1;
+}
+
+// The draw among the ids of x (all of the slice's, or its listed ones) by the
+// whole cluster. rest: of the ids that x leaves out, whose weight exact(key)
+// gives as that of smaller keys. Returns the index in x, -1 in other CTAs.
+template <bool ONE, typename S, typename E>
+__device__ int draw(Shared& s, const Row& r, const S& x, int first, const Rule& g, Range range,
+                    Rest rest, Team<ONE> t, E exact) {
+    u32 key = 0;            // kept: larger keys, and of the equal ones ids up to `last`
     int last = 0x7fffffff;
-    bool few = false;
-    if (k > 0 && k < a.V) {
-        const Border b = border<false>(s, r, x, 0, top, (u64)k, 0.0, false, rank, ctas);
+    if (g.k > 0) {
+        const Border b = border<false>(s, r, x, range, (u64)g.k, 0.0, rest, t);
         key = b.key;
-        few = b.ahead + b.ties <= kList;
+        range = {key, key_of(r.max_f), 0, (u32)min(b.ahead + b.ties, (u64)0xffffffffu)};
+        rest = {0, 0, false};
     }
-    if (p > 0.0 && p < 1.0) {
-        const Border b = border<true>(s, r, x, key, top, 0, p, few, rank, ctas);
+    if (g.p < 1.0) {
+        Border b;
+        u64 stay;
+        for (;;) {
+            b = border<true>(s, r, x, range, 0, g.p, rest, t);
+            const u64 w = weigh(r, s, value_of(b.key));
+            stay = w ? (b.target - b.ahead + w - 1) / w : b.ties;
+            if (rest.least == rest.most) break;
+            // the other end of the estimate: the same key, and as many of its ties?
+            const u64 most = share(g.p, b.total + rest.most);
+            if (most <= b.ahead + b.ties * w && (most - b.ahead + w - 1) / w == stay) break;
+            t.sync();
+            rest.least = rest.most = exact(range.from);
+        }
         key = b.key;
-        const u64 w = weigh(r, s, key);
-        const u64 stay = w ? (b.target - b.ahead + w - 1) / w : b.ties;
         if (stay < b.ties) {
             const int i = first_beyond(
-                s, x, s.told[7], rank, ctas, [&](int, u32 q) { return (u64)(q == key); },
+                s, x, s.told[7], t, [&](int, float v) { return (u64)(key_of(v) == key); },
                 [&](u64) { return stay - 1; });
-            if (i >= 0 && tid < (int)ctas) peer_store(&s.told[0][0], tid, (u64)(x.first + i));
-            row_sync(ctas);
+            if (i >= 0 && threadIdx.x < t.ctas)
+                t.store(&s.told[0][0], threadIdx.x, (u64)(first + x.id(i)));
+            t.sync();
             last = (int)s.told[0][0];
         }
     }
-    const double least_w = fmin(a.min_p.at(row), 1.0) * exp2((double)a.bits);
-    const u64 w_floor = least_w > 0.0 ? (u64)ceil(least_w) : 0;
-    const double u = a.u_wide ? static_cast<const double*>(a.u)[row]
-                              : (double)static_cast<const float*>(a.u)[row];
-    const int i = first_beyond(
-        s, x, s.told[8], rank, ctas,
-        [&](int j, u32 q) -> u64 {
-            if (q < key || (q == key && x.first + j > last)) return 0;
-            const u64 w = weigh(r, s, q);
-            return w < w_floor ? 0 : w;
+    return first_beyond(
+        s, x, s.told[8], t,
+        [&](int j, float v) -> u64 {
+            const u32 q = key_of(v);
+            const u64 w = weigh(r, s, v);  // for all: in a warp some lane needs it
+            return q < key || (q == key && first + x.id(j) > last) || w < g.w_floor ? 0 : w;
         },
-        [&](u64 total) {
-            const double t = u * (double)total;
-            return !(t > 0.0) ? 0ull : t >= (double)total ? total - 1 : min((u64)t, total - 1);
-        });
-    if (i >= 0 && tid == 0) a.out[row] = x.first + i;
-    row_sync(ctas);  // no CTA ends while another may still store into it
+        [&](u64 total) { return g.aim(total); });
 }
 
-template <typename T>
-int launch(const SampleArgs& a, int B, int ctas, cudaStream_t st) {
-    const size_t held = (size_t)(a.slice + 3) / 4 * 16;
-    const bool fits = held <= 200 * 1024;
-    const auto kern = fits ? sample_kernel<T, true> : sample_kernel<T, false>;
-    if (fits && held + sizeof(Shared) > 48 * 1024)
+// HELD: the slice is kept in shared memory, in front of a list of its places (as
+// many as it has). Otherwise the list is of kCand logits.
+template <typename T, bool HELD, bool ONE>
+__global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a) {
+    extern __shared__ __align__(16) float dyn[];
+    __shared__ Shared s;
+    const int tid = threadIdx.x;
+    const Team<ONE> t;
+    const int row = blockIdx.x / t.ctas;
+    const int first = min((long long)t.rank * a.slice, (long long)a.V);
+    Far<T> far;
+    {
+        const T* x = static_cast<const T*>(a.logits) + row * a.ld + first;
+        far.skip = (int)((uintptr_t)x & 15) / (int)sizeof(T);
+        far.x = x - far.skip;
+        far.n = min(a.slice, a.V - first) + far.skip;
+    }
+    const double T_ = a.temperature.at(row);
+    const bool greedy = !(T_ > 0.0);
+    Rule g;
+    g.k = a.top_k ? a.top_k[row] : a.one_k;
+    if (g.k < 0 || g.k >= a.V) g.k = 0;
+    g.p = a.top_p.at(row);
+    if (!(g.p > 0.0 && g.p < 1.0)) g.p = 1.0;
+    const double q = fmin(a.min_p.at(row), 1.0);
+    const double least_w = q * two_to(a.bits);
+    g.w_floor = least_w > 0.0 ? (u64)ceil(least_w) : 0;
+    g.u = a.u_wide ? static_cast<const double*>(a.u)[row]
+                   : (double)static_cast<const float*>(a.u)[row];
+    Row r;
+    r.scale = fmin(1.4426950408889634074 / T_, 1e300);
+    r.scale_f = (float)fmin(r.scale, 3e38);
+    r.unit = two_to(52 - a.bits);
+    const double reach = 64.0 / r.scale;
+    // (a scale that fp32 does not hold well: no estimates)
+    const bool bins = !greedy && (g.k > 0 || g.p < 1.0) && r.scale > 1e-30 && r.scale < 1e30 &&
+                      a.V < 1 << 20;
+    if (tid < kPow) s.pow[tid] = g_pow.v[tid];
+    if (bins) {
+        // The bins have to be in place before the row is read, its largest logit
+        // not known: they reach from 24 temperatures above the largest of the
+        // first kProbe logits to 32 below (beyond, every weight is 0), and at
+        // high temperatures over 112 at most. Where that is the wrong place the
+        // first or the last bin holds what matters, and the row goes on as if
+        // it had not been counted.
+        float v = -INFINITY;
+        const T* x = static_cast<const T*>(a.logits) + row * a.ld;
+#pragma unroll
+        for (int j = 0; j < kProbe / kThreads; ++j)
+            if (j * kThreads + tid < a.V) v = fmaxf(v, number<T>(x[j * kThreads + tid]));
+        const u32 k = __reduce_max_sync(0xffffffffu, key_of(v));
+        if ((tid & 31) == 0) s.warp_sum[tid >> 5] = k;
+        for (int b = tid; b < kCut; b += kThreads) s.count[b] = 0;
+        __syncthreads();
+        u32 first_most = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) first_most = max(first_most, (u32)s.warp_sum[w]);
+        const float t8 = (float)fmin(8.0 * T_, 16.0);
+        r.ref = (first_most == kNothing ? 0.0f : fminf(value_of(first_most), 3e38f)) + 3.0f * t8;
+        r.bin = fminf((kCut - 4) / (7.0f * t8), 3e38f);
+    }
+
+    // one pass over the slice: the largest; its id (greedy); the counts; the
+    // sum of the weights' estimates (top-p alone)
+    float best = -INFINITY, e[4] = {0, 0, 0, 0};
+    int best_at = 0;
+    const auto pass = [&](auto f) {
+        if constexpr (HELD) {
+            constexpr int P = Far<T>::P, U = Far<T>::U;
+            const int packs = far.packs();
+            for (int q = tid; q < packs; q += U * kThreads) {
+                float v[U][P];
+#pragma unroll
+                for (int j = 0; j < U; ++j)
+                    if (q + j * kThreads < packs) far.load(q + j * kThreads, v[j]);
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    if (q + j * kThreads >= packs) break;
+#pragma unroll
+                    for (int i = 0; i < P; i += 4)
+                        reinterpret_cast<float4*>(dyn)[((q + j * kThreads) * P + i) / 4] =
+                            make_float4(v[j][i], v[j][i + 1], v[j][i + 2], v[j][i + 3]);
+#pragma unroll
+                    for (int i = 0; i < P; ++i) f(v[j][i], i);
+                }
+            }
+        } else {
+            each(far, [&](int, float v, int i) { f(v, i); });
+        }
+    };
+    if (greedy) {
+        each(far, [&](int i, float v, int) {
+            best_at = v > best ? i : best_at;
+            best = fmaxf(best, v);
+        });
+    } else if (!bins) {
+        pass([&](float v, int) { best = fmaxf(best, v); });
+    } else if (g.k > 0) {
+        pass([&](float v, int) {
+            best = fmaxf(best, v);
+            atomicAdd(&s.count[linear_bin(r, v)], 1u);
+        });
+    } else {
+        pass([&](float v, int i) {
+            best = fmaxf(best, v);
+            atomicAdd(&s.count[linear_bin(r, v)], 1u);
+            e[i & 3] += fast_exp2((v - r.ref) * r.scale_f);
+        });
+    }
+    double sum = 0.0;
+    if (bins && g.k <= 0) {
+        sum = ((double)e[0] + e[1]) + ((double)e[2] + e[3]);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        __syncthreads();
+        if ((tid & 31) == 0) s.warp_sum[tid >> 5] = (u64)__double_as_longlong(sum);
+    }
+    u64 most = __reduce_max_sync(0xffffffffu, key_of(best));
+    const u32 id = (u32)most == key_of(best) ? (u32)(first + far.id(best_at)) : 0xffffffffu;
+    most = most << 32 | ~__reduce_min_sync(0xffffffffu, greedy ? id : 0);
+    if ((tid & 31) == 0) s.red[tid >> 5] = most;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) most = s.red[k] > most ? s.red[k] : most;
+    if (bins && g.k <= 0) {  // in the order of the warps, then of the CTAs
+        sum = 0.0;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) sum += __longlong_as_double((long long)s.warp_sum[k]);
+        t.tell(s.told[9], (u64)__double_as_longlong(sum));
+    }
+    t.tell(s.told[0], most);
+    t.sync();
+    sum = 0.0;
+#pragma unroll
+    for (int c = 0; c < (ONE ? 1 : kMaxCluster); ++c)
+        if (c < (int)t.ctas) {
+            most = s.told[0][c] > most ? s.told[0][c] : most;
+            if (bins && g.k <= 0) sum += __longlong_as_double((long long)s.told[9][c]);
+        }
+
+    const u32 top = (u32)(most >> 32);
+    if (top == kNothing || greedy) {
+        if (t.rank == 0 && tid == 0)
+            a.out[row] = top == kNothing ? -1 : (int)~(u32)most;
+        return;
+    }
+    r.max_f = value_of(top);
+    const auto x = [&] {
+        if constexpr (HELD)
+            return Near{dyn, far.n, far.skip};
+        else
+            return far;
+    }();
+    if (r.max_f == INFINITY) {  // nothing but the largest: its lowest id
+        const int i = first_beyond(
+            s, x, s.told[8], t, [&](int, float v) { return (u64)(v == INFINITY); },
+            [](u64) { return 0ull; });
+        if (i >= 0 && tid == 0) a.out[row] = first + x.id(i);
+        t.sync();  // no CTA ends while another may still read from it
+        return;
+    }
+    r.max = r.max_f;
+    r.cutoff = fmaxf(__double2float_ru(r.max - reach), -3.402823466e38f);
+    Range range{kNothing, top, 0, (u32)a.V};
+    const auto exact = [&](u32 from) {
+        u64 sum = 0;
+        each_weighed(r, s, x, [&](float v, u64 w) { sum += key_of(v) < from ? w : 0; });
+        t.tell(s.told[12], block_add(s, sum));
+        t.sync();
+        sum = 0;
+        for (u32 c = 0; c < t.ctas; ++c) sum += s.told[12][c];
+        return sum;
+    };
+    if (bins) {
+        Range found;
+        const u32 listed = cut(s, r, a.V, g.k, g.p, a.bits, t, sum, &found);
+        if (listed) range = found;
+        // every CTA of the cluster decides alike
+        if (listed && HELD ? listed <= (u32)a.V / 2 : listed && ONE && listed <= kCand) {
+            const float least = value_of(range.from);
+            float others = 0.0f;  // estimate of the weight that is not listed (top-p alone)
+            const auto finish = [&](const auto& l) {
+                if (g.k > 0 && listed <= kList) return draw_few(s, r, l, first, g, t);
+                Rest rest{0, 0, false};
+                if (g.k <= 0) {
+                    // Each 2^d is off by 2^-22 of itself, and by the roundings of
+                    // the difference, the scale and their product, 3 * 2^-24 |d|
+                    // ln 2; a thread adds up n / 2048 + 4 of them. The mean of
+                    // |d|, by weight, is the entropy of the weights less log2 of
+                    // their sum, at most log2(V / sum).
+                    double v = others;
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                    __syncthreads();
+                    if ((tid & 31) == 0) s.warp_sum[tid >> 5] = (u64)__double_as_longlong(v);
+                    __syncthreads();
+                    v = 0.0;
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) v += __longlong_as_double((long long)s.warp_sum[w]);
+                    t.tell(s.told[13], (u64)__double_as_longlong(v));
+                    t.sync();
+                    v = 0.0;
+                    for (u32 c = 0; c < t.ctas; ++c) v += __longlong_as_double((long long)s.told[13][c]);
+                    if (v > 0x1p-100) {
+                        const double mean = ilogb(a.V / v) + 1;
+                        const double off = 0x1p-22 + (far.n / 2048 + 8) * 0x1p-24 + 3 * 0x1p-24 * 0.694 * mean;
+                        const double units = v * two_to(a.bits), err = 1.01 * off * units + a.V;
+                        rest.least = units > err ? (u64)(units - err) : 0;
+                        rest.most = (u64)(units + err);  // (exact weights are rounded, too)
+                    } else {
+                        rest.most = a.V;
+                    }
+                }
+                const int i = draw(s, r, l, first, g, range, rest, t, exact);
+                t.sync();
+                return i < 0 ? -1 : first + l.id(i);
+            };
+            const auto listing = [&](u32* marks, auto put) {
+                return g.k > 0 ? list<false>(s, r, x, least, marks, &others, put)
+                               : list<true>(s, r, x, least, marks, &others, put);
+            };
+            if constexpr (HELD) {
+                unsigned short* at = reinterpret_cast<unsigned short*>(dyn + a.slice + 8);
+                u32* marks = reinterpret_cast<u32*>(at + a.slice + 8);
+                const int n = listing(marks, [&](u32 pos, int i) {
+                    at[pos] = (unsigned short)i;
+                });
+                const int id = finish(NearListed{x, at, n});
+                if (id >= 0 && tid == 0) a.out[row] = id;
+            } else {
+                u32* marks = reinterpret_cast<u32*>(dyn + kCand);
+                u32* at = reinterpret_cast<u32*>(dyn);  // places first, then the logits there
+                const int n = min(kCand, listing(marks, [&](u32 pos, int i) {
+                    if (pos < kCand) at[pos] = (u32)i;
+                }));
+#pragma unroll 4
+                for (int i = tid; i < n; i += kThreads) dyn[i] = x.value((int)at[i]);
+                __syncthreads();
+                const int m = finish(FarListed{dyn, n});
+                const int i = marked_place(s, x.n, marks, (u32)m);
+                if (i >= 0) a.out[row] = x.id(i);
+            }
+            return;
+        }
+    }
+    const int i = draw(s, r, x, first, g, range, Rest{0, 0, g.k <= 0}, t, exact);
+    if (i >= 0 && tid == 0) a.out[row] = first + x.id(i);
+    t.sync();
+}
+
+template <typename T, bool HELD, bool ONE>
+int start(const SampleArgs& a, int B, int ctas, size_t dyn, cudaStream_t st) {
+    const auto kern = sample_kernel<T, HELD, ONE>;
+    if (dyn + sizeof(Shared) > 48 * 1024)
         SN_TRY(cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                200 * 1024),
                           "sample"));
+    if (ONE) {
+        kern<<<B, kThreads, dyn, st>>>(a);
+        return cuda_check(cudaGetLastError(), "sample launch");
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)B * ctas);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = fits ? held : 0;
+    cfg.dynamicSmemBytes = dyn;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -553,6 +1199,30 @@ int launch(const SampleArgs& a, int B, int ctas, cudaStream_t st) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cuda_check(cudaLaunchKernelEx(&cfg, kern, a), "sample launch");
+}
+
+template <typename T>
+int launch(SampleArgs& a, int B, int sms, cudaStream_t st) {
+    // Rows enough to keep every SM busy with four CTAs: a row to a CTA. Fewer:
+    // slices of 8192 logits, cut further down to 2048 while the SMs have less
+    // than two CTAs each.
+    const bool one = B >= 4 * sms;
+    int ctas = 1;
+    while (!one && ctas < kMaxCluster &&
+           ((long long)ctas * 8192 < a.V ||
+            ((long long)B * ctas < 2ll * sms && (long long)ctas * 2048 < a.V)))
+        ctas *= 2;
+    a.slice = (int)(((long long)a.V + ctas - 1) / ctas + 7) / 8 * 8;
+    // the slice in fp32 behind up to 7 skipped places, a list of places in 16
+    // bits, and a bit for each
+    const size_t marks = (size_t)(a.slice + 8 + 31) / 32 * 4, held = (size_t)(a.slice + 8) * 6 + marks;
+    if (ctas == 1 && a.slice > 8192) {
+        const size_t dyn = 4 * kCand + marks;
+        if (dyn <= 200 * 1024) return start<T, false, true>(a, B, 1, dyn, st);
+    }
+    if (held > 200 * 1024) return start<T, false, false>(a, B, ctas, 0, st);
+    return ctas == 1 ? start<T, true, true>(a, B, 1, held, st)
+                     : start<T, true, false>(a, B, ctas, held, st);
 }
 
 }  // namespace
@@ -577,22 +1247,13 @@ extern "C" sn_status sn_abi_sample(const void* logits, int64_t ld, int32_t dtype
     CallerDevice dev;
     SN_TRY(dev.enter("sample", {{logits, size}, {u, u_f64 ? 8u : 4u}, {temperature, 8},
                                 {top_k, 4}, {top_p, 8}, {min_p, 8}, {tokens, 4}}));
-    // slices of 8192 keys (32 KB) leave room for six CTAs on an SM, so that one
-    // row's reads run under another's arithmetic; a few rows are cut further,
-    // until the SMs have two CTAs each
-    int ctas = 1;
-    while (ctas < kMaxCluster &&
-           ((long long)ctas * 8192 < V ||
-            ((long long)B * ctas < 2ll * dev.num_sms() && (long long)ctas * 2048 < V)))
-        ctas *= 2;
     SampleArgs a{logits, u, top_k, tokens, {temperature, temperature0}, {top_p, top_p0},
                  {min_p, min_p0}, ld, top_k0, u_f64, V, 0, 44};
-    a.slice = (int)(((long long)V + ctas - 1) / ctas + 7) / 8 * 8;
     while (std::ldexp((double)V, a.bits) >= std::ldexp(1.0, 62)) --a.bits;
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     switch (dtype) {
-        case SN_F32: return launch<float>(a, B, ctas, st);
-        case SN_BF16: return launch<__nv_bfloat16>(a, B, ctas, st);
-        default: return launch<__half>(a, B, ctas, st);
+        case SN_F32: return launch<float>(a, B, dev.num_sms(), st);
+        case SN_BF16: return launch<__nv_bfloat16>(a, B, dev.num_sms(), st);
+        default: return launch<__half>(a, B, dev.num_sms(), st);
     }
 }
