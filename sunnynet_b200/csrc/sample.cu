@@ -718,28 +718,46 @@ __device__ u32 cut(Shared& s, const Row& r, int V, int k, double p, int bits, Te
             const float slack = 0x1p-16f + 0x1p-21f * fabsf(d0);
             const float far = fminf(d0 - (b + 0.5f) * step * (1 + 0x1p-18f), 0.0f);
             const float near = b == 0 ? 0.0f : fminf(d0 - (b - 0.5f) * step * (1 - 0x1p-18f), 0.0f);
-            lo[j] = (u64)(n[j] * (unit_f * (1 - slack) * fast_exp2(far)));
+            // (the last bin has no far edge: -infinity lies in it)
+            lo[j] = b == kCut - 1 ? 0 : (u64)(n[j] * (unit_f * (1 - slack) * fast_exp2(far)));
             hi[j] = (u64)(n[j] * (unit_f * (1 + slack) * fast_exp2(near))) + n[j];
             lo_upto += lo[j];
             hi_upto += hi[j];
         }
-        lo_upto = block_upto(s, lo_upto) - lo_upto;
-        hi_upto = block_upto(s, hi_upto) - hi_upto;
+        const u64 lo_own = lo_upto, hi_own = hi_upto;
+        lo_upto = block_upto(s, lo_own);
+        hi_upto = block_upto(s, hi_own);
+        if (tid == kThreads - 1) s.found[1] = lo_upto, s.found[2] = hi_upto;
+        __syncthreads();
+        const u64 lo_all = s.found[1], hi_all = s.found[2];
+        __syncthreads();
+        lo_upto -= lo_own;
+        hi_upto -= hi_own;
+        // A bin lies at the border or behind it if the bins up to it reach p of
+        // the whole, or those behind it weigh no more than the rest; it lies
+        // ahead if those up to it do not, or those behind it weigh more. The
+        // bounds are a bin's width apart in what they sum up: for p near 1 the
+        // sums from behind are the sharper.
         const u64 sure = share(p, whole[1]), may = share(p, whole[0]);
-        u32 ahead = 0;
+        const u64 room = (u64)fmax(0.0, (1.0 - p) * (double)whole[0] - 2.0);
+        const u64 room_most = (u64)((1.0 - p) * (double)whole[1]) + 2;
+        u64 not_enough = 0, ahead = 0;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            counted += n[j];
-            if (lo_upto < sure && sure <= lo_upto + lo[j]) {
-                s.found[0] = N * tid + j;
-                s.found[1] = counted;
-            }
             lo_upto += lo[j];
             hi_upto += hi[j];
-            ahead += hi_upto < may;  // bins up to which the row is lighter (the sums ascend)
+            not_enough += !(lo_upto >= sure || hi_all - hi_upto <= room);
+            ahead += hi_upto < may || lo_all - lo_upto > room_most;  // (both descend along the bins)
         }
-        ahead = (u32)block_add(s, ahead);
-        if (tid == 0) s.found[3] = ahead;
+        const u64 both = block_add(s, not_enough << 32 | ahead);
+        const u32 bin = (u32)(both >> 32);
+        u32 upto = counted;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            upto += n[j];
+            if (bin == (u32)(N * tid + j)) s.found[1] = upto;
+        }
+        if (tid == 0) s.found[0] = bin, s.found[3] = min((u32)both, bin);
     }
     __syncthreads();
     // no bin, or the last, which has no far edge: every id can stay
