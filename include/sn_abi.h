@@ -242,8 +242,9 @@ sn_status sn_abi_layer_norm(const void* x, int64_t ldx, const void* w, const voi
                             int64_t rows, int32_t D, float eps, void* cuda_stream);
 /* Its gradients: dx (rows, D) contiguous, of `dtype`; dw, db (D) of `wdtype`,
  * overwritten; each may be NULL. The same input gives the same bits. ws: at
- * least sn_abi_layer_norm_bwd_ws bytes (asked with the arrays' GPU current)
- * when dw or db is wanted, free again when the work enqueued here is done. */
+ * least sn_abi_layer_norm_bwd_ws bytes (of the current GPU; the same for all
+ * of one kind) when dw or db is wanted, free again when the work enqueued here
+ * is done. */
 int64_t   sn_abi_layer_norm_bwd_ws(int64_t rows, int32_t D, int32_t dtype);
 sn_status sn_abi_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
                                 const void* w, const float* mean, const float* rstd, void* dx,

@@ -182,12 +182,24 @@ def check(rc: int, what: str = "") -> None:
         raise SnError(int(rc), f"{what}: {last_error()}")
 
 
+_DTYPE_CODES: dict = {}  # torch dtype -> SN_F32 / SN_BF16 / SN_F16 (sn_abi.h)
+
+
 def dtype_code(t) -> int:
     """SN_F32 / SN_BF16 / SN_F16 of a torch dtype (sn_abi.h)."""
-    code = {"torch.float32": 0, "torch.bfloat16": 1, "torch.float16": 2}.get(str(t))
+    if not _DTYPE_CODES:
+        import torch
+        _DTYPE_CODES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+    code = _DTYPE_CODES.get(t)
     if code is None:
         raise TypeError(f"float32, bfloat16 or float16 wanted, not {t}")
     return code
+
+
+def current_stream(tensor) -> int:
+    """torch's current stream of a CUDA tensor's device, as a raw handle."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(tensor.get_device())
 
 
 def ptr(x):

@@ -18,12 +18,19 @@
 // writes one row of partial sums, and a second small kernel adds the CTAs'
 // rows in order. No atomics: the same input gives the same bits.
 //
-// Rows wider than the register forms hold (kMaxWarpCols etc. below) take the
-// *_wide kernels, one CTA per row, which read a row again from cache for each
-// pass over it.
+// Rows of an odd width start anywhere in a 16-byte unit. They are still moved in
+// 16-byte packs: the packs are those of memory, a row's first and last being
+// partly its neighbours' (EDGE: those two element by element). A group of
+// threads that walks rows takes those at one distance from a boundary only, so
+// a thread keeps the same columns throughout.
+//
+// Rows wider than the register forms hold (see pick) take the *_wide kernels,
+// one CTA per row, which read a row again from cache for each pass over it.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <atomic>
 
 #include "caller.cuh"
 #include "ptx.cuh"
@@ -68,13 +75,45 @@ __device__ __forceinline__ void store_pack(T* p, const float (&f)[PACK]) {
     *reinterpret_cast<Pack<T, PACK>*>(p) = r;
 }
 
+// Columns [c, c + PACK) of a row at p as they are in memory, 0 where a row of D
+// has none (EDGE; c may be negative).
+template <typename T, int PACK, bool EDGE>
+__device__ __forceinline__ Pack<T, PACK> load_cols(const T* p, int c, int D) {
+    Pack<T, PACK> r;
+    if (c >= (EDGE ? 0 : c) && c + PACK <= D) {
+        r = *reinterpret_cast<const Pack<T, PACK>*>(p + c);
+    } else {
+#pragma unroll
+        for (int j = 0; j < PACK; ++j)
+            r.v[j] = EDGE && c + j >= 0 && c + j < D ? p[c + j] : from_f<T>(0.0f);
+    }
+    return r;
+}
+
+template <typename T, int PACK, bool EDGE>
+__device__ __forceinline__ void store_cols(T* p, int c, int D, const float (&f)[PACK]) {
+    if (!EDGE || (c >= 0 && c + PACK <= D)) {
+        store_pack<T, PACK>(p + c, f);
+    } else {
+#pragma unroll
+        for (int j = 0; j < PACK; ++j)
+            if (c + j >= 0 && c + j < D) p[c + j] = from_f<T>(f[j]);
+    }
+}
+
 // Weight or bias columns [c, c + PACK): fp32, or the rows' own type.
-template <typename T, int PACK>
-__device__ __forceinline__ void load_param(const void* w, int wide, int c, float other,
+template <typename T, int PACK, bool EDGE>
+__device__ __forceinline__ void load_param(const void* w, int wide, int c, int D, float other,
                                            float (&f)[PACK]) {
     if (!w) {
 #pragma unroll
         for (int j = 0; j < PACK; ++j) f[j] = other;
+    } else if (EDGE) {  // at no boundary of their own
+#pragma unroll
+        for (int j = 0; j < PACK; ++j) {
+            const int k = min(max(c + j, 0), D - 1);
+            f[j] = wide ? static_cast<const float*>(w)[k] : to_f(static_cast<const T*>(w)[k]);
+        }
     } else if (wide) {
         constexpr int Q = PACK < 4 ? PACK : 4;
 #pragma unroll
@@ -89,9 +128,15 @@ __device__ __forceinline__ void load_param(const void* w, int wide, int c, float
     }
 }
 
-// Sum over the threads that share a row; every one of them gets it. G lanes
-// of a warp, or (G == 0) the CTA, through `red` (32 floats, a buffer of its
-// own for each call between two of the same buffer's barriers).
+// Elements from the 16-byte boundary at or before p to p.
+template <typename T, bool EDGE>
+__device__ __forceinline__ int past_boundary(const T* p) {
+    return EDGE ? (int)((uintptr_t)p & 15) / (int)sizeof(T) : 0;
+}
+
+// Sums over the threads that share a row; every one of them gets them. G lanes
+// of a warp, or (G == 0) the CTA, through `red` (a buffer that is not written
+// again before another barrier of these).
 template <int G>
 __device__ __forceinline__ float row_sum(float v, float* red) {
     constexpr int S = G ? G : 32;
@@ -103,6 +148,24 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
         __syncthreads();
         v = 0.0f;
         for (int k = 0; k < nw; ++k) v += red[k];
+    }
+    return v;
+}
+
+template <int G>
+__device__ __forceinline__ float2 row_sums(float2 v, float2* red) {
+    constexpr int S = G ? G : 32;
+#pragma unroll
+    for (int o = S / 2; o; o >>= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    if (G == 0) {
+        const int w = threadIdx.x >> 5, nw = blockDim.x >> 5;
+        if ((threadIdx.x & 31) == 0) red[w] = v;
+        __syncthreads();
+        v = make_float2(0.0f, 0.0f);
+        for (int k = 0; k < nw; ++k) v.x += red[k].x, v.y += red[k].y;
     }
     return v;
 }
@@ -119,41 +182,46 @@ struct FwdArgs {
     float eps;
 };
 
-template <typename T, int PACK, int G, int NP>
+// A group of threads per row. (Groups that walk rows, each loading its next row
+// before it works on the one in hand, were slower: 43 us instead of 37 for
+// 32768 x 768 in fp32. Their registers cost more warps than the rows in flight
+// gain.)
+template <typename T, int PACK, int G, int NP, bool EDGE>
 __global__ void __launch_bounds__(G ? 128 : 512) norm_fwd_kernel(const FwdArgs a) {
+    constexpr int W = G ? G : 1;
     __shared__ float red[2][32];
-    const int lane = G ? (int)(threadIdx.x % (G ? G : 1)) : (int)threadIdx.x;
+    const int lane = G ? (int)(threadIdx.x % W) : (int)threadIdx.x;
     const int stride = G ? G : (int)blockDim.x;
     const long long row0 =
-        G ? blockIdx.x * (long long)(blockDim.x / (G ? G : 1)) + threadIdx.x / (G ? G : 1)
-          : blockIdx.x;
+        G ? blockIdx.x * (long long)(blockDim.x / W) + threadIdx.x / W : (long long)blockIdx.x;
     const bool live = row0 < a.rows;  // the other lanes still take part in the shuffles
     const long long row = live ? row0 : 0;
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    const int skip = past_boundary<T, EDGE>(x);
     float v[NP][PACK];
     float sum = 0.0f;
+    {
+        Pack<T, PACK> p[NP];
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-        const int c = (i * stride + lane) * PACK;
-        if (c < a.D) {
-            load_pack<T, PACK>(x + c, v[i]);
-        } else {
+        for (int i = 0; i < NP; ++i)
+            p[i] = load_cols<T, PACK, EDGE>(x, (i * stride + lane) * PACK - skip, a.D);
 #pragma unroll
-            for (int j = 0; j < PACK; ++j) v[i][j] = 0.0f;
-        }
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int j = 0; j < PACK; ++j) {
+                v[i][j] = to_f(p[i].v[j]);
+                sum += v[i][j];
+            }
     }
-#pragma unroll
-    for (int i = 0; i < NP; ++i)
-#pragma unroll
-        for (int j = 0; j < PACK; ++j) sum += v[i][j];
     const float mean = __fdiv_rn(row_sum<G>(sum, red[0]), (float)a.D);
     float sq = 0.0f;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-        const bool in = (i * stride + lane) * PACK < a.D;
+        const int c = (i * stride + lane) * PACK - skip;
 #pragma unroll
         for (int j = 0; j < PACK; ++j) {
             v[i][j] -= mean;
+            const bool in = EDGE ? c + j >= 0 && c + j < a.D : c < a.D;
             sq = in ? fmaf(v[i][j], v[i][j], sq) : sq;
         }
     }
@@ -167,29 +235,41 @@ __global__ void __launch_bounds__(G ? 128 : 512) norm_fwd_kernel(const FwdArgs a
     T* y = static_cast<T*>(a.y) + row * a.D;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-        const int c = (i * stride + lane) * PACK;
+        const int c = (i * stride + lane) * PACK - skip;
         if (c >= a.D) continue;
         float w[PACK], b[PACK];
-        load_param<T, PACK>(a.w, a.wide, c, 1.0f, w);
-        load_param<T, PACK>(a.b, a.wide, c, 0.0f, b);
+        load_param<T, PACK, EDGE>(a.w, a.wide, c, a.D, 1.0f, w);
+        load_param<T, PACK, EDGE>(a.b, a.wide, c, a.D, 0.0f, b);
 #pragma unroll
         for (int j = 0; j < PACK; ++j) v[i][j] = fmaf(v[i][j] * rstd, w[j], b[j]);
-        store_pack<T, PACK>(y + c, v[i]);
+        store_cols<T, PACK, EDGE>(y, c, a.D, v[i]);
     }
 }
 
 // Any width: three passes over the row, the last two from cache.
-template <typename T>
+template <typename T, int PACK, bool EDGE>
 __global__ void __launch_bounds__(512) norm_fwd_wide_kernel(const FwdArgs a) {
     __shared__ float red[2][32];
     const long long row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    const int skip = past_boundary<T, EDGE>(x), c0 = (int)threadIdx.x * PACK - skip;
+    const int by = (int)blockDim.x * PACK;
     float sum = 0.0f, sq = 0.0f;
-    for (int c = threadIdx.x; c < a.D; c += blockDim.x) sum += to_f(x[c]);
+#pragma unroll 4
+    for (int c = c0; c < a.D; c += by) {
+        const Pack<T, PACK> p = load_cols<T, PACK, EDGE>(x, c, a.D);
+#pragma unroll
+        for (int j = 0; j < PACK; ++j) sum += to_f(p.v[j]);
+    }
     const float mean = __fdiv_rn(row_sum<0>(sum, red[0]), (float)a.D);
-    for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
-        const float d = to_f(x[c]) - mean;
-        sq = fmaf(d, d, sq);
+#pragma unroll 4
+    for (int c = c0; c < a.D; c += by) {
+        const Pack<T, PACK> p = load_cols<T, PACK, EDGE>(x, c, a.D);
+#pragma unroll
+        for (int j = 0; j < PACK; ++j) {
+            const float d = to_f(p.v[j]) - mean;
+            sq = !EDGE || (c + j >= 0 && c + j < a.D) ? fmaf(d, d, sq) : sq;
+        }
     }
     const float rstd = __frsqrt_rn(__fdiv_rn(row_sum<0>(sq, red[1]), (float)a.D) + a.eps);
     if (threadIdx.x == 0) {
@@ -197,11 +277,15 @@ __global__ void __launch_bounds__(512) norm_fwd_wide_kernel(const FwdArgs a) {
         if (a.rstd) a.rstd[row] = rstd;
     }
     T* y = static_cast<T*>(a.y) + row * a.D;
-    for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
-        float w[1], b[1];
-        load_param<T, 1>(a.w, a.wide, c, 1.0f, w);
-        load_param<T, 1>(a.b, a.wide, c, 0.0f, b);
-        y[c] = from_f<T>(fmaf((to_f(x[c]) - mean) * rstd, w[0], b[0]));
+#pragma unroll 2
+    for (int c = c0; c < a.D; c += by) {
+        const Pack<T, PACK> p = load_cols<T, PACK, EDGE>(x, c, a.D);
+        float w[PACK], b[PACK], o[PACK];
+        load_param<T, PACK, EDGE>(a.w, a.wide, c, a.D, 1.0f, w);
+        load_param<T, PACK, EDGE>(a.b, a.wide, c, a.D, 0.0f, b);
+#pragma unroll
+        for (int j = 0; j < PACK; ++j) o[j] = fmaf((to_f(p.v[j]) - mean) * rstd, w[j], b[j]);
+        store_cols<T, PACK, EDGE>(y, c, a.D, o);
     }
 }
 
@@ -217,76 +301,137 @@ struct BwdArgs {
     int D, wide;
 };
 
-constexpr int kBwdThreads = 256;    // CTA of the warp-group forms
-constexpr int kMaxWarpCols = 1024;  // columns a warp-group form can hold
+// Threads of a CTA of the warp-group forms: each CTA leaves a row of partial
+// sums, so few large ones where registers allow.
+constexpr int bwd_threads(int elems) { return elems <= 8 ? 256 : 128; }
 
-template <typename T, int PACK, int G, int NP>
-__global__ void __launch_bounds__(G ? kBwdThreads : 512) norm_bwd_kernel(const BwdArgs a) {
-    __shared__ float red[4][32];
-    __shared__ float colsum[G ? 2 * G * NP * PACK : 1];
-    const int lane = G ? (int)(threadIdx.x % (G ? G : 1)) : (int)threadIdx.x;
+// Rows of a group on their way or in hand: 3, or 2 where a thread's part of a
+// row is large (a CTA's slots then leave room for others on the SM).
+constexpr int bwd_ahead(int bytes) { return bytes >= 64 ? 2 : 3; }
+
+// Bytes of a thread's slots: those rows of x and dy, and its weights in fp32.
+constexpr int bwd_slot_bytes(int elem, int elems) {
+    return elems * (2 * bwd_ahead(elem * elems) * elem + 4);
+}
+
+// The rows a group has yet to work on wait in shared memory, brought in by
+// cp.async: registers for them would cost the warps that hide what is left
+// (each thread reads back only what it copied itself, so no barrier is due).
+template <typename T, int PACK, int G, int NP, bool EDGE>
+__global__ void __launch_bounds__(G ? bwd_threads(PACK * NP) : 512) norm_bwd_kernel(const BwdArgs a) {
+    constexpr int W = G ? G : 1, kAhead = bwd_ahead(sizeof(T) * PACK * NP);
+    typedef Pack<T, PACK> P;
+    extern __shared__ __align__(128) unsigned char slots[];
+    __shared__ float2 red[2][32];
+    __shared__ float colsum[G ? 2 * W * NP * PACK : 1];
+    const int lane = G ? (int)(threadIdx.x % W) : (int)threadIdx.x;
     const int stride = G ? G : (int)blockDim.x;
-    const int per = G ? (int)(blockDim.x / (G ? G : 1)) : 1;  // rows a CTA has in hand
-    const int mine = G ? (int)(threadIdx.x / (G ? G : 1)) : 0;
+    // a CTA has `per` rows in hand; the step from one to the next of a group is
+    // a multiple of 8, after which rows begin at the same place in a 16-byte unit
+    const int per = G ? (int)(blockDim.x / W) : 1;
+    const int mine = G ? (int)(threadIdx.x / W) : 0;
     const float inv = __fdiv_rn(1.0f, (float)a.D);
+    const long long step = (long long)gridDim.x * per;
+    long long base = (long long)blockIdx.x * per;
+    const int skip = past_boundary<T, EDGE>(static_cast<const T*>(a.x) +
+                                            min(base + mine, a.rows - 1) * a.ldx);
+    const auto col = [&](int i) { return (i * stride + lane) * PACK - skip; };
+    P* const rows = reinterpret_cast<P*>(slots) + threadIdx.x;  // [kAhead][2][NP][threads]
+    const auto slot = [&](int stage, int which, int i) -> P* {
+        return rows + ((stage * 2 + which) * NP + i) * (int)blockDim.x;
+    };
+    Pack<float, PACK>* const weights =
+        reinterpret_cast<Pack<float, PACK>*>(reinterpret_cast<P*>(slots) +
+                                             kAhead * 2 * NP * blockDim.x) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        Pack<float, PACK> w;
+#pragma unroll
+        for (int j = 0; j < PACK; ++j) w.v[j] = 0.0f;
+        if (col(i) < a.D) load_param<T, PACK, EDGE>(a.w, a.wide, col(i), a.D, 1.0f, w.v);
+        weights[i * blockDim.x] = w;
+    }
     float aw[NP][PACK], ab[NP][PACK];
 #pragma unroll
     for (int i = 0; i < NP; ++i)
 #pragma unroll
         for (int j = 0; j < PACK; ++j) aw[i][j] = ab[i][j] = 0.0f;
 
-    int buf = 0;
-    for (long long base = (long long)blockIdx.x * per; base < a.rows;
-         base += (long long)gridDim.x * per) {
-        const bool live = base + mine < a.rows;
-        const long long row = live ? base + mine : 0;
-        const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-        const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
+    const auto fetch = [&](long long row, int stage) {
+        if (row < a.rows) {
+            const T* from[2] = {static_cast<const T*>(a.x) + row * a.ldx,
+                                static_cast<const T*>(a.dy) + row * a.lddy};
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int c = col(i);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if constexpr (sizeof(P) != 16) {
+                        *slot(stage, k, i) = load_cols<T, PACK, EDGE>(from[k], c, a.D);
+                    } else if (!EDGE || (c >= 0 && c + PACK <= a.D)) {
+                        if (c < a.D) cp_async16(slot(stage, k, i), from[k] + c, 16);
+                    } else if (c < a.D) {
+                        // partly a neighbouring row's, which is there to be read
+                        // but in front of the first row and behind the last
+                        const long long ld = k ? a.lddy : a.ldx, at = row * ld + c;
+                        if (at >= 0 && at + PACK <= (a.rows - 1) * ld + a.D)
+                            cp_async16(slot(stage, k, i), from[k] + c, 16);
+                        else
+                            *slot(stage, k, i) = load_cols<T, PACK, EDGE>(from[k], c, a.D);
+                    }
+                }
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead - 1; ++k) fetch(base + mine + k * step, k);
+    int stage = 0;
+    for (int buf = 0; base < a.rows; base += step, buf ^= 1) {
+        const long long row = base + mine;
+        const bool live = row < a.rows;
+        const float mean = live ? a.mean[row] : 0.0f, rstd = live ? a.rstd[row] : 0.0f;
+        fetch(row + (kAhead - 1) * step, stage == 0 ? kAhead - 1 : stage - 1);
+        cp_async_wait_group<kAhead - 1>();
         float xv[NP][PACK], gv[NP][PACK];
+        float2 sum = make_float2(0.0f, 0.0f);  // of du and du * xhat
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const int c = (i * stride + lane) * PACK;
-            if (live && c < a.D) {
-                load_pack<T, PACK>(x + c, xv[i]);
-                load_pack<T, PACK>(dy + c, gv[i]);
-            } else {
+            const int c = col(i);
+            if (!(live && c < a.D)) {
 #pragma unroll
                 for (int j = 0; j < PACK; ++j) xv[i][j] = gv[i][j] = 0.0f;
+                continue;
             }
-        }
-        const float mean = a.mean[row], rstd = a.rstd[row];
-        float s1 = 0.0f, s2 = 0.0f;  // sums of du and du * xhat
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int c = (i * stride + lane) * PACK;
-            if (!(live && c < a.D)) continue;
-            float w[PACK];
-            load_param<T, PACK>(a.w, a.wide, c, 1.0f, w);
+            const P x = *slot(stage, 0, i), g = *slot(stage, 1, i);
+            const Pack<float, PACK> w = weights[i * blockDim.x];
 #pragma unroll
             for (int j = 0; j < PACK; ++j) {
-                xv[i][j] = (xv[i][j] - mean) * rstd;
+                xv[i][j] = (to_f(x.v[j]) - mean) * rstd;
+                gv[i][j] = to_f(g.v[j]);
+                if (EDGE && (c + j < 0 || c + j >= a.D)) xv[i][j] = gv[i][j] = 0.0f;
                 aw[i][j] = fmaf(gv[i][j], xv[i][j], aw[i][j]);
                 ab[i][j] += gv[i][j];
-                gv[i][j] *= w[j];
-                s1 += gv[i][j];
-                s2 = fmaf(gv[i][j], xv[i][j], s2);
+                gv[i][j] *= w.v[j];
+                sum.x += gv[i][j];
+                sum.y = fmaf(gv[i][j], xv[i][j], sum.y);
             }
         }
+        stage = stage == kAhead - 1 ? 0 : stage + 1;
         if (!a.dx) continue;  // the whole grid alike
-        s1 = row_sum<G>(s1, red[buf]) * inv;
-        s2 = row_sum<G>(s2, red[buf + 1]) * inv;
-        buf ^= 2;  // a buffer is written again only behind the next row's barriers
+        sum = row_sums<G>(sum, red[buf]);
+        const float s1 = sum.x * inv, s2 = sum.y * inv;
         if (live) {
             T* dx = static_cast<T*>(a.dx) + row * a.D;
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                const int c = (i * stride + lane) * PACK;
+                const int c = col(i);
                 if (c >= a.D) continue;
                 float o[PACK];
 #pragma unroll
                 for (int j = 0; j < PACK; ++j)
                     o[j] = rstd * (gv[i][j] - s1 - xv[i][j] * s2);
-                store_pack<T, PACK>(dx + c, o);
+                store_cols<T, PACK, EDGE>(dx, c, a.D, o);
             }
         }
     }
@@ -295,37 +440,44 @@ __global__ void __launch_bounds__(G ? kBwdThreads : 512) norm_bwd_kernel(const B
     float* pb = pw + (size_t)gridDim.x * a.D;
     if (G == 0) {
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int c = (i * stride + lane) * PACK;
-            if (c >= a.D) continue;
+        for (int i = 0; i < NP; ++i)
 #pragma unroll
             for (int j = 0; j < PACK; ++j) {
-                pw[c + j] = aw[i][j];
-                pb[c + j] = ab[i][j];
+                const int c = (i * stride + lane) * PACK + j - skip;
+                if (c >= 0 && c < a.D) {
+                    pw[c] = aw[i][j];
+                    pb[c] = ab[i][j];
+                }
             }
-        }
         return;
     }
-    // groups of one warp by shuffles, then the warps one after the other
-    constexpr int cols = (G ? G : 1) * NP * PACK;
+    // groups of one warp by shuffles (where they share columns), then the warps
+    // one after the other
+    constexpr int cols = W * NP * PACK;
+    if (!EDGE) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i)
+        for (int i = 0; i < NP; ++i)
 #pragma unroll
-        for (int j = 0; j < PACK; ++j)
+            for (int j = 0; j < PACK; ++j)
 #pragma unroll
-            for (int o = 16; o >= (G ? G : 32); o >>= 1) {
-                aw[i][j] += __shfl_xor_sync(0xffffffffu, aw[i][j], o);
-                ab[i][j] += __shfl_xor_sync(0xffffffffu, ab[i][j], o);
-            }
-    for (int k = 0; k < (int)(blockDim.x >> 5); ++k) {
-        if ((int)(threadIdx.x >> 5) == k && (int)(threadIdx.x & 31) < (G ? G : 32)) {
+                for (int o = 16; o >= (G ? G : 32); o >>= 1) {
+                    aw[i][j] += __shfl_xor_sync(0xffffffffu, aw[i][j], o);
+                    ab[i][j] += __shfl_xor_sync(0xffffffffu, ab[i][j], o);
+                }
+    } else {
+        for (int c = threadIdx.x; c < 2 * cols; c += blockDim.x) colsum[c] = 0.0f;
+        __syncthreads();
+    }
+    for (int k = 0; k < (EDGE ? per : (int)(blockDim.x >> 5)); ++k) {
+        if (EDGE ? mine == k : (int)(threadIdx.x >> 5) == k && (int)(threadIdx.x & 31) < W) {
 #pragma unroll
             for (int i = 0; i < NP; ++i)
 #pragma unroll
                 for (int j = 0; j < PACK; ++j) {
-                    const int c = (i * stride + lane) * PACK + j;
-                    colsum[c] = (k ? colsum[c] : 0.0f) + aw[i][j];
-                    colsum[cols + c] = (k ? colsum[cols + c] : 0.0f) + ab[i][j];
+                    const int c = (i * stride + lane) * PACK + j - skip;
+                    if (EDGE && (c < 0 || c >= a.D)) continue;
+                    colsum[c] = (EDGE || k ? colsum[c] : 0.0f) + aw[i][j];
+                    colsum[cols + c] = (EDGE || k ? colsum[cols + c] : 0.0f) + ab[i][j];
                 }
         }
         __syncthreads();
@@ -337,118 +489,168 @@ __global__ void __launch_bounds__(G ? kBwdThreads : 512) norm_bwd_kernel(const B
 }
 
 // dx of rows of any width: two passes over the row, the second from cache.
-template <typename T>
+template <typename T, int PACK, bool EDGE>
 __global__ void __launch_bounds__(512) norm_dx_wide_kernel(const BwdArgs a) {
-    __shared__ float red[2][32];
+    __shared__ float2 red[32];
     const long long row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
+    const int skip = past_boundary<T, EDGE>(x), c0 = (int)threadIdx.x * PACK - skip;
+    const int by = (int)blockDim.x * PACK;
     const float mean = a.mean[row], rstd = a.rstd[row], inv = __fdiv_rn(1.0f, (float)a.D);
-    float s1 = 0.0f, s2 = 0.0f;
-    for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
-        float w[1];
-        load_param<T, 1>(a.w, a.wide, c, 1.0f, w);
-        const float g = to_f(dy[c]) * w[0];
-        s1 += g;
-        s2 = fmaf(g, (to_f(x[c]) - mean) * rstd, s2);
+    float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll 2
+    for (int c = c0; c < a.D; c += by) {
+        const Pack<T, PACK> p = load_cols<T, PACK, EDGE>(x, c, a.D);
+        const Pack<T, PACK> g = load_cols<T, PACK, EDGE>(dy, c, a.D);
+        float w[PACK];
+        load_param<T, PACK, EDGE>(a.w, a.wide, c, a.D, 1.0f, w);
+#pragma unroll
+        for (int j = 0; j < PACK; ++j) {
+            const float du = to_f(g.v[j]) * w[j];
+            sum.x += du;
+            sum.y = fmaf(du, (to_f(p.v[j]) - mean) * rstd, sum.y);
+        }
     }
-    s1 = row_sum<0>(s1, red[0]) * inv;
-    s2 = row_sum<0>(s2, red[1]) * inv;
+    sum = row_sums<0>(sum, red);
+    const float s1 = sum.x * inv, s2 = sum.y * inv;
     T* dx = static_cast<T*>(a.dx) + row * a.D;
-    for (int c = threadIdx.x; c < a.D; c += blockDim.x) {
-        float w[1];
-        load_param<T, 1>(a.w, a.wide, c, 1.0f, w);
-        dx[c] = from_f<T>(rstd * (to_f(dy[c]) * w[0] - s1 - (to_f(x[c]) - mean) * rstd * s2));
+#pragma unroll 2
+    for (int c = c0; c < a.D; c += by) {
+        const Pack<T, PACK> p = load_cols<T, PACK, EDGE>(x, c, a.D);
+        const Pack<T, PACK> g = load_cols<T, PACK, EDGE>(dy, c, a.D);
+        float w[PACK], o[PACK];
+        load_param<T, PACK, EDGE>(a.w, a.wide, c, a.D, 1.0f, w);
+#pragma unroll
+        for (int j = 0; j < PACK; ++j)
+            o[j] = rstd * (to_f(g.v[j]) * w[j] - s1 - (to_f(p.v[j]) - mean) * rstd * s2);
+        store_cols<T, PACK, EDGE>(dx, c, a.D, o);
     }
 }
 
-// Partial dw, db of any width: 32 columns per CTA column, the rows of slice
-// blockIdx.y over its 8 warps.
+// Partial dw, db of any width: a lane's columns lie 32 apart, kColsWide to a
+// CTA, the rows of slice blockIdx.y over its 8 warps.
+constexpr int kColsWide = 128;
+
 template <typename T>
 __global__ void __launch_bounds__(256) norm_cols_wide_kernel(const BwdArgs a) {
-    __shared__ float sw[8][32], sb[8][32];
+    constexpr int N = kColsWide / 32;
+    __shared__ float sums[2][8][kColsWide];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + lane;
+    const int c0 = blockIdx.x * kColsWide + lane;
     const long long lo = a.rows * blockIdx.y / gridDim.y, hi = a.rows * (blockIdx.y + 1) / gridDim.y;
-    float aw = 0.0f, ab = 0.0f;
-    if (c < a.D)
-        for (long long r = lo + w; r < hi; r += 8) {
-            const float g = to_f(static_cast<const T*>(a.dy)[r * a.lddy + c]);
-            const float xh = (to_f(static_cast<const T*>(a.x)[r * a.ldx + c]) - a.mean[r]) * a.rstd[r];
-            aw = fmaf(g, xh, aw);
-            ab += g;
+    float aw[N] = {}, ab[N] = {};
+#pragma unroll 4
+    for (long long r = lo + w; r < hi; r += 8) {
+        const T* dy = static_cast<const T*>(a.dy) + r * a.lddy;
+        const T* x = static_cast<const T*>(a.x) + r * a.ldx;
+        const float mean = a.mean[r], rstd = a.rstd[r];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int c = c0 + 32 * j;
+            const float g = c < a.D ? to_f(dy[c]) : 0.0f;
+            const float xh = c < a.D ? (to_f(x[c]) - mean) * rstd : 0.0f;
+            aw[j] = fmaf(g, xh, aw[j]);
+            ab[j] += g;
         }
-    sw[w][lane] = aw;
-    sb[w][lane] = ab;
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        sums[0][w][lane + 32 * j] = aw[j];
+        sums[1][w][lane + 32 * j] = ab[j];
+    }
     __syncthreads();
-    if (w < 2 && c < a.D) {
+    const int k = threadIdx.x / kColsWide, j = threadIdx.x % kColsWide;
+    const int c = blockIdx.x * kColsWide + j;
+    if (c < a.D) {
         float s = 0.0f;
-        for (int k = 0; k < 8; ++k) s += w ? sb[k][lane] : sw[k][lane];
-        a.part[((size_t)w * gridDim.y + blockIdx.y) * a.D + c] = s;
+        for (int i = 0; i < 8; ++i) s += sums[k][i][j];
+        a.part[((size_t)k * gridDim.y + blockIdx.y) * a.D + c] = s;
     }
 }
 
-// out[c] = sum of P partial rows, in order within each of 16 slices, then the
-// slices; blockIdx.y: 0 dw, 1 db.
+// out[c] = sum of P partial rows, in order within each of 32 slices, then the
+// slices; blockIdx.y: 0 dw, 1 db. A few dozen CTAs: it takes as long as its
+// chains of loads, so these are many and short.
 template <typename W>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(1024)
     norm_cols_kernel(const float* __restrict__ part, int P, int D, W* dw, W* db) {
-    __shared__ float s[16][32];
+    __shared__ float s[32][33];
     W* out = blockIdx.y ? db : dw;
     const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
     const float* p = part + (size_t)blockIdx.y * P * D + c;
     pdl_wait();
     float v = 0.0f;
-    if (out && c < D)
-        for (int r = k; r < P; r += 16) v += p[(size_t)r * D];
+    if (out && c < D) {
+#pragma unroll 16
+        for (int r = k; r < P; r += 32) v += p[(size_t)r * D];
+    }
     s[k][lane] = v;
     __syncthreads();
-    if (k == 0 && out && c < D) {
-        v = s[0][lane];
-        for (int i = 1; i < 16; ++i) v += s[i][lane];
-        out[c] = from_f<W>(v);
-    }
+    v = s[lane][k];  // column k of these, its slices over the lanes
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0 && out && blockIdx.x * 32 + k < D) out[blockIdx.x * 32 + k] = from_f<W>(v);
 }
 
 // How a row is laid over threads: G lanes of a warp (0: a CTA of `threads`),
-// NP packs of PACK elements each.
+// NP packs of PACK elements each. G == -1: no register form holds it.
 struct Form {
     int G, NP, threads;
 };
 
 int round32(int v) { return (v + 31) / 32 * 32; }
 
-// most: elements of a row a thread may hold. G == -1: no register form.
-Form pick(int D, int pack, int most, int cta_threads) {
-    const int packs = (D + pack - 1) / pack, np = most / pack;
+// A warp holds `warp_most` elements a lane at most, a thread of a CTA
+// `cta_most`, a CTA has 128 to 512 threads. A row in one warp needs no barrier
+// between its loads and its stores, so warps come first, with as many elements
+// as leave registers for some 16 warps on an SM; the CTA forms take the most
+// packs that still give 128 threads, for more rows in flight.
+Form pick(int packs, int pack, int warp_most, int cta_most) {
     if (pack > 1)
         for (int g = 4; g < 32; g *= 2)
             if (packs <= g) return {g, 1, 0};
-    const int need = (packs + 31) / 32;
-    for (int n : {1, 2, 3, 4, 6, 8, 16, 32})
-        if (n <= np && need <= n && n * 32 * pack <= kMaxWarpCols) return {32, n, 0};
-    for (int n : {1, 2, 4, 8, 16, 32})
-        if (n <= np && round32((packs + n - 1) / n) <= cta_threads)
+    for (int n : {1, 2, 3, 4, 6, 8, 12, 16, 32})
+        if (n * pack <= warp_most && packs <= n * 32) return {32, n, 0};
+    for (int n : {32, 16, 8, 4, 2, 1})
+        if (n * pack <= cta_most && (packs + n - 1) / n > 96 && round32((packs + n - 1) / n) <= 512)
             return {0, n, round32((packs + n - 1) / n)};
     return {-1, 0, 0};
 }
 
-constexpr int kFwdMost = 32, kBwdMost = 16, kBwdWarpMost = 24;
+// Packs of a row, one more where it may begin within one.
+int packs_of(int D, int pack, bool edge) { return (D + (edge ? pack - 1 : 0) + pack - 1) / pack; }
 
-template <typename T, int PACK, int G, int NP>
+// CTAs of a kernel that are on an SM at once, asked once for each.
+template <typename K>
+int resident(K kern, int threads, std::atomic<int>* known) {
+    int n = known->load(std::memory_order_relaxed);
+    if (!n) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess) {
+            cudaGetLastError();
+            return 1;
+        }
+        known->store(n < 1 ? 1 : n, std::memory_order_relaxed);
+    }
+    return n < 1 ? 1 : n;
+}
+
+template <typename T, int PACK, int G, int NP, bool EDGE>
 int fwd_launch(const FwdArgs& a, int threads, cudaStream_t st) {
     const int per = G ? 128 / (G ? G : 1) : 1;
     const long long blocks = (a.rows + per - 1) / per;
-    norm_fwd_kernel<T, PACK, G, NP><<<(unsigned)blocks, G ? 128 : threads, 0, st>>>(a);
+    norm_fwd_kernel<T, PACK, G, NP, EDGE><<<(unsigned)blocks, G ? 128 : threads, 0, st>>>(a);
     return cuda_check(cudaGetLastError(), "layer_norm launch");
 }
 
-template <typename T, int PACK>
+template <typename T, int PACK, bool EDGE>
 int fwd_dispatch(const FwdArgs& a, cudaStream_t st) {
-    const Form f = pick(a.D, PACK, kFwdMost, 512);
+    // 48 elements a lane: 1536 fp32 columns in one warp; single elements are
+    // the rare case of rows that share no boundary with their outputs
+    const Form f = pick(packs_of(a.D, PACK, EDGE), PACK, PACK == 1 ? 32 : 48, 32);
 #define SN_FWD(g, n) \
-    if (f.G == g && f.NP == n) return fwd_launch<T, PACK, g, n>(a, f.threads, st)
+    if (f.G == g && f.NP == n) return fwd_launch<T, PACK, g, n, EDGE>(a, f.threads, st)
     if constexpr (PACK > 1) {
         SN_FWD(4, 1);
         SN_FWD(8, 1);
@@ -458,9 +660,10 @@ int fwd_dispatch(const FwdArgs& a, cudaStream_t st) {
     SN_FWD(32, 2);
     SN_FWD(32, 3);
     SN_FWD(32, 4);
+    SN_FWD(32, 6);
     if constexpr (PACK <= 4) {
-        SN_FWD(32, 6);
         SN_FWD(32, 8);
+        SN_FWD(32, 12);
         SN_FWD(0, 8);
     }
     if constexpr (PACK == 1) {
@@ -473,51 +676,51 @@ int fwd_dispatch(const FwdArgs& a, cudaStream_t st) {
     SN_FWD(0, 2);
     SN_FWD(0, 4);
 #undef SN_FWD
-    norm_fwd_wide_kernel<T><<<(unsigned)a.rows, 512, 0, st>>>(a);
+    norm_fwd_wide_kernel<T, PACK, EDGE><<<(unsigned)a.rows, 512, 0, st>>>(a);
     return cuda_check(cudaGetLastError(), "layer_norm launch");
 }
 
+// How rows may be moved: in packs that begin where the rows do, in packs of
+// memory, or one element at a time.
+enum Move { kWhole, kEdge, kSingle };
+
 template <typename T>
-int fwd_typed(const FwdArgs& a, bool vec, cudaStream_t st) {
-    return vec ? fwd_dispatch<T, 16 / sizeof(T)>(a, st) : fwd_dispatch<T, 1>(a, st);
+int fwd_typed(const FwdArgs& a, Move move, cudaStream_t st) {
+    constexpr int P = 16 / sizeof(T);
+    return move == kWhole  ? fwd_dispatch<T, P, false>(a, st)
+           : move == kEdge ? fwd_dispatch<T, P, true>(a, st)
+                           : fwd_dispatch<T, 1, false>(a, st);
 }
 
-Form bwd_form(int D, int pack) {
-    const Form f = pick(D, pack, kBwdWarpMost, 512);
-    return f.G ? f : pick(D, pack, kBwdMost, 512);
-}
-
-// CTAs of the backward kernel: rows of the partial sums.
-int bwd_parts(long long rows, int D, int pack, int sms) {
-    const Form f = bwd_form(D, pack);
-    long long want, cap;
-    if (f.G < 0) {  // slices of norm_cols_wide_kernel
-        const int cols = (D + 31) / 32;
-        want = (rows + 63) / 64;
-        cap = (8ll * sms + cols - 1) / cols;
-    } else if (f.G) {
-        const int per = kBwdThreads / f.G;
-        want = (rows + per - 1) / per;
-        cap = 2ll * sms;
-    } else {
-        want = rows;
-        cap = (long long)sms * (f.threads <= 128 ? 4 : f.threads <= 256 ? 2 : 1);
+// Launches the backward kernel; a == nullptr: the CTAs of it that an SM holds.
+template <typename T, int PACK, int G, int NP, bool EDGE>
+int bwd_launch(const BwdArgs* a, int threads, int parts, cudaStream_t st) {
+    static std::atomic<int> known[17];  // by warps of a CTA
+    const auto kern = norm_bwd_kernel<T, PACK, G, NP, EDGE>;
+    const int n = G ? bwd_threads(PACK * NP) : threads;
+    const size_t dyn = (size_t)n * bwd_slot_bytes(sizeof(T), PACK * NP);
+    if (dyn > 40 * 1024)
+        SN_TRY(cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)dyn),
+                          "layer_norm_bwd"));
+    if (!a) {
+        int held = known[n / 32].load(std::memory_order_relaxed);
+        if (!held) {
+            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kern, n, dyn) != cudaSuccess)
+                cudaGetLastError();
+            held = held < 1 ? 1 : held;
+            known[n / 32].store(held, std::memory_order_relaxed);
+        }
+        return held;
     }
-    const long long p = want < cap ? want : cap;
-    return (int)(p < 1 ? 1 : p);
-}
-
-template <typename T, int PACK, int G, int NP>
-int bwd_launch(const BwdArgs& a, int threads, int parts, cudaStream_t st) {
-    norm_bwd_kernel<T, PACK, G, NP><<<parts, G ? kBwdThreads : threads, 0, st>>>(a);
+    kern<<<parts, n, dyn, st>>>(*a);
     return cuda_check(cudaGetLastError(), "layer_norm_bwd launch");
 }
 
-template <typename T, int PACK>
-int bwd_dispatch(const BwdArgs& a, int parts, cudaStream_t st) {
-    const Form f = bwd_form(a.D, PACK);
+template <typename T, int PACK, bool EDGE>
+int bwd_dispatch(const BwdArgs* a, const Form& f, int parts, cudaStream_t st) {
 #define SN_BWD(g, n) \
-    if (f.G == g && f.NP == n) return bwd_launch<T, PACK, g, n>(a, f.threads, parts, st)
+    if (f.G == g && f.NP == n) return bwd_launch<T, PACK, g, n, EDGE>(a, f.threads, parts, st)
     if constexpr (PACK > 1) {
         SN_BWD(4, 1);
         SN_BWD(8, 1);
@@ -526,13 +729,14 @@ int bwd_dispatch(const BwdArgs& a, int parts, cudaStream_t st) {
     SN_BWD(32, 1);
     SN_BWD(32, 2);
     SN_BWD(32, 3);
+    SN_BWD(32, 4);
     if constexpr (PACK <= 4) {
-        SN_BWD(32, 4);
         SN_BWD(32, 6);
+        SN_BWD(32, 8);
         SN_BWD(0, 4);
     }
     if constexpr (PACK == 1) {
-        SN_BWD(32, 8);
+        SN_BWD(32, 12);
         SN_BWD(32, 16);
         SN_BWD(0, 8);
         SN_BWD(0, 16);
@@ -540,35 +744,74 @@ int bwd_dispatch(const BwdArgs& a, int parts, cudaStream_t st) {
     SN_BWD(0, 1);
     SN_BWD(0, 2);
 #undef SN_BWD
-    if (a.dx) norm_dx_wide_kernel<T><<<(unsigned)a.rows, 512, 0, st>>>(a);
+    if (!a) return 1;
+    if (a->dx) norm_dx_wide_kernel<T, PACK, EDGE><<<(unsigned)a->rows, 512, 0, st>>>(*a);
     SN_TRY(cuda_check(cudaGetLastError(), "layer_norm_bwd launch"));
-    if (a.part) norm_cols_wide_kernel<T><<<dim3((a.D + 31) / 32, parts), 256, 0, st>>>(a);
+    if (a->part)
+        norm_cols_wide_kernel<T>
+            <<<dim3((a->D + kColsWide - 1) / kColsWide, parts), 256, 0, st>>>(*a);
     return cuda_check(cudaGetLastError(), "layer_norm_bwd launch");
 }
 
 template <typename T>
-int bwd_typed(const BwdArgs& a, bool vec, int sms, void* dw, void* db, cudaStream_t st) {
-    const int pack = vec ? 16 / (int)sizeof(T) : 1;
-    const int parts = a.rows ? bwd_parts(a.rows, a.D, pack, sms) : 0;
-    if (a.rows && (a.dx || a.part)) {
-        if (vec)
-            SN_TRY((bwd_dispatch<T, 16 / sizeof(T)>(a, parts, st)));
-        else
-            SN_TRY((bwd_dispatch<T, 1>(a, parts, st)));
-    }
-    if (!dw && !db) return SN_OK;
-    const dim3 grid((a.D + 31) / 32, 2);
-    return cuda_check(
-        a.wide ? launch_pdl(norm_cols_kernel<float>, grid, dim3(512), 0, st, (const float*)a.part,
-                            parts, a.D, (float*)dw, (float*)db)
-               : launch_pdl(norm_cols_kernel<T>, grid, dim3(512), 0, st, (const float*)a.part,
-                            parts, a.D, (T*)dw, (T*)db),
-        "layer_norm_bwd launch");
+int bwd_moved(const BwdArgs* a, const Form& f, Move move, int parts, cudaStream_t st) {
+    constexpr int P = 16 / sizeof(T);
+    return move == kWhole  ? bwd_dispatch<T, P, false>(a, f, parts, st)
+           : move == kEdge ? bwd_dispatch<T, P, true>(a, f, parts, st)
+                           : bwd_dispatch<T, 1, false>(a, f, parts, st);
 }
 
-// 16-byte loads and stores need 16-byte rows throughout.
-bool rows16(const void* p, long long ld, unsigned size) {
-    return ((uintptr_t)p & 15) == 0 && (ld * size) % 16 == 0;
+int bwd_any(const BwdArgs* a, const Form& f, Move move, int dtype, int parts, cudaStream_t st) {
+    switch (dtype) {
+        case SN_F32: return bwd_moved<float>(a, f, move, parts, st);
+        case SN_BF16: return bwd_moved<__nv_bfloat16>(a, f, move, parts, st);
+        default: return bwd_moved<__half>(a, f, move, parts, st);
+    }
+}
+
+Form bwd_form(int D, Move move, int dtype) {
+    const int pack = move == kSingle ? 1 : 16 / (int)dtype_size(dtype);
+    return pick(packs_of(D, pack, move == kEdge), pack, pack == 1 ? 16 : 32, 16);
+}
+
+// CTAs of the backward kernel, which are the rows of the partial sums: as many
+// as the SMs hold; a multiple of 8 where the rows are moved in packs of memory.
+int bwd_parts(long long rows, int D, Move move, int dtype, int sms) {
+    const Form f = bwd_form(D, move, dtype);
+    long long want, cap;
+    if (f.G < 0) {  // slices of norm_cols_wide_kernel
+        const int cols = (D + kColsWide - 1) / kColsWide;
+        want = (rows + 63) / 64;
+        cap = (8ll * sms + cols - 1) / cols;
+    } else {
+        // a CTA's partial sums are worth two of its rows: four rows to a group,
+        // as far as that leaves every SM a CTA
+        const int pack = move == kSingle ? 1 : 16 / (int)dtype_size(dtype);
+        const int per = f.G ? bwd_threads(f.NP * pack) / f.G : 1;
+        want = (rows + per - 1) / per;
+        want = want / 4 > sms ? want / 4 : want < sms ? want : sms;
+        const int held = bwd_any(nullptr, f, move, dtype, 0, nullptr);
+        cap = (long long)sms * (held < 1 ? 1 : held);
+    }
+    long long p = want < cap ? want : cap;
+    if (move == kEdge && f.G >= 0) p = (p + 7) / 8 * 8;
+    return (int)(p < 1 ? 1 : p);
+}
+
+template <typename W>
+int cols_launch(const float* part, int parts, int D, void* dw, void* db, cudaStream_t st) {
+    return cuda_check(launch_pdl(norm_cols_kernel<W>, dim3((D + 31) / 32, 2), dim3(1024), 0, st,
+                                 part, parts, D, static_cast<W*>(dw), static_cast<W*>(db)),
+                      "layer_norm_bwd launch");
+}
+
+// Two arrays of rows whose rows lie alike in 16-byte units.
+bool alike(const void* p, long long ldp, const void* q, long long ldq, unsigned size) {
+    return ((uintptr_t)p - (uintptr_t)q) % 16 == 0 && (ldp - ldq) * (long long)size % 16 == 0;
+}
+
+bool whole16(const void* p, long long ld, unsigned size) {
+    return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0;
 }
 
 bool shape_ok(long long rows, int D, long long ld) {
@@ -595,13 +838,17 @@ sn_status sn_abi_layer_norm(const void* x, int64_t ldx, const void* w, const voi
     CallerDevice dev;
     SN_TRY(dev.enter("layer_norm", {{x, size}, {w, ws}, {b, ws}, {y, size}, {mean, 4}, {rstd, 4}}));
     const FwdArgs a{x, w, b, y, mean, rstd, rows, ldx, D, wdtype == SN_F32, eps};
-    const bool vec = rows16(x, ldx, size) && rows16(y, D, size) && (!w || rows16(w, 0, ws)) &&
-                     (!b || rows16(b, 0, ws)) && D % (16 / size) == 0;
+    const bool like = alike(x, ldx, y, D, size);
+    const Move move = like && whole16(x, ldx, size) && D % (16 / size) == 0 &&
+                              (!w || whole16(w, 0, ws)) && (!b || whole16(b, 0, ws))
+                          ? kWhole
+                      : like ? kEdge
+                             : kSingle;
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     switch (dtype) {
-        case SN_F32: return fwd_typed<float>(a, vec, st);
-        case SN_BF16: return fwd_typed<__nv_bfloat16>(a, vec, st);
-        default: return fwd_typed<__half>(a, vec, st);
+        case SN_F32: return fwd_typed<float>(a, move, st);
+        case SN_BF16: return fwd_typed<__nv_bfloat16>(a, move, st);
+        default: return fwd_typed<__half>(a, move, st);
     }
 }
 
@@ -610,8 +857,12 @@ int64_t sn_abi_layer_norm_bwd_ws(int64_t rows, int32_t D, int32_t dtype) {
     if (!size || !shape_ok(rows, D, D)) return 0;
     CallerDevice dev;
     const int sms = dev.select("layer_norm_bwd_ws") == SN_OK ? dev.num_sms() : 148;
-    const int a = bwd_parts(rows, D, 1, sms), b = bwd_parts(rows, D, 16 / (int)size, sms);
-    return 8ll * (a > b ? a : b) * D;
+    int parts = 0;  // the most that any addresses lead to
+    for (Move move : {kWhole, kEdge, kSingle}) {
+        const int p = bwd_parts(rows, D, move, dtype, sms);
+        parts = p > parts ? p : parts;
+    }
+    return 8ll * parts * D;
 }
 
 sn_status sn_abi_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int64_t ldx,
@@ -635,13 +886,21 @@ sn_status sn_abi_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int
                     (long long)sn_abi_layer_norm_bwd_ws(rows, D, dtype));
     const BwdArgs a{dy, x, w, mean, rstd, dx, sums ? static_cast<float*>(ws) : nullptr, rows,
                     ldx, lddy, D, wdtype == SN_F32};
-    const bool vec = rows16(dy, lddy, size) && rows16(x, ldx, size) && (!w || rows16(w, 0, wsz)) &&
-                     (!dx || rows16(dx, D, size)) && D % (16 / size) == 0;
+    const bool like = alike(x, ldx, dy, lddy, size) && (!dx || alike(x, ldx, dx, D, size));
+    const Move move = like && whole16(x, ldx, size) && D % (16 / size) == 0 &&
+                              (!w || whole16(w, 0, wsz))
+                          ? kWhole
+                      : like ? kEdge
+                             : kSingle;
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
-    switch (dtype) {
-        case SN_F32: return bwd_typed<float>(a, vec, dev.num_sms(), dw, db, st);
-        case SN_BF16: return bwd_typed<__nv_bfloat16>(a, vec, dev.num_sms(), dw, db, st);
-        default: return bwd_typed<__half>(a, vec, dev.num_sms(), dw, db, st);
+    const int parts = rows ? bwd_parts(rows, D, move, dtype, dev.num_sms()) : 0;
+    if (rows && (dx || sums))
+        SN_TRY(bwd_any(&a, bwd_form(D, move, dtype), move, dtype, parts, st));
+    if (!sums) return SN_OK;
+    switch (wdtype) {
+        case SN_F32: return cols_launch<float>(a.part, parts, D, dw, db, st);
+        case SN_BF16: return cols_launch<__nv_bfloat16>(a.part, parts, D, dw, db, st);
+        default: return cols_launch<__half>(a.part, parts, D, dw, db, st);
     }
 }
 

@@ -21,11 +21,10 @@ can be captured into a CUDA graph.
 """
 from __future__ import annotations
 
-import ctypes
-from operator import attrgetter
+from array import array
 
 from . import _lib
-from ._lib import check, dtype_code, ptr
+from ._lib import check, current_stream, dtype_code, ptr
 from .runtime import bind_stream, load_runtime
 
 __all__ = ["load_kernel", "load_scan_kernel", "kernel_available", "set_kernel_threads",
@@ -205,9 +204,49 @@ def scan_auto(u, p, s0, chunk: int = 64, p_min_hint=None):
     return states, states[:, -1]
 
 
-def _stream(device) -> int:
+def _lib_loaded():
+    """The library, without a look at the file where it is loaded already."""
+    return _lib._lib or load_kernel()
+
+
+def _rows(t, D):
+    """t as rows of D values at one stride: (tensor, stride in elements)."""
+    if t.is_contiguous():
+        return t, D
+    t = t.reshape(-1, D)  # a view wherever the rows lie at one stride
+    n, ld = t.shape[0], t.stride(0)
+    if t.stride(1) != 1 or (n > 1 and ld < D):  # among these what a sum's gradient broadcasts
+        t, ld = t.contiguous(), D
+    return t, max(ld, D)
+
+
+def _norm_forward(x, weight, bias, eps, keep):
+    """(y, what the backward pass needs of the call: None unless keep)."""
+    D = x.shape[-1]
+    rows = x.numel() // D
+    x2, ld = _rows(x, D)
+    w = None if weight is None else weight.contiguous()
+    b = None if bias is None else bias.contiguous()
+    y = x.new_empty(x.shape)
+    code = dtype_code(x.dtype)
+    wcode = code if w is None and b is None else dtype_code((b if w is None else w).dtype)
+    mean = rstd = stats = None
+    if keep:
+        stats = x.new_empty(2 * rows, dtype=_float32())
+        mean = stats.data_ptr()
+        rstd = mean + 4 * rows
+    rc = _lib_loaded().sn_abi_layer_norm(
+        x2.data_ptr(), ld, None if w is None else w.data_ptr(),
+        None if b is None else b.data_ptr(), y.data_ptr(), mean, rstd, code, wcode, rows, D, eps,
+        current_stream(x))
+    if rc:
+        check(rc, "layer_norm")
+    return y, (x2, w, (stats, ld, code, wcode, rows, D)) if keep else None
+
+
+def _float32():
     import torch
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch.float32
 
 
 _NORM = None
@@ -218,89 +257,77 @@ def _norm_fn():
     if _NORM is not None:
         return _NORM
     import torch
+    types = (torch.float32, torch.bfloat16, torch.float16)
 
     class _Norm(torch.autograd.Function):
         @staticmethod
         def forward(ctx, x, weight, bias, eps):
-            D = x.shape[-1]
-            rows = x.numel() // D
-            x2 = x.reshape(rows, D)  # a view wherever the rows lie at one stride
-            if x2.stride(1) != 1 or (rows > 1 and x2.stride(0) < D):
-                x2 = x2.contiguous()
-            w, b = (None if t is None else t.contiguous() for t in (weight, bias))
-            y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            keep = any(ctx.needs_input_grad)
-            stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if keep else None
-            wdtype = dtype_code(next((t.dtype for t in (w, b) if t is not None), x.dtype))
-            check(load_kernel().sn_abi_layer_norm(
-                x2.data_ptr(), max(x2.stride(0), D), _addr(w), _addr(b), y.data_ptr(),
-                _addr(stats), _addr(stats) and stats[1:].data_ptr(), dtype_code(x.dtype), wdtype,
-                rows, D, eps, _stream(x.device)), "layer_norm")
-            if keep:
-                ctx.save_for_backward(x2, w, stats)
-                ctx.wdtype = wdtype
+            y, kept = _norm_forward(x, weight, bias, eps, True)
+            ctx.save_for_backward(kept[0], kept[1])
+            ctx.call = kept[2]
             return y
 
         @staticmethod
-        @torch.autograd.function.once_differentiable
         def backward(ctx, dy):
-            x, w, stats = ctx.saved_tensors
-            rows, D = x.shape
-            want_x, want_w, want_b = ctx.needs_input_grad[:3]
-            g = dy.reshape(rows, D)
-            if g.stride(1) != 1 or (rows > 1 and g.stride(0) < D):
-                g = g.contiguous()  # among them what a sum's gradient broadcasts
-            lib = load_kernel()
-            dx = torch.empty(dy.shape, dtype=x.dtype, device=x.device) if want_x else None
-            wt = (torch.float32, torch.bfloat16, torch.float16)[ctx.wdtype]
-            dw, db = (torch.empty(D, dtype=wt, device=x.device) if want else None
-                      for want in (want_w, want_b))
+            if torch.is_grad_enabled():  # create_graph: its own gradient is not there
+                raise RuntimeError("layer_norm can be differentiated once")
+            x, w = ctx.saved_tensors
+            stats, ldx, code, wcode, rows, D = ctx.call
+            want_x, want_w, want_b, _ = ctx.needs_input_grad
+            g, ldg = _rows(dy, D)
+            lib = _lib_loaded()
+            dx = g.new_empty(dy.shape) if want_x else None
+            dw = g.new_empty(D, dtype=types[wcode]) if want_w else None
+            db = g.new_empty(D, dtype=types[wcode]) if want_b else None
             ws, need = None, 0
             if want_w or want_b:
-                with torch.cuda.device(x.device):
-                    need = lib.sn_abi_layer_norm_bwd_ws(rows, D, dtype_code(x.dtype))
-                ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-            check(lib.sn_abi_layer_norm_bwd(
-                g.data_ptr(), max(g.stride(0), D), x.data_ptr(), max(x.stride(0), D), _addr(w),
-                stats.data_ptr(), stats[1:].data_ptr(), _addr(dx), _addr(dw), _addr(db),
-                _addr(ws), need, dtype_code(x.dtype), ctx.wdtype, rows, D, _stream(x.device)),
-                "layer_norm_bwd")
+                need = lib.sn_abi_layer_norm_bwd_ws(rows, D, code)
+                ws = g.new_empty(need, dtype=torch.uint8)
+            mean = stats.data_ptr()
+            rc = lib.sn_abi_layer_norm_bwd(
+                g.data_ptr(), ldg, x.data_ptr(), ldx, None if w is None else w.data_ptr(), mean,
+                mean + 4 * rows, None if dx is None else dx.data_ptr(),
+                None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
+                None if ws is None else ws.data_ptr(), need, code, wcode, rows, D,
+                current_stream(x))
+            if rc:
+                check(rc, "layer_norm_bwd")
             return dx, dw, db, None
 
     _NORM = _Norm
     return _NORM
 
 
-def _addr(t):
-    return None if t is None else t.data_ptr()
-
-
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x
     (float32, bfloat16 or float16; the variance biased; sums in fp32).
     weight, bias: None or (D,) of float32 or x's type. Differentiable in x,
-    weight and bias; rows may lie at a stride; the gradients do not depend on
-    scheduling."""
+    weight and bias; rows may lie at a stride. The same call gives the same
+    bits every time; a row's bits depend on its place among the rows only
+    where the width is no multiple of 16 bytes."""
+    import torch
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("layer_norm: x needs a last axis of at least one value")
     if not x.is_cuda:  # host tensors are staged, as by the other kernels
         to = lambda t: None if t is None else t.cuda()  # noqa: E731
         return layer_norm(x.cuda(), to(weight), to(bias), eps).to(x.device)
+    D, kind = x.shape[-1], None
     dtype_code(x.dtype)
-    params = [t for t in (weight, bias) if t is not None]
-    for t in params:
-        if tuple(t.shape) != (x.shape[-1],) or t.device != x.device or \
-                t.dtype != params[0].dtype or str(t.dtype) not in ("torch.float32", str(x.dtype)):
-            raise ValueError(f"layer_norm: weight and bias have {x.shape[-1]} values of float32 "
-                             f"or {x.dtype} on {x.device}, both the same")
+    for t in (weight, bias):
+        if t is not None:
+            if t.dim() != 1 or t.shape[0] != D or t.get_device() != x.get_device() or \
+                    (t.dtype != torch.float32 and t.dtype != x.dtype) or \
+                    (kind is not None and t.dtype != kind):
+                raise ValueError(f"layer_norm: weight and bias have {D} values of float32 or "
+                                 f"{x.dtype} on {x.device}, both the same")
+            kind = t.dtype
     if not eps >= 0:
         raise ValueError("layer_norm: eps must not be negative")
-    return _norm_fn().apply(x, weight, bias, float(eps))
-
-
-def _addresses(tensors):
-    import torch
-    return (ctypes.c_void_p * len(tensors))(*map(torch.Tensor.data_ptr, tensors))
+    if torch.is_grad_enabled() and (x.requires_grad or
+                                    (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        return _norm_fn().apply(x, weight, bias, float(eps))
+    return _norm_forward(x, weight, bias, float(eps), False)[0]
 
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, beta2=0.999,
@@ -317,49 +344,58 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, bet
     float64 one) may be on the GPU: then a captured step reads them anew at
     each replay."""
     import torch
-    params, grads, exp_avg, exp_avg_sq = map(list, (params, grads, exp_avg, exp_avg_sq))
+    Tensor = torch.Tensor
     lists = [params, grads, exp_avg, exp_avg_sq]
     if (avg_scale is None) != (sq_scale is None):
         raise ValueError("adamw_step: 8-bit states have avg_scale and sq_scale")
     bits = 32 if avg_scale is None else 8
-    scales = [] if bits == 32 else [list(avg_scale), list(sq_scale)]
-    n = len(params)
-    if any(len(x) != n for x in lists + scales):
+    if bits == 8:
+        lists += [avg_scale, sq_scale]
+    lists = [x if isinstance(x, (list, tuple)) else list(x) for x in lists]
+    n = len(lists[0])
+    if any(len(x) != n for x in lists):
         raise ValueError("adamw_step: the lists differ in length")
     if n == 0:
         return
-    sizes = list(map(torch.Tensor.numel, params))
-    if any(list(map(torch.Tensor.numel, x)) != sizes for x in lists[1:]):
-        raise ValueError("adamw_step: a gradient or state differs in size from its parameter")
-    if any(list(map(torch.Tensor.numel, x)) != [-(-k // STATE_BLOCK) for k in sizes]
-           for x in scales):
-        raise ValueError(f"adamw_step: one scale for each {STATE_BLOCK} values is wanted")
-    kinds = [set(map(attrgetter("dtype"), x)) for x in lists + scales]
-    state = torch.float32 if bits == 32 else torch.float8_e4m3fn
-    if any(len(k) != 1 for k in kinds) or kinds[2] != {state} or kinds[3] != {state} or \
-            any(k != {torch.float32} for k in kinds[4:]):
-        raise TypeError(f"adamw_step: params of one type, grads of one type, states of {state} "
-                        "and scales of float32 are wanted")
-    for x in lists + scales:
-        if not all(map(torch.Tensor.is_contiguous, x)):
-            raise ValueError("adamw_step: every tensor must be contiguous")
-    device = params[0].device
-    if device.type != "cuda" or len(set().union(*(map(torch.Tensor.get_device, x)
-                                                  for x in lists + scales))) != 1:
+    first = lists[0][0]
+    if not first.is_cuda:
         raise ValueError("adamw_step: every tensor must be on one GPU")
+    sizes = array("q", map(Tensor.numel, lists[0]))
+    for x in lists[1:4]:
+        if array("q", map(Tensor.numel, x)) != sizes:
+            raise ValueError("adamw_step: a gradient or state differs in size from its parameter")
+    if bits == 8:
+        blocks = array("q", [-(-k // STATE_BLOCK) for k in sizes])
+        for x in lists[4:]:
+            if array("q", map(Tensor.numel, x)) != blocks:
+                raise ValueError(f"adamw_step: one scale for each {STATE_BLOCK} values is wanted")
+    state = torch.float32 if bits == 32 else torch.float8_e4m3fn
+    for x, kind in zip(lists, (first.dtype, lists[1][0].dtype, state, state, torch.float32,
+                               torch.float32)):
+        for t in x:
+            if t.dtype is not kind:
+                raise TypeError("adamw_step: params of one type, grads of one type, states of "
+                                f"{state} and scales of float32 are wanted")
+        if not all(map(Tensor.is_contiguous, x)):
+            raise ValueError("adamw_step: every tensor must be contiguous")
     on_gpu = {}
     for name, v, dt in (("step", step, torch.int64), ("lr", lr, torch.float64)):
-        if isinstance(v, torch.Tensor):
-            if v.dtype != dt or v.numel() != 1 or v.device != device:
-                raise TypeError(f"adamw_step: {name} as a tensor is one {dt} value on {device}")
+        if isinstance(v, Tensor):
+            if v.dtype != dt or v.numel() != 1 or v.device != first.device:
+                raise TypeError(f"adamw_step: {name} as a tensor is one {dt} value on "
+                                f"{first.device}")
             on_gpu[name] = v.data_ptr()
-    at = [_addresses(x) for x in lists + scales]
-    where = [a for a, k in zip(at[0], sizes) if k]
-    if len(set(where)) != len(where):
+    # (that they are memory of one GPU is looked up by address, below)
+    at = [array("Q", map(Tensor.data_ptr, x)) for x in lists]
+    if len(set(at[0])) != n and len({a for a, k in zip(at[0], sizes) if k}) != \
+            sum(1 for k in sizes if k):
         raise ValueError("adamw_step: a parameter appears twice")
-    check(load_kernel().sn_abi_adamw_step(
-        n, *at[:4], *(at[4:] or (None, None)), (ctypes.c_int64 * n)(*sizes),
-        dtype_code(params[0].dtype), dtype_code(grads[0].dtype), bits,
+    to = [x.buffer_info()[0] for x in at]
+    rc = _lib_loaded().sn_abi_adamw_step(
+        n, *to[:4], *(to[4:] or (None, None)), sizes.buffer_info()[0], dtype_code(first.dtype),
+        dtype_code(lists[1][0].dtype), bits,
         0 if "step" in on_gpu else int(step), on_gpu.get("step"),
         0.0 if "lr" in on_gpu else float(lr), on_gpu.get("lr"), float(beta1), float(beta2),
-        float(eps), float(weight_decay), _stream(device)), "adamw_step")
+        float(eps), float(weight_decay), current_stream(first))
+    if rc:
+        check(rc, "adamw_step")

@@ -8,7 +8,8 @@ from __future__ import annotations
 
 import math
 
-from ._lib import check, dtype_code
+from . import _lib
+from ._lib import check, current_stream, dtype_code
 from .runtime import load_runtime
 
 __all__ = ["sample"]
@@ -19,8 +20,8 @@ def _setting(name, v, B, device, dtype):
     import torch
     if not isinstance(v, torch.Tensor):
         return None, v, None
-    if tuple(v.shape) != (B,) or v.device != device:
-        raise ValueError(f"sample: {name} is one number or {B} of them on {device}")
+    if v.dim() != 1 or v.shape[0] != B or v.get_device() != device:
+        raise ValueError(f"sample: {name} is one number or {B} of them on cuda:{device}")
     v = v.to(dtype).contiguous()
     return v.data_ptr(), 0, v
 
@@ -42,17 +43,18 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
     B, V = logits.shape
     if V == 0:
         raise ValueError("sample: no logits to draw from")
-    if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < V:
+    ld, along = logits.stride()
+    if V > 1 and along != 1 or B > 1 and ld < V:
         raise ValueError("sample: the logits of a row must lie side by side")
-    dev = logits.device
-    if tuple(u.shape) != (B,) or u.device != dev or \
+    dev = logits.get_device()
+    if u.dim() != 1 or u.shape[0] != B or u.get_device() != dev or \
             u.dtype not in (torch.float32, torch.float64):
-        raise ValueError(f"sample: u has {B} numbers of float32 or float64 on {dev}")
+        raise ValueError(f"sample: u has {B} numbers of float32 or float64 on cuda:{dev}")
     if out is None:
-        out = torch.empty(B, dtype=torch.int32, device=dev)
-    elif tuple(out.shape) != (B,) or out.dtype != torch.int32 or out.device != dev or \
-            not out.is_contiguous():
-        raise ValueError(f"sample: out has {B} contiguous int32 values on {dev}")
+        out = logits.new_empty(B, dtype=torch.int32)
+    elif out.dim() != 1 or out.shape[0] != B or out.dtype != torch.int32 or \
+            out.get_device() != dev or not out.is_contiguous():
+        raise ValueError(f"sample: out has {B} contiguous int32 values on cuda:{dev}")
     u = u.contiguous()
     t, t0, keep_t = _setting("temperature", temperature, B, dev, torch.float64)
     k, k0, keep_k = _setting("top_k", top_k, B, dev, torch.int32)
@@ -60,9 +62,10 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
     q, q0, keep_q = _setting("min_p", min_p, B, dev, torch.float64)
     if not math.isfinite(t0) or not math.isfinite(p0) or not q0 <= 1:
         raise ValueError("sample: temperature and top_p are finite, min_p is at most 1")
-    check(load_runtime().sn_abi_sample(
-        logits.data_ptr(), max(logits.stride(0), V), dtype_code(logits.dtype), u.data_ptr(),
+    rc = (_lib._lib or load_runtime()).sn_abi_sample(
+        logits.data_ptr(), max(ld, V), dtype_code(logits.dtype), u.data_ptr(),
         int(u.dtype == torch.float64), t, float(t0), k, max(0, min(int(k0), 0x7fffffff)), p,
-        float(p0), q, float(q0), B, V, out.data_ptr(), torch.cuda.current_stream(dev).cuda_stream),
-        "sample")
+        float(p0), q, float(q0), B, V, out.data_ptr(), current_stream(logits))
+    if rc:
+        check(rc, "sample")
     return out
