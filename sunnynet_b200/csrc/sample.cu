@@ -1117,18 +1117,28 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a)
         for (u32 c = 0; c < t.ctas; ++c) sum += s.told[12][c];
         return sum;
     };
+    u32 listed = 0;   // ids that can stay, where they are to be listed
+    float least = 0;  // their least logit
     if (bins) {
         Range found;
-        const u32 listed = cut(s, r, a.V, g.k, g.p, a.bits, t, sum, &found);
-        if (listed) range = found;
+        const u32 n = cut(s, r, a.V, g.k, g.p, a.bits, t, sum, &found);
+        if (n) range = found;
         // every CTA of the cluster decides alike
-        if (listed && HELD ? listed <= (u32)a.V / 2 : listed && ONE && listed <= kCand) {
-            const float least = value_of(range.from);
+        if (n && (HELD ? n <= (u32)a.V / 2 : ONE && n <= kCand)) listed = n;
+        least = value_of(range.from);
+    } else if (g.w_floor > 0 && g.k == 0 && g.p == 1.0 && (HELD || ONE)) {
+        // where x < max + T ln(min_p) by more than the roundings here, w is below min_p
+        const double edge = T_ * log(q);
+        least = __double2float_rd(r.max + edge - 1e-9 * fabs(edge));
+        listed = (u32)a.V;
+    }
+    if constexpr (HELD || ONE) {
+        if (listed) {
             float others = 0.0f;  // estimate of the weight that is not listed (top-p alone)
             const auto finish = [&](const auto& l) {
                 if (g.k > 0 && listed <= kList) return draw_few(s, r, l, first, g, t);
                 Rest rest{0, 0, false};
-                if (g.k <= 0) {
+                if (g.k <= 0 && g.p < 1.0) {
                     // Each 2^d is off by 2^-22 of itself, and by the roundings of
                     // the difference, the scale and their product, 3 * 2^-24 |d|
                     // ln 2; a thread adds up n / 2048 + 4 of them. The mean of
@@ -1162,8 +1172,8 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a)
                 return i < 0 ? -1 : first + l.id(i);
             };
             const auto listing = [&](u32* marks, auto put) {
-                return g.k > 0 ? list<false>(s, r, x, least, marks, &others, put)
-                               : list<true>(s, r, x, least, marks, &others, put);
+                return g.k <= 0 && g.p < 1.0 ? list<true>(s, r, x, least, marks, &others, put)
+                                             : list<false>(s, r, x, least, marks, &others, put);
             };
             if constexpr (HELD) {
                 unsigned short* at = reinterpret_cast<unsigned short*>(dyn + a.slice + 8);
@@ -1173,20 +1183,23 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a)
                 });
                 const int id = finish(NearListed{x, at, n});
                 if (id >= 0 && tid == 0) a.out[row] = id;
+                return;
             } else {
                 u32* marks = reinterpret_cast<u32*>(dyn + kCand);
                 u32* at = reinterpret_cast<u32*>(dyn);  // places first, then the logits there
-                const int n = min(kCand, listing(marks, [&](u32 pos, int i) {
+                const int n = listing(marks, [&](u32 pos, int i) {
                     if (pos < kCand) at[pos] = (u32)i;
-                }));
+                });
+                if (n <= kCand) {  // always where the bins counted them
 #pragma unroll 4
-                for (int i = tid; i < n; i += kThreads) dyn[i] = x.value((int)at[i]);
-                __syncthreads();
-                const int m = finish(FarListed{dyn, n});
-                const int i = marked_place(s, x.n, marks, (u32)m);
-                if (i >= 0) a.out[row] = x.id(i);
+                    for (int i = tid; i < n; i += kThreads) dyn[i] = x.value((int)at[i]);
+                    __syncthreads();
+                    const int m = finish(FarListed{dyn, n});
+                    const int i = marked_place(s, x.n, marks, (u32)m);
+                    if (i >= 0) a.out[row] = x.id(i);
+                    return;
+                }
             }
-            return;
         }
     }
     const int i = draw(s, r, x, first, g, range, Rest{0, 0, g.k <= 0}, t, exact);

@@ -227,7 +227,7 @@ def _norm_forward(x, weight, bias, eps, keep):
     x2, ld = _rows(x, D)
     w = None if weight is None else weight.contiguous()
     b = None if bias is None else bias.contiguous()
-    y = x.new_empty(x.shape)
+    y = _empty_like(x) if x2 is x else x.new_empty(x.shape)
     code = dtype_code(x.dtype)
     wcode = code if w is None and b is None else dtype_code((b if w is None else w).dtype)
     mean = rstd = stats = None
@@ -247,6 +247,11 @@ def _norm_forward(x, weight, bias, eps, keep):
 def _float32():
     import torch
     return torch.float32
+
+
+def _empty_like(t):
+    import torch
+    return torch.empty_like(t)
 
 
 _NORM = None
@@ -276,7 +281,7 @@ def _norm_fn():
             want_x, want_w, want_b, _ = ctx.needs_input_grad
             g, ldg = _rows(dy, D)
             lib = _lib_loaded()
-            dx = g.new_empty(dy.shape) if want_x else None
+            dx = (torch.empty_like(g) if g is dy else g.new_empty(dy.shape)) if want_x else None
             dw = g.new_empty(D, dtype=types[wcode]) if want_w else None
             db = g.new_empty(D, dtype=types[wcode]) if want_b else None
             ws, need = None, 0
