@@ -42,6 +42,7 @@ class SunnyBatch:
         self.vocab, self.dim, self.inner, self.rank, self.taps, self.layers, self.group, \
             self.wtype = (int(v) for v in d)
         self.nseq = int(nseq)
+        self._logits = None  # of step_sample
 
     def step(self, tokens, logits=None):
         t = _tokens(tokens)
@@ -60,6 +61,24 @@ class SunnyBatch:
         bind_stream(t, out)
         check(self._lib.sn_abi_sunny_step_argmax(self._h, ptr(t), B, ptr(out)), "sunny_argmax")
         return out
+
+    def step_sample(self, tokens, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """One token to each of the first B sequences, and the next ones (B,)
+        int32, drawn on the GPU with numbers u as ``sampling.sample`` does;
+        the logits stay there. Tokens and settings are host arrays (or single
+        settings) and the result is one, or all are CUDA tensors."""
+        import torch
+
+        from .sampling import sample, settings_to
+        on_gpu = hasattr(tokens, "data_ptr") and tokens.is_cuda
+        t = _tokens(tokens) if on_gpu else torch.from_numpy(_tokens(tokens)).cuda()
+        B = int(t.shape[0])
+        if self._logits is None:
+            self._logits = torch.empty(self.nseq, self.vocab, dtype=torch.float32, device=t.device)
+        logits = self.step(t, self._logits[:B])
+        rule = (u, temperature, top_k, top_p, min_p)
+        out = sample(logits, *(rule if on_gpu else settings_to(logits, *rule)))
+        return out if on_gpu else out.cpu().numpy()
 
     def prefill(self, tokens, chunk: int = 256, logits=None, want_logits: bool = True):
         """tokens (B, T) -> logits of the last position (B, vocab). Runs as

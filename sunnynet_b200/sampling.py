@@ -8,11 +8,13 @@ from __future__ import annotations
 
 import math
 
+import numpy as np
+
 from . import _lib
 from ._lib import check, current_stream, dtype_code
 from .runtime import load_runtime
 
-__all__ = ["sample"]
+__all__ = ["sample", "settings_to"]
 
 
 def _setting(name, v, B, device, dtype):
@@ -24,6 +26,20 @@ def _setting(name, v, B, device, dtype):
         raise ValueError(f"sample: {name} is one number or {B} of them on cuda:{device}")
     v = v.to(dtype).contiguous()
     return v.data_ptr(), 0, v
+
+
+def settings_to(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """u and the settings of ``sample``, from host arrays (or single numbers) to
+    the logits' GPU in one copy."""
+    import torch
+    B = logits.shape[0]
+    pack = np.zeros((5, B), np.float64)  # top_k is a whole number below 2^31: exact
+    for to, v in zip(pack, (u, temperature, top_p, min_p, np.clip(top_k, 0, 0x7fffffff))):
+        to[:] = v
+    if not np.isfinite(pack).all():
+        raise ValueError("sample: the settings are finite numbers")
+    u, t, p, q, k = torch.from_numpy(pack).to(logits.device)
+    return u, t, k.to(torch.int32), p, q
 
 
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):

@@ -25,9 +25,13 @@ request:
 
 Sampling follows the reference: temperature <= 0 is greedy (lowest id on
 ties); otherwise logits / temperature, top-k, then nucleus top-p (the most
-probable token always kept), drawn with the request's numpy generator. When
-every live request is greedy the step returns only the argmax ids from the
-device instead of all logits.
+probable token always kept) and min-p (ids of at least min_p times the most
+probable one's probability), drawn with the request's numpy generator. The
+logits stay on the device: when every live request is greedy the step returns
+only the argmax ids, otherwise each request gives one number of its generator
+and the draw is made there (``sampling.sample``; the same tokens as
+``sample_token`` draws from the same logits and generator). Only requests that
+record their logits bring them to the host.
 """
 from __future__ import annotations
 
@@ -42,8 +46,9 @@ from .model import SunnyBatch
 __all__ = ["sample_token", "CudaSunnyEngine", "Request", "BatchEngine"]
 
 
-def sample_token(logits, temperature=1.0, top_p=1.0, top_k=0, rng=None) -> int:
-    """Next token id from one row of logits (the reference's sampling rule)."""
+def sample_token(logits, temperature=1.0, top_p=1.0, top_k=0, rng=None, min_p=0.0) -> int:
+    """Next token id from one row of logits (the reference's sampling rule, and
+    min-p) on the host."""
     x = np.asarray(logits, np.float64)
     if temperature is None or temperature <= 0:
         return int(np.argmax(x))
@@ -61,6 +66,8 @@ def sample_token(logits, temperature=1.0, top_p=1.0, top_k=0, rng=None) -> int:
         z = np.full_like(z, -np.inf)
         z[order] = zs
     w = np.exp(z - np.max(z))
+    if min_p > 0.0:
+        w = np.where(w >= min(min_p, 1.0), w, 0.0)
     tot = w.sum()
     if not np.isfinite(tot) or tot <= 0:
         return int(np.argmax(x))
@@ -109,6 +116,7 @@ class Request:
     seed: int | None = None
     stop_ids: tuple = ()
     record_logits: bool = False  # keep the logits each token was drawn from (testing)
+    min_p: float = 0.0
     id: int = -1
     tokens: list = field(default_factory=list)
     logits: list = field(default_factory=list)
@@ -125,7 +133,9 @@ class BatchEngine:
 
     ``handle_factory(n)`` makes a handle of n sequences (default: a
     ``SunnyBatch`` of `blob`); it must offer prefill, step, step_argmax,
-    get_state_at, set_state_at and reset.
+    get_state_at, set_state_at and reset. Where it offers step_sample too, it
+    keeps its logits on the GPU (CUDA tokens give CUDA logits) and requests are
+    drawn there.
     """
 
     def __init__(self, blob=None, slots: int = 16, eos: int | None = None,
@@ -166,7 +176,10 @@ class BatchEngine:
         if logits_row is not None:
             if r.record_logits:
                 r.logits.append(np.array(logits_row, np.float32))
-            token = sample_token(logits_row, r.temperature, r.top_p, r.top_k, r._rng)
+            token = sample_token(logits_row, r.temperature, r.top_p, r.top_k, r._rng, r.min_p)
+        if token < 0:  # a draw from no logit above -inf
+            self._finish(r, "empty")
+            return
         if self.eos is not None and token == self.eos:
             self._finish(r, "eos")
             return
@@ -177,6 +190,23 @@ class BatchEngine:
             self._finish(r, "stop")
         elif len(r.tokens) >= r.max_tokens:
             self._finish(r, "length")
+
+    def _rule(self, requests):
+        """(u, temperature, top_k, top_p, min_p) for a draw of one token for each;
+        None (a slot without a request) is greedy. Only a request that draws
+        takes a number from its generator."""
+        rule = np.zeros((5, len(requests)))
+        rule[3] = 1.0
+        for j, r in enumerate(requests):
+            if r is not None and r.temperature is not None and r.temperature > 0:
+                rule[:, j] = (r._rng.random(), min(r.temperature, 1e300), r.top_k or 0,
+                              r.top_p if 0.0 < r.top_p < 1.0 else 1.0,
+                              min(r.min_p, 1.0) if r.min_p > 0.0 else 0.0)
+        return rule
+
+    def _on_gpu(self, requests) -> bool:
+        return hasattr(self.main, "step_sample") and \
+            not any(r.record_logits for r in requests)
 
     def _admit(self, events):
         free = [i for i, r in enumerate(self.slots) if r is None]
@@ -192,12 +222,23 @@ class BatchEngine:
         for T, group in sorted(by_len.items()):
             n = len(group)
             self.pre.reset()
-            lg = np.asarray(self.pre.prefill(np.array([r.prompt for r in group], np.int32),
-                                             chunk=self.chunk))
+            prompts = np.array([r.prompt for r in group], np.int32)
+            tokens = None
+            if self._on_gpu(group):
+                import torch
+
+                from .sampling import sample, settings_to
+                lg = self.pre.prefill(torch.from_numpy(prompts).cuda(), chunk=self.chunk)
+                tokens = sample(lg, *settings_to(lg, *self._rule(group))).tolist()
+            else:
+                lg = np.asarray(self.pre.prefill(prompts, chunk=self.chunk))
             s, h = self.pre.get_state_at(0, n)
             for j, r in enumerate(group):
                 self.main.set_state_at(r.slot, s[j:j + 1], h[j:j + 1])
-                self._take(r, logits_row=lg[j], events=events)
+                if tokens is not None:
+                    self._take(r, token=tokens[j], events=events)
+                else:
+                    self._take(r, logits_row=lg[j], events=events)
 
     def step(self) -> list:
         """Admit waiting requests, then one decode step for every live
@@ -214,6 +255,10 @@ class BatchEngine:
         if all(r.temperature is None or r.temperature <= 0 for r in live) and \
                 not any(r.record_logits for r in live):
             nxt = np.asarray(self.main.step_argmax(toks))
+            for r in live:
+                self._take(r, token=int(nxt[r.slot]), events=events)
+        elif self._on_gpu(live):
+            nxt = self.main.step_sample(toks, *self._rule(self.slots[:B]))
             for r in live:
                 self._take(r, token=int(nxt[r.slot]), events=events)
         else:

@@ -258,3 +258,64 @@ def test_refusals(sample):
     rc = L.sn_abi_sample(host.ctypes.data, 10, 0, u.data_ptr(), 0, None, 1.0, None, 0, None, 1.0,
                          None, 0.0, 3, 10, out.data_ptr(), None)
     assert rc == -1 and "device memory" in _lib.last_error()
+
+
+def test_engine_draws_on_the_gpu_what_the_host_draws():
+    """Requests of every kind of settings, served among others: the same tokens
+    from the GPU's draw as from numpy's on the same logits and generators."""
+    import tempfile
+    from pathlib import Path
+
+    from sunnynet_b200 import formats
+    from sunnynet_b200.model import SunnyBatch
+    from sunnynet_b200.serve import BatchEngine
+    shape = formats.SunnyShape(1500, 128, 224, 80, 4, 3)
+    rng = np.random.default_rng(5)
+    specs = [dict(temperature=0.8, top_k=40, top_p=0.95, seed=1), dict(),
+             dict(temperature=1.2, seed=2), dict(temperature=0.7, top_p=0.5, seed=3),
+             dict(temperature=1.5, min_p=0.05, seed=4), dict(temperature=1.0, top_k=3, seed=5),
+             dict(temperature=0.9, top_k=0, top_p=0.0, seed=6)]
+    prompts = [list(rng.integers(0, shape.vocab, n)) for n in (4, 9, 9, 3, 17, 4, 8)]
+    with tempfile.TemporaryDirectory() as td:
+        p = Path(td) / "m.usnn"
+        formats.write_usnn(p, formats.random_sunny(shape, seed=2, perturb=True))
+
+        class HostDraws(SunnyBatch):
+            step_sample = property()  # not offered
+
+        tokens = []
+        for factory in (SunnyBatch, HostDraws):
+            eng = BatchEngine(slots=3, prefill_chunk=8, handle_factory=lambda n: factory(p, n))
+            assert hasattr(eng.main, "step_sample") == (factory is SunnyBatch)
+            reqs = [eng.submit(q, 12, **s) for q, s in zip(prompts, specs)]
+            eng.run()
+            tokens.append([r.tokens for r in reqs])
+        assert tokens[0] == tokens[1] and all(len(t) == 12 for t in tokens[0])
+
+
+def test_step_sample_of_a_handle():
+    import tempfile
+    from pathlib import Path
+
+    from sunnynet_b200 import formats
+    from sunnynet_b200.model import SunnyBatch
+    shape = formats.SunnyShape(700, 64, 96, 32, 4, 2)
+    with tempfile.TemporaryDirectory() as td:
+        p = Path(td) / "m.usnn"
+        formats.write_usnn(p, formats.random_sunny(shape, seed=3, perturb=True))
+        a, b = SunnyBatch(p, 5), SunnyBatch(p, 5)
+        rng = np.random.default_rng(0)
+        toks = rng.integers(0, shape.vocab, 5).astype(np.int32)
+        T, k = np.array([0.0, 0.5, 1.0, 2.0, 0.8]), np.array([0, 5, 0, 50, 10])
+        for _ in range(4):
+            u = rng.random(5)
+            logits = np.asarray(b.step(toks))
+            want = [token(r, v, T=t, k=int(j)) for r, v, t, j in zip(logits.astype(np.float64), u, T, k)]
+            got = a.step_sample(toks, u, T, k)
+            assert got.dtype == np.int32 and got.tolist() == want
+            toks = got
+        c = lambda x: torch.from_numpy(x).cuda()  # noqa: E731
+        got = a.step_sample(c(toks), c(u), c(T), c(k.astype(np.int32)))
+        assert got.is_cuda and got.tolist() == [
+            token(r, v, T=t, k=int(j)) for r, v, t, j in
+            zip(np.asarray(b.step(toks)).astype(np.float64), u, T, k)]

@@ -115,3 +115,13 @@ def test_rejects_empty_prompt_and_zero_budget():
         eng.submit([], 3)
     with pytest.raises(ValueError):
         eng.submit([1], 0)
+
+
+def test_sample_token_min_p():
+    rng = np.random.default_rng(1)
+    lg = np.log(np.array([0.5, 0.3, 0.15, 0.05]))
+    draws = {sample_token(lg, 1.0, rng=rng, min_p=0.5) for _ in range(200)}
+    assert draws == {0, 1}  # at least half of the most probable one's 0.5
+    draws = {sample_token(lg, 1.0, top_k=3, rng=rng, min_p=0.05) for _ in range(300)}
+    assert draws == {0, 1, 2}
+    assert {sample_token(lg, 1.0, rng=rng, min_p=1.0) for _ in range(20)} == {0}
