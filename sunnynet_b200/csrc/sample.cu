@@ -329,6 +329,82 @@ struct Far {
     }
 };
 
+template <typename T>
+__device__ __forceinline__ T nothing();
+template <>
+__device__ __forceinline__ float nothing<float>() { return -INFINITY; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 nothing<__nv_bfloat16>() {
+    return __ushort_as_bfloat16(0xff80);
+}
+template <>
+__device__ __forceinline__ __half nothing<__half>() { return __ushort_as_half(0xfc00); }
+
+// A walk over a slice in the caller's memory in tiles of a pack to a thread, the
+// next kRing - 1 of them on their way to shared memory (cp.async) meanwhile: 16
+// bytes a thread and tile, where loads into registers had 4 packs in flight
+// and none while they were worked on (20 us for the first 592 rows of 32000
+// fp32 logits, and 16 from L2; 3.8 and 4.8 TB/s). A warp reads back what its
+// own lanes copied.
+constexpr int kRing = 8;
+static_assert(kRing * kThreads * 16 <= kCand * 4, "the list's room, not yet in use, holds the ring");
+
+template <typename T>
+struct Walk {
+    static constexpr int P = 16 / sizeof(T);
+    const Far<T>& x;
+    Pack<T, P>* ring;  // [kRing][kThreads]
+    int packs, tiles, ahead = 0;
+    __device__ Walk(const Far<T>& far, void* shared)
+        : x(far), ring(static_cast<Pack<T, P>*>(shared)), packs(far.packs()),
+          tiles((far.packs() + kThreads - 1) / kThreads) {
+        for (int k = 0; k < kRing - 1; ++k) fetch();
+    }
+    __device__ __forceinline__ void fetch() {
+        const int q = ahead * kThreads + threadIdx.x;
+        Pack<T, P>* to = ring + ahead % kRing * kThreads + threadIdx.x;
+        if (q < packs) {
+            if (q * P >= x.skip && (q + 1) * P <= x.n) {
+                cp_async16(to, x.x + (long long)q * P, 16);
+            } else {
+                Pack<T, P> p;
+#pragma unroll
+                for (int j = 0; j < P; ++j) {
+                    const int i = q * P + j;
+                    p.v[j] = i >= x.skip && i < x.n ? x.x[i] : nothing<T>();
+                }
+                *to = p;
+            }
+        }
+        cp_async_commit();
+        ++ahead;
+    }
+    // The warp's 32 packs of tile t, once they are there. (What is fetched next
+    // goes where the tile before this one lay.)
+    __device__ __forceinline__ const Pack<T, P>* tile(int t) {
+        __syncwarp();
+        fetch();
+        cp_async_wait_group<kRing - 1>();
+        __syncwarp();
+        return ring + t % kRing * kThreads + (threadIdx.x & ~31);
+    }
+};
+
+// f(place, logit, position in its pack) for each, padding included, ascending
+// within a thread.
+template <typename T, typename F>
+__device__ __forceinline__ void walk_all(const Far<T>& x, void* ring, F f) {
+    Walk<T> walk(x, ring);
+    for (int t = 0; t < walk.tiles; ++t) {
+        const auto* part = walk.tile(t);
+        const int q = t * kThreads + threadIdx.x;
+        if (q >= walk.packs) continue;
+        const auto p = part[threadIdx.x & 31];
+#pragma unroll
+        for (int e = 0; e < Walk<T>::P; ++e) f(q * Walk<T>::P + e, number<T>(p.v[e]), e);
+    }
+}
+
 // The same in shared memory, in fp32 and whole packs.
 struct Near {
     static constexpr int P = 4, U = 1;
@@ -390,13 +466,12 @@ __device__ __forceinline__ void each(const S& x, F f) {
 // of one, are formed side by side (each is a chain of a dozen operations).
 template <typename S, typename F>
 __device__ __forceinline__ void each_weighed(const Row& r, const Shared& s, const S& x, F f) {
-    constexpr int P = S::P, U = P == 1 ? S::U : 1;
+    constexpr int P = S::P, G = P == 1 ? S::U : 1;  // packs weighed side by side
     const int packs = x.packs();
-    for (int q = threadIdx.x; q < packs; q += U * kThreads) {
-        float v[U][P];
-        u64 w[U][P];
+    for (int q = threadIdx.x; q < packs; q += S::U * kThreads) {
+        float v[S::U][P];
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
+        for (int j = 0; j < S::U; ++j) {
             if (q + j * kThreads < packs) {
                 x.load(q + j * kThreads, v[j]);
             } else {
@@ -405,13 +480,17 @@ __device__ __forceinline__ void each_weighed(const Row& r, const Shared& s, cons
             }
         }
 #pragma unroll
-        for (int j = 0; j < U; ++j)
+        for (int j0 = 0; j0 < S::U; j0 += G) {
+            u64 w[G][P];
 #pragma unroll
-            for (int e = 0; e < P; ++e) w[j][e] = weigh(r, s, v[j][e]);
+            for (int j = 0; j < G; ++j)
 #pragma unroll
-        for (int j = 0; j < U; ++j)
+                for (int e = 0; e < P; ++e) w[j][e] = weigh(r, s, v[j0 + j][e]);
 #pragma unroll
-            for (int e = 0; e < P; ++e) f(v[j][e], w[j][e]);
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int e = 0; e < P; ++e) f(v[j0 + j][e], w[j][e]);
+        }
     }
 }
 
@@ -780,6 +859,25 @@ __device__ u32 cut(Shared& s, const Row& r, int V, int k, double p, int bits, Te
     return all;
 }
 
+// put(position, place) for each marked place in order; returns their number.
+template <typename F>
+__device__ int give_marked(Shared& s, int words, const u32* marks, F put) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    // a few neighbouring words to each thread
+    const int each = (words + kThreads - 1) / kThreads;
+    const int lo = min(tid * each, words), hi = min(lo + each, words);
+    u32 mine = 0;
+    for (int w = lo; w < hi; ++w) mine += __popc(marks[w]);
+    const u32 upto = (u32)block_upto(s, mine);
+    if (tid == kThreads - 1) s.found[0] = upto;
+    u32 at = upto - mine;
+    for (int w = lo; w < hi; ++w)
+        for (u32 m = marks[w]; m; m &= m - 1) put(at++, w * 32 + __ffs(m) - 1);
+    __syncthreads();
+    return (int)s.found[0];
+}
+
 // Marks the places of a slice's logits >= least, a bit each in words of 32, then
 // gives put(position, place) for each in order; returns their number. REST: the
 // weight of the others is estimated and added to *rest.
@@ -807,19 +905,46 @@ __device__ int list(Shared& s, const Row& r, const S& x, float least, u32* marks
             *rest += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
         }
     }
-    __syncthreads();
-    // a few neighbouring words to each thread
-    const int each = (words + kThreads - 1) / kThreads;
-    const int lo = min(tid * each, words), hi = min(lo + each, words);
-    u32 mine = 0;
-    for (int w = lo; w < hi; ++w) mine += __popc(marks[w]);
-    const u32 upto = (u32)block_upto(s, mine);
-    if (tid == kThreads - 1) s.found[0] = upto;
-    u32 at = upto - mine;
-    for (int w = lo; w < hi; ++w)
-        for (u32 m = marks[w]; m; m &= m - 1) put(at++, w * 32 + __ffs(m) - 1);
-    __syncthreads();
-    return (int)s.found[0];
+    return give_marked(s, words, marks, put);
+}
+
+// The same over a row that is not kept.
+template <bool REST, typename T, typename F>
+__device__ int list(Shared& s, const Row& r, const Far<T>& x, void* ring, float least, u32* marks,
+                    float* rest, F put) {
+    constexpr int P = 16 / sizeof(T);  // words of a warp's part of a tile
+    const int lane = threadIdx.x & 31, words = (x.n + 31) / 32;
+    Walk<T> walk(x, ring);
+    float before = 0.0f;
+    for (int t = 0; t < walk.tiles; ++t) {
+        const T* part = reinterpret_cast<const T*>(walk.tile(t));
+        const int w0 = (t * kThreads + (int)(threadIdx.x & ~31)) * P / 32;
+        float v[P];
+#pragma unroll
+        for (int j = 0; j < P; ++j) v[j] = number<T>(part[j * 32 + lane]);
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            const bool in = w0 + j < words && (w0 + j) * 32 + lane < x.n;
+            v[j] = in ? v[j] : -INFINITY;  // (a tile's end that was not copied)
+            const u32 m = __ballot_sync(0xffffffffu, v[j] >= least);
+            if (lane == j && w0 + j < words) marks[w0 + j] = m;
+        }
+        if (REST) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < P; j += 2) {
+                const float a = v[j] >= least ? 0.0f : fast_exp2((v[j] - r.max_f) * r.scale_f);
+                const float b =
+                    v[j + 1] >= least ? 0.0f : fast_exp2((v[j + 1] - r.max_f) * r.scale_f);
+                sum += a + b;
+            }
+            // two tiles' at a time: half as many roundings
+            if (t & 1) *rest += before + sum;
+            before = t & 1 ? 0.0f : sum;
+        }
+    }
+    *rest += before;
+    return give_marked(s, words, marks, put);
 }
 
 // Place of the m-th marked, from 0, in the thread that finds it; -1 in others.
@@ -1030,15 +1155,21 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a)
                     for (int i = 0; i < P; ++i) f(v[j][i], i);
                 }
             }
+        } else if constexpr (ONE) {
+            walk_all(far, dyn, [&](int, float v, int i) { f(v, i); });
         } else {
             each(far, [&](int, float v, int i) { f(v, i); });
         }
     };
     if (greedy) {
-        each(far, [&](int i, float v, int) {
+        const auto keep = [&](int i, float v, int) {
             best_at = v > best ? i : best_at;
             best = fmaxf(best, v);
-        });
+        };
+        if constexpr (!HELD && ONE)
+            walk_all(far, dyn, keep);
+        else
+            each(far, keep);
     } else if (!bins) {
         pass([&](float v, int) { best = fmaxf(best, v); });
     } else if (g.k > 0) {
@@ -1172,8 +1303,13 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a)
                 return i < 0 ? -1 : first + l.id(i);
             };
             const auto listing = [&](u32* marks, auto put) {
-                return g.k <= 0 && g.p < 1.0 ? list<true>(s, r, x, least, marks, &others, put)
-                                             : list<false>(s, r, x, least, marks, &others, put);
+                if constexpr (HELD)
+                    return g.k <= 0 && g.p < 1.0 ? list<true>(s, r, x, least, marks, &others, put)
+                                                 : list<false>(s, r, x, least, marks, &others, put);
+                else
+                    return g.k <= 0 && g.p < 1.0
+                               ? list<true>(s, r, x, dyn, least, marks, &others, put)
+                               : list<false>(s, r, x, dyn, least, marks, &others, put);
             };
             if constexpr (HELD) {
                 unsigned short* at = reinterpret_cast<unsigned short*>(dyn + a.slice + 8);
