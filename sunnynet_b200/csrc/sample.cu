@@ -116,6 +116,7 @@ struct Shared {
     u64 told[14][kMaxCluster];  // a value of each CTA, one line per exchange
     u64 red[kWarps];
     u64 warp_sum[kWarps];
+    u64 third[kWarps];
     alignas(16) u32 count[kCut];  // of cut()
     alignas(16) u32 lo[kBins], hi[kBins];  // a bin's count or weight, as two words, of border()
     u32 list[2][kList], listed[2];  // keys of the border's bin, of top-k and of top-p
@@ -274,6 +275,30 @@ __device__ __forceinline__ u64 block_upto(Shared& s, u64 v) {
     return v;
 }
 
+// Three of those at once.
+__device__ __forceinline__ void block_upto3(Shared& s, u64 (&v)[3], u64 (&all)[3]) {
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+            const u64 x = __shfl_up_sync(0xffffffffu, v[j], o);
+            if (lane >= o) v[j] += x;
+        }
+    if (lane == 31) s.red[w] = v[0], s.warp_sum[w] = v[1], s.third[w] = v[2];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 3; ++j) all[j] = 0;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+        if (k == w)
+#pragma unroll
+            for (int j = 0; j < 3; ++j) v[j] += all[j];
+        all[0] += s.red[k], all[1] += s.warp_sum[k], all[2] += s.third[k];
+    }
+    __syncthreads();
+}
+
 // Sum over the CTA's threads, the same in all.
 __device__ __forceinline__ u64 block_add(Shared& s, u64 v) {
     v = warp_add(v);
@@ -340,53 +365,68 @@ __device__ __forceinline__ __nv_bfloat16 nothing<__nv_bfloat16>() {
 template <>
 __device__ __forceinline__ __half nothing<__half>() { return __ushort_as_half(0xfc00); }
 
-// A walk over a slice in the caller's memory in tiles of a pack to a thread, the
-// next kRing - 1 of them on their way to shared memory (cp.async) meanwhile: 16
-// bytes a thread and tile, where loads into registers had 4 packs in flight
-// and none while they were worked on (20 us for the first 592 rows of 32000
-// fp32 logits, and 16 from L2; 3.8 and 4.8 TB/s). A warp reads back what its
-// own lanes copied.
-constexpr int kRing = 8;
-static_assert(kRing * kThreads * 16 <= kCand * 4, "the list's room, not yet in use, holds the ring");
+// A walk over a slice in the caller's memory in tiles of kTile packs to a
+// thread, the next kRing - 1 of them on their way to shared memory (cp.async)
+// meanwhile. Loads into registers had 4 packs in flight and none while they
+// were worked on: 20 us instead of 14 for the first 592 rows of 32000 fp32
+// logits. A warp reads back what its own lanes copied.
+constexpr int kRing = 4, kTile = 2;
 
 template <typename T>
 struct Walk {
     static constexpr int P = 16 / sizeof(T);
     const Far<T>& x;
-    Pack<T, P>* ring;  // [kRing][kThreads]
+    Pack<T, P>* ring;  // [kRing][warps][kTile][32]
     int packs, tiles, ahead = 0;
     __device__ Walk(const Far<T>& far, void* shared)
         : x(far), ring(static_cast<Pack<T, P>*>(shared)), packs(far.packs()),
-          tiles((far.packs() + kThreads - 1) / kThreads) {
+          tiles((far.packs() + kTile * kThreads - 1) / (kTile * kThreads)) {
         for (int k = 0; k < kRing - 1; ++k) fetch();
     }
+    // First pack of the calling warp's part of tile t: kTile * 32 packs.
+    __device__ __forceinline__ int first(int t) const {
+        return (t * kThreads + (int)(threadIdx.x & ~31)) * kTile;
+    }
+    __device__ __forceinline__ Pack<T, P>* part(int t) const {
+        return ring + ((t % kRing) * kThreads + (threadIdx.x & ~31)) * kTile;
+    }
+    __device__ __forceinline__ bool inner(int t) const { return t > 0 && t + 1 < tiles; }
     __device__ __forceinline__ void fetch() {
-        const int q = ahead * kThreads + threadIdx.x;
-        Pack<T, P>* to = ring + ahead % kRing * kThreads + threadIdx.x;
-        if (q < packs) {
-            if (q * P >= x.skip && (q + 1) * P <= x.n) {
-                cp_async16(to, x.x + (long long)q * P, 16);
-            } else {
-                Pack<T, P> p;
+        const int lane = threadIdx.x & 31;
+        Pack<T, P>* to = part(ahead);
+        const int q0 = first(ahead);
+        if (inner(ahead)) {
 #pragma unroll
-                for (int j = 0; j < P; ++j) {
-                    const int i = q * P + j;
-                    p.v[j] = i >= x.skip && i < x.n ? x.x[i] : nothing<T>();
+            for (int n = 0; n < kTile; ++n)
+                cp_async16(to + n * 32 + lane, x.x + (long long)(q0 + n * 32 + lane) * P, 16);
+        } else if (ahead < tiles) {
+#pragma unroll
+            for (int n = 0; n < kTile; ++n) {
+                const int q = q0 + n * 32 + lane;
+                if (q * P >= x.skip && (q + 1) * P <= x.n) {
+                    cp_async16(to + n * 32 + lane, x.x + (long long)q * P, 16);
+                } else {  // in part or wholly beside the slice
+                    Pack<T, P> p;
+#pragma unroll
+                    for (int j = 0; j < P; ++j) {
+                        const int i = q * P + j;
+                        p.v[j] = i >= x.skip && i < x.n ? x.x[i] : nothing<T>();
+                    }
+                    to[n * 32 + lane] = p;
                 }
-                *to = p;
             }
         }
         cp_async_commit();
         ++ahead;
     }
-    // The warp's 32 packs of tile t, once they are there. (What is fetched next
-    // goes where the tile before this one lay.)
+    // The warp's part of tile t, once it is there. (What is fetched next goes
+    // where the tile before this one lay.)
     __device__ __forceinline__ const Pack<T, P>* tile(int t) {
         __syncwarp();
         fetch();
         cp_async_wait_group<kRing - 1>();
         __syncwarp();
-        return ring + t % kRing * kThreads + (threadIdx.x & ~31);
+        return part(t);
     }
 };
 
@@ -395,13 +435,17 @@ struct Walk {
 template <typename T, typename F>
 __device__ __forceinline__ void walk_all(const Far<T>& x, void* ring, F f) {
     Walk<T> walk(x, ring);
+    const int lane = threadIdx.x & 31;
     for (int t = 0; t < walk.tiles; ++t) {
         const auto* part = walk.tile(t);
-        const int q = t * kThreads + threadIdx.x;
-        if (q >= walk.packs) continue;
-        const auto p = part[threadIdx.x & 31];
+        const int q0 = walk.first(t) + lane;
 #pragma unroll
-        for (int e = 0; e < Walk<T>::P; ++e) f(q * Walk<T>::P + e, number<T>(p.v[e]), e);
+        for (int n = 0; n < kTile; ++n) {
+            const auto p = part[n * 32 + lane];
+#pragma unroll
+            for (int e = 0; e < Walk<T>::P; ++e)
+                f((q0 + n * 32) * Walk<T>::P + e, number<T>(p.v[e]), e);
+        }
     }
 }
 
@@ -538,10 +582,9 @@ __device__ Border border(Shared& s, const Row& r, const S& x, const Range& in, u
     u64 base = BY_WEIGHT ? 0 : in.ahead;
     int shift = max(0, 32 - __clz(to - from) - 9);  // (to - from) >> shift < 512
     int bin = -1;
-    // few enough to gather at once: for a weight, only with nothing else to weigh
-    bool few = in.keys <= kList && (!BY_WEIGHT || (in.ahead == 0 && !rest.below));
+    bool few = in.keys <= kList;  // enough to gather at once
     u64 total = 0;
-    for (bool first = true;; first = false) {
+    for (bool first = true;; first = false) {  // (or a first round of `few` that were not)
         if (!few) {
             for (int b = tid; b < kBins; b += kThreads) s.lo[b] = s.hi[b] = 0;
             __syncthreads();
@@ -601,14 +644,28 @@ __device__ Border border(Shared& s, const Row& r, const S& x, const Range& in, u
         if (tid == 0) s.listed[BY_WEIGHT] = 0, s.least = 0xffffffffu, s.most = 0;
         __syncthreads();
         u32 least = 0xffffffffu, most = 0;
-        each(x, [&](int, float f, int) {
-            const u32 k = key_of(f);
-            if (k < from || k > to || (!few && (int)((to - k) >> shift) != bin)) return;
+        const auto gather = [&](u32 k) {
             least = min(least, k);
             most = max(most, k);
             const u32 at = atomicAdd(&s.listed[BY_WEIGHT], 1u);
             if (at < kList) list[at] = k;
-        });
+        };
+        if (BY_WEIGHT && few) {  // the first round, without a histogram before
+            u64 above = 0, below = 0;
+            each_weighed(r, s, x, [&](float f, u64 w) {
+                const u32 k = key_of(f);
+                above += k > to ? w : 0;
+                below += k < from ? w : 0;
+                if (k >= from && k <= to) gather(k);
+            });
+            t.tell(s.told[10], block_add(s, above));
+            if (rest.below) t.tell(s.told[11], block_add(s, below));
+        } else {
+            each(x, [&](int, float f, int) {
+                const u32 k = key_of(f);
+                if (k >= from && k <= to && (few || (int)((to - k) >> shift) == bin)) gather(k);
+            });
+        }
         least = __reduce_min_sync(0xffffffffu, least);
         most = __reduce_max_sync(0xffffffffu, most);
         if ((tid & 31) == 0 && least <= most) {
@@ -623,6 +680,10 @@ __device__ Border border(Shared& s, const Row& r, const S& x, const Range& in, u
         u64 count = 0;
         least = 0xffffffffu, most = 0;
         for (u32 c = 0; c < t.ctas; ++c) {
+            if (BY_WEIGHT && few) {
+                base += s.told[10][c];
+                if (rest.below) total += s.told[11][c];
+            }
             count += told[0][c];
             least = min(least, (u32)told[1][c]);
             most = max(most, (u32)told[2][c]);
@@ -631,7 +692,7 @@ __device__ Border border(Shared& s, const Row& r, const S& x, const Range& in, u
         to = most;
         if (from == to) {  // one key, however often
             if (BY_WEIGHT && target == 0) {
-                total = count * weigh(r, s, value_of(from));
+                total += base + count * weigh(r, s, value_of(from));
                 target = share(p, total + rest.least);
             }
             return {from, base, count, total, target};
@@ -645,7 +706,7 @@ __device__ Border border(Shared& s, const Row& r, const S& x, const Range& in, u
             s.all[tid] = mine;  // no key behind the last
             if (BY_WEIGHT) s.weight[tid] = w;
             if (BY_WEIGHT && target == 0) {
-                total = block_add(s, w);
+                total += base + block_add(s, w);
                 target = share(p, total + rest.least);
             }
             __syncthreads();
@@ -761,7 +822,7 @@ __device__ u32 cut(Shared& s, const Row& r, int V, int k, double p, int bits, Te
     if (k <= 0) {
         // 2^-12 is more than its terms' 2^-22, the roundings of exponents up to
         // 200 (3 * 2^-24 * 200 * ln 2 < 2^-15) and those of sums of 2^10 terms
-        sum *= exp2(((double)r.ref - r.max) * r.scale);
+        sum *= fast_exp2((float)(((double)r.ref - r.max) * r.scale));
         if (!(sum >= 0.5 && sum < 2.0 * V)) return 0;  // ref is too far off
         const double units = sum * two_to(bits);
         whole[0] = (u64)(units * (1 - 0x1p-12));
@@ -772,46 +833,39 @@ __device__ u32 cut(Shared& s, const Row& r, int V, int k, double p, int bits, Te
     t.add_up(&s.count[N * tid], sums);
 #pragma unroll
     for (int j = 0; j < N; ++j) own += n[j] = (u32)sums[j];
-    u32 counted = (u32)block_upto(s, own) - own;  // before this thread's bins
-    if (tid == 0) s.found[0] = kCut, s.found[3] = 0;
-    __syncthreads();
-    // found: the border's bin or a farther one, ids up to it, ids in it; and
-    // how many nearest bins are surely ahead of the border
+    // found: the border's bin or a farther one, ids up to it, ids ahead of the
+    // range; and how many nearest bins are surely ahead of the border
     if (k > 0) {
+        u32 counted = (u32)block_upto(s, own) - own;  // before this thread's bins
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             if (counted < (u32)k && (u32)k <= counted + n[j]) {
                 s.found[0] = s.found[3] = N * tid + j;
                 s.found[1] = counted + n[j];
-                s.found[2] = n[j];
+                s.found[2] = counted;
             }
             counted += n[j];
         }
     } else {  // the weight of a bin's ids is between those of its edges
         const float step = (float)(r.scale / r.bin), unit_f = (float)two_to(bits);
         const float d0 = (float)(((double)r.ref - r.max) * r.scale);  // bin 0's middle
-        u64 lo[N], hi[N], lo_upto = 0, hi_upto = 0;
+        const float slack = 0x1p-16f + 0x1p-21f * fabsf(d0);
+        u64 lo[N], hi[N], upto[3] = {0, 0, own}, all[3];
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const int b = N * tid + j;
-            const float slack = 0x1p-16f + 0x1p-21f * fabsf(d0);
             const float far = fminf(d0 - (b + 0.5f) * step * (1 + 0x1p-18f), 0.0f);
             const float near = b == 0 ? 0.0f : fminf(d0 - (b - 0.5f) * step * (1 - 0x1p-18f), 0.0f);
             // (the last bin has no far edge: -infinity lies in it)
             lo[j] = b == kCut - 1 ? 0 : (u64)(n[j] * (unit_f * (1 - slack) * fast_exp2(far)));
             hi[j] = (u64)(n[j] * (unit_f * (1 + slack) * fast_exp2(near))) + n[j];
-            lo_upto += lo[j];
-            hi_upto += hi[j];
+            upto[0] += lo[j];
+            upto[1] += hi[j];
         }
-        const u64 lo_own = lo_upto, hi_own = hi_upto;
-        lo_upto = block_upto(s, lo_own);
-        hi_upto = block_upto(s, hi_own);
-        if (tid == kThreads - 1) s.found[1] = lo_upto, s.found[2] = hi_upto;
-        __syncthreads();
-        const u64 lo_all = s.found[1], hi_all = s.found[2];
-        __syncthreads();
-        lo_upto -= lo_own;
-        hi_upto -= hi_own;
+        const u64 lo_own = upto[0], hi_own = upto[1];
+        block_upto3(s, upto, all);
+        u64 lo_upto = upto[0] - lo_own, hi_upto = upto[1] - hi_own;
+        u32 counted = (u32)upto[2] - own;
         // A bin lies at the border or behind it if the bins up to it reach p of
         // the whole, or those behind it weigh no more than the rest; it lies
         // ahead if those up to it do not, or those behind it weigh more. The
@@ -825,18 +879,19 @@ __device__ u32 cut(Shared& s, const Row& r, int V, int k, double p, int bits, Te
         for (int j = 0; j < N; ++j) {
             lo_upto += lo[j];
             hi_upto += hi[j];
-            not_enough += !(lo_upto >= sure || hi_all - hi_upto <= room);
-            ahead += hi_upto < may || lo_all - lo_upto > room_most;  // (both descend along the bins)
+            not_enough += !(lo_upto >= sure || all[1] - hi_upto <= room);
+            ahead += hi_upto < may || all[0] - lo_upto > room_most;  // (both descend along the bins)
         }
         const u64 both = block_add(s, not_enough << 32 | ahead);
-        const u32 bin = (u32)(both >> 32);
-        u32 upto = counted;
+        const u32 bin = (u32)(both >> 32), near = min((u32)both, bin);
+        if (tid == 0) s.found[0] = bin, s.found[3] = near, s.found[2] = 0;
+        __syncthreads();
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            upto += n[j];
-            if (bin == (u32)(N * tid + j)) s.found[1] = upto;
+            counted += n[j];
+            if (bin == (u32)(N * tid + j)) s.found[1] = counted;
+            if (near == (u32)(N * tid + j + 1)) s.found[2] = counted;
         }
-        if (tid == 0) s.found[0] = bin, s.found[3] = min((u32)both, bin);
     }
     __syncthreads();
     // no bin, or the last, which has no far edge: every id can stay
@@ -852,9 +907,9 @@ __device__ u32 cut(Shared& s, const Row& r, int V, int k, double p, int bits, Te
     __syncthreads();
     range->from = s.edge[0];
     range->to = s.edge[1];
-    range->ahead = k > 0 ? s.found[1] - s.found[2] : range->to < key_of(r.max_f);
     const u32 all = open && k <= 0 ? (u32)V : (u32)s.found[1];
-    range->keys = k > 0 ? (u32)s.found[2] : all;
+    range->ahead = s.found[2];
+    range->keys = all - (u32)s.found[2];
     __syncthreads();
     return all;
 }
@@ -882,7 +937,7 @@ __device__ int give_marked(Shared& s, int words, const u32* marks, F put) {
 // gives put(position, place) for each in order; returns their number. REST: the
 // weight of the others is estimated and added to *rest.
 template <bool REST, typename S, typename F>
-__device__ int list(Shared& s, const Row& r, const S& x, float least, u32* marks, float* rest,
+__device__ int list(Shared& s, const Row& r, const S& x, float least, u32* marks, double* rest,
                     F put) {
     constexpr int U = 8;
     const int tid = threadIdx.x, words = (x.n + 31) / 32;
@@ -902,7 +957,7 @@ __device__ int list(Shared& s, const Row& r, const S& x, float least, u32* marks
 #pragma unroll
             for (int j = 0; j < U; ++j)
                 v[j] = v[j] >= least ? 0.0f : fast_exp2((v[j] - r.max_f) * r.scale_f);
-            *rest += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            *rest += (double)(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])));
         }
     }
     return give_marked(s, words, marks, put);
@@ -911,39 +966,30 @@ __device__ int list(Shared& s, const Row& r, const S& x, float least, u32* marks
 // The same over a row that is not kept.
 template <bool REST, typename T, typename F>
 __device__ int list(Shared& s, const Row& r, const Far<T>& x, void* ring, float least, u32* marks,
-                    float* rest, F put) {
-    constexpr int P = 16 / sizeof(T);  // words of a warp's part of a tile
+                    double* rest, F put) {
+    constexpr int N = kTile * 16 / sizeof(T);  // words of a warp's part of a tile
     const int lane = threadIdx.x & 31, words = (x.n + 31) / 32;
     Walk<T> walk(x, ring);
-    float before = 0.0f;
     for (int t = 0; t < walk.tiles; ++t) {
         const T* part = reinterpret_cast<const T*>(walk.tile(t));
-        const int w0 = (t * kThreads + (int)(threadIdx.x & ~31)) * P / 32;
-        float v[P];
+        const int w0 = walk.first(t) * Walk<T>::P / 32;
+        float v[N];
+        u32 mine = 0;
 #pragma unroll
-        for (int j = 0; j < P; ++j) v[j] = number<T>(part[j * 32 + lane]);
-#pragma unroll
-        for (int j = 0; j < P; ++j) {
-            const bool in = w0 + j < words && (w0 + j) * 32 + lane < x.n;
-            v[j] = in ? v[j] : -INFINITY;  // (a tile's end that was not copied)
+        for (int j = 0; j < N; ++j) {
+            v[j] = number<T>(part[j * 32 + lane]);
             const u32 m = __ballot_sync(0xffffffffu, v[j] >= least);
-            if (lane == j && w0 + j < words) marks[w0 + j] = m;
+            mine = lane == j ? m : mine;
         }
+        if (lane < N && w0 + lane < words) marks[w0 + lane] = mine;
         if (REST) {
-            float sum = 0.0f;
+            float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < P; j += 2) {
-                const float a = v[j] >= least ? 0.0f : fast_exp2((v[j] - r.max_f) * r.scale_f);
-                const float b =
-                    v[j + 1] >= least ? 0.0f : fast_exp2((v[j + 1] - r.max_f) * r.scale_f);
-                sum += a + b;
-            }
-            // two tiles' at a time: half as many roundings
-            if (t & 1) *rest += before + sum;
-            before = t & 1 ? 0.0f : sum;
+            for (int j = 0; j < N; ++j)
+                sum[j & 1] += v[j] >= least ? 0.0f : fast_exp2((v[j] - r.max_f) * r.scale_f);
+            *rest += (double)(sum[0] + sum[1]);
         }
     }
-    *rest += before;
     return give_marked(s, words, marks, put);
 }
 
@@ -1265,16 +1311,16 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a)
     }
     if constexpr (HELD || ONE) {
         if (listed) {
-            float others = 0.0f;  // estimate of the weight that is not listed (top-p alone)
+            double others = 0.0;  // estimate of the weight that is not listed (top-p alone)
             const auto finish = [&](const auto& l) {
                 if (g.k > 0 && listed <= kList) return draw_few(s, r, l, first, g, t);
                 Rest rest{0, 0, false};
                 if (g.k <= 0 && g.p < 1.0) {
-                    // Each 2^d is off by 2^-22 of itself, and by the roundings of
-                    // the difference, the scale and their product, 3 * 2^-24 |d|
-                    // ln 2; a thread adds up n / 2048 + 4 of them. The mean of
-                    // |d|, by weight, is the entropy of the weights less log2 of
-                    // their sum, at most log2(V / sum).
+                    // Each 2^d is off by 2^-22 of itself, by the roundings of the
+                    // difference and the product and by the scale's in fp32,
+                    // (2 * 2^-24 + that) |d| ln 2, and by 10 of sums in fp32. The
+                    // mean of |d|, by weight, is the entropy of the weights less
+                    // log2 of their sum, at most log2(V / sum).
                     double v = others;
 #pragma unroll
                     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -1290,7 +1336,9 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a)
                     for (u32 c = 0; c < t.ctas; ++c) v += __longlong_as_double((long long)s.told[13][c]);
                     if (v > 0x1p-100) {
                         const double mean = ilogb(a.V / v) + 1;
-                        const double off = 0x1p-22 + (far.n / 2048 + 8) * 0x1p-24 + 3 * 0x1p-24 * 0.694 * mean;
+                        const double scale = fabs(r.scale_f / r.scale - 1.0);
+                        const double off = 0x1p-22 + 10 * 0x1p-24 +
+                                           (2 * 0x1p-24 + scale) * 0.694 * mean;
                         const double units = v * two_to(a.bits), err = 1.01 * off * units + a.V;
                         rest.least = units > err ? (u64)(units - err) : 0;
                         rest.most = (u64)(units + err);  // (exact weights are rounded, too)
