@@ -488,6 +488,112 @@ __global__ void __launch_bounds__(G ? bwd_threads(PACK * NP) : 512) norm_bwd_ker
     }
 }
 
+// Forward over many 16-bit rows of an odd width: a lane's columns lie at no
+// boundary of the weights, and loading these one by one for each row took most
+// of norm_fwd_kernel's time (3000 x 8190 in bf16: 86 us, and 53 here). Here
+// groups walk rows that lie alike, as in the backward kernel, a thread's weights
+// and biases in its slots beside the rows on their way. The CTAs that an SM
+// holds, and the loads on their way with them, are the bound now.
+template <typename T, int PACK, int G, int NP>
+__global__ void __launch_bounds__(G ? 128 : 512) norm_fwd_walk_kernel(const FwdArgs a) {
+    constexpr int W = G ? G : 1, kAhead = bwd_ahead(sizeof(T) * PACK * NP);
+    typedef Pack<T, PACK> P;
+    typedef Pack<float, PACK> F;
+    extern __shared__ __align__(128) unsigned char slots[];
+    __shared__ float red[4][32];
+    const int lane = G ? (int)(threadIdx.x % W) : (int)threadIdx.x;
+    const int stride = G ? G : (int)blockDim.x;
+    const int per = G ? (int)(blockDim.x / W) : 1;
+    const int mine = G ? (int)(threadIdx.x / W) : 0;
+    const long long step = (long long)gridDim.x * per;  // a multiple of 8
+    long long base = (long long)blockIdx.x * per;
+    const int skip = past_boundary<T, true>(static_cast<const T*>(a.x) +
+                                            min(base + mine, a.rows - 1) * a.ldx);
+    const auto col = [&](int i) { return (i * stride + lane) * PACK - skip; };
+    P* const rows = reinterpret_cast<P*>(slots) + threadIdx.x;  // [kAhead][NP][threads]
+    const auto slot = [&](int stage, int i) -> P* {
+        return rows + (stage * NP + i) * (int)blockDim.x;
+    };
+    F* const weights = reinterpret_cast<F*>(reinterpret_cast<P*>(slots) +
+                                            kAhead * NP * blockDim.x) + threadIdx.x;
+    F* const biases = weights + NP * blockDim.x;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        F w, b;
+        load_param<T, PACK, true>(a.w, a.wide, col(i), a.D, 1.0f, w.v);
+        load_param<T, PACK, true>(a.b, a.wide, col(i), a.D, 0.0f, b.v);
+        weights[i * blockDim.x] = w;
+        biases[i * blockDim.x] = b;
+    }
+    const auto fetch = [&](long long row, int stage) {
+        if (row < a.rows) {
+            const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int c = col(i);
+                const long long at = row * a.ldx + c;
+                // (partly a neighbouring row's, as in the backward kernel)
+                if (c < a.D && at >= 0 && at + PACK <= (a.rows - 1) * a.ldx + a.D)
+                    cp_async16(slot(stage, i), x + c, 16);
+                else
+                    *slot(stage, i) = load_cols<T, PACK, true>(x, c, a.D);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int k = 0; k < kAhead - 1; ++k) fetch(base + mine + k * step, k);
+    int stage = 0;
+    for (int buf = 0; base < a.rows; base += step, buf ^= 2) {
+        const long long row = base + mine;
+        const bool live = row < a.rows;
+        fetch(row + (kAhead - 1) * step, stage == 0 ? kAhead - 1 : stage - 1);
+        cp_async_wait_group<kAhead - 1>();
+        float v[NP][PACK];
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int c = col(i);
+            P x;
+            if (live) x = *slot(stage, i);
+#pragma unroll
+            for (int j = 0; j < PACK; ++j) {
+                v[i][j] = live && c + j >= 0 && c + j < a.D ? to_f(x.v[j]) : 0.0f;
+                sum += v[i][j];
+            }
+        }
+        stage = stage == kAhead - 1 ? 0 : stage + 1;
+        const float mean = __fdiv_rn(row_sum<G>(sum, red[buf]), (float)a.D);
+        float sq = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int c = col(i);
+#pragma unroll
+            for (int j = 0; j < PACK; ++j) {
+                v[i][j] -= mean;
+                sq = c + j >= 0 && c + j < a.D ? fmaf(v[i][j], v[i][j], sq) : sq;
+            }
+        }
+        const float rstd =
+            __frsqrt_rn(__fdiv_rn(row_sum<G>(sq, red[buf + 1]), (float)a.D) + a.eps);
+        if (!live) continue;
+        if (lane == 0) {
+            if (a.mean) a.mean[row] = mean;
+            if (a.rstd) a.rstd[row] = rstd;
+        }
+        T* y = static_cast<T*>(a.y) + row * a.D;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int c = col(i);
+            if (c >= a.D) continue;
+            const F w = weights[i * blockDim.x], b = biases[i * blockDim.x];
+#pragma unroll
+            for (int j = 0; j < PACK; ++j) v[i][j] = fmaf(v[i][j] * rstd, w.v[j], b.v[j]);
+            store_cols<T, PACK, true>(y, c, a.D, v[i]);
+        }
+    }
+}
+
 // dx of rows of any width: two passes over the row, the second from cache.
 template <typename T, int PACK, bool EDGE>
 __global__ void __launch_bounds__(512) norm_dx_wide_kernel(const BwdArgs a) {
@@ -622,22 +728,48 @@ Form pick(int packs, int pack, int warp_most, int cta_most) {
 // Packs of a row, one more where it may begin within one.
 int packs_of(int D, int pack, bool edge) { return (D + (edge ? pack - 1 : 0) + pack - 1) / pack; }
 
-// CTAs of a kernel that are on an SM at once, asked once for each.
+// CTAs of a kernel that an SM holds, asked once for each size of CTA.
 template <typename K>
-int resident(K kern, int threads, std::atomic<int>* known) {
-    int n = known->load(std::memory_order_relaxed);
-    if (!n) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess) {
+int resident(K kern, int threads, size_t dyn, std::atomic<int>* known) {
+    int held = known[threads / 32].load(std::memory_order_relaxed);
+    if (!held) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kern, threads, dyn) != cudaSuccess)
             cudaGetLastError();
-            return 1;
-        }
-        known->store(n < 1 ? 1 : n, std::memory_order_relaxed);
+        held = held < 1 ? 1 : held;
+        known[threads / 32].store(held, std::memory_order_relaxed);
     }
-    return n < 1 ? 1 : n;
+    return held;
+}
+
+template <typename K>
+int allow_smem(K kern, size_t dyn, const char* what) {
+    if (dyn <= 40 * 1024) return SN_OK;
+    return cuda_check(
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)dyn), what);
 }
 
 template <typename T, int PACK, int G, int NP, bool EDGE>
-int fwd_launch(const FwdArgs& a, int threads, cudaStream_t st) {
+int fwd_launch(const FwdArgs& a, int threads, int sms, cudaStream_t st) {
+    if constexpr (EDGE && sizeof(T) == 2) {
+        // With eight rows for each group of an SM. 16-bit, before and now: 4000
+        // x 5003 62 and 33 us, 40000 x 601 68 and 45, 8192 x 2047 50 and 36; 600
+        // rows of 4001, four for each, 9.7 and 10.4. In fp32, where twice the
+        // packs carry the same loads of weights, 3000 x 8190 goes from 52 to 58
+        // us and the others stay within 2 us.
+        static std::atomic<int> known[17];
+        const auto kern = norm_fwd_walk_kernel<T, PACK, G, NP>;
+        const int n = G ? 128 : threads, per = G ? n / (G ? G : 1) : 1;
+        const size_t dyn =
+            (size_t)n * NP * PACK * (bwd_ahead(sizeof(T) * PACK * NP) * sizeof(T) + 8);
+        if ((a.w || a.b) && dyn <= 200 * 1024 && a.rows >= 8ll * sms * per) {
+            SN_TRY(allow_smem(kern, dyn, "layer_norm"));
+            const long long cap = (long long)sms * resident(kern, n, dyn, known) / 8 * 8;
+            const long long want = (a.rows / 3 + per - 1) / per;
+            const long long ctas = want < cap ? (want + 7) / 8 * 8 : cap;
+            kern<<<(unsigned)ctas, n, dyn, st>>>(a);
+            return cuda_check(cudaGetLastError(), "layer_norm launch");
+        }
+    }
     const int per = G ? 128 / (G ? G : 1) : 1;
     const long long blocks = (a.rows + per - 1) / per;
     norm_fwd_kernel<T, PACK, G, NP, EDGE><<<(unsigned)blocks, G ? 128 : threads, 0, st>>>(a);
@@ -645,12 +777,12 @@ int fwd_launch(const FwdArgs& a, int threads, cudaStream_t st) {
 }
 
 template <typename T, int PACK, bool EDGE>
-int fwd_dispatch(const FwdArgs& a, cudaStream_t st) {
+int fwd_dispatch(const FwdArgs& a, int sms, cudaStream_t st) {
     // 48 elements a lane: 1536 fp32 columns in one warp; single elements are
     // the rare case of rows that share no boundary with their outputs
     const Form f = pick(packs_of(a.D, PACK, EDGE), PACK, PACK == 1 ? 32 : 48, 32);
 #define SN_FWD(g, n) \
-    if (f.G == g && f.NP == n) return fwd_launch<T, PACK, g, n, EDGE>(a, f.threads, st)
+    if (f.G == g && f.NP == n) return fwd_launch<T, PACK, g, n, EDGE>(a, f.threads, sms, st)
     if constexpr (PACK > 1) {
         SN_FWD(4, 1);
         SN_FWD(8, 1);
@@ -685,11 +817,11 @@ int fwd_dispatch(const FwdArgs& a, cudaStream_t st) {
 enum Move { kWhole, kEdge, kSingle };
 
 template <typename T>
-int fwd_typed(const FwdArgs& a, Move move, cudaStream_t st) {
+int fwd_typed(const FwdArgs& a, Move move, int sms, cudaStream_t st) {
     constexpr int P = 16 / sizeof(T);
-    return move == kWhole  ? fwd_dispatch<T, P, false>(a, st)
-           : move == kEdge ? fwd_dispatch<T, P, true>(a, st)
-                           : fwd_dispatch<T, 1, false>(a, st);
+    return move == kWhole  ? fwd_dispatch<T, P, false>(a, sms, st)
+           : move == kEdge ? fwd_dispatch<T, P, true>(a, sms, st)
+                           : fwd_dispatch<T, 1, false>(a, sms, st);
 }
 
 // Launches the backward kernel; a == nullptr: the CTAs of it that an SM holds.
@@ -699,20 +831,8 @@ int bwd_launch(const BwdArgs* a, int threads, int parts, cudaStream_t st) {
     const auto kern = norm_bwd_kernel<T, PACK, G, NP, EDGE>;
     const int n = G ? bwd_threads(PACK * NP) : threads;
     const size_t dyn = (size_t)n * bwd_slot_bytes(sizeof(T), PACK * NP);
-    if (dyn > 40 * 1024)
-        SN_TRY(cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)dyn),
-                          "layer_norm_bwd"));
-    if (!a) {
-        int held = known[n / 32].load(std::memory_order_relaxed);
-        if (!held) {
-            if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&held, kern, n, dyn) != cudaSuccess)
-                cudaGetLastError();
-            held = held < 1 ? 1 : held;
-            known[n / 32].store(held, std::memory_order_relaxed);
-        }
-        return held;
-    }
+    SN_TRY(allow_smem(kern, dyn, "layer_norm_bwd"));
+    if (!a) return resident(kern, n, dyn, known);
     kern<<<parts, n, dyn, st>>>(*a);
     return cuda_check(cudaGetLastError(), "layer_norm_bwd launch");
 }
@@ -846,9 +966,9 @@ sn_status sn_abi_layer_norm(const void* x, int64_t ldx, const void* w, const voi
                              : kSingle;
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     switch (dtype) {
-        case SN_F32: return fwd_typed<float>(a, move, st);
-        case SN_BF16: return fwd_typed<__nv_bfloat16>(a, move, st);
-        default: return fwd_typed<__half>(a, move, st);
+        case SN_F32: return fwd_typed<float>(a, move, dev.num_sms(), st);
+        case SN_BF16: return fwd_typed<__nv_bfloat16>(a, move, dev.num_sms(), st);
+        default: return fwd_typed<__half>(a, move, dev.num_sms(), st);
     }
 }
 

@@ -64,7 +64,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kCut = 1024;     // bins of the first histogram, four to a thread
 constexpr int kBins = 512;     // of the others, two to a thread
 constexpr int kList = 256;     // keys resolved by comparing them all: one to a thread
-constexpr int kCand = 8192;    // logits a CTA that keeps no slice lists: 32 KB, four CTAs on an SM
+constexpr int kCand = 8192;    // logits a CTA that keeps no slice can list, at least: 32 KB, four CTAs on an SM
 constexpr int kProbe = 4 * kThreads;  // first logits of a row, from which the bins take their place
 constexpr int kPow = 128;      // table of 2^(j/128)
 constexpr int kMaxCluster = 8;
@@ -98,7 +98,7 @@ struct SampleArgs {
     int32_t* out;
     Setting temperature, top_p, min_p;
     long long ld;
-    int one_k, u_wide, V, slice, bits;
+    int one_k, u_wide, V, slice, bits, cand;
 };
 
 // Bits of x ordered like the numbers, -0 taken for 0.
@@ -1116,7 +1116,7 @@ __device__ int draw(Shared& s, const Row& r, const S& x, int first, const Rule& 
 }
 
 // HELD: the slice is kept in shared memory, in front of a list of its places (as
-// many as it has). Otherwise the list is of kCand logits.
+// many as it has). Otherwise the list is of a.cand logits.
 template <typename T, bool HELD, bool ONE>
 __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a) {
     extern __shared__ __align__(16) float dyn[];
@@ -1301,7 +1301,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a)
         const u32 n = cut(s, r, a.V, g.k, g.p, a.bits, t, sum, &found);
         if (n) range = found;
         // every CTA of the cluster decides alike
-        if (n && (HELD ? n <= (u32)a.V / 2 : ONE && n <= kCand)) listed = n;
+        if (n && (HELD ? n <= (u32)a.V / 2 : ONE && n <= (u32)a.cand)) listed = n;
         least = value_of(range.from);
     } else if (g.w_floor > 0 && g.k == 0 && g.p == 1.0 && (HELD || ONE)) {
         // where x < max + T ln(min_p) by more than the roundings here, w is below min_p
@@ -1369,13 +1369,13 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a)
                 if (id >= 0 && tid == 0) a.out[row] = id;
                 return;
             } else {
-                u32* marks = reinterpret_cast<u32*>(dyn + kCand);
+                u32* marks = reinterpret_cast<u32*>(dyn + a.cand);
                 u32* at = reinterpret_cast<u32*>(dyn);  // places first, then the logits there
                 const int n = listing(marks, [&](u32 pos, int i) {
-                    if (pos < kCand) at[pos] = (u32)i;
+                    if (pos < (u32)a.cand) at[pos] = (u32)i;
                 });
-                if (n <= kCand) {  // always where the bins counted them
-#pragma unroll 4
+                if (n <= a.cand) {  // always where the bins counted them
+#pragma unroll 8
                     for (int i = tid; i < n; i += kThreads) dyn[i] = x.value((int)at[i]);
                     __syncthreads();
                     const int m = finish(FarListed{dyn, n});
@@ -1418,10 +1418,11 @@ int start(const SampleArgs& a, int B, int ctas, size_t dyn, cudaStream_t st) {
 
 template <typename T>
 int launch(SampleArgs& a, int B, int sms, cudaStream_t st) {
-    // Rows enough to keep every SM busy with four CTAs: a row to a CTA. Fewer:
-    // slices of 8192 logits, cut further down to 2048 while the SMs have less
-    // than two CTAs each.
-    const bool one = B >= 4 * sms;
+    // A row for every SM: a row to a CTA (256 x 32000 top-k takes 24 us so, 48 in
+    // clusters of 4; 160 x 32000 23 and 33). Fewer: slices of 8192 logits, cut
+    // further down to 2048 while the SMs have less than two CTAs each (one row
+    // of 32000 takes 13 us in eight CTAs).
+    const bool one = B >= sms;
     int ctas = 1;
     while (!one && ctas < kMaxCluster &&
            ((long long)ctas * 8192 < a.V ||
@@ -1432,7 +1433,9 @@ int launch(SampleArgs& a, int B, int sms, cudaStream_t st) {
     // bits, and a bit for each
     const size_t marks = (size_t)(a.slice + 8 + 31) / 32 * 4, held = (size_t)(a.slice + 8) * 6 + marks;
     if (ctas == 1 && a.slice > 8192) {
-        const size_t dyn = 4 * kCand + marks;
+        // the more rows an SM has at once the shorter their lists
+        a.cand = B >= 4 * sms ? kCand : B >= 2 * sms ? 3 * kCand / 2 : 11 * kCand / 4;
+        const size_t dyn = 4 * (size_t)a.cand + marks;
         if (dyn <= 200 * 1024) return start<T, false, true>(a, B, 1, dyn, st);
     }
     if (held > 200 * 1024) return start<T, false, false>(a, B, ctas, 0, st);
@@ -1463,7 +1466,7 @@ extern "C" sn_status sn_abi_sample(const void* logits, int64_t ld, int32_t dtype
     SN_TRY(dev.enter("sample", {{logits, size}, {u, u_f64 ? 8u : 4u}, {temperature, 8},
                                 {top_k, 4}, {top_p, 8}, {min_p, 8}, {tokens, 4}}));
     SampleArgs a{logits, u, top_k, tokens, {temperature, temperature0}, {top_p, top_p0},
-                 {min_p, min_p0}, ld, top_k0, u_f64, V, 0, 44};
+                 {min_p, min_p0}, ld, top_k0, u_f64, V, 0, 44, 0};
     while (std::ldexp((double)V, a.bits) >= std::ldexp(1.0, 62)) --a.bits;
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     switch (dtype) {

@@ -178,6 +178,20 @@ def test_strided_rows_and_shapes(norm, dtype):
     assert ((g[0].double() - want[1].sum(0)).abs() <= bound + 60 * torch.finfo(dtype).smallest_normal).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,D", [(30001, 7), (20000, 33), (9477, 250), (5003, 1001), (2500, 2047),
+                                    (1190, 5003)])
+def test_many_rows_of_an_odd_width(norm, rows, D, dtype):
+    """Rows that a group of threads walks, the last of them not all alike; the
+    rows and the weights of a view, of both types, and with one of the two only."""
+    x, w, b, _ = inputs(rows, D + 5, dtype, torch.float32, 2)
+    for off, ww, bb in ((0, w, b), (3, w.to(dtype), b.to(dtype)), (5, None, b), (1, w, None)):
+        view = x[:, off:off + D]
+        ww, bb = (t if t is None else t[off:off + D] for t in (ww, bb))
+        want, err = truth(view, ww, bb, 1e-5)
+        near(norm(view, ww, bb), want, err, dtype)
+
+
 def test_no_rows_constant_rows_and_large_means(norm):
     w, b = torch.rand(48, device="cuda").requires_grad_(), torch.rand(48, device="cuda").requires_grad_()
     x = torch.empty(0, 48, device="cuda", requires_grad=True)
