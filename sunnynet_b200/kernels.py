@@ -344,7 +344,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, bet
     and for each the states, updated in place: exp_avg and exp_avg_sq in
     float32, or, with avg_scale and sq_scale (float32, one for each
     ``STATE_BLOCK`` values), float8_e4m3fn codes of the first moment and of
-    the square root of the second. All contiguous, on one GPU; no parameter
+    the square root of the second. All contiguous, on one GPU; none
     twice. `step` counts from 1. step (an int64 tensor of one value) and lr (a
     float64 one) may be on the GPU: then a captured step reads them anew at
     each replay."""
@@ -392,9 +392,11 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, bet
             on_gpu[name] = v.data_ptr()
     # (that they are memory of one GPU is looked up by address, below)
     at = [array("Q", map(Tensor.data_ptr, x)) for x in lists]
-    if len(set(at[0])) != n and len({a for a, k in zip(at[0], sizes) if k}) != \
-            sum(1 for k in sizes if k):
-        raise ValueError("adamw_step: a parameter appears twice")
+    written = at[0] + at[2] + at[3]
+    if len(set(written)) != 3 * n:  # (those without a value have no address)
+        written = [x for x, k in zip(written, list(sizes) * 3) if k]
+        if len(set(written)) != len(written):
+            raise ValueError("adamw_step: a parameter or state appears twice")
     to = [x.buffer_info()[0] for x in at]
     rc = _lib_loaded().sn_abi_adamw_step(
         n, *to[:4], *(to[4:] or (None, None)), sizes.buffer_info()[0], dtype_code(first.dtype),
@@ -404,3 +406,4 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, bet
         float(eps), float(weight_decay), current_stream(first))
     if rc:
         check(rc, "adamw_step")
+    torch.autograd.graph.increment_version(lists[0])  # a graph that saved one must not use it

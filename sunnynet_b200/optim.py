@@ -77,12 +77,16 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
+        """A state dict of this class or of torch.optim.AdamW (states of 32 bits)."""
         super().load_state_dict(state_dict)
+        for g in self.param_groups:
+            g.setdefault("state_bits", 32)
         # torch gives states their parameter's type: put back the saved ones
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):
             if i in state_dict["state"]:
-                self.state[p] = {k: v.detach().to(p.device, copy=True)
+                self.state[p] = {k: int(v) if k == "step" else
+                                 v.detach().to(p.device, copy=True)
                                  if isinstance(v, torch.Tensor) else v
                                  for k, v in state_dict["state"][i].items()}

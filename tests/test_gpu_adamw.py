@@ -119,6 +119,35 @@ def test_bits_of_the_update(adamw_step, kind, bits, offset):
     assert all(torch.equal(a, b) for a, b in zip(lists[1], grads))
 
 
+def test_roots_and_quotients_of_every_size(adamw_step):
+    """p = -(m / 2) / (2 sqrt(3 v / 4) + eps), each operation rounded once (the
+    rates are powers of two), for magnitudes inside and outside 2^-80 .. 2^80,
+    against torch's division and root, which round correctly."""
+    n = 1 << 21
+    g = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda: torch.rand(n, device="cuda", generator=g, dtype=torch.float64)  # noqa: E731
+    for lo, hi in ((-75, 75), (-20, 4), (-130, 120)):
+        m = ((r() - 0.5).sign() * (1 + r()) * 2.0 ** (lo + (hi - lo) * r()).floor()).float()
+        v = ((1 + r()) * 2.0 ** (lo + (hi - lo) * r()).floor()).float()
+        for eps in (1e-8, 0.0):
+            p, state = torch.zeros(n, device="cuda"), [m.clone(), v.clone()]
+            adamw_step([p], [torch.zeros(n, device="cuda")], state[:1], state[1:], 1, lr=0.5,
+                       beta1=0.5, beta2=0.75, eps=eps, weight_decay=0.0)
+            want = 0 - (m * 0.5) / ((v * 0.75).sqrt() * 2.0 + torch.tensor(eps, device="cuda"))
+            assert torch.equal(p, want), (lo, hi, eps)
+            assert torch.equal(state[0], m * 0.5) and torch.equal(state[1], v * 0.75)
+
+
+def test_a_step_is_seen_by_autograd(adamw_step):
+    """A graph that saved a parameter refuses its backward pass after the step."""
+    p, g, m, v = make([64], KINDS[0], 32)
+    p[0].requires_grad_()
+    loss = (p[0] * p[0]).sum()
+    adamw_step([p[0].detach()], g, m, v, 1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_a_large_launch_and_many_tensors(adamw_step, bits):
     """The wide chunks, and more tensors than one launch takes."""
@@ -274,6 +303,26 @@ def test_optimizer_state_saved_and_loaded(bits, tmp_path):
     assert all(ob.state[p]["exp_avg"].dtype == want and ob.state[p]["step"] == 4 for p in b)
 
 
+def test_state_of_torchs_optimizer_is_loaded():
+    """One more step of either from there; bounds as in test_optimizer_follows_torch."""
+    from sunnynet_b200.optim import AdamW
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(500, device="cuda", generator=g).requires_grad_()
+    b = torch.optim.AdamW([x], lr=1e-2)
+    for _ in range(3):
+        x.grad = torch.randn(500, device="cuda", generator=g)
+        b.step()
+    y = x.detach().clone().requires_grad_()
+    a = AdamW([y])
+    a.load_state_dict(b.state_dict())
+    x.grad = torch.randn(500, device="cuda", generator=g)
+    y.grad = x.grad.clone()
+    a.step(), b.step()
+    assert a.state[y]["step"] == 4
+    h = 2.0 ** -24
+    assert ((x.double() - y.double()).abs() <= 16 * h * 4e-2 + 3 * h * (x.abs() + 1)).all()
+
+
 def test_refusals(adamw_step):
     from sunnynet_b200.optim import AdamW
     def lists():
@@ -284,6 +333,8 @@ def test_refusals(adamw_step):
     bad = [
         lambda: adamw_step(p, g[:1], m, v, 1), lambda: adamw_step(p, g, m, v, 0),
         lambda: adamw_step([p[0], p[0]], [g[0], g[0]], [m[0], m[0]], [v[0], v[0]], 1),
+        lambda: adamw_step(p, g, [m[0], m[1]], [v[0], m[1]], 1),
+        lambda: adamw_step(p, g, [p[0], m[1]], v, 1),
         lambda: adamw_step([p[0].cpu(), p[1]], g, m, v, 1),
         lambda: adamw_step([p[0].half(), p[1]], g, m, v, 1),
         lambda: adamw_step([x.double() for x in p], g, m, v, 1),
