@@ -1435,6 +1435,7 @@ int launch(SampleArgs& a, int B, int sms, cudaStream_t st) {
     if (ctas == 1 && a.slice > 8192) {
         // the more rows an SM has at once the shorter their lists
         a.cand = B >= 4 * sms ? kCand : B >= 2 * sms ? 3 * kCand / 2 : 11 * kCand / 4;
+        if (4 * (size_t)a.cand + marks > 200 * 1024) a.cand = kCand;
         const size_t dyn = 4 * (size_t)a.cand + marks;
         if (dyn <= 200 * 1024) return start<T, false, true>(a, B, 1, dyn, st);
     }

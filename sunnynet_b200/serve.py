@@ -30,8 +30,10 @@ probable one's probability), drawn with the request's numpy generator. The
 logits stay on the device: when every live request is greedy the step returns
 only the argmax ids, otherwise each request gives one number of its generator
 and the draw is made there (``sampling.sample``; the same tokens as
-``sample_token`` draws from the same logits and generator). Only requests that
-record their logits bring them to the host.
+``sample_token`` draws from the same logits and generator; of logits that are
+NaN the draw takes none, and a request left without any logit above -infinity
+ends as "empty"). Only requests that record their logits bring them to the
+host.
 """
 from __future__ import annotations
 

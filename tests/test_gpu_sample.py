@@ -170,6 +170,19 @@ def test_long_rows(sample, V):
         assert np.array_equal(got, [token(r, v, **rule) for r, v in zip(x, u)]), rule
 
 
+@pytest.mark.parametrize("V", [70001, 930001, 1040001])
+@pytest.mark.parametrize("copies", [55, 110, 220])
+def test_long_rows_of_many_requests(sample, V, copies):
+    """A CTA to each of 165, 330 and 660 rows, their lists of three lengths."""
+    rng = np.random.default_rng(V)
+    t, x = rows_of(rng.standard_normal((3, V)) * 2, torch.bfloat16)
+    u = np.array([0.3, 0.8, 0.95])
+    many, us = t.repeat(copies, 1), torch.from_numpy(u).cuda().repeat(copies)
+    for rule in ({"k": 9000}, {"k": 20000, "p": 0.8}, {"p": 0.6}):
+        got = sample(many, us, **names(rule)).cpu().numpy().reshape(copies, 3)
+        assert (got == [token(r, v, **rule) for r, v in zip(x, u)]).all(), rule
+
+
 def test_borders_among_crowded_logits(sample):
     """Thousands of distinct logits within one bin of the first histogram: the later rounds."""
     rng = np.random.default_rng(8)
