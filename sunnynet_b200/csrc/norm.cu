@@ -128,6 +128,16 @@ __device__ __forceinline__ void load_param(const void* w, int wide, int c, int D
     }
 }
 
+// Whether some of columns [c, c + PACK) are none of a row of D, so that each has
+// to be asked for. The first and the last pack of a row that a CTA shares (8190
+// columns in bf16 take 48 us so, 52 where every column is asked for); of a row
+// in a warp, where most warps hold such a pack, always (20000 x 333 in bf16 20
+// us, and 22 with a branch).
+template <int PACK, int G>
+__device__ __forceinline__ bool sticks_out(int c, int D) {
+    return G || c < 0 || c + PACK > D;
+}
+
 // Elements from the 16-byte boundary at or before p to p.
 template <typename T, bool EDGE>
 __device__ __forceinline__ int past_boundary(const T* p) {
@@ -219,11 +229,14 @@ __global__ void __launch_bounds__(G ? 128 : 512) norm_fwd_kernel(const FwdArgs a
     for (int i = 0; i < NP; ++i) {
         const int c = (i * stride + lane) * PACK - skip;
 #pragma unroll
-        for (int j = 0; j < PACK; ++j) {
-            v[i][j] -= mean;
-            const bool in = EDGE ? c + j >= 0 && c + j < a.D : c < a.D;
-            sq = in ? fmaf(v[i][j], v[i][j], sq) : sq;
+        for (int j = 0; j < PACK; ++j) v[i][j] -= mean;
+        if (sticks_out<PACK, G>(c, a.D)) {
+#pragma unroll
+            for (int j = 0; j < PACK; ++j)
+                if (EDGE ? c + j < 0 || c + j >= a.D : c >= a.D) v[i][j] = 0.0f;
         }
+#pragma unroll
+        for (int j = 0; j < PACK; ++j) sq = fmaf(v[i][j], v[i][j], sq);
     }
     const float rstd =
         __frsqrt_rn(__fdiv_rn(row_sum<G>(sq, red[1]), (float)a.D) + a.eps);
@@ -314,6 +327,31 @@ constexpr int bwd_slot_bytes(int elem, int elems) {
     return elems * (2 * bwd_ahead(elem * elems) * elem + 4);
 }
 
+// A thread's PACK fp32 values of its i-th pack, in runs of 16 bytes so that a
+// warp's accesses meet no bank twice.
+template <int PACK, typename Q>
+__device__ __forceinline__ void put_wide(Q* to, int i, const float* v) {
+    constexpr int R = sizeof(Q) / sizeof(float);
+#pragma unroll
+    for (int h = 0; h < PACK / R; ++h) {
+        Q q;
+#pragma unroll
+        for (int j = 0; j < R; ++j) q.v[j] = v[h * R + j];
+        to[(i * (PACK / R) + h) * (int)blockDim.x] = q;
+    }
+}
+
+template <int PACK, typename Q>
+__device__ __forceinline__ void get_wide(const Q* from, int i, float* v) {
+    constexpr int R = sizeof(Q) / sizeof(float);
+#pragma unroll
+    for (int h = 0; h < PACK / R; ++h) {
+        const Q q = from[(i * (PACK / R) + h) * (int)blockDim.x];
+#pragma unroll
+        for (int j = 0; j < R; ++j) v[h * R + j] = q.v[j];
+    }
+}
+
 // The rows a group has yet to work on wait in shared memory, brought in by
 // cp.async: registers for them would cost the warps that hide what is left
 // (each thread reads back only what it copied itself, so no barrier is due).
@@ -340,16 +378,17 @@ __global__ void __launch_bounds__(G ? bwd_threads(PACK * NP) : 512) norm_bwd_ker
     const auto slot = [&](int stage, int which, int i) -> P* {
         return rows + ((stage * 2 + which) * NP + i) * (int)blockDim.x;
     };
-    Pack<float, PACK>* const weights =
-        reinterpret_cast<Pack<float, PACK>*>(reinterpret_cast<P*>(slots) +
-                                             kAhead * 2 * NP * blockDim.x) + threadIdx.x;
+    Pack<float, PACK <= 4 ? PACK : 4>* const weights =
+        reinterpret_cast<Pack<float, PACK <= 4 ? PACK : 4>*>(reinterpret_cast<P*>(slots) +
+                                                            kAhead * 2 * NP * blockDim.x) +
+        threadIdx.x;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         Pack<float, PACK> w;
 #pragma unroll
         for (int j = 0; j < PACK; ++j) w.v[j] = 0.0f;
         if (col(i) < a.D) load_param<T, PACK, EDGE>(a.w, a.wide, col(i), a.D, 1.0f, w.v);
-        weights[i * blockDim.x] = w;
+        put_wide<PACK>(weights, i, w.v);
     }
     float aw[NP][PACK], ab[NP][PACK];
 #pragma unroll
@@ -387,10 +426,21 @@ __global__ void __launch_bounds__(G ? bwd_threads(PACK * NP) : 512) norm_bwd_ker
 #pragma unroll
     for (int k = 0; k < kAhead - 1; ++k) fetch(base + mine + k * step, k);
     int stage = 0;
+    // a row's statistics are asked for while the row before it is worked on, in 16
+    // bits (32768 x 768: 42 us without, 38 with; in fp32, where the rows take
+    // longer to come, their registers cost as much: 57 and 59)
+    constexpr bool kAsk = sizeof(T) == 2;
+    float mean = 0.0f, rstd = 0.0f, next_mean = 0.0f, next_rstd = 0.0f;
+    if (kAsk && base + mine < a.rows) next_mean = a.mean[base + mine], next_rstd = a.rstd[base + mine];
     for (int buf = 0; base < a.rows; base += step, buf ^= 1) {
         const long long row = base + mine;
         const bool live = row < a.rows;
-        const float mean = live ? a.mean[row] : 0.0f, rstd = live ? a.rstd[row] : 0.0f;
+        if (kAsk) {
+            mean = next_mean, rstd = next_rstd;
+            if (row + step < a.rows) next_mean = a.mean[row + step], next_rstd = a.rstd[row + step];
+        } else {
+            mean = live ? a.mean[row] : 0.0f, rstd = live ? a.rstd[row] : 0.0f;
+        }
         fetch(row + (kAhead - 1) * step, stage == 0 ? kAhead - 1 : stage - 1);
         cp_async_wait_group<kAhead - 1>();
         float xv[NP][PACK], gv[NP][PACK];
@@ -404,7 +454,8 @@ __global__ void __launch_bounds__(G ? bwd_threads(PACK * NP) : 512) norm_bwd_ker
                 continue;
             }
             const P x = *slot(stage, 0, i), g = *slot(stage, 1, i);
-            const Pack<float, PACK> w = weights[i * blockDim.x];
+            Pack<float, PACK> w;
+            get_wide<PACK>(weights, i, w.v);
 #pragma unroll
             for (int j = 0; j < PACK; ++j) {
                 xv[i][j] = (to_f(x.v[j]) - mean) * rstd;
@@ -490,7 +541,7 @@ __global__ void __launch_bounds__(G ? bwd_threads(PACK * NP) : 512) norm_bwd_ker
 
 // Forward over many 16-bit rows of an odd width: a lane's columns lie at no
 // boundary of the weights, and loading these one by one for each row took most
-// of norm_fwd_kernel's time (3000 x 8190 in bf16: 86 us, and 53 here). Here
+// of norm_fwd_kernel's time (3000 x 8190 in bf16: 86 us, and 48 here). Here
 // groups walk rows that lie alike, as in the backward kernel, a thread's weights
 // and biases in its slots beside the rows on their way. The CTAs that an SM
 // holds, and the loads on their way with them, are the bound now.
@@ -498,7 +549,7 @@ template <typename T, int PACK, int G, int NP>
 __global__ void __launch_bounds__(G ? 128 : 512) norm_fwd_walk_kernel(const FwdArgs a) {
     constexpr int W = G ? G : 1, kAhead = bwd_ahead(sizeof(T) * PACK * NP);
     typedef Pack<T, PACK> P;
-    typedef Pack<float, PACK> F;
+    typedef Pack<float, PACK <= 4 ? PACK : 4> F;
     extern __shared__ __align__(128) unsigned char slots[];
     __shared__ float red[4][32];
     const int lane = G ? (int)(threadIdx.x % W) : (int)threadIdx.x;
@@ -516,14 +567,14 @@ __global__ void __launch_bounds__(G ? 128 : 512) norm_fwd_walk_kernel(const FwdA
     };
     F* const weights = reinterpret_cast<F*>(reinterpret_cast<P*>(slots) +
                                             kAhead * NP * blockDim.x) + threadIdx.x;
-    F* const biases = weights + NP * blockDim.x;
+    F* const biases = weights + NP * (PACK <= 4 ? 1 : PACK / 4) * blockDim.x;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-        F w, b;
+        Pack<float, PACK> w, b;
         load_param<T, PACK, true>(a.w, a.wide, col(i), a.D, 1.0f, w.v);
         load_param<T, PACK, true>(a.b, a.wide, col(i), a.D, 0.0f, b.v);
-        weights[i * blockDim.x] = w;
-        biases[i * blockDim.x] = b;
+        put_wide<PACK>(weights, i, w.v);
+        put_wide<PACK>(biases, i, b.v);
     }
     const auto fetch = [&](long long row, int stage) {
         if (row < a.rows) {
@@ -556,9 +607,10 @@ __global__ void __launch_bounds__(G ? 128 : 512) norm_fwd_walk_kernel(const FwdA
             const int c = col(i);
             P x;
             if (live) x = *slot(stage, i);
+            const bool all = live && !sticks_out<PACK, G>(c, a.D);
 #pragma unroll
             for (int j = 0; j < PACK; ++j) {
-                v[i][j] = live && c + j >= 0 && c + j < a.D ? to_f(x.v[j]) : 0.0f;
+                v[i][j] = all || (live && c + j >= 0 && c + j < a.D) ? to_f(x.v[j]) : 0.0f;
                 sum += v[i][j];
             }
         }
@@ -568,10 +620,11 @@ __global__ void __launch_bounds__(G ? 128 : 512) norm_fwd_walk_kernel(const FwdA
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             const int c = col(i);
+            const bool all = !sticks_out<PACK, G>(c, a.D);
 #pragma unroll
             for (int j = 0; j < PACK; ++j) {
                 v[i][j] -= mean;
-                sq = c + j >= 0 && c + j < a.D ? fmaf(v[i][j], v[i][j], sq) : sq;
+                sq = all || (c + j >= 0 && c + j < a.D) ? fmaf(v[i][j], v[i][j], sq) : sq;
             }
         }
         const float rstd =
@@ -586,7 +639,9 @@ __global__ void __launch_bounds__(G ? 128 : 512) norm_fwd_walk_kernel(const FwdA
         for (int i = 0; i < NP; ++i) {
             const int c = col(i);
             if (c >= a.D) continue;
-            const F w = weights[i * blockDim.x], b = biases[i * blockDim.x];
+            Pack<float, PACK> w, b;
+            get_wide<PACK>(weights, i, w.v);
+            get_wide<PACK>(biases, i, b.v);
 #pragma unroll
             for (int j = 0; j < PACK; ++j) v[i][j] = fmaf(v[i][j] * rstd, w.v[j], b.v[j]);
             store_cols<T, PACK, true>(y, c, a.D, v[i]);
@@ -752,7 +807,7 @@ template <typename T, int PACK, int G, int NP, bool EDGE>
 int fwd_launch(const FwdArgs& a, int threads, int sms, cudaStream_t st) {
     if constexpr (EDGE && sizeof(T) == 2) {
         // With eight rows for each group of an SM. 16-bit, before and now: 4000
-        // x 5003 62 and 33 us, 40000 x 601 68 and 45, 8192 x 2047 50 and 36; 600
+        // x 5003 62 and 30 us, 40000 x 601 68 and 45, 8192 x 2047 50 and 35; 600
         // rows of 4001, four for each, 9.7 and 10.4. In fp32, where twice the
         // packs carry the same loads of weights, 3000 x 8190 goes from 52 to 58
         // us and the others stay within 2 us.
