@@ -3,9 +3,8 @@
     python -m sunnynet_b200.build [--force] [--verbose]
 
 The library links the CUDA runtime statically and exports only the C ABI
-declared in include/*.h (no torch types cross it). Beside it _tensor_lists.so
-is built, an extension module for the installed torch that reads lists of
-tensors (csrc/tensor_lists.cpp).
+declared in include/*.h (no torch types cross it). Beside it _torch_calls.so
+is built, an extension module for the installed torch (csrc/torch_calls.cpp).
 """
 from __future__ import annotations
 
@@ -25,7 +24,7 @@ CSRC = PKG / "csrc"
 INCLUDE = REPO / "include"
 BUILD = PKG / "_build"
 LIB = PKG / "libsunnynet_cuda.so"
-LISTS = PKG / "_tensor_lists.so"
+TORCH_CALLS = PKG / "_torch_calls.so"
 
 SOURCES = ["runtime.cu", "abi.cu", "recur.cu", "quant4.cu", "gemm.cu", "tc_gemm.cu", "sunny.cu",
            "rwkv7.cu", "scan_noalloc.cu", "sunny_fused.cu", "w4a8_tc.cu", "argmax.cu",
@@ -64,22 +63,23 @@ def _compile(src: Path, obj: Path, extra, verbose: bool):
     return obj
 
 
-def _build_lists(force: bool) -> None:
+def _build_torch_calls(force: bool) -> None:
     """The extension module for the torch that is installed (its headers give the
     tensors' layout; the symbols come from its loaded libraries)."""
     spec = importlib.util.find_spec("torch")
     if spec is None:
         return
     torch = Path(spec.origin).parent
-    src = CSRC / "tensor_lists.cpp"
-    made = LISTS.stat().st_mtime if LISTS.exists() else 0.0
+    src = CSRC / "torch_calls.cpp"
+    made = TORCH_CALLS.stat().st_mtime if TORCH_CALLS.exists() else 0.0
     if not force and made > max(src.stat().st_mtime, (torch / "version.py").stat().st_mtime):
         return
     inc = [torch / "include", torch / "include" / "torch" / "csrc" / "api" / "include",
-           sysconfig.get_paths()["include"]]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-fPIC", "-shared", "-o", str(LISTS),
+           sysconfig.get_paths()["include"], Path(nvcc()).resolve().parent.parent / "include",
+           INCLUDE]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-fPIC", "-shared", "-o", str(TORCH_CALLS),
            str(src), *[x for i in inc for x in ("-isystem", str(i))],
-           "-L", str(torch / "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python"]
+           "-L", str(torch / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {src.name}:\n{r.stderr[-4000:]}")
@@ -101,7 +101,7 @@ def build(force: bool = False, verbose: bool = False, extra=()) -> Path:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stderr[-4000:]}")
-    _build_lists(force)
+    _build_torch_calls(force)
     return LIB
 
 

@@ -209,112 +209,30 @@ def _lib_loaded():
     return _lib._lib or load_kernel()
 
 
-def _tensor_lists():
-    """The extension module that reads lists of tensors."""
-    try:
-        from . import _tensor_lists as m
-    except ImportError as e:
-        raise RuntimeError("sunnynet_b200/_tensor_lists.so is missing or of another torch: "
-                           "python -m sunnynet_b200.build") from e
-    return m
+_TORCH_CALLS = None
+
+
+def _torch_calls():
+    """The extension module for torch's tensors, given the library's entry points."""
+    global _TORCH_CALLS
+    if _TORCH_CALLS is None:
+        try:
+            import torch  # noqa: F401  (its libraries first)
+
+            from . import _torch_calls as m
+        except ImportError as e:
+            raise RuntimeError("sunnynet_b200/_torch_calls.so is missing or of another torch: "
+                               "python -m sunnynet_b200.build") from e
+        lib = load_kernel()
+        m.use(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            lib.sn_abi_layer_norm, lib.sn_abi_layer_norm_bwd, lib.sn_abi_layer_norm_bwd_ws,
+            lib.sn_abi_last_error)))
+        _TORCH_CALLS = m
+    return _TORCH_CALLS
 
 
 def _address(data: bytes) -> int:
     return ctypes.cast(data, ctypes.c_void_p).value
-
-
-def _rows(t, D):
-    """t as rows of D values at one stride: (tensor, stride in elements)."""
-    if t.is_contiguous():
-        return t, D
-    t = t.reshape(-1, D)  # a view wherever the rows lie at one stride
-    n, ld = t.shape[0], t.stride(0)
-    if t.stride(1) != 1 or (n > 1 and ld < D):  # among these what a sum's gradient broadcasts
-        t, ld = t.contiguous(), D
-    return t, max(ld, D)
-
-
-def _norm_forward(x, weight, bias, eps, keep):
-    """(y, what the backward pass needs of the call: None unless keep)."""
-    D = x.shape[-1]
-    rows = x.numel() // D
-    x2, ld = _rows(x, D)
-    w = None if weight is None else weight.contiguous()
-    b = None if bias is None else bias.contiguous()
-    y = _empty_like(x) if x2 is x else x.new_empty(x.shape)
-    code = dtype_code(x.dtype)
-    wcode = code if w is None and b is None else dtype_code((b if w is None else w).dtype)
-    mean = rstd = stats = None
-    if keep:
-        stats = x.new_empty(2 * rows, dtype=_float32())
-        mean = stats.data_ptr()
-        rstd = mean + 4 * rows
-    rc = _lib_loaded().sn_abi_layer_norm(
-        x2.data_ptr(), ld, None if w is None else w.data_ptr(),
-        None if b is None else b.data_ptr(), y.data_ptr(), mean, rstd, code, wcode, rows, D, eps,
-        current_stream(x))
-    if rc:
-        check(rc, "layer_norm")
-    return y, (x2, w, (stats, ld, code, wcode, rows, D)) if keep else None
-
-
-def _float32():
-    import torch
-    return torch.float32
-
-
-def _empty_like(t):
-    import torch
-    return torch.empty_like(t)
-
-
-_NORM = None
-
-
-def _norm_fn():
-    global _NORM
-    if _NORM is not None:
-        return _NORM
-    import torch
-    types = (torch.float32, torch.bfloat16, torch.float16)
-
-    class _Norm(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, x, weight, bias, eps):
-            y, kept = _norm_forward(x, weight, bias, eps, True)
-            ctx.save_for_backward(kept[0], kept[1])
-            ctx.call = kept[2]
-            return y
-
-        @staticmethod
-        def backward(ctx, dy):
-            if torch.is_grad_enabled():  # create_graph: its own gradient is not there
-                raise RuntimeError("layer_norm can be differentiated once")
-            x, w = ctx.saved_tensors
-            stats, ldx, code, wcode, rows, D = ctx.call
-            want_x, want_w, want_b, _ = ctx.needs_input_grad
-            g, ldg = _rows(dy, D)
-            lib = _lib_loaded()
-            dx = (torch.empty_like(g) if g is dy else g.new_empty(dy.shape)) if want_x else None
-            dw = g.new_empty(D, dtype=types[wcode]) if want_w else None
-            db = g.new_empty(D, dtype=types[wcode]) if want_b else None
-            ws, need = None, 0
-            if want_w or want_b:
-                need = lib.sn_abi_layer_norm_bwd_ws(rows, D, code)
-                ws = g.new_empty(need, dtype=torch.uint8)
-            mean = stats.data_ptr()
-            rc = lib.sn_abi_layer_norm_bwd(
-                g.data_ptr(), ldg, x.data_ptr(), ldx, None if w is None else w.data_ptr(), mean,
-                mean + 4 * rows, None if dx is None else dx.data_ptr(),
-                None if dw is None else dw.data_ptr(), None if db is None else db.data_ptr(),
-                None if ws is None else ws.data_ptr(), need, code, wcode, rows, D,
-                current_stream(x))
-            if rc:
-                check(rc, "layer_norm_bwd")
-            return dx, dw, db, None
-
-    _NORM = _Norm
-    return _NORM
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
@@ -342,11 +260,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
             kind = t.dtype
     if not eps >= 0:
         raise ValueError("layer_norm: eps must not be negative")
-    if torch.is_grad_enabled() and (x.requires_grad or
-                                    (weight is not None and weight.requires_grad) or
-                                    (bias is not None and bias.requires_grad)):
-        return _norm_fn().apply(x, weight, bias, float(eps))
-    return _norm_forward(x, weight, bias, float(eps), False)[0]
+    return _torch_calls().layer_norm(x, weight, bias, eps)
 
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, beta2=0.999,
@@ -378,7 +292,7 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, bet
         return
     first, grad = lists[0][0], lists[1][0]
     state = torch.float32 if bits == 32 else torch.float8_e4m3fn
-    at, sizes = _tensor_lists().read(
+    at, sizes = _torch_calls().read(
         tuple(lists), (first.dtype, grad.dtype, state, state, torch.float32, torch.float32)[:len(lists)],
         STATE_BLOCK)
     on_gpu = {}
