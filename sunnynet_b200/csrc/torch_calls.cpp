@@ -6,9 +6,9 @@
 // model (146 tensors, six lists with 8-bit states) 200 us of calls, as long as
 // the update itself takes on the GPU; here 25 us.
 //
-// layer_norm: the call and its node in the autograd graph. As a Function in
-// Python a call and its gradients took 110 us, half of it torch's own for any
-// such Function.
+// layer_norm: the call and its node in the autograd graph. A call and its
+// gradients take 75 us of the host's time (torch's own layer norm 70), as a
+// Function in Python 110; a call without a graph 8 us instead of 11.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
