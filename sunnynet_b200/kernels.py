@@ -243,8 +243,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     bits every time; a row's bits depend on its place among the rows only
     where the width is no multiple of 16 bytes."""
     import torch
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError("layer_norm: x needs a last axis of at least one value")
+    if x.dim() == 0 or not 0 < x.shape[-1] < 1 << 31:
+        raise ValueError("layer_norm: x needs a last axis of 1 to 2^31 - 1 values")
     if not x.is_cuda:  # host tensors are staged, as by the other kernels
         to = lambda t: None if t is None else t.cuda()  # noqa: E731
         return layer_norm(x.cuda(), to(weight), to(bias), eps).to(x.device)

@@ -57,8 +57,8 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
     if logits.dim() != 2 or not logits.is_cuda:
         raise ValueError("sample: logits (B, V) on a GPU are wanted")
     B, V = logits.shape
-    if V == 0:
-        raise ValueError("sample: no logits to draw from")
+    if not 0 < V < 1 << 31 or B >= 1 << 31:
+        raise ValueError("sample: rows of 1 to 2^31 - 1 logits are wanted, and fewer rows than 2^31")
     ld, along = logits.stride()
     if V > 1 and along != 1 or B > 1 and ld < V:
         raise ValueError("sample: the logits of a row must lie side by side")

@@ -260,11 +260,58 @@ def test_host_tensors_are_staged(norm):
     near(gw, want[2], err[2], torch.float32)
 
 
+def test_differentiated_once_and_inputs_unchanged(norm):
+    x, w, b, dy = inputs(8, 40, torch.float32, torch.float32, 11)
+    x.requires_grad_(), w.requires_grad_()
+    y = norm(x, w, b)
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        torch.autograd.grad(y, x, dy, create_graph=True)
+    y = norm(x, w, b)
+    with torch.no_grad():
+        x.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(y, x, dy)
+    with torch.no_grad():
+        assert not norm(x, w, b).requires_grad
+    assert not norm(x.detach(), w.detach(), b).requires_grad
+
+
+def test_two_threads_on_streams_of_their_own(norm):
+    import threading
+
+    from sunnynet_b200.kernels import adamw_step
+    from sunnynet_b200.sampling import sample
+
+    def run(seed, out):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            x, w, b, dy = inputs(700, 515, torch.bfloat16, torch.float32, seed)
+            x.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+            m, v = torch.zeros_like(w), torch.zeros_like(w)
+            u = torch.linspace(0, 0.99, 700, device="cuda")
+            for t in range(1, 30):
+                y = norm(x, w, b)
+                gx, gw, gb = torch.autograd.grad(y, (x, w, b), dy)
+                adamw_step([w.detach()], [gw], [m], [v], t)
+                tokens = sample(y.detach(), u, top_k=9, top_p=0.9)
+            torch.cuda.current_stream().synchronize()
+            out.append([a.detach().clone() for a in (y, gx, gb, w, tokens)])
+            torch.cuda.current_stream().synchronize()
+
+    alone, beside = [[], []], [[], []]
+    for s in range(2):
+        run(s, alone[s])
+    threads = [threading.Thread(target=run, args=(s, beside[s])) for s in range(2)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    for a, c in zip(alone, beside):
+        assert all(torch.equal(p, q) for p, q in zip(a[0], c[0]))
+
+
 def test_refusals(norm):
     x, w = torch.randn(4, 8, device="cuda"), torch.ones(8, device="cuda")
     for bad in (lambda: norm(x.double()), lambda: norm(x, w[:7]), lambda: norm(x, w.half()),
                 lambda: norm(x, w.cpu()), lambda: norm(x, w, w.bfloat16()), lambda: norm(x[:, :0]),
-                lambda: norm(x.sum()), lambda: norm(x, w, None, -1.0)):
+                lambda: norm(x.sum()), lambda: norm(x, w, None, -1.0),
+                lambda: norm(x[:1, :1].expand(1, 1 << 32))):
         with pytest.raises((ValueError, TypeError)):
             bad()
     from sunnynet_b200 import _lib
