@@ -565,7 +565,7 @@ def ref_sunny(path, S, B, budget_s=10.0):
         stepf = lambda h, t, buf: L.sn_step(h, int(t), buf)
         cores = max(1, int(L.sn_recommended_threads()))
     else:
-        raise RuntimeError("oracle/_ref is not built; the CPU baseline needs the reference runtime")
+        return {"unavailable": "oracle/_ref, the reference runtime, is not built"}
     rng = np.random.default_rng(0)
     if B == 1:
         L.sn_set_threads(cores)
@@ -733,7 +733,7 @@ def ref_prefill(path, S, budget_s=15.0):
     sunnynet.c:347-349) on one sequence, all physical cores."""
     import oracle
     if not oracle.ref_available():
-        raise RuntimeError("oracle/_ref is not built; the CPU baseline needs the reference runtime")
+        return {"unavailable": "oracle/_ref, the reference runtime, is not built"}
     L = oracle.ref_model()
     cores = max(1, int(L.sn_recommended_threads()))
     L.sn_set_threads(cores)
@@ -897,7 +897,7 @@ def ref_rwkv(path, S, B, budget_s=10.0):
     import threading
     import oracle
     if not oracle.ref_available():
-        raise RuntimeError("oracle/_ref is not built; the CPU baseline needs the reference runtime")
+        return {"unavailable": "oracle/_ref, the reference runtime, is not built"}
     L = oracle.ref_abi()
     cores = max(1, int(oracle.ref_model().sn_recommended_threads()))
     K = 1 if B == 1 else min(cores, B, 32)
@@ -961,6 +961,9 @@ def main():
         if dist.rank != 0:
             return 0
         res, base = WORKLOADS[args.config](args, torch, dist, ours=False)
+        if "unavailable" in base:
+            print(json.dumps({"impl": "reference", "unavailable": base["unavailable"]}))
+            return 0
         res.update({"impl": "reference", "value": base["value"], "n_gpus": args.gpus,
                     "steps": args.steps, "warmup": args.warmup,
                     "scaling": SCALING.get(args.config, "weak"),
