@@ -20,7 +20,7 @@
 //
 // What bounds a batch of rows is not HBM but the instructions spent on a logit:
 // an exact weight takes about 40, 14 of them in 64 bits. So what can be kept is
-// narrowed first. A histogram over 512 bins, linear from the largest logit down,
+// narrowed first. A histogram over 1024 bins, linear from the largest logit down,
 // counts the logits; for top-k the bins down to the k-th, for top-p those whose
 // count times the bin's least weight reaches p of the row's weight (estimated
 // from above in fp32) hold every id that can stay. The ids of those bins are
@@ -43,6 +43,10 @@
 // for every SM a row belongs to one CTA, which keeps no more than the list and
 // reads the row from L2 again: the cost of a CTA's fixed steps (scans,
 // searches) is then spread over the whole row.
+//
+// One row of 32000 fp32 logits with top-k 40 and top-p 0.95 takes 13 us, a chain
+// of waits; 1024 of them 58 us with top-k 40, of which 22 are the pass over the
+// logits, and 121 us with top-p 0.9, which keeps some thousands of each.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -64,7 +68,8 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kCut = 1024;     // bins of the first histogram, four to a thread
 constexpr int kBins = 512;     // of the others, two to a thread
 constexpr int kList = 256;     // keys resolved by comparing them all: one to a thread
-constexpr int kCand = 8192;    // logits a CTA that keeps no slice can list, at least: 32 KB, four CTAs on an SM
+constexpr int kCand = 8192;    // logits a CTA that keeps no slice can list, at least: 32 KB,
+                               // four CTAs on an SM
 constexpr int kProbe = 4 * kThreads;  // first logits of a row, from which the bins take their place
 constexpr int kPow = 128;      // table of 2^(j/128)
 constexpr int kMaxCluster = 8;

@@ -216,14 +216,17 @@ def _torch_calls():
     """The extension module for torch's tensors, given the library's entry points."""
     global _TORCH_CALLS
     if _TORCH_CALLS is None:
-        try:
-            import torch  # noqa: F401  (its libraries first)
+        import torch  # noqa: F401  (its libraries first)
 
+        from . import build
+        lib = load_kernel()
+        if not build.TORCH_CALLS.exists():  # as load_runtime does with the library
+            build.build()
+        try:
             from . import _torch_calls as m
         except ImportError as e:
-            raise RuntimeError("sunnynet_b200/_torch_calls.so is missing or of another torch: "
-                               "python -m sunnynet_b200.build") from e
-        lib = load_kernel()
+            raise RuntimeError(f"{build.TORCH_CALLS} was built for another torch; run "
+                               "`python -m sunnynet_b200.build --force`") from e
         m.use(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
             lib.sn_abi_layer_norm, lib.sn_abi_layer_norm_bwd, lib.sn_abi_layer_norm_bwd_ws,
             lib.sn_abi_last_error)))

@@ -88,3 +88,20 @@ def test_python_refusals_before_the_library():
         kernels.adamw_step([x], [], [x], [x], 1)
     with pytest.raises(ValueError):
         kernels.layer_norm(torch.zeros(3, 0))
+
+
+def test_lists_of_tensors_are_refused_before_a_gpu_is_asked(lib):
+    from sunnynet_b200 import kernels
+    read = kernels._torch_calls().read
+    a, f = [torch.zeros(3), torch.zeros(0)], torch.float32
+    for bad, error, text in (
+            (lambda: read((a, a), (f, f), 256), ValueError, "one GPU"),
+            (lambda: read((a, a[:1]), (f, f), 256), ValueError, "one GPU|length"),
+            (lambda: read((a,), (torch.float64,), 256), TypeError, "float64"),
+            (lambda: read(([1.0],), (f,), 256), TypeError, "tensors"),
+            (lambda: read((iter(a),), (f,), 256), TypeError, "lists"),
+            (lambda: read((a,), (f, f), 256), ValueError, "dtype"),
+            (lambda: read((a,), (3,), 256), TypeError, "dtype"),
+            (lambda: kernels._torch_calls().layer_norm(1, None, None, 0.1), TypeError, "tensors")):
+        with pytest.raises(error, match=text):
+            bad()
