@@ -146,6 +146,15 @@ struct Team {
         else
             cluster_sync();
     }
+    // Another CTA's shared memory may be touched once that CTA runs: each says so
+    // when it starts, and waits for the others in front of its first tell(). The
+    // pass over the row lies between the two, so the wait is over by then.
+    __device__ __forceinline__ void started() const {
+        if (!ONE && ctas > 1) cluster_arrive_relaxed();
+    }
+    __device__ __forceinline__ void all_started() const {
+        if (!ONE && ctas > 1) cluster_wait();
+    }
     // Reads of another CTA's shared memory take several hundred cycles: the
     // callers issue all of theirs before they use the first.
     __device__ __forceinline__ u32 read(const u32* local, u32 from) const {
@@ -1128,6 +1137,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a)
     __shared__ Shared s;
     const int tid = threadIdx.x;
     const Team<ONE> t;
+    t.started();
     const int row = blockIdx.x / t.ctas;
     const int first = min((long long)t.rank * a.slice, (long long)a.V);
     Far<T> far;
@@ -1250,6 +1260,7 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a)
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kWarps; ++k) most = s.red[k] > most ? s.red[k] : most;
+    t.all_started();
     if (bins && g.k <= 0) {  // in the order of the warps, then of the CTAs
         sum = 0.0;
 #pragma unroll
