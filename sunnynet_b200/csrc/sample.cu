@@ -908,7 +908,7 @@ __device__ u32 cut(Shared& s, const Row& r, int V, int k, double p, int bits, Te
         }
     }
     __syncthreads();
-    // no bin, or the last, which has no far edge: every id can stay
+    // no bin, the last, which has no far edge, or the one before it: every id can stay
     const int bin = (int)s.found[0], ahead = (int)s.found[3];
     const bool open = bin >= kCut - 2;
     if (tid < 32) {
@@ -921,7 +921,7 @@ __device__ u32 cut(Shared& s, const Row& r, int V, int k, double p, int bits, Te
     __syncthreads();
     range->from = s.edge[0];
     range->to = s.edge[1];
-    const u32 all = open && k <= 0 ? (u32)V : (u32)s.found[1];
+    const u32 all = open ? (u32)V : (u32)s.found[1];  // (bins behind the border's are in, too)
     range->ahead = s.found[2];
     range->keys = all - (u32)s.found[2];
     __syncthreads();
@@ -1031,25 +1031,29 @@ struct Rule {
     }
 };
 
-// The draw among the listed ids of a top-k row, kList of the whole row at most,
-// by the CTA of rank 0: a thread for each id, which counts and weighs those
-// ahead of it. The lists are in order of id. Returns the id (first + x.id), -1
-// in other CTAs.
+// The draw among the listed ids of a top-k row, if they are kList at most in all
+// CTAs together (what was listed counts here, not what the bins foretold), by the
+// CTA of rank 0: a thread for each id, which counts and weighs those ahead of
+// it. The lists are in order of id. *drawn: the id (first + x.id), -1 in other
+// CTAs. False, in every CTA alike, where they are more.
 template <bool ONE, typename L>
-__device__ int draw_few(Shared& s, const Row& r, const L& x, int first, const Rule& g,
-                        Team<ONE> t) {
+__device__ bool draw_few(Shared& s, const Row& r, const L& x, int first, const Rule& g,
+                         Team<ONE> t, int* drawn) {
     const int tid = threadIdx.x;
+    u64* told = s.told[13];  // (a line of top-p without top-k)
     // each CTA leaves its keys and ids where rank 0 reads them
-    for (int i = tid; i < x.n; i += kThreads) {
+    for (int i = tid; i < min(x.n, kList); i += kThreads) {
         s.list[0][i] = key_of(x.value(i));
         s.list[1][i] = (u32)(first + x.id(i));
     }
-    if (tid == 0) t.store(&s.told[1][t.rank], 0, (u64)x.n);
+    t.tell(told, (u64)x.n);
     t.sync();
+    u64 count = 0;
+    for (u32 c = 0; c < t.ctas; ++c) count += told[c];
+    if (count > kList) return false;
     if (t.rank == 0) {
-        u32 at, count = 0;
-        for (u32 c = 0; c < t.ctas; ++c) count += (u32)s.told[1][c];
-        const u32 c = t.place(s.told[1], tid, &at);
+        u32 at;
+        const u32 c = t.place(told, tid, &at);
         const bool in = c < t.ctas;
         const u32 mine = in ? t.read(&s.list[0][at], c) : 0;
         const u32 id = in ? t.read(&s.list[1][at], c) : 0;
@@ -1077,7 +1081,8 @@ __device__ int draw_few(Shared& s, const Row& r, const L& x, int first, const Ru
         if (stays && goal < upto && goal >= upto - w) s.found[0] = id;
     }
     t.sync();  // no CTA ends while rank 0 may still read from it
-    return t.rank == 0 ? (int)s.found[0] : -1;
+    *drawn = t.rank == 0 ? (int)s.found[0] : -1;
+    return true;
 }
 
 // The draw among the ids of x (all of the slice's, or its listed ones) by the
@@ -1329,7 +1334,8 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(const SampleArgs a)
         if (listed) {
             double others = 0.0;  // estimate of the weight that is not listed (top-p alone)
             const auto finish = [&](const auto& l) {
-                if (g.k > 0 && listed <= kList) return draw_few(s, r, l, first, g, t);
+                int few;
+                if (g.k > 0 && listed <= kList && draw_few(s, r, l, first, g, t, &few)) return few;
                 Rest rest{0, 0, false};
                 if (g.k <= 0 && g.p < 1.0) {
                     // Each 2^d is off by 2^-22 of itself, by the roundings of the

@@ -1,5 +1,12 @@
-"""The draw's rows at their edges. Tokens are compared exactly with the rule in 64
-bits, as in test_gpu_sample."""
+"""The draw where few ids can stay or the border lies far below the largest logit:
+low temperatures and rows with fewer allowed ids than top-k; clusters that start
+beside other work.
+
+The bins that narrow a row down reach 32 temperatures below the largest of its
+first 1024 logits, 56 / 1020 of a temperature each; the last two have no far edge
+that counts. Tokens are compared exactly with the rule in 64 bits, as in
+test_gpu_sample.
+"""
 from __future__ import annotations
 
 import numpy as np
@@ -9,6 +16,26 @@ from test_gpu_sample import names, rows_of, sample, token  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
+
+
+BIN = 56 / 1020  # of a temperature
+
+
+def far_rows(rng, n, V, T, k, below):
+    """Rows whose k-th logit lies `below` temperatures under the largest, which is
+    among the first 1024; the others lie farther down."""
+    x = -T * (below + 0.3 + 20 * rng.random((n, V)))
+    for r in x:
+        at = rng.choice(V, k, replace=False)
+        r[at] = -T * 3 * rng.random(k)
+        if k > 1:
+            r[at[-1]] = -T * below
+        at = at[0]
+        if at >= 1024:
+            r[rng.integers(min(V, 1024))], r[at] = 0.0, -T * (below + 0.3)
+        else:
+            r[at] = 0.0
+    return x
 
 
 @pytest.mark.parametrize("n,V", [(1, 32000), (9, 5003), (70, 9001)])
@@ -31,3 +58,16 @@ def test_clusters_that_start_beside_other_work(sample, n, V):  # noqa: F811
         got += [sample(t, c, **names(rule)), sample(t, c, 0.0)]
     torch.cuda.synchronize()
     assert all(g.tolist() == want for g in got[::2]) and all(g.tolist() == greedy for g in got[1::2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V", [(1, 1000), (1, 32000), (3, 8192), (40, 9001), (160, 5003), (160, 16384)])
+def test_the_kth_logit_in_the_last_bins(sample, n, V, dtype):  # noqa: F811
+    """Bins 1021, 1022 and 1023 (the largest lies in bin 437), and far behind them."""
+    rng = np.random.default_rng(V)
+    for T, k, b in ((1.0, 2, 1022), (1.0, 40, 1021), (1.0, 40, 1022), (1.0, 40, 1023), (0.1, 100, 1022),
+                    (0.15, 40, 1021.52), (0.5, 256, 1022), (0.25, 300, 1022), (1.0, 40, 1100)):
+        t, x = rows_of(far_rows(rng, n, V, T, k, (b - 437.14) * BIN), dtype)
+        u = rng.random(n)
+        got = sample(t, torch.from_numpy(u).cuda(), T, top_k=k).cpu().numpy()
+        assert np.array_equal(got, [token(r, v, T=T, k=k) for r, v in zip(x, u)]), (T, k, b)
