@@ -947,6 +947,14 @@ __device__ int give_marked(Shared& s, int words, const u32* marks, F put) {
     return (int)s.found[0];
 }
 
+// Which of the 32 places of word w are a slice's, [skip, n) (skip < 32): those beside
+// it read as -infinity, which is no less than a `least` of -infinity.
+__device__ __forceinline__ u32 places(int w, int skip, int n) {
+    const int left = n - w * 32;
+    const u32 m = left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u;
+    return w == 0 ? m & ~0u << skip : m;
+}
+
 // Marks the places of a slice's logits >= least, a bit each in words of 32, then
 // gives put(position, place) for each in order; returns their number. REST: the
 // weight of the others is estimated and added to *rest.
@@ -965,7 +973,7 @@ __device__ int list(Shared& s, const Row& r, const S& x, float least, u32* marks
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             const u32 m = __ballot_sync(0xffffffffu, v[j] >= least);
-            if ((tid & 31) == j && w0 + j < words) marks[w0 + j] = m;
+            if ((tid & 31) == j && w0 + j < words) marks[w0 + j] = m & places(w0 + j, x.skip, x.n);
         }
         if (REST) {
 #pragma unroll
@@ -995,7 +1003,8 @@ __device__ int list(Shared& s, const Row& r, const Far<T>& x, void* ring, float 
             const u32 m = __ballot_sync(0xffffffffu, v[j] >= least);
             mine = lane == j ? m : mine;
         }
-        if (lane < N && w0 + lane < words) marks[w0 + lane] = mine;
+        if (lane < N && w0 + lane < words)
+            marks[w0 + lane] = mine & places(w0 + lane, x.skip, x.n);
         if (REST) {
             float sum[2] = {0.0f, 0.0f};
 #pragma unroll

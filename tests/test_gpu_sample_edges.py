@@ -71,3 +71,50 @@ def test_the_kth_logit_in_the_last_bins(sample, n, V, dtype):  # noqa: F811
         u = rng.random(n)
         got = sample(t, torch.from_numpy(u).cuda(), T, top_k=k).cpu().numpy()
         assert np.array_equal(got, [token(r, v, T=T, k=k) for r, v in zip(x, u)]), (T, k, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V,gap,off", [(200, 20011, 0, 0), (300, 10003, 0, 1), (200, 9973, 13, 3), (150, 20001, 5, 0),
+                                         (160, 5003, 0, 1), (40, 9001, 3, 0), (2, 32001, 0, 5)])
+def test_fewer_allowed_ids_than_top_k(sample, n, V, gap, off, dtype):  # noqa: F811
+    """Ten allowed ids, the first of each row among them and the largest of all; what
+    lies between the rows and behind the last is larger still."""
+    rng = np.random.default_rng(V)
+    flat = np.full(off + n * (V + gap) + 64, 3e4)
+    x = np.full((n, V), -np.inf)
+    for r in x:
+        r[rng.choice(V, 8, replace=False)] = rng.standard_normal(8)
+        r[:2] = 20.0 + rng.random(2)
+    np.lib.stride_tricks.as_strided(flat[off:], (n, V), ((V + gap) * 8, 8))[:] = x
+    f, _ = rows_of(flat, dtype)
+    t = f[0].as_strided((n, V), (V + gap, 1), off)
+    x = t.double().cpu().numpy()
+    u = rng.random(n)
+    for rule in ({"k": 40}, {"T": 12.0, "k": 40}, {"T": 0.1, "k": 40, "p": 0.9}, {"T": 9.0, "k": 300, "q": 0.1},
+                 {"T": 5.0, "p": 0.97}, {"T": 1e300, "q": 0.5}):
+        got = sample(t, torch.from_numpy(u).cuda(), **names(rule)).cpu().numpy()
+        assert np.array_equal(got, [token(r, v, **rule) for r, v in zip(x, u)]), rule
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,V", [(60, 1000), (2, 32000), (160, 5003), (160, 20011), (300, 10003)])
+def test_low_temperatures(sample, n, V, dtype):  # noqa: F811
+    rng = np.random.default_rng(V + n)
+    t, x = rows_of(rng.standard_normal((n, V)) * 2.5, dtype)
+    u = rng.random(n)
+    for T in (0.05, 0.1, 0.2):
+        for k in (5, 40, 300):
+            got = sample(t, torch.from_numpy(u).cuda(), T, top_k=k).cpu().numpy()
+            assert np.array_equal(got, [token(r, v, T=T, k=k) for r, v in zip(x, u)]), (T, k)
+
+
+@pytest.mark.parametrize("n,V", [(5, 1001), (1, 32001), (160, 5003), (160, 20011)])
+def test_every_id_can_stay(sample, n, V):  # noqa: F811
+    """Borders in the open bin of wide rows, and a min-p edge below every number."""
+    rng = np.random.default_rng(V)
+    t, x = rows_of(rng.standard_normal((n, V)) * 30, torch.float32)
+    u = rng.random(n)
+    for rule in ({"T": 60.0, "p": 0.9}, {"T": 60.0, "k": V - 3}, {"T": 60.0, "k": V // 2, "p": 0.9},
+                 {"T": 1e300, "q": 0.5}, {"T": 1e39, "q": 1e-3}):
+        got = sample(t, torch.from_numpy(u).cuda(), **names(rule)).cpu().numpy()
+        assert np.array_equal(got, [token(r, v, **rule) for r, v in zip(x, u)]), rule
