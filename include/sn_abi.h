@@ -232,7 +232,7 @@ int32_t     sn_abi_rwkv7_dims(const SnAbiRwkv7* m, int32_t* dims8); /* vocab,D,H
 #define SN_BF16  1
 #define SN_F16   2
 
-/* Layer norm of `rows` rows of D values: y = (x - mean) * rstd * w + b, the
+/* Layer norm of `rows` rows of D values (1 to 2^31 - 2^14): y = (x - mean) * rstd * w + b, the
  * variance biased, rstd = 1 / sqrt(var + eps). x has rows at a stride of ldx
  * elements, y is contiguous; both are of `dtype`. w, b (D) are of `wdtype`:
  * SN_F32 or `dtype`; either may be NULL (1, 0). mean, rstd (rows) fp32 are

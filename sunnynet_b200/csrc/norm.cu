@@ -992,8 +992,12 @@ bool whole16(const void* p, long long ld, unsigned size) {
     return (uintptr_t)p % 16 == 0 && ld * size % 16 == 0;
 }
 
+// The widest row: the wide kernels count columns in 32 bits, up to four steps of
+// 512 packs beyond the row's end.
+constexpr int kMaxWidth = 0x7fffffff - 0x4000 + 1;
+
 bool shape_ok(long long rows, int D, long long ld) {
-    return rows >= 0 && rows < (1ll << 31) && D > 0 && ld >= D;
+    return rows >= 0 && rows < (1ll << 31) && D > 0 && D <= kMaxWidth && ld >= D;
 }
 
 }  // namespace

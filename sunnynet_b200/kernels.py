@@ -31,6 +31,7 @@ __all__ = ["load_kernel", "load_scan_kernel", "kernel_available", "set_kernel_th
            "CoreCUDA", "core_forward", "step_core", "dw_step", "ScanCUDA", "scan_auto",
            "layer_norm", "adamw_step", "STATE_BLOCK"]
 
+_MAX_WIDTH = (1 << 31) - (1 << 14)  # of layer_norm's rows
 STATE_BLOCK = 256  # values of an 8-bit optimiser state that share one scale
 
 
@@ -246,8 +247,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     bits every time; a row's bits depend on its place among the rows only
     where the width is no multiple of 16 bytes."""
     import torch
-    if x.dim() == 0 or not 0 < x.shape[-1] < 1 << 31:
-        raise ValueError("layer_norm: x needs a last axis of 1 to 2^31 - 1 values")
+    if x.dim() == 0 or not 0 < x.shape[-1] <= _MAX_WIDTH:
+        raise ValueError("layer_norm: x needs a last axis of 1 to 2^31 - 2^14 values")
     if not x.is_cuda:  # host tensors are staged, as by the other kernels
         to = lambda t: None if t is None else t.cuda()  # noqa: E731
         return layer_norm(x.cuda(), to(weight), to(bias), eps).to(x.device)
