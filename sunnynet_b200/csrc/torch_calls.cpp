@@ -13,6 +13,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
@@ -155,6 +156,11 @@ PyObject* layer_norm(PyObject*, PyObject* args) {
     if (!PyArg_ParseTuple(args, "OOOd", &xo, &wo, &bo, &eps)) return nullptr;
     at::Tensor x, w, b;
     if (!tensor_of(xo, &x) || !tensor_of(wo, &w) || !tensor_of(bo, &b)) return nullptr;
+    // (neither path carries a tangent on)
+    const auto moves = [](const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); };
+    TORCH_CHECK(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
+                  (moves(x) || moves(w) || moves(b))),
+                "layer_norm has no forward-mode derivative");
     const auto grows = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
     if (at::GradMode::is_enabled() && (grows(x) || grows(w) || grows(b)))
         return THPVariable_Wrap(

@@ -243,7 +243,8 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the last axis of x
     (float32, bfloat16 or float16; the variance biased; sums in fp32).
     weight, bias: None or (D,) of float32 or x's type. Differentiable in x,
-    weight and bias; rows may lie at a stride. The same call gives the same
+    weight and bias, once and in reverse mode (a tensor with a forward-mode
+    tangent is refused); rows may lie at a stride. The same call gives the same
     bits every time; a row's bits depend on its place among the rows only
     where the width is no multiple of 16 bytes."""
     import torch
