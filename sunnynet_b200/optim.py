@@ -77,7 +77,16 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """A state dict of this class or of torch.optim.AdamW (states of 32 bits)."""
+        """A state dict of this class or of torch.optim.AdamW (states of 32 bits).
+        One that asks for what this class does not do (maximize, amsgrad, weight
+        decay that is not decoupled, states of 8 bits where it has none) is
+        refused, and nothing is changed."""
+        for mine, g in zip(self.param_groups, state_dict["param_groups"]):
+            if g.get("maximize") or g.get("amsgrad") or not g.get("decoupled_weight_decay", True):
+                raise ValueError("AdamW: maximize, amsgrad and weight decay that is not decoupled "
+                                 "are not supported")
+            if "state_bits" not in g and mine["state_bits"] != 32:
+                raise ValueError("AdamW: this optimiser has states of 8 bits, the state dict of 32")
         super().load_state_dict(state_dict)
         for g in self.param_groups:
             g.setdefault("state_bits", 32)
