@@ -77,10 +77,10 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """A state dict of this class or of torch.optim.AdamW (states of 32 bits).
-        One that asks for what this class does not do (maximize, amsgrad, weight
-        decay that is not decoupled, states of 8 bits where it has none) is
-        refused, and nothing is changed."""
+        """A state dict of this class or of torch.optim.AdamW (states of 32 bits,
+        kept in float32 here). One that asks for what this class does not do
+        (maximize, amsgrad, weight decay that is not decoupled, states of 8 bits
+        where it has none) is refused, and nothing is changed."""
         for mine, g in zip(self.param_groups, state_dict["param_groups"]):
             if g.get("maximize") or g.get("amsgrad") or not g.get("decoupled_weight_decay", True):
                 raise ValueError("AdamW: maximize, amsgrad and weight decay that is not decoupled "
@@ -91,11 +91,12 @@ class AdamW(torch.optim.Optimizer):
         for g in self.param_groups:
             g.setdefault("state_bits", 32)
         # torch gives states their parameter's type: put back the saved ones
-        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        params = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(ids, params):
-            if i in state_dict["state"]:
-                self.state[p] = {k: int(v) if k == "step" else
-                                 v.detach().to(p.device, copy=True)
-                                 if isinstance(v, torch.Tensor) else v
-                                 for k, v in state_dict["state"][i].items()}
+        for g, saved in zip(self.param_groups, state_dict["param_groups"]):
+            wide = ("exp_avg", "exp_avg_sq") if g["state_bits"] == 32 else ()  # torch's may be narrower
+            for p, i in zip(g["params"], saved["params"]):
+                if i in state_dict["state"]:
+                    self.state[p] = {k: int(v) if k == "step" else
+                                     v.detach().to(p.device, torch.float32 if k in wide else v.dtype,
+                                                   copy=True).contiguous()
+                                     if isinstance(v, torch.Tensor) else v
+                                     for k, v in state_dict["state"][i].items()}

@@ -30,3 +30,18 @@ def test_state_dicts_that_ask_for_more_are_refused(flag):
     with pytest.raises(ValueError, match="8 bits" if flag == "bits" else "not supported"):
         opt.load_state_dict(saved)
     assert opt.state_dict() == before
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_states_are_kept_in_float32(dtype):
+    from sunnynet_b200.optim import AdamW
+    x, saved = stepped(dtype)
+    saved["state"][0]["exp_avg"] = saved["state"][0]["exp_avg"].t().contiguous().t()  # of another layout
+    opt = AdamW([x])
+    opt.load_state_dict(saved)
+    s = opt.state[x]
+    assert s["step"] == 2 and opt.param_groups[0]["lr"] == 1e-2
+    for k in ("exp_avg", "exp_avg_sq"):
+        assert s[k].dtype == torch.float32 and s[k].is_contiguous()
+        assert torch.equal(s[k], saved["state"][0][k].float())
+        assert s[k].data_ptr() != saved["state"][0][k].data_ptr()
