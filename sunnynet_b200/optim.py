@@ -82,7 +82,8 @@ class AdamW(torch.optim.Optimizer):
         (maximize, amsgrad, weight decay that is not decoupled, states of 8 bits
         where it has none) is refused, and nothing is changed."""
         for mine, g in zip(self.param_groups, state_dict["param_groups"]):
-            if g.get("maximize") or g.get("amsgrad") or not g.get("decoupled_weight_decay", True):
+            if g.get("maximize") or g.get("amsgrad") or \
+                    (g.get("weight_decay") and not g.get("decoupled_weight_decay", True)):
                 raise ValueError("AdamW: maximize, amsgrad and weight decay that is not decoupled "
                                  "are not supported")
             if "state_bits" not in g and mine["state_bits"] != 32:

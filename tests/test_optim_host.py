@@ -45,3 +45,12 @@ def test_states_are_kept_in_float32(dtype):
         assert s[k].dtype == torch.float32 and s[k].is_contiguous()
         assert torch.equal(s[k], saved["state"][0][k].float())
         assert s[k].data_ptr() != saved["state"][0][k].data_ptr()
+
+
+def test_without_weight_decay_it_need_not_be_decoupled():
+    from sunnynet_b200.optim import AdamW
+    x, saved = stepped(weight_decay=0.0)
+    saved["param_groups"][0]["decoupled_weight_decay"] = False
+    opt = AdamW([x])
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["weight_decay"] == 0.0 and opt.state[x]["step"] == 2
