@@ -24,6 +24,7 @@
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "sn_abi.h"
@@ -194,8 +195,8 @@ PyObject** items(PyObject* list, Py_ssize_t* n) {
 // read(lists, dtypes, block) -> (addresses, sizes): of k lists of n tensors, as
 // k * n unsigned and n signed 64-bit numbers. List i has tensors of dtypes[i],
 // all contiguous and on one GPU. Lists 0 to 3 agree in their sizes, the others
-// have one value for each `block` of those. No address of lists 0, 2, 3 ...
-// (what is written) appears twice.
+// have one value for each `block` of those. No memory of lists 0, 2, 3 ...
+// (what is written) belongs to two of their tensors.
 PyObject* read(PyObject*, PyObject* args) {
     PyObject *lists, *dtypes;
     long long block;
@@ -209,7 +210,8 @@ PyObject* read(PyObject*, PyObject* args) {
     try {
         Py_ssize_t n = 0;
         if (!items(PyTuple_GET_ITEM(lists, 0), &n)) return nullptr;
-        std::vector<uint64_t> at(k * n), written;
+        std::vector<uint64_t> at(k * n);
+        std::vector<std::pair<uint64_t, uint64_t>> written;  // begin and end
         std::vector<int64_t> sizes(n);
         c10::Device device(c10::kCPU);
         for (Py_ssize_t i = 0; i < k; ++i) {
@@ -255,12 +257,15 @@ PyObject* read(PyObject*, PyObject* args) {
                     return nullptr;
                 }
                 at[i * n + j] = reinterpret_cast<uint64_t>(size ? t.data_ptr() : nullptr);
-                if (size && i != 1) written.push_back(at[i * n + j]);
+                if (size && i != 1)
+                    written.emplace_back(at[i * n + j], at[i * n + j] + size * t.element_size());
             }
         }
         std::sort(written.begin(), written.end());
-        if (std::adjacent_find(written.begin(), written.end()) != written.end()) {
-            PyErr_SetString(PyExc_ValueError, "a parameter or state appears twice");
+        if (std::adjacent_find(written.begin(), written.end(), [](const auto& a, const auto& b) {
+                return b.first < a.second;
+            }) != written.end()) {
+            PyErr_SetString(PyExc_ValueError, "a parameter or state appears twice, or overlaps another");
             return nullptr;
         }
         return Py_BuildValue("(y#y#)", reinterpret_cast<const char*>(at.data()),

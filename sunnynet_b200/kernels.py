@@ -277,10 +277,10 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, bet
     and for each the states, updated in place: exp_avg and exp_avg_sq in
     float32, or, with avg_scale and sq_scale (float32, one for each
     ``STATE_BLOCK`` values), float8_e4m3fn codes of the first moment and of
-    the square root of the second. All contiguous, on one GPU; none
-    twice. `step` counts from 1. step (an int64 tensor of one value) and lr (a
-    float64 one) may be on the GPU: then a captured step reads them anew at
-    each replay."""
+    the square root of the second. All contiguous, on one GPU; no parameter or
+    state twice, or overlapping another. `step` counts from 1. step (an int64
+    tensor of one value) and lr (a float64 one) may be on the GPU: then a
+    captured step reads them anew at each replay."""
     import torch
     Tensor = torch.Tensor
     lists = [params, grads, exp_avg, exp_avg_sq]
