@@ -24,6 +24,8 @@ def _setting(name, v, B, device, dtype):
         return None, v, None
     if v.dim() != 1 or v.shape[0] != B or v.get_device() != device:
         raise ValueError(f"sample: {name} is one number or {B} of them on cuda:{device}")
+    if dtype == torch.int32 and v.dtype != dtype:  # beyond 31 bits: every id, as a number would
+        v = v.to(torch.int64).clamp(0, 0x7fffffff)
     v = v.to(dtype).contiguous()
     return v.data_ptr(), 0, v
 
@@ -48,11 +50,11 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
     [0, 1) (float32 or float64).
 
     temperature, top_k, top_p, min_p: a number for all rows, or a tensor (B,)
-    on the logits' GPU (float64, top_k int32; others are converted by a kernel
-    each). temperature <= 0 takes the lowest id of the largest logit. top_k of
-    0 (or >= V), top_p of 1 and min_p of 0 keep every id; ids as likely as the
-    k-th stay. A row without a logit above -inf gives -1. Only enqueues, on
-    torch's current stream of that GPU."""
+    on the logits' GPU (float64, top_k int32; others are converted there).
+    temperature <= 0 takes the lowest id of the largest logit. top_k of 0 (or
+    >= V), top_p of 1 and min_p of 0 keep every id; ids as likely as the k-th
+    stay. A row without a logit above -inf gives -1. Only enqueues, on torch's
+    current stream of that GPU."""
     import torch
     if logits.dim() != 2 or not logits.is_cuda:
         raise ValueError("sample: logits (B, V) on a GPU are wanted")

@@ -118,3 +118,14 @@ def test_every_id_can_stay(sample, n, V):  # noqa: F811
                  {"T": 1e300, "q": 0.5}, {"T": 1e39, "q": 1e-3}):
         got = sample(t, torch.from_numpy(u).cuda(), **names(rule)).cpu().numpy()
         assert np.array_equal(got, [token(r, v, **rule) for r, v in zip(x, u)]), rule
+
+
+def test_top_k_beyond_31_bits(sample):  # noqa: F811
+    """In a wider type: as many ids as a number of that size would keep."""
+    rng = np.random.default_rng(6)
+    t, x = rows_of(rng.standard_normal((4, 500)), torch.float32)
+    u = np.array([0.9, 0.97, 0.5, 0.99])
+    k = torch.tensor([(1 << 32) + 1, 3, -(1 << 33) + 2, (1 << 31) + 2], device="cuda")
+    want = [token(r, v, k=j) for r, v, j in zip(x, u, (0, 3, 0, 0))]
+    assert sample(t, torch.from_numpy(u).cuda(), top_k=k).tolist() == want
+    assert sample(t, torch.from_numpy(u).cuda(), top_k=k.double()).tolist() == want
