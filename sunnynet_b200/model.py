@@ -65,20 +65,21 @@ class SunnyBatch:
     def step_sample(self, tokens, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """One token to each of the first B sequences, and the next ones (B,)
         int32, drawn on the GPU with numbers u as ``sampling.sample`` does;
-        the logits stay there. Tokens and settings are host arrays (or single
-        settings) and the result is one, or all are CUDA tensors."""
+        the logits stay there. Tokens and settings are host arrays (numpy or
+        torch, or single settings) and the result is one like the tokens, or all
+        are CUDA tensors."""
         import torch
 
         from .sampling import sample, settings_to
         on_gpu = hasattr(tokens, "data_ptr") and tokens.is_cuda
-        t = _tokens(tokens) if on_gpu else torch.from_numpy(_tokens(tokens)).cuda()
+        t = _tokens(tokens) if on_gpu else torch.as_tensor(_tokens(tokens)).cuda()
         B = int(t.shape[0])
         if self._logits is None:
             self._logits = torch.empty(self.nseq, self.vocab, dtype=torch.float32, device=t.device)
         logits = self.step(t, self._logits[:B])
         rule = (u, temperature, top_k, top_p, min_p)
         out = sample(logits, *(rule if on_gpu else settings_to(logits, *rule)))
-        return out if on_gpu else out.cpu().numpy()
+        return out if on_gpu else out.cpu() if hasattr(tokens, "data_ptr") else out.cpu().numpy()
 
     def prefill(self, tokens, chunk: int = 256, logits=None, want_logits: bool = True):
         """tokens (B, T) -> logits of the last position (B, vocab). Runs as

@@ -129,3 +129,23 @@ def test_top_k_beyond_31_bits(sample):  # noqa: F811
     want = [token(r, v, k=j) for r, v, j in zip(x, u, (0, 3, 0, 0))]
     assert sample(t, torch.from_numpy(u).cuda(), top_k=k).tolist() == want
     assert sample(t, torch.from_numpy(u).cuda(), top_k=k.double()).tolist() == want
+
+
+def test_step_sample_of_torch_tensors_on_the_host():
+    import tempfile
+    from pathlib import Path
+
+    from sunnynet_b200 import formats
+    from sunnynet_b200.model import SunnyBatch
+    shape = formats.SunnyShape(700, 64, 96, 32, 4, 2)
+    with tempfile.TemporaryDirectory() as td:
+        p = Path(td) / "m.usnn"
+        formats.write_usnn(p, formats.random_sunny(shape, seed=3, perturb=True))
+        a, b = SunnyBatch(p, 3), SunnyBatch(p, 3)
+        toks, u, k = np.array([5, 600, 31], np.int32), np.array([0.1, 0.5, 0.9]), np.array([0, 7, 40])
+        for _ in range(3):
+            want = b.step_sample(toks, u, 0.8, k)
+            got = a.step_sample(torch.from_numpy(toks), torch.from_numpy(u), 0.8, torch.from_numpy(k))
+            assert isinstance(want, np.ndarray) and got.dtype == torch.int32 and not got.is_cuda
+            assert got.tolist() == want.tolist()
+            toks = want
