@@ -38,6 +38,7 @@ host.
 from __future__ import annotations
 
 import collections
+import importlib.util
 import itertools
 from dataclasses import dataclass, field
 
@@ -130,6 +131,10 @@ class Request:
         self._rng = np.random.default_rng(self.seed)
 
 
+def _greedy(r: Request) -> bool:
+    return r.temperature is None or not r.temperature > 0
+
+
 class BatchEngine:
     """Continuous batching over `slots` sequences of one batched handle.
 
@@ -137,7 +142,8 @@ class BatchEngine:
     ``SunnyBatch`` of `blob`); it must offer prefill, step, step_argmax,
     get_state_at, set_state_at and reset. Where it offers step_sample too, it
     keeps its logits on the GPU (CUDA tokens give CUDA logits) and requests are
-    drawn there.
+    drawn there, which needs torch; greedy requests do not, and without it the
+    others are drawn on the host.
     """
 
     def __init__(self, blob=None, slots: int = 16, eos: int | None = None,
@@ -152,6 +158,7 @@ class BatchEngine:
         self.waiting: collections.deque = collections.deque()
         self.finished: list = []
         self._ids = itertools.count()
+        self._torch = importlib.util.find_spec("torch") is not None
 
     # ------------------------------------------------------------- requests
     def submit(self, prompt, max_tokens: int, **sampling) -> Request:
@@ -200,15 +207,16 @@ class BatchEngine:
         rule = np.zeros((5, len(requests)))
         rule[3] = 1.0
         for j, r in enumerate(requests):
-            if r is not None and r.temperature is not None and r.temperature > 0:
+            if r is not None and not _greedy(r):
                 rule[:, j] = (r._rng.random(), min(r.temperature, 1e300), r.top_k or 0,
                               r.top_p if 0.0 < r.top_p < 1.0 else 1.0,
                               min(r.min_p, 1.0) if r.min_p > 0.0 else 0.0)
         return rule
 
     def _on_gpu(self, requests) -> bool:
-        return hasattr(self.main, "step_sample") and \
-            not any(r.record_logits for r in requests)
+        """Whether these requests' tokens are drawn on the GPU."""
+        return self._torch and hasattr(self.main, "step_sample") and \
+            not all(_greedy(r) for r in requests) and not any(r.record_logits for r in requests)
 
     def _admit(self, events):
         free = [i for i, r in enumerate(self.slots) if r is None]
@@ -254,7 +262,7 @@ class BatchEngine:
         toks = np.zeros(B, np.int32)
         for r in live:
             toks[r.slot] = r.tokens[-1]
-        if all(r.temperature is None or r.temperature <= 0 for r in live) and \
+        if all(_greedy(r) for r in live) and \
                 not any(r.record_logits for r in live):
             nxt = np.asarray(self.main.step_argmax(toks))
             for r in live:
