@@ -71,18 +71,27 @@ def _build_torch_calls(force: bool) -> None:
         return
     torch = Path(spec.origin).parent
     src = CSRC / "torch_calls.cpp"
+    # the entry points' signatures are compiled in: their header counts as a source
+    made_of = [src, torch / "version.py", Path(__file__), *INCLUDE.glob("*.h")]
     made = TORCH_CALLS.stat().st_mtime if TORCH_CALLS.exists() else 0.0
-    if not force and made > max(src.stat().st_mtime, (torch / "version.py").stat().st_mtime):
+    if not force and made > max(p.stat().st_mtime for p in made_of):
         return
+    # in place of the old module only when it is whole: another process may be loading
+    # that one, or building as well
+    new = TORCH_CALLS.with_name(f"{TORCH_CALLS.name}.{os.getpid()}")
     inc = [torch / "include", torch / "include" / "torch" / "csrc" / "api" / "include",
            sysconfig.get_paths()["include"], Path(nvcc()).resolve().parent.parent / "include",
            INCLUDE]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-fPIC", "-shared", "-o", str(TORCH_CALLS),
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++20", "-fPIC", "-shared", "-o", str(new),
            str(src), *[x for i in inc for x in ("-isystem", str(i))],
            "-L", str(torch / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"g++ failed on {src.name}:\n{r.stderr[-4000:]}")
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"g++ failed on {src.name}:\n{r.stderr[-4000:]}")
+        os.replace(new, TORCH_CALLS)
+    finally:
+        new.unlink(missing_ok=True)
 
 
 def build(force: bool = False, verbose: bool = False, extra=()) -> Path:
