@@ -281,7 +281,8 @@ sn_status sn_abi_adamw_step(int32_t count, void* const* params, const void* cons
  * those, in descending order and equal ones by id, each whose predecessors
  * weigh less than top_p of them all; min_p keeps the weights of at least
  * min_p; the token is the first id whose weight and those of the ids before
- * it exceed u times the kept weight. NaN counts as -infinity; a row of
+ * it exceed u times the kept weight. Weights are rounded to 2^-44 of the
+ * largest (coarser above 2^18 ids). NaN counts as -infinity; a row of
  * nothing else gives -1; a largest logit of +infinity is taken itself. */
 sn_status sn_abi_sample(const void* logits, int64_t ld, int32_t dtype, const void* u,
                         int32_t u_f64, const double* temperature, double temperature0,

@@ -11,8 +11,8 @@
 // (4 to 32 lanes of a warp, or a whole CTA) between its one read and its
 // write, so the variance is the two-pass one (sum of squared differences
 // from the mean) at no extra traffic. All sums are fp32. 32768 x 768 in fp32:
-// forward 37 us, backward with the weights' gradients 57 (0.83 and 0.81 of the
-// copy rate); in bf16 25 and 38 (0.62, 0.60), where a row's instructions and the
+// forward 37 us, backward with the weights' gradients 57 (0.83 and 0.80 of the
+// copy rate); in bf16 25 and 39 (0.62, 0.59), where a row's instructions and the
 // rows that the registers leave room for count as much as its bytes.
 //
 // The weight gradients need a sum down the rows: each thread of the backward
@@ -28,7 +28,8 @@
 // a thread keeps the same columns throughout.
 //
 // Rows wider than the register forms hold (see pick) take the *_wide kernels,
-// one CTA per row, which read a row again from cache for each pass over it.
+// one CTA per row, which read a row again from cache for each pass over it (1000
+// x 33000 in fp32: forward 78 us, 0.52 of the copy rate, backward 171, 0.35).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -36,7 +36,8 @@ def settings_to(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     import torch
     B = logits.shape[0]
     pack = np.zeros((5, B), np.float64)  # top_k is a whole number below 2^31: exact
-    for to, v in zip(pack, (u, temperature, top_p, min_p, np.clip(np.asarray(top_k), 0, 0x7fffffff))):
+    k = np.clip(np.asarray(top_k), 0, 0x7fffffff)
+    for to, v in zip(pack, (u, temperature, top_p, min_p, k)):
         to[:] = v
     if not np.isfinite(pack).all():
         raise ValueError("sample: the settings are finite numbers")

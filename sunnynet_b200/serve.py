@@ -29,11 +29,13 @@ probable token always kept) and min-p (ids of at least min_p times the most
 probable one's probability), drawn with the request's numpy generator. The
 logits stay on the device: when every live request is greedy the step returns
 only the argmax ids, otherwise each request gives one number of its generator
-and the draw is made there (``sampling.sample``; the same tokens as
-``sample_token`` draws from the same logits and generator; of logits that are
-NaN the draw takes none, and a request left without any logit above -infinity
-ends as "empty"). Only requests that record their logits bring them to the
-host.
+and the draw is made there (``sampling.sample``). It draws what
+``sample_token`` draws from the same logits and generator but where that number,
+or top-p, meets a border between two ids to about V * 2^-45: the weights there
+are whole multiples of 2^-44 of the largest (coarser above 2^18 ids), here
+doubles. Of logits that are NaN the draw takes none, and a request left without
+any logit above -infinity ends as "empty". Only requests that record their
+logits bring them to the host.
 """
 from __future__ import annotations
 
