@@ -45,6 +45,7 @@ extern "C" {
 #define SN_CAP_RECUR_BWD    (1u << 9)  /* sn_abi_recur_bwd */
 #define SN_CAP_TRAIN        (1u << 10) /* sn_abi_layer_norm, _bwd, sn_abi_adamw_step */
 #define SN_CAP_SAMPLE       (1u << 11) /* sn_abi_sample */
+#define SN_CAP_LINEAR_ATTENTION (1u << 12) /* sn_abi_linear_attention_* */
 
 /* Status codes (reference sn_abi.h:41-46, docs/ABI.md:55-68) */
 #define SN_OK              0
@@ -289,6 +290,46 @@ sn_status sn_abi_sample(const void* logits, int64_t ld, int32_t dtype, const voi
                         const int32_t* top_k, int32_t top_k0, const double* top_p,
                         double top_p0, const double* min_p, double min_p0, int32_t B,
                         int32_t V, int32_t* tokens, void* cuda_stream);
+
+/* Linear attention with a decay for each head (SN_CAP_LINEAR_ATTENTION):
+ *   S_t = exp(log_decay_t) S_(t-1) + k_t v_t^T     o_t = scale * S_t^T q_t
+ * q, k (B, T, Hk, dk) and v (B, T, H, dv) of `dtype`, the values of a head side
+ * by side, the other strides in elements (sequence, token, head; any, zero too).
+ * H is a multiple of Hk: head h reads head h / (H / Hk) of q and k. dk, dv: 1 to
+ * 128. log_decay fp32 by its strides: zeros for the first two where a head has
+ * one decay for all tokens; what leaves less than 2^-256 (minus infinity too)
+ * leaves nothing. state (B, H, dk, dv) fp32: before the first token, NULL for
+ * zeros. lengths (B) or NULL: tokens from there on are not read, leave the
+ * state as it is, and their outputs (and gradients) are zeros. */
+typedef struct {
+    const void *q, *k, *v;
+    const float* log_decay;
+    const float* state;
+    const int32_t* lengths;
+    int64_t q_stride[3], k_stride[3], v_stride[3], log_decay_stride[3];
+    int32_t dtype, B, T, H, Hk, dk, dv;
+    float scale;
+} SnAbiLinearAttention;
+/* Bytes of workspace of the calls below (-1 where they would refuse the sizes).
+ * head_gates: dlog_decay is (H), else (B, T, H). */
+int64_t   sn_abi_linear_attention_ws(const SnAbiLinearAttention* a, int32_t backward,
+                                     int32_t head_gates);
+/* out (B, T, H, dv) contiguous, of `dtype`; state_out (B, H, dk, dv) fp32. The
+ * same call gives the same bits. */
+sn_status sn_abi_linear_attention(const SnAbiLinearAttention* a, void* out, float* state_out,
+                                  void* ws, int64_t ws_bytes, void* cuda_stream);
+/* Gradients: dq, dk (B, T, Hk, dk) and dv (B, T, H, dv), contiguous, of `dtype`;
+ * dlog_decay fp32 and dstate (of the first state) may be NULL; dstate_out, that
+ * of state_out, may be NULL (zeros). */
+sn_status sn_abi_linear_attention_bwd(const SnAbiLinearAttention* a, const void* dout,
+                                      const int64_t* dout_stride, const float* dstate_out, void* dq,
+                                      void* dk, void* dv, float* dlog_decay, int32_t head_gates,
+                                      float* dstate, void* ws, int64_t ws_bytes, void* cuda_stream);
+/* One token of each sequence (T = 1; the token strides, state and lengths of `a`
+ * are not read): state, its sequences state_stride values apart, is updated in
+ * place; out (B, H, dv) contiguous. */
+sn_status sn_abi_linear_attention_step(const SnAbiLinearAttention* a, float* state,
+                                       int64_t state_stride, void* out, void* cuda_stream);
 
 #ifdef __cplusplus
 }

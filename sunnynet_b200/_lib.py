@@ -81,6 +81,10 @@ SIGNATURES = {
     "sn_abi_adamw_step": (I32, [I32, V, V, V, V, V, V, V, I32, I32, I32, I64, V, F64, V, F64, F64,
                                 F64, F64, V]),
     "sn_abi_sample": (I32, [V, I64, I32, V, I32, V, F64, V, I32, V, F64, V, F64, I32, I32, V, V]),
+    "sn_abi_linear_attention_ws": (I64, [V, I32, I32]),
+    "sn_abi_linear_attention": (I32, [V, V, V, V, I64, V]),
+    "sn_abi_linear_attention_bwd": (I32, [V, V, V, V, V, V, V, V, I32, V, V, I64, V]),
+    "sn_abi_linear_attention_step": (I32, [V, V, I64, V, V]),
     # recur.h
     "sn_set_threads": (None, [CI]),
     "sn_threads": (CI, []),
@@ -123,6 +127,14 @@ SIGNATURES = {
     "sn_rk_vocab": (CI, [V]),
     "sn_rk_ready": (CI, [V]),
 }
+
+
+class LinearAttention(ctypes.Structure):
+    """SnAbiLinearAttention (sn_abi.h)."""
+    _fields_ = [(n, V) for n in ("q", "k", "v", "log_decay", "state", "lengths")] + \
+        [(n + "_stride", I64 * 3) for n in ("q", "k", "v", "log_decay")] + \
+        [(n, I32) for n in ("dtype", "B", "T", "H", "Hk", "dk", "dv")] + [("scale", F32)]
+
 
 STATUS = {0: "OK", -1: "E_INVAL", -2: "E_NOMEM", -3: "E_IO", -4: "E_FORMAT",
           -5: "E_UNSUPPORTED", -6: "E_DEVICE"}

@@ -1,0 +1,377 @@
+"""Linear attention with a decay for each head, its gradients and its form for
+single tokens, against the recurrence in 64 bits (its gradients by autograd).
+
+Tolerances. Every output is a sum of products of the inputs, so the same
+recurrence of their absolute values bounds the sum of the magnitudes of its
+terms (M below, one number for each output). A term meets at most
+ - float32 and float16: three matrix products, each of two factors in two bf16
+   parts: 2^-17 for each factor and 2^-16 for the product of the low parts that
+   is left out, 2^-15; decays of 2^-20 (ex2.approx: 2^-22, and the sums of the
+   decays, 2^-24 of at most 2^5 where 2^-c is worth anything); fp32 sums of up to
+   64 + 128 terms in a chunk and one more for each chunk of a sequence, 2^-24
+   each: 3 * 2^-15 + 2^-20 + (192 + T / 32) 2^-24 < 2^-13 for T up to 8192;
+ - bfloat16: one more rounding to bf16 for what lies between two products (a
+   score, or the state), 2^-8, and the second-order part of both: 2^-8 + 2^-13;
+   the states and the gradient of the decays have none: 2^-13.
+The store adds a half step of the stored type.
+"""
+from __future__ import annotations
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+FINE = 2.0 ** -13
+
+
+@pytest.fixture(scope="module")
+def kernels():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from sunnynet_b200 import kernels
+    return kernels
+
+
+def recurrence(q, k, v, log_decay, state, lengths, scale):
+    """The definition, token by token, in the inputs' type."""
+    B, T, H, dv = v.shape
+    Hk, dk = q.shape[2:]
+    q, k = (x.repeat_interleave(H // Hk, 2) for x in (q, k))
+    f = log_decay.exp().expand(B, T, H)
+    S = torch.zeros(B, H, dk, dv, dtype=v.dtype, device=v.device) if state is None else state
+    out = []
+    for t in range(T):
+        new = S * f[:, t, :, None, None] + k[:, t, :, :, None] * v[:, t, :, None, :]
+        o = (q[:, t, :, :, None] * new).sum(2) * scale
+        if lengths is not None:
+            on = (t < lengths)[:, None, None]
+            new, o = torch.where(on[..., None], new, S), torch.where(on, o, 0.0)
+        S = new
+        out.append(o)
+    return torch.stack(out, 1) if T else torch.zeros_like(v), S
+
+
+def make(B, T, H, Hk, dk, dv, dtype, decay="token", state=True, lengths=None, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed + 1000 * T + dk)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=gen)  # noqa: E731
+    x = {"q": r(B, T, Hk, dk).to(dtype), "k": r(B, T, Hk, dk).to(dtype), "v": r(B, T, H, dv).to(dtype)}
+    if decay == "head":
+        x["log_decay"] = -torch.exp2(-1.0 - 7.0 * torch.rand(H, device="cuda", generator=gen))
+    else:
+        x["log_decay"] = -torch.nn.functional.softplus(r(B, T, H) * 2 - 2)
+    x["state"] = r(B, H, dk, dv) if state else None
+    x["lengths"] = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    return x
+
+
+def truth(x, scale, ends=None):
+    """(out, state[, gradients of what requires them]) in 64 bits, and the same of absolute values."""
+    got = []
+    for take in (lambda t: t, torch.abs):
+        leaves = {n: (take(t.detach().double()) if n not in ("lengths", "log_decay") else
+                      t.detach().double() if n == "log_decay" else t) if t is not None else None
+                  for n, t in x.items()}
+        if ends is not None:
+            for n, t in leaves.items():
+                if t is not None and n != "lengths":
+                    t.requires_grad_()
+        out, state = recurrence(**leaves, scale=scale)
+        res = [out, state]
+        if ends is not None:
+            into = [t for n, t in leaves.items() if t is not None and n != "lengths"]
+            outs = [(o, take(e.double())) for o, e in zip((out, state), ends) if e is not None]
+            res += torch.autograd.grad([o for o, _ in outs], into, [e for _, e in outs], allow_unused=True,
+                                       materialize_grads=True)
+        got.append([t.detach() for t in res])
+    return got
+
+
+def near(got, want, most, dtype, rough):
+    """rough: roundings to bf16 between products."""
+    assert got.dtype == dtype and got.shape == want.shape
+    e = torch.finfo(dtype).eps / 2
+    bound = ((2.0 ** -8 if rough else 0.0) + FINE) * most
+    tiny = torch.finfo(dtype).smallest_normal * e  # half a step below the normal numbers
+    bad = ~((got.double() - want).abs() <= bound + e * (want.abs() + bound) + tiny).flatten()
+    if bad.any():
+        at = bad.nonzero()[:4, 0]
+        pytest.fail(f"{int(bad.sum())} of {got.numel()}: at {at.tolist()} {got.flatten()[at].tolist()} for "
+                    f"{want.flatten()[at].tolist()}, bound {bound.flatten()[at].tolist()}")
+    if want.numel() >= 4096 and want.norm() > 0:
+        # as independent roundings (at most 2^-8 / sqrt 3 for each value and each of two stages) add up
+        far = float((got.double() - want).norm() / want.norm())
+        assert far <= (2.0 ** -8 if dtype == torch.bfloat16 else e + 2.0 ** -15), far
+
+
+SIZES = [(1, 1, 1, 1, 1, 1), (2, 3, 2, 1, 5, 7), (1, 64, 2, 2, 64, 64), (2, 65, 3, 3, 64, 48), (1, 63, 1, 1, 33, 17),
+         (2, 130, 4, 2, 64, 64), (1, 31, 2, 1, 128, 128), (2, 97, 3, 1, 72, 127), (1, 200, 2, 1, 16, 100),
+         (1, 700, 3, 3, 64, 32), (2, 1100, 2, 1, 40, 72), (1, 1000, 2, 2, 128, 128), (1, 515, 1, 1, 9, 3),
+         (5, 70, 100, 50, 8, 8)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,H,Hk,dk,dv", SIZES)
+def test_outputs_and_states(kernels, B, T, H, Hk, dk, dv, dtype):
+    for n, (decay, state) in enumerate((("token", True), ("head", False))):
+        x = make(B, T, H, Hk, dk, dv, dtype, decay, state, seed=n)
+        got = kernels.linear_attention(**x, scale=0.3)
+        (out, S), (mo, ms) = truth(x, 0.3)
+        near(got[0], out, mo, dtype, dtype == torch.bfloat16)
+        near(got[1], S, ms, torch.float32, False)
+
+
+def gradients(kernels, x, scale, ends):
+    leaves = {n: t.detach().clone().requires_grad_() if t is not None and n != "lengths" else t for n, t in x.items()}
+    out = kernels.linear_attention(**leaves, scale=scale)
+    into = [t for n, t in leaves.items() if t is not None and n != "lengths"]
+    outs = [(o, e) for o, e in zip(out, ends) if e is not None]
+    return [t.detach() for t in out] + list(torch.autograd.grad([o for o, _ in outs], into, [e for _, e in outs]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,H,Hk,dk,dv", SIZES)
+def test_gradients(kernels, B, T, H, Hk, dk, dv, dtype):
+    for n, (decay, state) in enumerate((("token", True), ("head", False))):
+        x = make(B, T, H, Hk, dk, dv, dtype, decay, state, seed=n)
+        gen = torch.Generator(device="cuda").manual_seed(7)
+        ends = (torch.randn(B, T, H, dv, device="cuda", generator=gen).to(dtype),
+                torch.randn(B, H, dk, dv, device="cuda", generator=gen) if state else None)
+        got = gradients(kernels, x, 0.3, ends)
+        want, most = truth(x, 0.3, ends)
+        rough = dtype == torch.bfloat16
+        kinds = [(dtype, rough), (torch.float32, False)] + [(dtype, rough)] * 3 + [(torch.float32, False)] * 2
+        for g, w, m, (kind, coarse) in zip(got, want, most, kinds):
+            near(g, w, m, kind, coarse)
+
+
+def test_gradients_against_differences(kernels):
+    """Central differences of the 64-bit recurrence along random directions; the
+    sum's error is that of near(), the differences' own below 1e-8 of it."""
+    x = make(1, 150, 2, 1, 24, 40, torch.float32)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    ends = (torch.randn(1, 150, 2, 40, device="cuda", generator=gen), torch.randn(1, 2, 24, 40, device="cuda", generator=gen))
+    got = gradients(kernels, x, 0.3, ends)[2:]
+    _, most = truth(x, 0.3, ends)
+    wide = {n: t.double() if t is not None else None for n, t in x.items()}
+    loss = lambda y: sum(float((o * e.double()).sum()) for o, e in zip(recurrence(**y, scale=0.3), ends))  # noqa: E731
+    for (n, g), m in zip(zip(("q", "k", "v", "log_decay", "state"), got), most[2:]):
+        way = torch.randn(g.shape, device="cuda", generator=gen, dtype=torch.float64)
+        h = 1e-5
+        diff = (loss({**wide, n: wide[n] + h * way}) - loss({**wide, n: wide[n] - h * way})) / (2 * h)
+        assert abs(diff - float((g.double() * way).sum())) <= 2 * FINE * float((m * way.abs()).sum()), n
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,lengths", [(100, [100, 64, 1, 0, 65]), (1300, [1300, 600, 0, 513, 1024])])
+def test_padded_batches(kernels, T, lengths, dtype):
+    """What lies behind a sequence's end is not read: NaN there leaves no trace."""
+    x = make(5, T, 2, 1, 64, 32, dtype, lengths=lengths)
+    ends = (torch.randn(5, T, 2, 32, device="cuda").to(dtype), torch.randn(5, 2, 64, 32, device="cuda"))
+    want, most = truth(x, 0.2, ends)
+    behind = torch.arange(T, device="cuda") >= x["lengths"][:, None]
+    for n in ("q", "k", "v", "log_decay"):
+        x[n][behind] = float("nan")
+    ends[0][behind] = float("nan")
+    got = gradients(kernels, x, 0.2, ends)
+    rough = dtype == torch.bfloat16
+    for g, w, m, (kind, coarse) in zip(got, want, most, [(dtype, rough), (torch.float32, False)] + [(dtype, rough)] * 3 +
+                                       [(torch.float32, False)] * 2):
+        near(g, w, m, kind, coarse)
+    for g in (got[0], *got[2:6]):
+        assert (g[behind] == 0).all()
+
+
+@pytest.mark.parametrize("T", [40, 900])
+def test_decays_that_forget(kernels, T):
+    """Minus infinity begins anew: several sequences in one row give what each alone gives."""
+    x = make(1, T, 3, 3, 64, 64, torch.float32, state=False)
+    cuts = [0, 1, 7, T // 2, T // 2 + 1, T - 3]
+    for c in cuts:
+        x["log_decay"][:, c] = -float("inf")
+    x["log_decay"][:, 3] = -1e30
+    x["log_decay"][:, 5] = 0.0
+    x["state"] = torch.randn(1, 3, 64, 64, device="cuda")  # forgotten at once
+    out, S = kernels.linear_attention(**x, scale=1.0)
+    cuts.insert(2, 3)
+    for a, b in zip(cuts, cuts[1:] + [T]):
+        part = {n: x[n][:, a:b] for n in ("q", "k", "v", "log_decay")}
+        part["log_decay"] = part["log_decay"].clamp_min(-1e4)
+        (o, s), (mo, ms) = truth({**part, "state": None, "lengths": None}, 1.0)
+        near(out[:, a:b], o, mo, torch.float32, False)
+    near(S, s, ms, torch.float32, False)
+    # near tokens keep their weight exactly however far the sum of decays is from zero
+    x["log_decay"][:] = -40.0
+    x["log_decay"][:, 20] = 0.0
+    out, _ = kernels.linear_attention(**x, scale=1.0)
+    (o, _), (mo, _) = truth(x, 1.0)
+    near(out, o, mo, torch.float32, False)
+
+
+def test_values_without_finite_numbers_stay_in_their_place(kernels):
+    """A NaN in v reaches its own column of what comes after it, and nothing before."""
+    x = make(1, 200, 2, 2, 64, 64, torch.float32, state=False)
+    clean, _ = kernels.linear_attention(**x)
+    x["v"][0, 130, 1, 5] = float("nan")
+    out, S = kernels.linear_attention(**x)
+    assert out[0, 130:, 1, 5].isnan().all() and S[0, 1, :, 5].isnan().all()
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    hit[0, 128:, 1] = True  # (the chunk of the token shares its products' rows)
+    assert torch.equal(out[~hit], clean[~hit])
+    assert not out[0, :130].isnan().any() and not out[0, :, 0].isnan().any()
+
+
+def test_layouts(kernels):
+    """Views of one projection, of transposed tensors, at odd addresses, broadcast ones."""
+    for dtype in DTYPES:
+        for dk, dv, off in ((64, 64, 0), (64, 64, 1), (24, 40, 3), (33, 65, 0)):
+            wide = torch.randn(2, 300, off + 2 * 2 * dk + 4 * dv, device="cuda").to(dtype)
+            q, k, v = wide[..., off:].split([2 * dk, 2 * dk, 4 * dv], 2)
+            x = {"q": q.unflatten(2, (2, dk)), "k": k.unflatten(2, (2, dk)), "v": v.unflatten(2, (4, dv)),
+                 "log_decay": -torch.rand(300, 4, 2, device="cuda").permute(2, 0, 1), "state": None, "lengths": None}
+            x["state"] = torch.randn(2, dk, dv, 4, device="cuda").permute(0, 3, 1, 2)
+            whole = {n: t.contiguous() if t is not None else None for n, t in x.items()}
+            for a, b in zip(kernels.linear_attention(**x), kernels.linear_attention(**whole)):
+                assert torch.equal(a, b)
+            x["q"] = whole["q"].transpose(1, 3).contiguous().transpose(1, 3)
+            x["k"] = whole["k"][:1, :1].expand(2, 300, 2, dk)
+            whole["k"] = x["k"].contiguous()
+            for a, b in zip(kernels.linear_attention(**x), kernels.linear_attention(**whole)):
+                assert torch.equal(a, b)
+    x = make(2, 200, 2, 2, 64, 64, torch.bfloat16)
+    base = gradients(kernels, x, 0.1, (torch.ones(2, 200, 2, 64, device="cuda", dtype=torch.bfloat16), None))
+    same = gradients(kernels, x, 0.1, (torch.ones((), device="cuda", dtype=torch.bfloat16).expand(2, 200, 2, 64), None))
+    assert all(torch.equal(a, b) for a, b in zip(base, same))
+
+
+def test_nothing_to_do(kernels):
+    x = make(2, 0, 3, 1, 8, 16, torch.float32)
+    out, S = kernels.linear_attention(**x)
+    assert out.shape == (2, 0, 3, 16) and torch.equal(S, x["state"])
+    got = gradients(kernels, x, 1.0, (out, torch.ones_like(S)))
+    assert torch.equal(got[-1], torch.ones_like(S)) and got[2].shape == (2, 0, 1, 8)
+    x = make(0, 5, 3, 1, 8, 16, torch.float32, decay="head")
+    out, S = kernels.linear_attention(**x)
+    assert out.shape == (0, 5, 3, 16) and S.shape == (0, 3, 8, 16)
+    got = gradients(kernels, x, 1.0, (out, None))
+    assert torch.equal(got[-2], torch.zeros(3, device="cuda"))
+    assert kernels.linear_attention_step(x["q"][:, 0], x["k"][:, 0], x["v"][:, 0], x["log_decay"], S).shape == (0, 3, 16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,Hk,dk,dv", [(1, 12, 12, 64, 64), (3, 4, 2, 128, 128), (5, 3, 1, 7, 33), (2, 2, 2, 1, 1),
+                                          (300, 2, 1, 40, 72), (2, 3, 3, 100, 4), (4, 1, 1, 128, 2)])
+def test_single_tokens(kernels, B, H, Hk, dk, dv, dtype):
+    """fp32 throughout: a state takes three roundings and the decay's 2^-21 a token,
+    an output a sum of dk more."""
+    x = make(B, 6, H, Hk, dk, dv, dtype)
+    wide = torch.randn(B, 2, H, dk, dv, device="cuda")
+    wide[:, 0] = x["state"]
+    S, other = wide[:, 0], wide[:, 1].clone()
+    want, most = truth(x, 0.3)
+    for t in range(6):
+        at = lambda n: x[n][:, t]  # noqa: B023,E731
+        out = kernels.linear_attention_step(at("q"), at("k"), at("v"), at("log_decay"), S, 0.3)
+        err = (dk + 40) * 2.0 ** -24 + 6 * 2.0 ** -21
+        e = torch.finfo(dtype).eps / 2
+        assert out.dtype == dtype
+        far = (out.double() - want[0][:, t]).abs()
+        assert (far <= err * most[0][:, t] + e * (want[0][:, t].abs() + err * most[0][:, t])).all()
+    assert ((S.double() - want[1]).abs() <= 6 * (2.0 ** -22 + 2.0 ** -21) * most[1]).all()
+    assert torch.equal(wide[:, 1], other)
+    # one decay for each head, and one that forgets
+    head = torch.full((H,), -0.5, device="cuda")
+    head[0] = -float("inf")
+    before = S.double().clone()
+    kernels.linear_attention_step(x["q"][:, 0], x["k"][:, 0], x["v"][:, 0], head, S, 0.3)
+    k, v = x["k"][:, 0].double().repeat_interleave(H // Hk, 1), x["v"][:, 0].double()
+    to = before * head.double().exp()[:, None, None] + k[..., None] * v[:, :, None]
+    assert ((S.double() - to).abs() <= 2.0 ** -20 * (before.abs() + (k[..., None] * v[:, :, None]).abs())).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_prompt_in_parts_and_its_next_tokens(kernels, dtype):
+    """A whole prompt; in three parts, the state handed on; by single tokens."""
+    x = make(2, 700, 4, 2, 64, 64, dtype)
+    x["lengths"] = None
+    want, most = truth(x, 0.2)
+    S, outs = x["state"], []
+    for a, b in ((0, 1), (1, 333), (333, 690)):
+        part = {n: x[n][:, a:b] for n in ("q", "k", "v", "log_decay")}
+        out, S = kernels.linear_attention(**part, state=S, scale=0.2)
+        outs.append(out)
+    for t in range(690, 700):
+        outs.append(kernels.linear_attention_step(*(x[n][:, t] for n in ("q", "k", "v", "log_decay")), S, 0.2)[:, None])
+    near(torch.cat(outs, 1), want[0], most[0], dtype, dtype == torch.bfloat16)
+    near(S, want[1], most[1], torch.float32, False)
+
+
+def test_same_bits_captured_and_on_other_streams(kernels):
+    xs = [make(1, 1500, 3, 3, 64, 64, torch.bfloat16, seed=n) for n in range(2)]
+    want = [kernels.linear_attention(**x) for x in xs]
+    again = kernels.linear_attention(**xs[0])
+    assert all(torch.equal(a, b) for a, b in zip(want[0], again))
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for x in xs:  # two graphs, run at the same time: each has its own workspace
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(kernels.linear_attention(**x))
+        graphs.append(g)
+    for _ in range(3):
+        for pair in got:
+            for t in pair:
+                t.zero_()
+        torch.cuda.synchronize()
+        sides = [torch.cuda.Stream() for _ in graphs]
+        for g, s in zip(graphs, sides):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    ends = (torch.ones_like(want[0][0]), None)
+    first = gradients(kernels, xs[0], 1.0, ends)
+    for a, b in zip(first, gradients(kernels, xs[0], 1.0, ends)):
+        assert torch.equal(a, b)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = gradients(kernels, xs[0], 1.0, ends)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, other))
+
+
+def test_only_once_differentiable_and_versions(kernels):
+    x = make(1, 10, 2, 2, 8, 8, torch.float32)
+    x["q"].requires_grad_()
+    out, S = kernels.linear_attention(**x)
+    (dq,) = torch.autograd.grad(out.sum(), x["q"], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.sum(), x["q"])
+    state = torch.zeros(1, 2, 8, 8, device="cuda")
+    w = torch.ones(1, 2, 8, 8, device="cuda", requires_grad=True)
+    y = (w * state).sum()
+    kernels.linear_attention_step(x["q"].detach()[:, 0], x["k"][:, 0], x["v"][:, 0], x["log_decay"][:, 0], state)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+
+
+def test_refusals_on_the_gpu(kernels):
+    x = make(2, 5, 4, 2, 8, 16, torch.float32)
+    for change in ({"q": x["q"][:, :4]}, {"k": x["k"][..., :7]}, {"v": x["v"][:, :, :3]}, {"q": x["q"].bfloat16()},
+                   {"v": x["v"].cpu()}, {"log_decay": x["log_decay"].double()}, {"log_decay": x["log_decay"][:, :1]},
+                   {"log_decay": x["log_decay"].cpu()}, {"state": x["state"][:1]}, {"state": x["state"].bfloat16()},
+                   {"lengths": torch.ones(2, device="cuda")}, {"lengths": torch.ones(3, dtype=torch.int32, device="cuda")},
+                   {"q": torch.zeros(2, 5, 2, 129, device="cuda"), "k": torch.zeros(2, 5, 2, 129, device="cuda"), "state": None}):
+        with pytest.raises((ValueError, TypeError)):
+            kernels.linear_attention(**{**x, **change})
+    s = {n: x[n][:, 0] for n in ("q", "k", "v", "log_decay")}
+    for state in (x["state"].bfloat16(), x["state"][:1], x["state"].cpu(), x["state"].transpose(2, 3).contiguous().transpose(2, 3),
+                  x["state"].clone().requires_grad_()):
+        with pytest.raises((ValueError, RuntimeError)):
+            kernels.linear_attention_step(**s, state=state)
+    from sunnynet_b200._lib import SnError
+    with pytest.raises(SnError, match="overlap"):
+        kernels.linear_attention_step(**s, state=x["state"][:1].expand(2, 4, 8, 16))
