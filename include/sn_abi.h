@@ -331,6 +331,44 @@ sn_status sn_abi_linear_attention_bwd(const SnAbiLinearAttention* a, const void*
 sn_status sn_abi_linear_attention_step(const SnAbiLinearAttention* a, float* state,
                                        int64_t state_stride, void* out, void* cuda_stream);
 
+/* Rows of an embedding (SN_CAP_TRAIN): out[i] = scale * W[token_i], n rows of D
+ * values, contiguous; W (V, D) with rows `ld` values apart, both of `dtype`;
+ * tokens int32 or int64 (token_bits). A token outside [0, V) gives a row of NaN.
+ * Its gradient: dW[v] = scale * the sum of dout[i] over token_i = v, in fp32 and
+ * in the order of i; dW (V, D) contiguous, overwritten; dout with rows `ld`
+ * values apart. The same call gives the same bits. */
+sn_status sn_abi_embedding(const void* tokens, int32_t token_bits, int64_t n, const void* W,
+                           int64_t ld, int64_t V, int32_t D, int32_t dtype, float scale, void* out,
+                           void* cuda_stream);
+int64_t   sn_abi_embedding_bwd_ws(int64_t n, int64_t V, int32_t D);
+sn_status sn_abi_embedding_bwd(const void* tokens, int32_t token_bits, int64_t n, const void* dout,
+                               int64_t ld, int64_t V, int32_t D, int32_t dtype, float scale, void* dW,
+                               void* ws, int64_t ws_bytes, void* cuda_stream);
+
+/* The norm of all values of `count` tensors (SN_CAP_TRAIN): lists (in host
+ * memory) of device addresses, sizes and types (SN_F32, SN_BF16, SN_F16, mixed
+ * at will). norm = sqrt(sum of squares), factor = min(1, max_norm / (norm +
+ * 1e-6)), each one fp32 value on the GPU or NULL; a NaN among the values makes
+ * both NaN. clip_grads also multiplies every value by the factor in place
+ * (where it is 1, nothing is written); no tensor may then appear twice or
+ * overlap another. The same call gives the same bits. */
+int64_t   sn_abi_grad_norm_ws(int32_t count, const int64_t* sizes);
+sn_status sn_abi_grad_norm(int32_t count, const void* const* grads, const int64_t* sizes,
+                           const int32_t* dtypes, double max_norm, float* norm, float* factor,
+                           void* ws, int64_t ws_bytes, void* cuda_stream);
+sn_status sn_abi_clip_grads(int32_t count, void* const* grads, const int64_t* sizes,
+                            const int32_t* dtypes, double max_norm, float* norm, float* factor,
+                            void* ws, int64_t ws_bytes, void* cuda_stream);
+/* sn_abi_adamw_step with every gradient multiplied by *grad_scale (one fp32
+ * value on the GPU, such as the factor above) as it is read. */
+sn_status sn_abi_adamw_step_scaled(int32_t count, void* const* params, const void* const* grads,
+                                   void* const* avg, void* const* sq, float* const* avg_scale,
+                                   float* const* sq_scale, const int64_t* sizes, int32_t dtype,
+                                   int32_t grad_dtype, int32_t state_bits, int64_t step,
+                                   const int64_t* step_dev, double lr, const double* lr_dev,
+                                   double beta1, double beta2, double eps, double weight_decay,
+                                   const float* grad_scale, void* cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

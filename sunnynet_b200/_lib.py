@@ -81,6 +81,14 @@ SIGNATURES = {
     "sn_abi_adamw_step": (I32, [I32, V, V, V, V, V, V, V, I32, I32, I32, I64, V, F64, V, F64, F64,
                                 F64, F64, V]),
     "sn_abi_sample": (I32, [V, I64, I32, V, I32, V, F64, V, I32, V, F64, V, F64, I32, I32, V, V]),
+    "sn_abi_embedding": (I32, [V, I32, I64, V, I64, I64, I32, I32, F32, V, V]),
+    "sn_abi_embedding_bwd_ws": (I64, [I64, I64, I32]),
+    "sn_abi_embedding_bwd": (I32, [V, I32, I64, V, I64, I64, I32, I32, F32, V, V, I64, V]),
+    "sn_abi_grad_norm_ws": (I64, [I32, V]),
+    "sn_abi_grad_norm": (I32, [I32, V, V, V, F64, V, V, V, I64, V]),
+    "sn_abi_clip_grads": (I32, [I32, V, V, V, F64, V, V, V, I64, V]),
+    "sn_abi_adamw_step_scaled": (I32, [I32, V, V, V, V, V, V, V, I32, I32, I32, I64, V, F64, V, F64,
+                                       F64, F64, F64, V, V]),
     "sn_abi_linear_attention_ws": (I64, [V, I32, I32]),
     "sn_abi_linear_attention": (I32, [V, V, V, V, I64, V]),
     "sn_abi_linear_attention_bwd": (I32, [V, V, V, V, V, V, V, V, I32, V, V, I64, V]),

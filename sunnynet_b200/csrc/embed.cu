@@ -1,0 +1,534 @@
+// The rows of an embedding for given tokens, scaled, and the gradient of the
+// embedding (no counterpart among the reference's kernels: its decode copies one
+// row a step, its training loop leaves both to torch).
+//
+//   out[i] = scale * W[token_i]        dW[v] = scale * sum of dout[i] over token_i = v
+//
+// Forward: a copy, bound by HBM. A token outside the vocabulary gives a row of
+// NaN, and no gradient: the device has no other way to tell.
+//
+// Gradient: the tokens are sorted by a stable radix sort of eight bits a pass
+// (two launches each: the counts of every tile, then ranks and places), so that
+// each row's tokens lie side by side in their order and are added in it: the
+// same bits every time, no atomics. Bound by HBM (dout read, dW written once) from some
+// ten thousand tokens on, and by the launches below. While they sort, further
+// CTAs of the same launches fill dW with zeros, which costs nothing then: most
+// rows of a vocabulary occur in no batch, and those that do are overwritten.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "caller.cuh"
+#include "ptx.cuh"
+#include "runtime.cuh"
+
+namespace sn {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ float to_f(T x) {
+    if constexpr (sizeof(T) == 4)
+        return x;
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        return __bfloat162float(x);
+    else
+        return __half2float(x);
+}
+template <typename T>
+__device__ __forceinline__ T from_f(float x) {
+    if constexpr (sizeof(T) == 4)
+        return x;
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        return __float2bfloat16_rn(x);
+    else
+        return __float2half_rn(x);
+}
+
+// N values of T, read and written at once.
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+    T v[N];
+};
+
+// x / d for x < 2^31, by one product.
+struct Divide {
+    unsigned d, mul, shift;
+    explicit Divide(unsigned n = 1) : d(n), mul(0), shift(0) {
+        while ((1ull << shift) < n) ++shift;
+        mul = (unsigned)(((1ull << 32) * ((1ull << shift) - n)) / n + 1);
+    }
+    __device__ __forceinline__ unsigned of(unsigned x) const { return (__umulhi(x, mul) + x) >> shift; }
+};
+
+// The row of token i, or -1.
+__device__ __forceinline__ long long row_of(const void* tokens, bool wide, long long i, long long V) {
+    const long long t = wide ? static_cast<const long long*>(tokens)[i] : static_cast<const int*>(tokens)[i];
+    return t >= 0 && t < V ? t : -1;
+}
+
+// ----------------------------------------------------------------- forward
+constexpr int kThreads = 256;
+
+// A CTA copies `rows` rows of `packs` packs, a thread U packs at a time.
+template <typename T, int N, int U>
+__global__ void __launch_bounds__(kThreads)
+rows_kernel(const void* tokens, bool wide, const T* W, long long ld, long long V, T* out, long long n, int D,
+            unsigned rows, unsigned packs, Divide by, float scale) {
+    const long long first = blockIdx.x * (long long)rows;
+    const unsigned todo = (unsigned)min((long long)rows, n - first) * packs;
+    for (unsigned i0 = threadIdx.x; i0 < todo; i0 += U * kThreads) {
+        Pack<T, N> x[U];
+        long long row[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const unsigned i = i0 + u * kThreads, r = by.of(i);
+            row[u] = i < todo ? row_of(tokens, wide, first + r, V) : -1;
+            if (row[u] >= 0)
+                x[u] = *reinterpret_cast<const Pack<T, N>*>(W + row[u] * ld + (i - r * packs) * N);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const unsigned i = i0 + u * kThreads, r = by.of(i);
+            if (i >= todo) break;
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                x[u].v[k] = from_f<T>(row[u] >= 0 ? to_f(x[u].v[k]) * scale : __int_as_float(0x7fffffff));
+            *reinterpret_cast<Pack<T, N>*>(out + (first + r) * D + (i - r * packs) * N) = x[u];
+        }
+    }
+}
+
+// -------------------------------------------------------------------- sort
+constexpr int kTiles = 148;  // at most: a tile of the tokens for each SM
+constexpr int kBins = 256;
+
+struct Sorting {
+    const void* tokens;  // of the first pass
+    bool wide;
+    long long V;
+    const uint2* from;  // of the others: token and place
+    uint2* to;
+    int* counts;  // tiles x kBins
+    int n, tiles, per, shift;
+    float4* zeros;  // what further CTAs fill
+    long long zero_packs;
+};
+
+__device__ __forceinline__ uint2 entry(const Sorting& s, int i) {
+    if (s.from) return s.from[i];
+    const long long r = row_of(s.tokens, s.wide, i, s.V);
+    return make_uint2((unsigned)(r < 0 ? s.V : r), (unsigned)i);  // strangers behind all others
+}
+
+__device__ __forceinline__ void fill_zeros(const Sorting& s) {
+    const long long ctas = gridDim.x - s.tiles;
+    for (long long i = (blockIdx.x - s.tiles) * (long long)blockDim.x + threadIdx.x; i < s.zero_packs;
+         i += ctas * blockDim.x)
+        s.zeros[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+}
+
+__global__ void __launch_bounds__(1024) count_kernel(const Sorting s) {
+    pdl_trigger();
+    if (blockIdx.x >= (unsigned)s.tiles) return fill_zeros(s);  // (dW is this call's own since its first launch)
+    __shared__ int count[kBins];
+    for (int i = threadIdx.x; i < kBins; i += blockDim.x) count[i] = 0;
+    __syncthreads();
+    pdl_wait();
+    const int lo = blockIdx.x * s.per, hi = min(s.n, lo + s.per);
+    for (int i = lo + threadIdx.x; i < hi; i += blockDim.x) atomicAdd(&count[entry(s, i).x >> s.shift & (kBins - 1)], 1);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBins; i += blockDim.x) s.counts[blockIdx.x * kBins + i] = count[i];
+}
+
+// A thread for each of the tile's tokens, WARPS * 32 at a time, in their order.
+template <int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) place_kernel(const Sorting s) {
+    pdl_trigger();
+    if (blockIdx.x >= (unsigned)s.tiles) return fill_zeros(s);
+    constexpr int PARTS = WARPS * 32 / kBins;
+    __shared__ int at[kBins], part[PARTS][kBins][2], warp_sum[kBins / 32];
+    __shared__ int seen[WARPS][kBins];  // of a warp, in this round
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bin = tid % kBins;
+    for (int i = tid; i < WARPS * kBins; i += WARPS * 32) (&seen[0][0])[i] = 0;
+    pdl_wait();
+    // where this tile's tokens of each bin begin: behind those of lower bins, and of earlier tiles
+    {
+        int all = 0, before = 0;
+#pragma unroll 8
+        for (int t = tid / kBins; t < s.tiles; t += PARTS) {
+            const int c = s.counts[t * kBins + bin];
+            all += c;
+            before += t < (int)blockIdx.x ? c : 0;
+        }
+        part[tid / kBins][bin][0] = all;
+        part[tid / kBins][bin][1] = before;
+        __syncthreads();
+        int sum = 0;
+        if (tid < kBins) {
+            all = before = 0;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) all += part[p][tid][0], before += part[p][tid][1];
+            sum = all;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int y = __shfl_up_sync(0xffffffffu, sum, d);
+                if (lane >= d) sum += y;
+            }
+            if (lane == 31) warp_sum[warp] = sum;
+        }
+        __syncthreads();
+        if (tid < kBins) {
+            for (int w = 0; w < warp; ++w) sum += warp_sum[w];
+            at[tid] = sum - all + before;
+        }
+        __syncthreads();
+    }
+    const int lo = blockIdx.x * s.per, hi = min(s.n, lo + s.per);
+    for (int base = lo; base < hi; base += WARPS * 32) {
+        const int i = base + tid;
+        const bool in = i < hi;
+        const uint2 e = in ? entry(s, i) : make_uint2(0, 0);
+        const unsigned d = e.x >> s.shift & (kBins - 1);
+        const unsigned peers = __match_any_sync(0xffffffffu, in ? d : kBins);
+        const int rank = __popc(peers & ((1u << lane) - 1));
+        if (in && rank == 0) seen[warp][d] = __popc(peers);
+        __syncthreads();
+        if (tid < kBins) {  // counts of the warps become their first places
+            int next = at[tid];
+#pragma unroll 8
+            for (int w = 0; w < WARPS; ++w) {
+                const int c = seen[w][tid];
+                seen[w][tid] = next;
+                next += c;
+            }
+            at[tid] = next;
+        }
+        __syncthreads();
+        if (in) s.to[seen[warp][d] + rank] = e;
+        __syncthreads();
+        if (base + WARPS * 32 < hi)
+            for (int j = tid; j < WARPS * kBins; j += WARPS * 32) (&seen[0][0])[j] = 0;
+        __syncthreads();
+    }
+}
+
+// --------------------------------------------------------------------- sums
+// The sorted tokens in chunks of `per`. A row whose tokens are at most `per`
+// belongs to the chunk in which they begin, and is written by it; those of a
+// longer one are summed up to each chunk's border and joined by a second
+// kernel: a piece that began in its chunk lies in slot 2 c + 1, one that goes
+// on in it from the last in slot 2 c.
+constexpr int kMaxChunk = 512;
+constexpr int kColumns = 128;  // threads of a CTA, each with a pack of columns
+
+struct Summing {
+    const uint2* sorted;
+    int n, per;
+    long long V, ld;
+    int D;
+    float* pieces;  // slots x D
+    float scale;
+};
+
+// Whether sorted token i exists and is of row r.
+__device__ __forceinline__ bool is(const Summing& s, long long i, unsigned r) {
+    return i < s.n && s.sorted[i].x == r;
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kColumns) sum_kernel(const Summing s, const T* dout, T* dW) {
+    pdl_trigger();
+    pdl_wait();
+    extern __shared__ uint2 window[];  // sorted tokens [a - per, b + per + 1)
+    __shared__ int first_, last_;
+    const int per = s.per, a = blockIdx.x * per, b = min(s.n, a + per), w0 = max(0, a - per);
+    const int w1 = (int)min((long long)s.n, (long long)b + per + 1);
+    for (int i = w0 + threadIdx.x; i < w1; i += kColumns) window[i - w0] = s.sorted[i];
+    if (threadIdx.x == 0) first_ = a, last_ = b;
+    __syncthreads();
+    const auto key = [&](int i) { return window[i - w0].x; };
+    // where the tokens of the row of token i (in the chunk) begin, or a - per
+    const auto begin_of = [&](int i) {
+        const unsigned r = key(i);
+        int lo = w0, hi = i;  // the first of r in [w0, i]
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (key(mid) >= r)
+                hi = mid;
+            else
+                lo = mid + 1;
+        }
+        return lo;
+    };
+    const auto long_row = [&](int begin, unsigned r) { return (long long)begin + per < w1 && key(begin + per) == r; };
+    const unsigned ra = key(a), rb = key(b - 1);
+    const bool on = a > 0 && key(a - 1) == ra;  // the first row began before
+    const int sa = begin_of(a), sb = begin_of(b - 1);
+    // (where it began at or before w0 > 0, token a itself is `per` behind w0: long)
+    const bool long_a = long_row(sa, ra), long_b = long_row(sb, rb);
+    if (on && !long_a)
+        for (int i = a + threadIdx.x; i < w1; i += kColumns)
+            if (key(i) != ra && key(i - 1) == ra) first_ = i;
+    if (on && !long_a && threadIdx.x == 0 && key(w1 - 1) == ra) first_ = w1;  // none behind it
+    if (b < s.n && key(b) == rb && !long_b)
+        for (int i = b + threadIdx.x; i < w1; i += kColumns)
+            if (key(i - 1) == rb && (i + 1 == w1 || key(i + 1) != rb) && key(i) == rb) last_ = i + 1;
+    __syncthreads();
+    const int first = first_, last = last_;
+    const bool cut = b < s.n && key(b) == rb && long_b;  // the last row goes on behind
+    const int col = (blockIdx.y * kColumns + threadIdx.x) * N;
+    if (first >= b || col >= s.D) return;
+    // (a short row's tokens behind b are this chunk's only if they begin in it)
+    constexpr int U = 8;
+    float sum[N] = {};
+    for (int i0 = first; i0 < last; i0 += U) {
+        Pack<T, N> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u < last && key(i0 + u) < s.V)
+                x[u] = *reinterpret_cast<const Pack<T, N>*>(dout + (long long)window[i0 + u - w0].y * s.ld + col);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u;
+            if (i >= last) break;
+            const unsigned r = key(i);
+            if (r >= s.V) break;
+#pragma unroll
+            for (int k = 0; k < N; ++k) sum[k] += to_f(x[u].v[k]);
+            if (i + 1 < last && key(i + 1) == r) continue;
+            // the row's last token in this chunk
+            const bool head = on && long_a && r == ra, tail = cut && r == rb;
+            if (head || tail) {
+                float* to = s.pieces + (2ll * blockIdx.x + (head ? 0 : 1)) * s.D + col;
+#pragma unroll
+                for (int k = 0; k < N; ++k) to[k] = sum[k];
+            } else {
+                Pack<T, N> y;
+#pragma unroll
+                for (int k = 0; k < N; ++k) y.v[k] = from_f<T>(sum[k] * s.scale);
+                *reinterpret_cast<Pack<T, N>*>(dW + (long long)r * s.D + col) = y;
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k) sum[k] = 0.0f;
+        }
+    }
+}
+
+// The pieces of the long row that begins in this chunk, if one does.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_kernel(const Summing s, T* dW) {
+    pdl_wait();
+    const int per = s.per, a = blockIdx.x * per, b = a + per;
+    if (b >= s.n) return;
+    const unsigned r = s.sorted[b].x;
+    if (r >= s.V || s.sorted[b - 1].x != r || (a > 0 && s.sorted[a - 1].x == r)) return;
+    int lo = a, hi = b - 1;  // where it begins
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (s.sorted[mid].x == r)
+            hi = mid;
+        else
+            lo = mid + 1;
+    }
+    if (!is(s, (long long)lo + per, r)) return;
+    int m0 = blockIdx.x + 1, m1 = (s.n - 1) / per;  // the last chunk whose first token is its
+    while (m0 < m1) {
+        const int mid = (m0 + m1 + 1) >> 1;
+        if (s.sorted[(long long)mid * per].x == r)
+            m0 = mid;
+        else
+            m1 = mid - 1;
+    }
+    for (int col = threadIdx.x; col < s.D; col += kThreads) {
+        float sum = s.pieces[(2ll * blockIdx.x + 1) * s.D + col];
+#pragma unroll 8
+        for (int c = blockIdx.x + 1; c <= m0; ++c) sum += s.pieces[2ll * c * s.D + col];
+        dW[(long long)r * s.D + col] = from_f<T>(sum * s.scale);
+    }
+}
+
+template <typename... P, typename... A>
+int launch_behind(void (*kernel)(P...), dim3 ctas, int threads, int smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = ctas;
+    c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    return cuda_check(cudaLaunchKernelEx(&c, kernel, args...), "embedding launch");
+}
+
+// Bytes of the widest access that fits addresses, strides and width.
+int width_of(const void* a, const void* b, long long ld, int D, unsigned e) {
+    int w = 16;
+    while (w > (int)e && ((uintptr_t)a % w || (uintptr_t)b % w || ld * e % w || (long long)D * e % w)) w /= 2;
+    return w;
+}
+
+template <typename F>
+int by_type(int dtype, F&& f) {
+    return dtype == SN_F32 ? f(0.0f) : dtype == SN_BF16 ? f(__nv_bfloat16()) : f(__half());
+}
+// f(type, values of an access)
+template <typename F>
+int by_access(int dtype, int width, F&& f) {
+    return by_type(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        constexpr int E = sizeof(T);
+        if (width == 16) return f(t, std::integral_constant<int, 16 / E>());
+        if (width == 8) return f(t, std::integral_constant<int, 8 / E>());
+        if constexpr (E == 2)
+            if (width == 4) return f(t, std::integral_constant<int, 2>());
+        return f(t, std::integral_constant<int, 1>());
+    });
+}
+
+int check_call(const char* what, int64_t n, int64_t V, int32_t D, int64_t ld, int32_t dtype, float scale) {
+    if (!dtype_size(dtype)) return fail(SN_E_INVAL, "%s: dtype %d", what, dtype);
+    if (n < 0 || V < 0 || D < 0 || n > 0x7fffffffll || V >= 0x7fffffffll || D > 1 << 30)
+        return fail(SN_E_INVAL, "%s: %lld tokens, %lld rows of %d", what, (long long)n, (long long)V, D);
+    if (ld < 0 || ld >= 1ll << 44) return fail(SN_E_INVAL, "%s: rows %lld values apart", what, (long long)ld);
+    if (!std::isfinite(scale)) return fail(SN_E_INVAL, "%s: the scale is not finite", what);
+    return SN_OK;
+}
+
+// How the tokens are cut up, and the workspace in bytes.
+struct Plan {
+    int tiles, per, passes, chunk;
+    long long chunks, list, counts, pieces, bytes;
+};
+Plan plan_of(long long n, long long V, int D) {
+    Plan p;
+    const auto up = [](long long b) { return (b + 255) / 256 * 256; };
+    p.tiles = (int)std::max(1ll, std::min((long long)kTiles, (n + 255) / 256));
+    p.per = (int)((n + p.tiles - 1) / p.tiles);
+    p.passes = 1;
+    while (V >> 8 * p.passes) ++p.passes;  // (V itself marks strangers)
+    // about 14 chunks to an SM, of 16 tokens at least
+    p.chunk = 16;
+    while (p.chunk < kMaxChunk && (n + p.chunk - 1) / p.chunk > 148 * 14) p.chunk *= 2;
+    p.chunks = (n + p.chunk - 1) / p.chunk;
+    p.list = up(n * 8);
+    p.counts = up((long long)p.tiles * kBins * 4);
+    p.pieces = up(p.chunks * 2 * D * 4);
+    p.bytes = 2 * p.list + p.counts + p.pieces;
+    return p;
+}
+
+}  // namespace
+}  // namespace sn
+
+using namespace sn;
+
+extern "C" {
+
+sn_status sn_abi_embedding(const void* tokens, int32_t token_bits, int64_t n, const void* W, int64_t ld, int64_t V,
+                           int32_t D, int32_t dtype, float scale, void* out, void* cuda_stream) {
+    SN_TRY(check_call("embedding", n, V, D, ld, dtype, scale));
+    if (token_bits != 32 && token_bits != 64) return fail(SN_E_INVAL, "embedding: tokens have 32 or 64 bits");
+    if (!n || !D) return SN_OK;
+    if (!tokens || !out || (V && !W)) return fail(SN_E_INVAL, "embedding: null pointer");
+    const unsigned e = dtype_size(dtype);
+    CallerDevice dev;
+    SN_TRY(dev.enter("embedding", {{tokens, (unsigned)token_bits / 8}, {W, e}, {out, e}}));
+    const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+    return by_access(dtype, width_of(W, out, ld, D, e), [&](auto t, auto vec) {
+        typedef decltype(t) T;
+        constexpr int N = decltype(vec)::value;
+        const unsigned packs = (unsigned)(D / N);
+        // four packs of a thread at once where that leaves a CTA for every SM
+        const bool many = n * packs >= 148ll * 4 * kThreads;
+        const unsigned rows = std::max(1u, (many ? 4u : 1u) * kThreads / packs);
+        const unsigned ctas = (unsigned)((n + rows - 1) / rows);
+        auto* kernel = many ? rows_kernel<T, N, 4> : rows_kernel<T, N, 1>;
+        kernel<<<ctas, kThreads, 0, st>>>(tokens, token_bits == 64, static_cast<const T*>(W), ld, V,
+                                          static_cast<T*>(out), n, D, rows, packs, Divide(packs), scale);
+        return cuda_check(cudaGetLastError(), "embedding launch");
+    });
+}
+
+int64_t sn_abi_embedding_bwd_ws(int64_t n, int64_t V, int32_t D) {
+    if (check_call("embedding_bwd_ws", n, V, D, 0, SN_F32, 1.0f) != SN_OK) return -1;
+    return n && V && D ? plan_of(n, V, D).bytes : 0;
+}
+
+sn_status sn_abi_embedding_bwd(const void* tokens, int32_t token_bits, int64_t n, const void* dout, int64_t ld,
+                               int64_t V, int32_t D, int32_t dtype, float scale, void* dW, void* ws,
+                               int64_t ws_bytes, void* cuda_stream) {
+    SN_TRY(check_call("embedding_bwd", n, V, D, ld, dtype, scale));
+    if (token_bits != 32 && token_bits != 64) return fail(SN_E_INVAL, "embedding_bwd: tokens have 32 or 64 bits");
+    if (!V || !D) return SN_OK;
+    if (!dW || (n && (!tokens || !dout))) return fail(SN_E_INVAL, "embedding_bwd: null pointer");
+    const unsigned e = dtype_size(dtype);
+    CallerDevice dev;
+    SN_TRY(dev.enter("embedding_bwd",
+                     {{tokens, n ? (unsigned)token_bits / 8 : 1}, {dout, n ? e : 1}, {dW, e}, {ws, 16}}));
+    const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+    const long long bytes = V * (long long)D * e;
+    if (!n) return cuda_check(cudaMemsetAsync(dW, 0, bytes, st), "embedding_bwd");
+    const Plan p = plan_of(n, V, D);
+    if (!ws || ws_bytes < p.bytes)
+        return fail(SN_E_INVAL, "embedding_bwd: a workspace of %lld bytes is wanted", p.bytes);
+    char* at = static_cast<char*>(ws);
+    uint2* lists[2] = {reinterpret_cast<uint2*>(at), reinterpret_cast<uint2*>(at + p.list)};
+    Sorting s = {};
+    s.tokens = tokens, s.wide = token_bits == 64, s.V = V;
+    s.counts = reinterpret_cast<int*>(at + 2 * p.list);
+    s.n = (int)n, s.tiles = p.tiles, s.per = p.per;
+    // the zeros, a part to each launch; where they do not come in packs, by a launch of their own
+    const bool packed = (uintptr_t)dW % 16 == 0;
+    const long long packs = packed ? bytes / 16 : 0, share = (packs + 2 * p.passes - 1) / (2 * p.passes);
+    if (bytes % 16 || !packed)
+        SN_TRY(cuda_check(cudaMemsetAsync(static_cast<char*>(dW) + packs * 16, 0, bytes - packs * 16, st),
+                          "embedding_bwd"));
+    long long done = 0;
+    const auto zeros = [&] {
+        s.zeros = reinterpret_cast<float4*>(dW) + done;
+        s.zero_packs = std::min(share, packs - done);
+        done += s.zero_packs;
+        return (unsigned)std::min((s.zero_packs + 4095) / 4096, 148ll * 4);
+    };
+    const bool big = p.per >= 512;
+    for (int i = 0; i < p.passes; ++i) {
+        s.shift = 8 * i;
+        s.from = i ? lists[(i - 1) & 1] : nullptr;
+        s.to = lists[i & 1];
+        const int threads = big ? 1024 : 256;
+        if (i == 0) {
+            const unsigned more = zeros();
+            count_kernel<<<p.tiles + more, threads, 0, st>>>(s);
+            SN_TRY(cuda_check(cudaGetLastError(), "embedding launch"));
+        } else {
+            const unsigned more = zeros();
+            SN_TRY(launch_behind(count_kernel, dim3(p.tiles + more), threads, 0, st, s));
+        }
+        const unsigned more = zeros();
+        SN_TRY(launch_behind(big ? place_kernel<32> : place_kernel<8>, dim3(p.tiles + more), threads, 0, st, s));
+    }
+    Summing m = {};
+    m.sorted = lists[(p.passes - 1) & 1];
+    m.n = (int)n, m.per = p.chunk, m.V = V, m.ld = ld, m.D = D;
+    m.pieces = reinterpret_cast<float*>(at + 2 * p.list + p.counts);
+    m.scale = scale;
+    SN_TRY(by_access(dtype, width_of(dout, dW, ld, D, e), [&](auto t, auto vec) {
+        typedef decltype(t) T;
+        constexpr int N = decltype(vec)::value;
+        const unsigned slabs = (unsigned)((D / N + kColumns - 1) / kColumns);
+        return launch_behind(sum_kernel<T, N>, dim3((unsigned)p.chunks, slabs), kColumns, (3 * p.chunk + 1) * 8, st, m,
+                             static_cast<const T*>(dout), static_cast<T*>(dW));
+    }));
+    return by_type(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        return launch_behind(join_kernel<T>, dim3((unsigned)p.chunks), kThreads, 0, st, m, static_cast<T*>(dW));
+    });
+}
+
+}  // extern "C"

@@ -278,8 +278,72 @@ PyObject* read(PyObject*, PyObject* args) {
     }
 }
 
+// read_grads(list, apart) -> (addresses, sizes, types, index of the GPU): tensors
+// of float types on one GPU, whose values fill one run of memory in any order;
+// with `apart`, no memory belongs to two of them.
+PyObject* read_grads(PyObject*, PyObject* args) {
+    PyObject* list;
+    int apart;
+    if (!PyArg_ParseTuple(args, "Op", &list, &apart)) return nullptr;
+    try {
+        Py_ssize_t n = 0;
+        PyObject** const of = items(list, &n);
+        if (!of) return nullptr;
+        std::vector<uint64_t> at(n);
+        std::vector<int64_t> sizes(n);
+        std::vector<int32_t> types(n);
+        std::vector<std::pair<uint64_t, uint64_t>> written;
+        c10::Device device(c10::kCPU);
+        for (Py_ssize_t j = 0; j < n; ++j) {
+            if (!THPVariable_Check(of[j])) {
+                PyErr_SetString(PyExc_TypeError, "tensors are wanted");
+                return nullptr;
+            }
+            const at::Tensor& t = THPVariable_Unpack(of[j]);
+            if (t.layout() != at::kStrided) {
+                PyErr_SetString(PyExc_ValueError, "sparse gradients are not supported");
+                return nullptr;
+            }
+            const at::ScalarType type = t.scalar_type();
+            if (type != at::kFloat && type != at::kBFloat16 && type != at::kHalf) {
+                PyErr_SetString(PyExc_TypeError, "gradients are of float32, bfloat16 or float16");
+                return nullptr;
+            }
+            if (j == 0) device = t.device();
+            if (!t.device().is_cuda() || t.device() != device) {
+                PyErr_SetString(PyExc_ValueError, "every gradient must be on one GPU");
+                return nullptr;
+            }
+            if (!t.is_non_overlapping_and_dense()) {
+                PyErr_SetString(PyExc_ValueError, "a gradient's values must fill one run of memory");
+                return nullptr;
+            }
+            sizes[j] = t.numel();
+            types[j] = code(type);
+            at[j] = reinterpret_cast<uint64_t>(sizes[j] ? t.data_ptr() : nullptr);
+            if (apart && sizes[j]) written.emplace_back(at[j], at[j] + sizes[j] * t.element_size());
+        }
+        std::sort(written.begin(), written.end());
+        if (std::adjacent_find(written.begin(), written.end(), [](const auto& a, const auto& b) {
+                return b.first < a.second;
+            }) != written.end()) {
+            PyErr_SetString(PyExc_ValueError, "a gradient appears twice, or overlaps another");
+            return nullptr;
+        }
+        return Py_BuildValue("(y#y#y#i)", reinterpret_cast<const char*>(at.data()),
+                             static_cast<Py_ssize_t>(n * 8), reinterpret_cast<const char*>(sizes.data()),
+                             static_cast<Py_ssize_t>(n * 8), reinterpret_cast<const char*>(types.data()),
+                             static_cast<Py_ssize_t>(n * 4), n ? (int)device.index() : -1);
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+
 PyMethodDef methods[] = {
     {"read", read, METH_VARARGS, "read(lists, dtypes, block) -> (addresses, sizes)"},
+    {"read_grads", read_grads, METH_VARARGS,
+     "read_grads(list, apart) -> (addresses, sizes, types, index of the GPU)"},
     {"layer_norm", layer_norm, METH_VARARGS, "layer_norm(x, weight, bias, eps) -> y"},
     {"use", use, METH_VARARGS, "use(addresses of the library's entry points)"},
     {nullptr, nullptr, 0, nullptr}};

@@ -29,7 +29,8 @@ from .runtime import bind_stream, load_runtime
 
 __all__ = ["load_kernel", "load_scan_kernel", "kernel_available", "set_kernel_threads",
            "CoreCUDA", "core_forward", "step_core", "dw_step", "ScanCUDA", "scan_auto",
-           "layer_norm", "adamw_step", "STATE_BLOCK", "linear_attention", "linear_attention_step"]
+           "layer_norm", "adamw_step", "STATE_BLOCK", "embedding", "grad_norm", "clip_grads",
+           "linear_attention", "linear_attention_step"]
 
 _MAX_WIDTH = (1 << 31) - (1 << 14)  # of layer_norm's rows
 STATE_BLOCK = 256  # values of an 8-bit optimiser state that share one scale
@@ -269,7 +270,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
 
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, beta2=0.999,
-               eps=1e-8, weight_decay=0.01, avg_scale=None, sq_scale=None) -> None:
+               eps=1e-8, weight_decay=0.01, avg_scale=None, sq_scale=None, grad_scale=None) -> None:
     """One AdamW step (decoupled weight decay) of all `params` in place, in one
     launch for each few hundred tensors.
 
@@ -280,7 +281,8 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, bet
     the square root of the second. All contiguous, on one GPU; no parameter or
     state twice, or overlapping another. `step` counts from 1. step (an int64
     tensor of one value) and lr (a float64 one) may be on the GPU: then a
-    captured step reads them anew at each replay."""
+    captured step reads them anew at each replay. grad_scale: one float32 value on
+    the GPU that multiplies every gradient as it is read (``grad_norm``'s factor)."""
     import torch
     Tensor = torch.Tensor
     lists = [params, grads, exp_avg, exp_avg_sq]
@@ -307,16 +309,134 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, bet
                 raise TypeError(f"adamw_step: {name} as a tensor is one {dt} value on "
                                 f"{first.device}")
             on_gpu[name] = v.data_ptr()
+    if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or
+                                   grad_scale.device != first.device):
+        raise TypeError(f"adamw_step: grad_scale is one float32 value on {first.device}")
     to = [_address(at) + 8 * n * i for i in range(len(lists))]
-    rc = _lib_loaded().sn_abi_adamw_step(
+    rc = _lib_loaded().sn_abi_adamw_step_scaled(
         n, *to[:4], *(to[4:] or (None, None)), _address(sizes), dtype_code(first.dtype),
         dtype_code(grad.dtype), bits,
         0 if "step" in on_gpu else int(step), on_gpu.get("step"),
         0.0 if "lr" in on_gpu else float(lr), on_gpu.get("lr"), float(beta1), float(beta2),
-        float(eps), float(weight_decay), current_stream(first))
+        float(eps), float(weight_decay), None if grad_scale is None else grad_scale.data_ptr(),
+        current_stream(first))
     if rc:
         check(rc, "adamw_step")
     torch.autograd.graph.increment_version(lists[0])  # a graph that saved one must not use it
+
+
+def _embedding_forward(tokens, weight, scale):
+    import torch
+    V, D = weight.shape
+    out = torch.empty(*tokens.shape, D, dtype=weight.dtype, device=weight.device)
+    rc = _lib_loaded().sn_abi_embedding(
+        tokens.data_ptr(), 8 * tokens.element_size(), tokens.numel(), weight.data_ptr(), weight.stride(0), V, D,
+        dtype_code(weight.dtype), scale, out.data_ptr(), current_stream(weight))
+    if rc:
+        check(rc, "embedding")
+    return out
+
+
+_EMBEDDING = None
+
+
+def _embedding_fn():
+    global _EMBEDDING
+    if _EMBEDDING is not None:
+        return _EMBEDDING
+    import torch
+
+    class _Embedding(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, tokens, weight, scale):
+            ctx.save_for_backward(tokens)
+            ctx.weight, ctx.scale = (weight.shape, weight.dtype), scale
+            return _embedding_forward(tokens, weight, scale)
+
+        @staticmethod
+        @torch.autograd.function.once_differentiable
+        def backward(ctx, dout):
+            (tokens,) = ctx.saved_tensors
+            (V, D), dtype = ctx.weight
+            rows = dout.reshape(tokens.numel(), D)  # a view wherever the rows lie at one stride
+            if D > 1 and rows.stride(1) != 1:
+                rows = rows.contiguous()
+            dw = torch.empty(V, D, dtype=dtype, device=dout.device)
+            lib, n = _lib_loaded(), tokens.numel()
+            need = lib.sn_abi_embedding_bwd_ws(n, V, D)
+            ws = torch.empty(need, dtype=torch.uint8, device=dout.device) if need > 0 else None
+            rc = lib.sn_abi_embedding_bwd(
+                tokens.data_ptr(), 8 * tokens.element_size(), n, rows.data_ptr(), rows.stride(0), V, D,
+                dtype_code(dtype), ctx.scale, dw.data_ptr(), None if ws is None else ws.data_ptr(), max(need, 0),
+                current_stream(dout))
+            if rc:
+                check(rc, "embedding_bwd")
+            return None, dw, None
+
+    _EMBEDDING = _Embedding
+    return _EMBEDDING
+
+
+def embedding(tokens, weight, scale: float = 1.0):
+    """weight[tokens] * scale: rows (..., D) of weight (V, D) (float32, bfloat16
+    or float16, on a GPU; rows may lie at a stride) for int32 or int64 tokens of
+    any shape on that GPU. A token outside [0, V) gives a row of NaN, and adds
+    nothing to the gradient. Differentiable once in weight: its gradient is dense,
+    sums each row's tokens in fp32 in their order, and is the same bits every time."""
+    import torch
+    if weight.dim() != 2 or not weight.is_cuda:
+        raise ValueError("embedding: weight (V, D) on a GPU is wanted")
+    if tokens.dtype not in (torch.int32, torch.int64) or tokens.device != weight.device:
+        raise ValueError(f"embedding: tokens are int32 or int64 on {weight.device}")
+    dtype_code(weight.dtype)
+    tokens = tokens.contiguous()
+    if weight.shape[1] > 1 and weight.stride(1) != 1:
+        weight = weight.contiguous()
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return _embedding_fn().apply(tokens, weight, float(scale))
+    return _embedding_forward(tokens, weight, float(scale))
+
+
+def _norm_call(name, grads, max_norm, apart):
+    """The call of a list of gradients: (norm and factor, the list)."""
+    import torch
+    if not isinstance(grads, (list, tuple)):
+        grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if not grads:
+        raise ValueError(f"{name}: no gradients")
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"{name}: max_norm must not be negative")
+    at, sizes, types, _ = _torch_calls().read_grads(grads, apart)
+    lib, n = _lib_loaded(), len(grads)
+    need = lib.sn_abi_grad_norm_ws(n, _address(sizes))
+    ws = torch.empty(2 + need // 4, dtype=torch.float32, device=grads[0].device)
+    to = ws.data_ptr()
+    rc = getattr(lib, "sn_abi_" + name)(n, _address(at), _address(sizes), _address(types), max_norm, to, to + 4,
+                                        to + 8, need, current_stream(ws))
+    if rc:
+        check(rc, name)
+    return ws, grads
+
+
+def grad_norm(grads, max_norm=float("inf")):
+    """(norm, factor) of a list of gradients (float32, bfloat16 and float16 mixed
+    at will, on one GPU), each one float32 value on the GPU: the square root of
+    the sum of all squares, and min(1, max_norm / (norm + 1e-6)), which
+    ``adamw_step`` takes as grad_scale. Squares are added in fp32 over a few values
+    and in fp64 above; the same bits every time."""
+    ws, _ = _norm_call("grad_norm", grads, max_norm, False)
+    return ws[0], ws[1]
+
+
+def clip_grads(grads, max_norm):
+    """The norm of a list of gradients, all of which are scaled in place to a norm
+    of max_norm where theirs is larger. (With ``adamw_step`` as the next step,
+    ``grad_norm`` and its factor spare the pass that writes them.)"""
+    import torch
+    ws, grads = _norm_call("clip_grads", grads, max_norm, True)
+    torch.autograd.graph.increment_version(grads)
+    return ws[0]
 
 
 _MAX_HEAD = 128  # values of a head of linear_attention

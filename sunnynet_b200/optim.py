@@ -17,16 +17,21 @@ class AdamW(torch.optim.Optimizer):
     as float8_e4m3fn codes with a scale for each ``kernels.STATE_BLOCK`` values
     (2.03 bytes a parameter instead of 8). Parameters are contiguous tensors on
     a GPU. The step number lives on the host: to capture a step into a CUDA
-    graph, call ``kernels.adamw_step`` with a step tensor."""
+    graph, call ``kernels.adamw_step`` with a step tensor. ``max_norm``: gradients
+    whose common norm (of all groups) is larger are scaled to it as the step reads
+    them, .grad stays as it is; ``grad_norm`` is then the last step's norm, on the GPU."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
-                 state_bits=32):
+                 state_bits=32, max_norm=None):
+        if max_norm is not None and not max_norm >= 0:
+            raise ValueError("AdamW: max_norm must not be negative")
         if state_bits not in (8, 32):
             raise ValueError("AdamW: states have 8 or 32 bits")
         if not (lr >= 0 and eps >= 0 and weight_decay >= 0):
             raise ValueError("AdamW: lr, eps and weight_decay must not be negative")
         if not all(0 <= b < 1 for b in betas):
             raise ValueError("AdamW: betas are in [0, 1)")
+        self.max_norm, self.grad_norm = max_norm, None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
                                       weight_decay=weight_decay, state_bits=state_bits))
 
@@ -54,6 +59,12 @@ class AdamW(torch.optim.Optimizer):
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step in a capture would repeat one step number: call "
                                "kernels.adamw_step with a step tensor")
+        factor = None
+        if self.max_norm is not None:
+            grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
+            if grads:
+                grads = [g if g.layout != torch.strided else g.contiguous() for g in grads]
+                self.grad_norm, factor = kernels.grad_norm(grads, self.max_norm)
         for group in self.param_groups:
             bits = group["state_bits"]
             alike = collections.defaultdict(list)  # one call takes one kind of tensors
@@ -71,7 +82,7 @@ class AdamW(torch.optim.Optimizer):
                     pick("exp_avg"), pick("exp_avg_sq"), t, group["lr"], *group["betas"],
                     group["eps"], group["weight_decay"],
                     pick("avg_scale") if bits == 8 else None,
-                    pick("sq_scale") if bits == 8 else None)
+                    pick("sq_scale") if bits == 8 else None, factor)
                 for _, s in these:
                     s["step"] = t
         return loss
