@@ -59,11 +59,28 @@ __device__ __forceinline__ void ldsm4t(uint32_t* r, uint32_t at) {
                  : "memory");
 }
 __device__ __forceinline__ void mma(float* c, const uint32_t* a, const uint32_t* b) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
         "{%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+
+// a * b + c of two bf16 each, rounded once.
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t neg2(uint32_t a) {
+    uint32_t r;
+    asm("neg.bf16x2 %0, %1;" : "=r"(r) : "r"(a));
+    return r;
+}
+__device__ __forceinline__ void stsm4(uint32_t at, const uint32_t* r) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3])
+                 : "memory");
 }
 
 // The product of A (PA planes) and B (PB planes) into two neighbouring column
@@ -110,59 +127,87 @@ struct Tile {
     }
 };
 
-// Tokens [t0, t0 + C) of one head, `d` values each (D with zeros behind them),
-// `stride` values from one token to the next; tokens from `end` on are zeros,
-// whatever lies there. `whole`: base and stride are multiples of 16 bytes (of 8
-// for float16) and d fills whole packs. bf16 goes by cp.async: the caller waits.
+// A tile of tokens on its way to shared memory: [t0, t0 + C) of one head, `d`
+// values each (D with zeros behind them), `stride` values from one token to the
+// next; tokens from `end` on are zeros, whatever lies there. `whole`: base and
+// stride are multiples of 16 bytes (of 8 for float16) and d fills whole packs.
+// fetch() asks for the values and put() brings them, between which the caller may
+// work; bf16 goes by cp.async in fetch(), for which the caller waits instead.
 template <typename T, int C, int D, int THREADS>
-__device__ __forceinline__ void load_tokens(bf16* dst, const T* src, long long stride, int t0, int end,
-                                            int d, bool whole) {
-    constexpr int LD = D + 8, PLANE = C * LD;
-    if (whole) {
-        constexpr int W = std::is_same<T, bf16>::value ? 8 : 4;  // values of a pack
-        constexpr int PACKS = C * D / W;
-#pragma unroll
-        for (int n = 0; n < PACKS / THREADS; ++n) {
-            const int i = n * THREADS + threadIdx.x, row = i / (D / W), col = i % (D / W) * W;
-            const bool in = t0 + row < end && col < d;
-            const T* from = src + (in ? (long long)(t0 + row) * stride + col : 0);
+struct Fetch {
+    static constexpr bool DIRECT = std::is_same<T, bf16>::value;
+    static constexpr int W = DIRECT ? 8 : 4;  // values of a pack
+    static constexpr int N = C * D / W / THREADS, LD = D + 8, PLANE = C * LD;
+    static_assert(C * D / W % THREADS == 0, "whole rounds of packs");
+    typedef typename std::conditional<sizeof(T) == 4, float4, uint2>::type Raw;
+    Raw raw[DIRECT ? 1 : N];
+
+    // Packs of a row are the work of neighbouring threads; a thread's rows lie ROWS apart.
+    static constexpr int PER_ROW = D / W, ROWS = THREADS / PER_ROW;
+    static_assert(THREADS % PER_ROW == 0, "whole rows for the threads");
+
+    __device__ __forceinline__ void fetch(bf16* dst, const T* src, long long stride, int t0, int end, int d,
+                                          bool whole) {
+        if (whole) {
+            const int row = threadIdx.x / PER_ROW, col = threadIdx.x % PER_ROW * W;
+            const int rows = col < d ? end - t0 - row : 0;  // of the thread's that hold values
+            const T* from = src + (long long)(t0 + row) * stride + col;
             bf16* to = dst + row * LD + col;
-            if constexpr (std::is_same<T, bf16>::value) {
-                cp_async16(to, from, in ? 16 : 0);
-            } else {
-                float x[4] = {};
-                if (in) {
-                    if constexpr (std::is_same<T, float>::value) {
-                        const float4 f = *reinterpret_cast<const float4*>(from);
-                        x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-                    } else {
-                        const uint2 f = *reinterpret_cast<const uint2*>(from);
-                        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&f.x));
-                        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&f.y));
-                        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-                    }
-                }
-                const uint2 hi = {pack2(x[0], x[1]), pack2(x[2], x[3])};
-                const uint2 lo = {rest2(x[0], x[1], hi.x), rest2(x[2], x[3], hi.y)};
-                *reinterpret_cast<uint2*>(to) = hi;
-                *reinterpret_cast<uint2*>(to + PLANE) = lo;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const bool in = n * ROWS < rows;
+                if constexpr (DIRECT)
+                    cp_async16(to + n * ROWS * LD, in ? from : src, in ? 16 : 0);
+                else
+                    raw[n] = in ? *reinterpret_cast<const Raw*>(from) : Raw();
+                from += ROWS * stride;
+            }
+        } else if constexpr (DIRECT) {
+            for (int i = threadIdx.x; i < C * D; i += THREADS) {
+                const int row = i / D, col = i % D;
+                dst[row * LD + col] = t0 + row < end && col < d ? src[(long long)(t0 + row) * stride + col]
+                                                                : __float2bfloat16_rn(0.0f);
             }
         }
-    } else {
-        for (int i = threadIdx.x; i < C * D; i += THREADS) {
-            const int row = i / D, col = i % D;
-            const bool in = t0 + row < end && col < d;
-            const float x = in ? to_f(src[(long long)(t0 + row) * stride + col]) : 0.0f;
-            const bf16 hi = __float2bfloat16_rn(x);
-            dst[row * LD + col] = hi;
-            if constexpr (planes_of<T> == 2)
-                dst[PLANE + row * LD + col] = __float2bfloat16_rn(x - __bfloat162float(hi));
+    }
+
+    __device__ __forceinline__ void put(bf16* dst, const T* src, long long stride, int t0, int end, int d,
+                                        bool whole) {
+        if constexpr (!DIRECT) {
+            if (whole) {
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
+                    const int i = n * THREADS + threadIdx.x, row = i / (D / W), col = i % (D / W) * W;
+                    bf16* to = dst + row * LD + col;
+                    float x[4];
+                    if constexpr (sizeof(T) == 4) {
+                        x[0] = raw[n].x, x[1] = raw[n].y, x[2] = raw[n].z, x[3] = raw[n].w;
+                    } else {
+                        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&raw[n].x));
+                        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&raw[n].y));
+                        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+                    }
+                    const uint2 hi = {pack2(x[0], x[1]), pack2(x[2], x[3])};
+                    const uint2 lo = {rest2(x[0], x[1], hi.x), rest2(x[2], x[3], hi.y)};
+                    *reinterpret_cast<uint2*>(to) = hi;
+                    *reinterpret_cast<uint2*>(to + PLANE) = lo;
+                }
+            } else {
+                for (int i = threadIdx.x; i < C * D; i += THREADS) {
+                    const int row = i / D, col = i % D;
+                    const bool in = t0 + row < end && col < d;
+                    const float x = in ? to_f(src[(long long)(t0 + row) * stride + col]) : 0.0f;
+                    const bf16 hi = __float2bfloat16_rn(x);
+                    dst[row * LD + col] = hi;
+                    dst[PLANE + row * LD + col] = __float2bfloat16_rn(x - __bfloat162float(hi));
+                }
+            }
         }
     }
-}
+};
 
 // The sums c of a chunk's log decays in powers of two, up to and with each
-// token. near + far is c to 2^-29: near a multiple of 1/16, so that near_t -
+// token. near + far is c to 2^-28: near a multiple of 1/16, so that near_t -
 // near_s is exact and the decay between two tokens as good as their
 // difference, however far both are from the chunk's start.
 template <int C>
@@ -171,6 +216,9 @@ struct alignas(16) Decays {
     float from_start[C];  // 2^c_t
     float to_end[C];      // 2^(c_C - c_t)
     float whole;          // 2^c_C
+    float unused[3];
+    // 2^(c_t - c_s)
+    __device__ __forceinline__ float between(int t, int s) const;
 };
 
 __device__ __forceinline__ float exp2_of(float x) {
@@ -179,38 +227,77 @@ __device__ __forceinline__ float exp2_of(float x) {
     return y;
 }
 
-// By one whole warp. A log decay below -256 (in powers of two) leaves nothing
-// in 32 bits, however long the chunk: it is taken as -256, minus infinity too.
 template <int C>
-__device__ __forceinline__ void decays(Decays<C>* to, const float* g, long long stride, int t0, int end) {
+__device__ __forceinline__ float Decays<C>::between(int t, int s) const {
+    return exp2_of(near[t] - near[s] + (far[t] - far[s]));
+}
+
+// What a chunk's tokens weigh in its state, each as the sum of two bf16: pairs of
+// tokens, the high parts in x, the low ones in y.
+template <int C>
+struct alignas(16) Weights {
+    uint2 pair[C / 2];
+};
+
+// By one whole warp, from a lane's C / 32 log decays (zeros behind the end), in
+// the tokens' order. The sums are whole numbers of 2^-40: no rounding, and half
+// the latency of fp64. A log decay beyond 256 (in powers of two) either way leaves
+// nothing, or no finite number, in 32 bits: it is taken as 256, infinities too. A
+// NaN makes every sum from its token on one.
+// The weights are to_end, or (back) scale * from_start.
+template <int C>
+__device__ __forceinline__ void decays(Decays<C>* to, Weights<C>* weights, const float* g, bool back,
+                                       float scale) {
     constexpr int N = C / 32;
+    constexpr float kLog2e = 1.44269504088896340736f, kRest = 1.92596299e-8f;  // their sum is log2(e) to 2^-50
     const int l = lane_id();
-    double c[N], sum = 0.0;
+    long long c[N], sum = 0;
+    int bad = N;  // the lane's first NaN
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int t = t0 + l * N + i;
-        double x = t < end ? (double)g[(long long)t * stride] * 1.4426950408889634074 : 0.0;
-        if (x < -256.0) x = -256.0;  // (a NaN stays)
-        c[i] = sum += x;
+        if (bad == N && g[i] != g[i]) bad = i;
+        const float x = fminf(fmaxf(g[i], -178.0f), 178.0f);
+        const float hi = x * kLog2e, lo = fmaf(x, kLog2e, -hi) + x * kRest;
+        c[i] = sum += __float2ll_rn(hi * 0x1p40f) + __float2ll_rn(lo * 0x1p40f);
     }
-    double before = sum;
+    const unsigned wrong = __ballot_sync(0xffffffffu, bad < N);
+    const int first = wrong ? __ffs(wrong) - 1 : 32;  // the lane of the first NaN
+    long long before = sum;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-        const double y = __shfl_up_sync(0xffffffffu, before, d);
+        const long long y = __shfl_up_sync(0xffffffffu, before, d);
         if (l >= d) before += y;
     }
-    const double all = __shfl_sync(0xffffffffu, before, 31);
+    const long long all = __shfl_sync(0xffffffffu, before, 31);
     before -= sum;
+    const float nan = __int_as_float(0x7fffffff);
+    float w[N];
+    const auto value = [](long long x) {  // (the high part is exact)
+        const int whole = (int)(x >> 36);
+        return make_float2((float)whole * 0.0625f, (float)(x - ((long long)whole << 36)) * 0x1p-40f);
+    };
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const double x = before + c[i];
-        const float near = rintf((float)x * 16.0f) * 0.0625f;
-        to->near[l * N + i] = near;
-        to->far[l * N + i] = (float)(x - (double)near);
-        to->from_start[l * N + i] = exp2_of((float)x);
-        to->to_end[l * N + i] = exp2_of((float)(all - x));
+        const bool poor = l > first || (l == first && i >= bad);
+        const float2 x = value(before + c[i]), y = value(all - before - c[i]);
+        to->near[l * N + i] = poor ? nan : x.x;
+        to->far[l * N + i] = x.y;
+        const float from_start = poor ? nan : exp2_of(x.x + x.y), to_end = wrong ? nan : exp2_of(y.x + y.y);
+        to->from_start[l * N + i] = from_start;
+        to->to_end[l * N + i] = to_end;
+        w[i] = back ? from_start * scale : to_end;
     }
-    if (l == 0) to->whole = exp2_of((float)all);
+    if constexpr (N > 1) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const uint32_t hi = pack2(w[i], w[i + 1]);
+            weights->pair[(l * N + i) / 2] = make_uint2(hi, rest2(w[i], w[i + 1], hi));
+        }
+    }
+    if (l == 0) {
+        const float2 x = value(all);
+        to->whole = wrong ? nan : exp2_of(x.x + x.y);
+    }
 }
 
 }  // namespace la
