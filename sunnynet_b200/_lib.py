@@ -137,13 +137,6 @@ SIGNATURES = {
 }
 
 
-class LinearAttention(ctypes.Structure):
-    """SnAbiLinearAttention (sn_abi.h)."""
-    _fields_ = [(n, V) for n in ("q", "k", "v", "log_decay", "state", "lengths")] + \
-        [(n + "_stride", I64 * 3) for n in ("q", "k", "v", "log_decay")] + \
-        [(n, I32) for n in ("dtype", "B", "T", "H", "Hk", "dk", "dv")] + [("scale", F32)]
-
-
 STATUS = {0: "OK", -1: "E_INVAL", -2: "E_NOMEM", -3: "E_IO", -4: "E_FORMAT",
           -5: "E_UNSUPPORTED", -6: "E_DEVICE"}
 

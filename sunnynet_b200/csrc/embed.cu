@@ -54,50 +54,47 @@ struct alignas(sizeof(T) * N) Pack {
     T v[N];
 };
 
-// x / d for x < 2^31, by one product.
-struct Divide {
-    unsigned d, mul, shift;
-    explicit Divide(unsigned n = 1) : d(n), mul(0), shift(0) {
-        while ((1ull << shift) < n) ++shift;
-        mul = (unsigned)(((1ull << 32) * ((1ull << shift) - n)) / n + 1);
-    }
-    __device__ __forceinline__ unsigned of(unsigned x) const { return (__umulhi(x, mul) + x) >> shift; }
-};
-
 // The row of token i, or -1.
 __device__ __forceinline__ long long row_of(const void* tokens, bool wide, long long i, long long V) {
     const long long t = wide ? static_cast<const long long*>(tokens)[i] : static_cast<const int*>(tokens)[i];
     return t >= 0 && t < V ? t : -1;
 }
 
+// x * f for a pack, rounded once to fp32 and once to T.
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> scaled(const Pack<T, N>& x, float f) {
+    Pack<T, N> y;
+#pragma unroll
+    for (int k = 0; k < N; ++k) y.v[k] = from_f<T>(to_f(x.v[k]) * f);
+    return y;
+}
+
 // ----------------------------------------------------------------- forward
 constexpr int kThreads = 256;
 
-// A CTA copies `rows` rows of `packs` packs, a thread U packs at a time.
-template <typename T, int N, int U>
+// LANES neighbouring threads copy a row, U packs of each on their way at once.
+template <typename T, int N, int LANES>
 __global__ void __launch_bounds__(kThreads)
 rows_kernel(const void* tokens, bool wide, const T* W, long long ld, long long V, T* out, long long n, int D,
-            unsigned rows, unsigned packs, Divide by, float scale) {
-    const long long first = blockIdx.x * (long long)rows;
-    const unsigned todo = (unsigned)min((long long)rows, n - first) * packs;
-    for (unsigned i0 = threadIdx.x; i0 < todo; i0 += U * kThreads) {
+            float scale) {
+    constexpr int U = LANES == 32 ? 4 : 2;
+    const long long i = (blockIdx.x * (long long)kThreads + threadIdx.x) / LANES;
+    if (i >= n) return;
+    const long long row = row_of(tokens, wide, i, V);
+    const float f = row >= 0 ? scale : __int_as_float(0x7fffffff);
+    const T* from = W + (row >= 0 ? row * ld : 0);
+    T* to = out + i * D;
+    for (int c = threadIdx.x % LANES * N; c < D; c += U * LANES * N) {
         Pack<T, N> x[U];
-        long long row[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const unsigned i = i0 + u * kThreads, r = by.of(i);
-            row[u] = i < todo ? row_of(tokens, wide, first + r, V) : -1;
-            if (row[u] >= 0)
-                x[u] = *reinterpret_cast<const Pack<T, N>*>(W + row[u] * ld + (i - r * packs) * N);
+            const int at = c + u * LANES * N;
+            if (at < D && V) x[u] = *reinterpret_cast<const Pack<T, N>*>(from + at);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const unsigned i = i0 + u * kThreads, r = by.of(i);
-            if (i >= todo) break;
-#pragma unroll
-            for (int k = 0; k < N; ++k)
-                x[u].v[k] = from_f<T>(row[u] >= 0 ? to_f(x[u].v[k]) * scale : __int_as_float(0x7fffffff));
-            *reinterpret_cast<Pack<T, N>*>(out + (first + r) * D + (i - r * packs) * N) = x[u];
+            const int at = c + u * LANES * N;
+            if (at < D) *reinterpret_cast<Pack<T, N>*>(to + at) = scaled(x[u], f);
         }
     }
 }
@@ -105,6 +102,7 @@ rows_kernel(const void* tokens, bool wide, const T* W, long long ld, long long V
 // -------------------------------------------------------------------- sort
 constexpr int kTiles = 148;  // at most: a tile of the tokens for each SM
 constexpr int kBins = 256;
+constexpr int kSort = 1024;  // threads of a CTA: tokens of a tile that are placed at once
 
 struct Sorting {
     const void* tokens;  // of the first pass
@@ -114,8 +112,10 @@ struct Sorting {
     uint2* to;
     int* counts;  // tiles x kBins
     int n, tiles, per, shift;
+    int* joins;  // how many rows a later kernel joins: set to none by the first launch
     float4* zeros;  // what further CTAs fill
     long long zero_packs;
+    int zero_rest;  // bytes behind those
 };
 
 __device__ __forceinline__ uint2 entry(const Sorting& s, int i) {
@@ -129,10 +129,13 @@ __device__ __forceinline__ void fill_zeros(const Sorting& s) {
     for (long long i = (blockIdx.x - s.tiles) * (long long)blockDim.x + threadIdx.x; i < s.zero_packs;
          i += ctas * blockDim.x)
         s.zeros[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (blockIdx.x == (unsigned)s.tiles && threadIdx.x < (unsigned)s.zero_rest)
+        reinterpret_cast<char*>(s.zeros + s.zero_packs)[threadIdx.x] = 0;
 }
 
-__global__ void __launch_bounds__(1024) count_kernel(const Sorting s) {
+__global__ void __launch_bounds__(kSort) count_kernel(const Sorting s) {
     pdl_trigger();
+    if (blockIdx.x == 0 && threadIdx.x == 0 && !s.from) *s.joins = 0;
     if (blockIdx.x >= (unsigned)s.tiles) return fill_zeros(s);  // (dW is this call's own since its first launch)
     __shared__ int count[kBins];
     for (int i = threadIdx.x; i < kBins; i += blockDim.x) count[i] = 0;
@@ -144,12 +147,11 @@ __global__ void __launch_bounds__(1024) count_kernel(const Sorting s) {
     for (int i = threadIdx.x; i < kBins; i += blockDim.x) s.counts[blockIdx.x * kBins + i] = count[i];
 }
 
-// A thread for each of the tile's tokens, WARPS * 32 at a time, in their order.
-template <int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) place_kernel(const Sorting s) {
+// A thread for each of the tile's tokens, kSort at a time, in their order.
+__global__ void __launch_bounds__(kSort) place_kernel(const Sorting s) {
     pdl_trigger();
     if (blockIdx.x >= (unsigned)s.tiles) return fill_zeros(s);
-    constexpr int PARTS = WARPS * 32 / kBins;
+    constexpr int WARPS = kSort / 32, PARTS = kSort / kBins;
     __shared__ int at[kBins], part[PARTS][kBins][2], warp_sum[kBins / 32];
     __shared__ int seen[WARPS][kBins];  // of a warp, in this round
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bin = tid % kBins;
@@ -158,7 +160,7 @@ __global__ void __launch_bounds__(WARPS * 32) place_kernel(const Sorting s) {
     // where this tile's tokens of each bin begin: behind those of lower bins, and of earlier tiles
     {
         int all = 0, before = 0;
-#pragma unroll 8
+#pragma unroll 16
         for (int t = tid / kBins; t < s.tiles; t += PARTS) {
             const int c = s.counts[t * kBins + bin];
             all += c;
@@ -231,13 +233,9 @@ struct Summing {
     long long V, ld;
     int D;
     float* pieces;  // slots x D
+    int *joins, *list;  // the chunks in which a row of several pieces begins, in any order
     float scale;
 };
-
-// Whether sorted token i exists and is of row r.
-__device__ __forceinline__ bool is(const Summing& s, long long i, unsigned r) {
-    return i < s.n && s.sorted[i].x == r;
-}
 
 template <typename T, int N>
 __global__ void __launch_bounds__(kColumns) sum_kernel(const Summing s, const T* dout, T* dW) {
@@ -278,76 +276,100 @@ __global__ void __launch_bounds__(kColumns) sum_kernel(const Summing s, const T*
         for (int i = b + threadIdx.x; i < w1; i += kColumns)
             if (key(i - 1) == rb && (i + 1 == w1 || key(i + 1) != rb) && key(i) == rb) last_ = i + 1;
     __syncthreads();
-    const int first = first_, last = last_;
     const bool cut = b < s.n && key(b) == rb && long_b;  // the last row goes on behind
+    if (cut && rb < s.V && !(on && ra == rb) && blockIdx.y == 0 && threadIdx.x == 0)
+        s.list[atomicAdd(s.joins, 1)] = blockIdx.x;
+    const int first = first_;
+    int last = last_;
+    if (key(last - 1) >= s.V) {  // strangers are no one's
+        int lo = first < last ? first : last, hi = last;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (key(mid) >= s.V)
+                hi = mid;
+            else
+                lo = mid + 1;
+        }
+        last = lo;
+    }
     const int col = (blockIdx.y * kColumns + threadIdx.x) * N;
-    if (first >= b || col >= s.D) return;
     // (a short row's tokens behind b are this chunk's only if they begin in it)
+    if (first >= b || first >= last || col >= s.D) return;
     constexpr int U = 8;
+    const T* const from = dout + col;
     float sum[N] = {};
     for (int i0 = first; i0 < last; i0 += U) {
         Pack<T, N> x[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (i0 + u < last && key(i0 + u) < s.V)
-                x[u] = *reinterpret_cast<const Pack<T, N>*>(dout + (long long)window[i0 + u - w0].y * s.ld + col);
+            x[u] = *reinterpret_cast<const Pack<T, N>*>(from + (long long)window[min(i0 + u, last - 1) - w0].y * s.ld);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = i0 + u;
-            if (i >= last) break;
-            const unsigned r = key(i);
-            if (r >= s.V) break;
+            if (i < last) {
 #pragma unroll
-            for (int k = 0; k < N; ++k) sum[k] += to_f(x[u].v[k]);
-            if (i + 1 < last && key(i + 1) == r) continue;
-            // the row's last token in this chunk
-            const bool head = on && long_a && r == ra, tail = cut && r == rb;
-            if (head || tail) {
-                float* to = s.pieces + (2ll * blockIdx.x + (head ? 0 : 1)) * s.D + col;
+                for (int k = 0; k < N; ++k) sum[k] += to_f(x[u].v[k]);
+                const unsigned r = key(i);
+                if (i + 1 == last || key(i + 1) != r) {  // the row's last token in this chunk
+                    const bool head = on && long_a && r == ra, tail = cut && r == rb;
+                    if (head || tail) {
+                        float* to = s.pieces + (2ll * blockIdx.x + (head ? 0 : 1)) * s.D + col;
 #pragma unroll
-                for (int k = 0; k < N; ++k) to[k] = sum[k];
-            } else {
-                Pack<T, N> y;
+                        for (int k = 0; k < N; ++k) to[k] = sum[k];
+                    } else {
+                        Pack<T, N> y;
 #pragma unroll
-                for (int k = 0; k < N; ++k) y.v[k] = from_f<T>(sum[k] * s.scale);
-                *reinterpret_cast<Pack<T, N>*>(dW + (long long)r * s.D + col) = y;
+                        for (int k = 0; k < N; ++k) y.v[k] = from_f<T>(sum[k] * s.scale);
+                        *reinterpret_cast<Pack<T, N>*>(dW + (long long)r * s.D + col) = y;
+                    }
+#pragma unroll
+                    for (int k = 0; k < N; ++k) sum[k] = 0.0f;
+                }
             }
-#pragma unroll
-            for (int k = 0; k < N; ++k) sum[k] = 0.0f;
         }
     }
 }
 
-// The pieces of the long row that begins in this chunk, if one does.
+// The pieces of the rows that have several, a slab of 128 columns of a row at a
+// time: each warp takes every kJoin-th piece, and the warps' sums are added in
+// their order.
+constexpr int kJoin = 8;  // warps
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) join_kernel(const Summing s, T* dW) {
+__global__ void __launch_bounds__(kJoin * 32) join_kernel(const Summing s, T* dW) {
     pdl_wait();
-    const int per = s.per, a = blockIdx.x * per, b = a + per;
-    if (b >= s.n) return;
-    const unsigned r = s.sorted[b].x;
-    if (r >= s.V || s.sorted[b - 1].x != r || (a > 0 && s.sorted[a - 1].x == r)) return;
-    int lo = a, hi = b - 1;  // where it begins
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (s.sorted[mid].x == r)
-            hi = mid;
-        else
-            lo = mid + 1;
-    }
-    if (!is(s, (long long)lo + per, r)) return;
-    int m0 = blockIdx.x + 1, m1 = (s.n - 1) / per;  // the last chunk whose first token is its
-    while (m0 < m1) {
-        const int mid = (m0 + m1 + 1) >> 1;
-        if (s.sorted[(long long)mid * per].x == r)
-            m0 = mid;
-        else
-            m1 = mid - 1;
-    }
-    for (int col = threadIdx.x; col < s.D; col += kThreads) {
-        float sum = s.pieces[(2ll * blockIdx.x + 1) * s.D + col];
+    __shared__ float part[kJoin][128];
+    const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, slabs = (s.D + 127) / 128, todo = *s.joins * slabs;
+    for (int item = blockIdx.x; item < todo; item += gridDim.x) {
+        const int first = s.list[item / slabs], col = item % slabs * 128 + l;
+        const unsigned r = s.sorted[(first + 1) * s.per].x;  // (it goes on in the next chunk)
+        // the last chunk whose first token is the row's: 32 places of what is left at once
+        int last = first + 1, hi = (s.n - 1) / s.per;
+        while (last < hi) {
+            const int step = (hi - last + 32) / 32, m = last + l * step;
+            const int yes = __popc(__ballot_sync(0xffffffffu, m <= hi && s.sorted[min(m, hi) * s.per].x == r));
+            last += (yes - 1) * step;
+            hi = min(hi, last + step - 1);
+        }
+        float sum[4] = {};
 #pragma unroll 8
-        for (int c = blockIdx.x + 1; c <= m0; ++c) sum += s.pieces[2ll * c * s.D + col];
-        dW[(long long)r * s.D + col] = from_f<T>(sum * s.scale);
+        for (int c = first + warp; c <= last; c += kJoin) {
+            const float* from = s.pieces + (2ll * c + (c == first)) * s.D;
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (col + k * 32 < s.D) sum[k] += from[col + k * 32];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) part[warp][k * 32 + l] = sum[k];
+        __syncthreads();
+        const int c = item % slabs * 128 + threadIdx.x;
+        if (threadIdx.x < 128 && c < s.D) {
+            float x = part[0][threadIdx.x];
+#pragma unroll
+            for (int w = 1; w < kJoin; ++w) x += part[w][threadIdx.x];
+            dW[(long long)r * s.D + c] = from_f<T>(x * s.scale);
+        }
+        __syncthreads();
     }
 }
 
@@ -403,12 +425,12 @@ int check_call(const char* what, int64_t n, int64_t V, int32_t D, int64_t ld, in
 // How the tokens are cut up, and the workspace in bytes.
 struct Plan {
     int tiles, per, passes, chunk;
-    long long chunks, list, counts, pieces, bytes;
+    long long chunks, list, counts, joins, pieces, bytes;
 };
 Plan plan_of(long long n, long long V, int D) {
     Plan p;
     const auto up = [](long long b) { return (b + 255) / 256 * 256; };
-    p.tiles = (int)std::max(1ll, std::min((long long)kTiles, (n + 255) / 256));
+    p.tiles = (int)std::max(1ll, std::min((long long)kTiles, (n + kSort - 1) / kSort));
     p.per = (int)((n + p.tiles - 1) / p.tiles);
     p.passes = 1;
     while (V >> 8 * p.passes) ++p.passes;  // (V itself marks strangers)
@@ -418,8 +440,9 @@ Plan plan_of(long long n, long long V, int D) {
     p.chunks = (n + p.chunk - 1) / p.chunk;
     p.list = up(n * 8);
     p.counts = up((long long)p.tiles * kBins * 4);
+    p.joins = up((p.chunks + 1) * 4);
     p.pieces = up(p.chunks * 2 * D * 4);
-    p.bytes = 2 * p.list + p.counts + p.pieces;
+    p.bytes = 2 * p.list + p.counts + p.joins + p.pieces;
     return p;
 }
 
@@ -443,14 +466,18 @@ sn_status sn_abi_embedding(const void* tokens, int32_t token_bits, int64_t n, co
     return by_access(dtype, width_of(W, out, ld, D, e), [&](auto t, auto vec) {
         typedef decltype(t) T;
         constexpr int N = decltype(vec)::value;
-        const unsigned packs = (unsigned)(D / N);
-        // four packs of a thread at once where that leaves a CTA for every SM
-        const bool many = n * packs >= 148ll * 4 * kThreads;
-        const unsigned rows = std::max(1u, (many ? 4u : 1u) * kThreads / packs);
-        const unsigned ctas = (unsigned)((n + rows - 1) / rows);
-        auto* kernel = many ? rows_kernel<T, N, 4> : rows_kernel<T, N, 1>;
-        kernel<<<ctas, kThreads, 0, st>>>(tokens, token_bits == 64, static_cast<const T*>(W), ld, V,
-                                          static_cast<T*>(out), n, D, rows, packs, Divide(packs), scale);
+        const auto go = [&](auto lanes) {
+            constexpr int L = decltype(lanes)::value;
+            rows_kernel<T, N, L><<<(unsigned)((n * L + kThreads - 1) / kThreads), kThreads, 0, st>>>(
+                tokens, token_bits == 64, static_cast<const T*>(W), ld, V, static_cast<T*>(out), n, D, scale);
+        };
+        // a warp to a row, or as many lanes as it has packs
+        if (D / N > 16)
+            go(std::integral_constant<int, 32>());
+        else if (D / N > 4)
+            go(std::integral_constant<int, 8>());
+        else
+            go(std::integral_constant<int, 2>());
         return cuda_check(cudaGetLastError(), "embedding launch");
     });
 }
@@ -482,41 +509,40 @@ sn_status sn_abi_embedding_bwd(const void* tokens, int32_t token_bits, int64_t n
     Sorting s = {};
     s.tokens = tokens, s.wide = token_bits == 64, s.V = V;
     s.counts = reinterpret_cast<int*>(at + 2 * p.list);
+    s.joins = reinterpret_cast<int*>(at + 2 * p.list + p.counts);
     s.n = (int)n, s.tiles = p.tiles, s.per = p.per;
-    // the zeros, a part to each launch; where they do not come in packs, by a launch of their own
+    // the zeros, a part to each launch; where they do not begin at a pack, by one of their own
     const bool packed = (uintptr_t)dW % 16 == 0;
     const long long packs = packed ? bytes / 16 : 0, share = (packs + 2 * p.passes - 1) / (2 * p.passes);
-    if (bytes % 16 || !packed)
-        SN_TRY(cuda_check(cudaMemsetAsync(static_cast<char*>(dW) + packs * 16, 0, bytes - packs * 16, st),
-                          "embedding_bwd"));
+    if (!packed) SN_TRY(cuda_check(cudaMemsetAsync(dW, 0, bytes, st), "embedding_bwd"));
     long long done = 0;
     const auto zeros = [&] {
         s.zeros = reinterpret_cast<float4*>(dW) + done;
         s.zero_packs = std::min(share, packs - done);
         done += s.zero_packs;
-        return (unsigned)std::min((s.zero_packs + 4095) / 4096, 148ll * 4);
+        s.zero_rest = packed && done == packs ? (int)(bytes % 16) : 0;
+        return (unsigned)std::min((s.zero_packs + 4095) / 4096 + (s.zero_rest > 0), 148ll * 4);
     };
-    const bool big = p.per >= 512;
     for (int i = 0; i < p.passes; ++i) {
         s.shift = 8 * i;
         s.from = i ? lists[(i - 1) & 1] : nullptr;
         s.to = lists[i & 1];
-        const int threads = big ? 1024 : 256;
         if (i == 0) {
             const unsigned more = zeros();
-            count_kernel<<<p.tiles + more, threads, 0, st>>>(s);
+            count_kernel<<<p.tiles + more, kSort, 0, st>>>(s);
             SN_TRY(cuda_check(cudaGetLastError(), "embedding launch"));
         } else {
             const unsigned more = zeros();
-            SN_TRY(launch_behind(count_kernel, dim3(p.tiles + more), threads, 0, st, s));
+            SN_TRY(launch_behind(count_kernel, dim3(p.tiles + more), kSort, 0, st, s));
         }
         const unsigned more = zeros();
-        SN_TRY(launch_behind(big ? place_kernel<32> : place_kernel<8>, dim3(p.tiles + more), threads, 0, st, s));
+        SN_TRY(launch_behind(place_kernel, dim3(p.tiles + more), kSort, 0, st, s));
     }
     Summing m = {};
     m.sorted = lists[(p.passes - 1) & 1];
     m.n = (int)n, m.per = p.chunk, m.V = V, m.ld = ld, m.D = D;
-    m.pieces = reinterpret_cast<float*>(at + 2 * p.list + p.counts);
+    m.joins = s.joins, m.list = s.joins + 1;
+    m.pieces = reinterpret_cast<float*>(at + 2 * p.list + p.counts + p.joins);
     m.scale = scale;
     SN_TRY(by_access(dtype, width_of(dout, dW, ld, D, e), [&](auto t, auto vec) {
         typedef decltype(t) T;
@@ -527,7 +553,9 @@ sn_status sn_abi_embedding_bwd(const void* tokens, int32_t token_bits, int64_t n
     }));
     return by_type(dtype, [&](auto t) {
         typedef decltype(t) T;
-        return launch_behind(join_kernel<T>, dim3((unsigned)p.chunks), kThreads, 0, st, m, static_cast<T*>(dW));
+        const long long most = (p.chunks + 1) / 2 * ((D + 127) / 128);  // (a row of several pieces has two chunks)
+        return launch_behind(join_kernel<T>, dim3((unsigned)std::min(most, 148ll * 8)), kJoin * 32, 0, st, m,
+                             static_cast<T*>(dW));
     });
 }
 

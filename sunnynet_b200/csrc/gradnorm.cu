@@ -10,9 +10,9 @@
 // to the largest count.
 //
 // Bound by HBM: the norm reads every value once, clipping once more, and writes
-// it. One wave of CTAs takes the values, each one run of one tensor; what the
-// first pass read last is still in L2 when the second begins, so that goes
-// through each run from its end.
+// it. One wave of CTAs takes the tensors' runs of a few thousand values in turn;
+// what the first pass read last is still in L2 when the second begins, so that
+// goes from the last run to the first.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,8 +28,8 @@ namespace sn {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWave = 148 * 8;     // runs that the values are cut into (and one more for each tensor)
-constexpr int kLeast = 4096;       // values of a run, or a multiple
+constexpr int kWave = 148 * 8;     // CTAs at most, each with one part of the sum
+constexpr int kRun = 16384, kShort = 4096;  // values of a run; of a small model's, for more CTAs
 constexpr int kFew = 32, kMany = 1280;  // tensors of a launch: 30 of the 32 KB of parameters
 
 struct Run {
@@ -41,8 +41,8 @@ struct Run {
 
 template <int N>
 struct Runs {
-    int count;
-    long long per;  // values of a run
+    int count, runs;
+    int per;  // values of a run
     Run t[N];
 };
 
@@ -80,8 +80,8 @@ union Pack {
 
 // Values of a run before its first multiple of 16 bytes.
 template <typename T>
-__device__ __forceinline__ long long head_of(const T* p, long long n) {
-    const long long k = (16 - (reinterpret_cast<uintptr_t>(p) & 15)) % 16 / sizeof(T);
+__device__ __forceinline__ int head_of(const T* p, int n) {
+    const int k = (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) % 16 / sizeof(T));
     return k < n ? k : n;
 }
 
@@ -109,32 +109,31 @@ __device__ __forceinline__ double squares(const uint4& w) {
 constexpr int kAhead = 4;  // loads of a thread on their way
 
 template <typename T>
-__device__ __forceinline__ double square_run(const T* p, long long n) {
+__device__ __forceinline__ double square_run(const T* p, int n) {
     constexpr int V = 16 / sizeof(T);
-    const long long head = head_of(p, n), packs = (n - head) / V, tail = head + packs * V;
+    const int head = head_of(p, n), packs = (n - head) / V, tail = head + packs * V;
     double sum = 0.0;
-    for (long long i = threadIdx.x; i < head + (n - tail); i += kThreads) {
+    for (int i = threadIdx.x; i < head + (n - tail); i += kThreads) {
         const double x = (double)to_f(p[i < head ? i : tail + (i - head)]);
         sum = fma(x, x, sum);
     }
     const uint4* at = reinterpret_cast<const uint4*>(p + head);
-    long long i = threadIdx.x;
-    for (; i + (kAhead - 1) * kThreads < packs; i += kAhead * kThreads) {
+    for (int i = threadIdx.x; i < packs; i += kAhead * kThreads) {
         uint4 w[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) w[k] = at[i + k * kThreads];
+        for (int k = 0; k < kAhead; ++k)
+            w[k] = i + k * kThreads < packs ? at[i + k * kThreads] : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < kAhead; ++k) sum += squares<T>(w[k]);
     }
-    for (; i < packs; i += kThreads) sum += squares<T>(at[i]);
     return sum;
 }
 
 template <typename T>
-__device__ __forceinline__ void scale_run(T* p, long long n, float f) {
+__device__ __forceinline__ void scale_run(T* p, int n, float f) {
     constexpr int V = 16 / sizeof(T);
-    const long long head = head_of(p, n), packs = (n - head) / V, tail = head + packs * V;
-    for (long long i = threadIdx.x; i < head + (n - tail); i += kThreads) {
+    const int head = head_of(p, n), packs = (n - head) / V, tail = head + packs * V;
+    for (int i = threadIdx.x; i < head + (n - tail); i += kThreads) {
         T* at = p + (i < head ? i : tail + (i - head));
         *at = from_f<T>(to_f(*at) * f);
     }
@@ -146,15 +145,15 @@ __device__ __forceinline__ void scale_run(T* p, long long n, float f) {
         for (int j = 0; j < V; ++j) q.v[j] = from_f<T>(to_f(q.v[j]) * f);
         return q.w;
     };
-    long long i = packs - 1 - threadIdx.x;
-    for (; i - (kAhead - 1) * kThreads >= 0; i -= kAhead * kThreads) {
+    for (int i = threadIdx.x; i < packs; i += kAhead * kThreads) {
         uint4 w[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) w[k] = at[i - k * kThreads];
+        for (int k = 0; k < kAhead; ++k)
+            if (i + k * kThreads < packs) w[k] = at[i + k * kThreads];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) at[i - k * kThreads] = scaled(w[k]);
+        for (int k = 0; k < kAhead; ++k)
+            if (i + k * kThreads < packs) at[i + k * kThreads] = scaled(w[k]);
     }
-    for (; i >= 0; i -= kThreads) at[i] = scaled(at[i]);
 }
 
 // Sum over the CTA, in thread 0 of it.
@@ -169,18 +168,26 @@ __device__ __forceinline__ double cta_sum(double x) {
     return x;
 }
 
+// f(values, how many) of run c.
+template <int N, typename F>
+__device__ __forceinline__ void with_run(const Runs<N>& a, int c, F&& f) {
+    const Run& t = a.t[find(a, c)];
+    const long long lo = (long long)(c - t.first) * a.per, left = t.n - lo;
+    const int n = left < a.per ? (int)left : a.per;
+    if (t.dtype == SN_F32)
+        f(static_cast<float*>(t.p) + lo, n);
+    else if (t.dtype == SN_BF16)
+        f(static_cast<__nv_bfloat16*>(t.p) + lo, n);
+    else
+        f(static_cast<__half*>(t.p) + lo, n);
+}
+
 template <int N>
 __global__ void __launch_bounds__(kThreads) square_kernel(const __grid_constant__ Runs<N> a, double* parts) {
     pdl_trigger();
-    const Run& t = a.t[find(a, blockIdx.x)];
-    const long long lo = (blockIdx.x - t.first) * a.per, n = min(a.per, t.n - lo);
-    double x;
-    if (t.dtype == SN_F32)
-        x = square_run(static_cast<const float*>(t.p) + lo, n);
-    else if (t.dtype == SN_BF16)
-        x = square_run(static_cast<const __nv_bfloat16*>(t.p) + lo, n);
-    else
-        x = square_run(static_cast<const __half*>(t.p) + lo, n);
+    double x = 0.0;
+    for (int c = blockIdx.x; c < a.runs; c += gridDim.x)
+        with_run(a, c, [&](const auto* p, int n) { x += square_run(p, n); });
     x = cta_sum(x);
     if (threadIdx.x == 0) parts[blockIdx.x] = x;
 }
@@ -222,14 +229,8 @@ scale_kernel(const __grid_constant__ Runs<N> a, const double* parts, int n_parts
         if (factor) *factor = r.y;
     }
     if (r.y == 1.0f) return;
-    const Run& t = a.t[find(a, blockIdx.x)];
-    const long long lo = (blockIdx.x - t.first) * a.per, n = min(a.per, t.n - lo);
-    if (t.dtype == SN_F32)
-        scale_run(static_cast<float*>(t.p) + lo, n, r.y);
-    else if (t.dtype == SN_BF16)
-        scale_run(static_cast<__nv_bfloat16*>(t.p) + lo, n, r.y);
-    else
-        scale_run(static_cast<__half*>(t.p) + lo, n, r.y);
+    for (int c = a.runs - 1 - blockIdx.x; c >= 0; c -= gridDim.x)
+        with_run(a, c, [&](auto* p, int n) { scale_run(p, n, r.y); });
 }
 
 // Launched so that it may start when the kernel before has, and waits for it.
@@ -269,21 +270,13 @@ int check_list(const char* what, const Call& c, double max_norm, long long* tota
     return SN_OK;
 }
 
-long long run_values(long long total) {
-    const long long per = (total + kWave - 1) / kWave;
-    return std::max(1ll, (per + kLeast - 1) / kLeast) * kLeast;
-}
+// How a list is cut up: launches of up to kMany tensors, each of up to kWave CTAs.
+int run_values(long long total) { return total >= 2ll * kWave * kRun ? kRun : kShort; }
 
-long long runs_of(const Call& c, long long per) {
-    long long n = 0;
-    for (int i = 0; i < c.count; ++i) n += (c.sizes[i] + per - 1) / per;
-    return n;
-}
-
-// Launches of up to kMany tensors: f(runs, ctas, runs before them).
+// f(runs, CTAs, parts before them) for each launch; how many parts there are.
 template <typename F>
-int each_launch(const Call& c, long long per, F&& f) {
-    long long before = 0;
+int each_launch(const Call& c, int per, long long* parts, F&& f) {
+    *parts = 0;
     for (int i = 0; i < c.count;) {
         Runs<kMany> a;
         a.count = 0;
@@ -291,20 +284,26 @@ int each_launch(const Call& c, long long per, F&& f) {
         long long n = 0;
         for (; i < c.count && a.count < kMany; ++i)
             if (c.sizes[i]) {
-                a.t[a.count++] = {c.grads[i], c.sizes[i], (int)n, c.dtypes[i]};
-                n += (c.sizes[i] + per - 1) / per;
+                const long long more = (c.sizes[i] + per - 1) / per;
+                if (n + more > 0x7fffffffll - kWave) {
+                    if (a.count) break;
+                    return fail(SN_E_INVAL, "grad_norm: a tensor of %lld values", (long long)c.sizes[i]);
+                }
+                a.t[a.count++] = {c.grads ? c.grads[i] : nullptr, c.sizes[i], (int)n, c.dtypes ? c.dtypes[i] : 0};
+                n += more;
             }
         if (!a.count) break;
+        a.runs = (int)n;
+        const unsigned ctas = (unsigned)std::min(n, (long long)kWave);
         if (a.count <= kFew) {
             Runs<kFew> b;
-            b.count = a.count;
-            b.per = per;
+            b.count = a.count, b.runs = a.runs, b.per = per;
             for (int k = 0; k < a.count; ++k) b.t[k] = a.t[k];
-            SN_TRY(f(b, (unsigned)n, before));
+            SN_TRY(f(b, ctas, *parts));
         } else {
-            SN_TRY(f(a, (unsigned)n, before));
+            SN_TRY(f(a, ctas, *parts));
         }
-        before += n;
+        *parts += ctas;
     }
     return SN_OK;
 }
@@ -313,8 +312,9 @@ int norm_or_clip(const char* what, const Call& c, double max_norm, bool clip, fl
                  int64_t ws_bytes, void* cuda_stream) {
     long long total;
     SN_TRY(check_list(what, c, max_norm, &total));
-    const long long per = run_values(total), n = runs_of(c, per);
-    if (n > 0x7fffffffll) return fail(SN_E_INVAL, "%s: too many tensors", what);
+    const int per = run_values(total);
+    long long n = 0;
+    SN_TRY(each_launch(c, per, &n, [](const auto&, unsigned, long long) { return SN_OK; }));
     if (n && (!ws || ws_bytes < n * 8)) return fail(SN_E_INVAL, "%s: a workspace of %lld bytes is wanted", what, n * 8);
     CallerDevice dev;
     for (int i = 0; i < c.count; ++i)
@@ -323,19 +323,19 @@ int norm_or_clip(const char* what, const Call& c, double max_norm, bool clip, fl
     SN_TRY(dev.select(what));
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     double* parts = static_cast<double*>(ws);
-    SN_TRY(each_launch(c, per, [&](const auto& a, unsigned ctas, long long before) {
+    SN_TRY(each_launch(c, per, &n, [&](const auto& a, unsigned ctas, long long before) {
         constexpr int N = sizeof(a.t) / sizeof(a.t[0]);
         square_kernel<N><<<ctas, kThreads, 0, st>>>(a, parts + before);
         return cuda_check(cudaGetLastError(), "grad_norm launch");
     }));
-    if (!clip || !n) return launch_behind(norm_kernel, 1u, st, (const double*)parts, (int)n, max_norm, norm, factor);
-    return each_launch(c, per, [&](const auto& a, unsigned ctas, long long before) {
+    const int count = (int)n;
+    if (!clip || !n) return launch_behind(norm_kernel, 1u, st, (const double*)parts, count, max_norm, norm, factor);
+    return each_launch(c, per, &n, [&](const auto& a, unsigned ctas, long long before) {
         constexpr int N = sizeof(a.t) / sizeof(a.t[0]);
-        (void)before;
         // (only the first of several may start early: its launch is the one behind the squares)
         if (!before)
-            return launch_behind(scale_kernel<N>, ctas, st, a, (const double*)parts, (int)n, max_norm, norm, factor);
-        scale_kernel<N><<<ctas, kThreads, 0, st>>>(a, parts, (int)n, max_norm, nullptr, nullptr);
+            return launch_behind(scale_kernel<N>, ctas, st, a, (const double*)parts, count, max_norm, norm, factor);
+        scale_kernel<N><<<ctas, kThreads, 0, st>>>(a, parts, count, max_norm, nullptr, nullptr);
         return cuda_check(cudaGetLastError(), "clip_grads launch");
     });
 }
@@ -354,7 +354,10 @@ int64_t sn_abi_grad_norm_ws(int32_t count, const int64_t* sizes) {
         if (sizes[i] < 0 || sizes[i] > (1ll << 46) - total) return -1;
         total += sizes[i];
     }
-    return 8 * runs_of({count, nullptr, sizes, nullptr}, run_values(total));
+    long long n = 0;
+    const int rc = each_launch({count, nullptr, sizes, nullptr}, run_values(total), &n,
+                               [](const auto&, unsigned, long long) { return SN_OK; });
+    return rc == SN_OK ? 8 * n : -1;
 }
 
 sn_status sn_abi_grad_norm(int32_t count, const void* const* grads, const int64_t* sizes, const int32_t* dtypes,

@@ -9,6 +9,10 @@
 // layer_norm: the call and its node in the autograd graph. A call and its
 // gradients take 75 us of the host's time (torch's own layer norm 70), as a
 // Function in Python 110; a call without a graph 8 us instead of 11.
+//
+// embedding, linear_attention (calls and nodes alike) and linear_attention_step:
+// with their checks in Python they took 20 to 30 us of the host's time a call,
+// longer than most of their kernels.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -21,7 +25,10 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
+#include <initializer_list>
+#include <optional>
 #include <stdexcept>
 #include <string>
 #include <utility>
@@ -37,6 +44,13 @@ struct {
     decltype(&sn_abi_layer_norm_bwd) norm_bwd = nullptr;
     decltype(&sn_abi_layer_norm_bwd_ws) norm_bwd_ws = nullptr;
     decltype(&sn_abi_last_error) last_error = nullptr;
+    decltype(&sn_abi_embedding) embedding = nullptr;
+    decltype(&sn_abi_embedding_bwd) embedding_bwd = nullptr;
+    decltype(&sn_abi_embedding_bwd_ws) embedding_bwd_ws = nullptr;
+    decltype(&sn_abi_linear_attention) attention = nullptr;
+    decltype(&sn_abi_linear_attention_bwd) attention_bwd = nullptr;
+    decltype(&sn_abi_linear_attention_ws) attention_ws = nullptr;
+    decltype(&sn_abi_linear_attention_step) attention_step = nullptr;
 } lib;
 
 std::string last_error() {
@@ -142,7 +156,7 @@ struct Norm : torch::autograd::Function<Norm> {
 bool tensor_of(PyObject* o, at::Tensor* t) {
     if (o == Py_None) return true;
     if (!THPVariable_Check(o)) {
-        PyErr_SetString(PyExc_TypeError, "layer_norm: tensors are wanted");
+        PyErr_SetString(PyExc_TypeError, "tensors are wanted");
         return false;
     }
     *t = THPVariable_Unpack(o);
@@ -171,14 +185,292 @@ PyObject* layer_norm(PyObject*, PyObject* args) {
     END_HANDLE_TH_ERRORS
 }
 
-// use(layer_norm, layer_norm_bwd, layer_norm_bwd_ws, last_error): their addresses.
+bool float_type(const at::Tensor& t) {
+    const at::ScalarType k = t.scalar_type();
+    return k == at::kFloat || k == at::kBFloat16 || k == at::kHalf;
+}
+
+bool wants_grad(std::initializer_list<at::Tensor> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const at::Tensor& t : ts)
+        if (t.defined() && t.requires_grad()) return true;
+    return false;
+}
+
+// (no call here carries a tangent on)
+void no_tangent(const char* what, std::initializer_list<at::Tensor> ts) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const at::Tensor& t : ts)
+        TORCH_CHECK(!(t.defined() && t._fw_grad(0).defined()), what, " has no forward-mode derivative");
+}
+
+at::Tensor space(int64_t bytes, const at::Tensor& like) {
+    return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
+// ------------------------------------------------------------------ embedding
+at::Tensor embedding_forward(const at::Tensor& tokens, const at::Tensor& w, double scale) {
+    std::vector<int64_t> sizes(tokens.sizes().begin(), tokens.sizes().end());
+    sizes.push_back(w.size(1));
+    at::Tensor out = at::empty(sizes, w.options());
+    const int rc = lib.embedding(address(tokens), 8 * (int32_t)tokens.element_size(), tokens.numel(), address(w),
+                                 w.stride(0), w.size(0), (int32_t)w.size(1), code(w.scalar_type()), (float)scale,
+                                 address(out), stream_of(w));
+    TORCH_CHECK(rc == SN_OK, "embedding: ", last_error());
+    return out;
+}
+
+struct Embedding : torch::autograd::Function<Embedding> {
+    static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& tokens,
+                              const at::Tensor& w, double scale) {
+        ctx->save_for_backward({tokens});
+        ctx->saved_data["rows"] = w.size(0);
+        ctx->saved_data["scale"] = scale;
+        return embedding_forward(tokens, w, scale);
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "embedding can be differentiated once");
+        const at::Tensor tokens = ctx->get_saved_variables()[0], &dout = grads[0];
+        const int64_t V = ctx->saved_data["rows"].toInt(), D = dout.size(-1), n = tokens.numel();
+        at::Tensor rows = dout.reshape({n, D});  // a view wherever the rows lie at one stride
+        if (D > 1 && rows.stride(1) != 1) rows = rows.contiguous();
+        at::Tensor dw = at::empty({V, D}, dout.options());
+        const int64_t need = lib.embedding_bwd_ws(n, V, (int32_t)D);
+        const at::Tensor ws = space(need, dout);
+        const int rc = lib.embedding_bwd(address(tokens), 8 * (int32_t)tokens.element_size(), n, address(rows),
+                                         rows.stride(0), V, (int32_t)D, code(dout.scalar_type()),
+                                         (float)ctx->saved_data["scale"].toDouble(), address(dw), address(ws),
+                                         need, stream_of(dout));
+        TORCH_CHECK(rc == SN_OK, "embedding_bwd: ", last_error());
+        return {at::Tensor(), dw, at::Tensor()};
+    }
+};
+
+// embedding(tokens, weight, scale)
+PyObject* embedding(PyObject*, PyObject* args) {
+    HANDLE_TH_ERRORS
+    PyObject *to, *wo;
+    double scale;
+    if (!PyArg_ParseTuple(args, "OOd", &to, &wo, &scale)) return nullptr;
+    at::Tensor tokens, w;
+    if (!tensor_of(to, &tokens) || !tensor_of(wo, &w)) return nullptr;
+    TORCH_CHECK_VALUE(w.defined() && w.dim() == 2 && w.is_cuda() && w.size(1) <= 1 << 30 && w.size(0) < 0x7fffffff,
+                      "embedding: weight (V, D) on a GPU is wanted");
+    TORCH_CHECK_TYPE(float_type(w), "embedding: weight is float32, bfloat16 or float16");
+    TORCH_CHECK_VALUE(tokens.defined() && (tokens.scalar_type() == at::kInt || tokens.scalar_type() == at::kLong) &&
+                          tokens.device() == w.device() && tokens.numel() <= 0x7fffffff,
+                      "embedding: tokens are int32 or int64 on the weight's GPU");
+    TORCH_CHECK_VALUE(std::isfinite(scale), "embedding: the scale is not finite");
+    no_tangent("embedding", {w});
+    tokens = tokens.contiguous();
+    if (w.size(1) > 1 && w.stride(1) != 1) w = w.contiguous();
+    if (wants_grad({w})) return THPVariable_Wrap(Embedding::apply(tokens, w, scale));
+    return THPVariable_Wrap(embedding_forward(tokens, w, scale));
+    END_HANDLE_TH_ERRORS
+}
+
+// ----------------------------------------------------------- linear attention
+constexpr int64_t kMaxHead = 128;
+
+// The checked arguments of a call. Tensors are made fit for it in place.
+SnAbiLinearAttention attention_call(const char* what, at::Tensor& q, at::Tensor& k, at::Tensor& v,
+                                    at::Tensor& decay, at::Tensor* state, at::Tensor* lengths, double scale) {
+    TORCH_CHECK_VALUE(q.dim() == 4 && v.dim() == 4 && k.sizes() == q.sizes() && v.size(0) == q.size(0) &&
+                          v.size(1) == q.size(1),
+                      what, ": q and k are (B, T, Hk, dk), v (B, T, H, dv)");
+    const int64_t B = q.size(0), T = q.size(1), Hk = q.size(2), dk = q.size(3), H = v.size(2), dv = v.size(3);
+    TORCH_CHECK_VALUE(Hk > 0 && H > 0 && H % Hk == 0 && dk > 0 && dk <= kMaxHead && dv > 0 && dv <= kMaxHead, what,
+                      ": heads of 1 to 128 values, H a multiple of Hk");
+    TORCH_CHECK_VALUE(T < 0x7fffffff - 128 && B * H <= 0x7fffffff, what, ": sizes beyond 31 bits");
+    TORCH_CHECK_TYPE(float_type(v), what, ": q, k and v are float32, bfloat16 or float16");
+    TORCH_CHECK_VALUE(v.is_cuda() && q.scalar_type() == v.scalar_type() && k.scalar_type() == v.scalar_type() &&
+                          q.device() == v.device() && k.device() == v.device(),
+                      what, ": q, k and v are of one type, on one GPU");
+    TORCH_CHECK_VALUE(decay.scalar_type() == at::kFloat && decay.device() == v.device() &&
+                          (decay.sizes() == at::IntArrayRef({H}) || decay.sizes() == at::IntArrayRef({B, T, H})),
+                      what, ": log_decay is float32 of (H) or (B, T, H) on the GPU of the others");
+    TORCH_CHECK_VALUE(std::isfinite(scale), what, ": the scale is not finite");
+    SnAbiLinearAttention a = {};
+    if (state && state->defined()) {
+        TORCH_CHECK_VALUE(state->scalar_type() == at::kFloat && state->device() == v.device() &&
+                              state->sizes() == at::IntArrayRef({B, H, dk, dv}),
+                          what, ": state is float32 of (B, H, dk, dv) on the GPU of the others");
+        *state = state->contiguous();
+        a.state = state->data_ptr<float>();
+    }
+    if (lengths && lengths->defined()) {
+        TORCH_CHECK_VALUE(lengths->scalar_type() == at::kInt && lengths->device() == v.device() &&
+                              lengths->sizes() == at::IntArrayRef({B}),
+                          what, ": lengths are (B) int32 values on the GPU of the others");
+        *lengths = lengths->contiguous();
+        a.lengths = lengths->data_ptr<int32_t>();
+    }
+    const auto rows = [](at::Tensor& t, const void** p, int64_t* stride) {
+        if (t.size(3) > 1 && t.stride(3) != 1) t = t.contiguous();
+        *p = t.data_ptr();
+        for (int i = 0; i < 3; ++i) stride[i] = t.stride(i);
+    };
+    rows(q, &a.q, a.q_stride);
+    rows(k, &a.k, a.k_stride);
+    rows(v, &a.v, a.v_stride);
+    a.log_decay = decay.data_ptr<float>();
+    for (int i = 0; i < 3; ++i)
+        a.log_decay_stride[i] = decay.dim() == 3 ? decay.stride(i) : i == 2 ? decay.stride(0) : 0;
+    a.dtype = code(v.scalar_type());
+    a.B = (int32_t)B, a.T = (int32_t)T, a.H = (int32_t)H, a.Hk = (int32_t)Hk, a.dk = (int32_t)dk, a.dv = (int32_t)dv;
+    a.scale = (float)scale;
+    return a;
+}
+
+std::pair<at::Tensor, at::Tensor> attention_forward(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor decay,
+                                                    at::Tensor state, at::Tensor lengths, double scale) {
+    const SnAbiLinearAttention a = attention_call("linear_attention", q, k, v, decay, &state, &lengths, scale);
+    at::Tensor out = at::empty(v.sizes(), v.options());
+    at::Tensor end = at::empty({a.B, a.H, a.dk, a.dv}, v.options().dtype(at::kFloat));
+    const int64_t need = lib.attention_ws(&a, 0, 0);
+    const at::Tensor ws = space(need, v);
+    const int rc = lib.attention(&a, address(out), end.data_ptr<float>(), address(ws), need, stream_of(v));
+    TORCH_CHECK(rc == SN_OK, "linear_attention: ", last_error());
+    return {out, end};
+}
+
+struct Attention : torch::autograd::Function<Attention> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
+                                                  const at::Tensor& k, const at::Tensor& v,
+                                                  const at::Tensor& decay,
+                                                  const std::optional<at::Tensor>& state_,
+                                                  const std::optional<at::Tensor>& lengths_, double scale) {
+        const at::Tensor state = state_.value_or(at::Tensor()), lengths = lengths_.value_or(at::Tensor());
+        ctx->save_for_backward({q, k, v, decay, state, lengths});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["scale"] = scale;
+        auto [out, end] = attention_forward(q, k, v, decay, state, lengths, scale);
+        return {out, end};
+    }
+
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                   torch::autograd::variable_list grads) {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "linear_attention can be differentiated once");
+        auto saved = ctx->get_saved_variables();
+        at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &decay = saved[3], &state = saved[4];
+        const bool has_state = state.defined();
+        const auto qs = q.sizes().vec(), ks = k.sizes().vec();
+        const SnAbiLinearAttention a = attention_call("linear_attention_bwd", q, k, v, decay, &state, &saved[5],
+                                                      ctx->saved_data["scale"].toDouble());
+        at::Tensor dout = grads[0], dend = grads[1];
+        if (!dout.defined()) dout = at::zeros(v.sizes(), v.options());
+        if (a.dv > 1 && dout.stride(3) != 1) dout = dout.contiguous();
+        if (dend.defined()) dend = dend.contiguous();
+        at::Tensor dq = at::empty(qs, q.options()), dk = at::empty(ks, k.options()),
+                   dv = at::empty(v.sizes(), v.options()), dg, ds;
+        if (ctx->needs_input_grad(3)) dg = at::empty(decay.sizes(), decay.options());
+        if (has_state && ctx->needs_input_grad(4)) ds = at::empty(state.sizes(), state.options());
+        const int32_t heads = dg.defined() && decay.dim() == 1;
+        if (a.B) {
+            const int64_t need = lib.attention_ws(&a, 1, heads);
+            const at::Tensor ws = space(need, v);
+            const int64_t stride[3] = {dout.stride(0), dout.stride(1), dout.stride(2)};
+            const int rc = lib.attention_bwd(&a, address(dout), stride, static_cast<float*>(address(dend)),
+                                             address(dq), address(dk), address(dv),
+                                             static_cast<float*>(address(dg)), heads,
+                                             static_cast<float*>(address(ds)), address(ws), need, stream_of(v));
+            TORCH_CHECK(rc == SN_OK, "linear_attention_bwd: ", last_error());
+        } else if (dg.defined()) {
+            dg.zero_();
+        }
+        return {dq, dk, dv, dg, ds, at::Tensor(), at::Tensor()};
+    }
+};
+
+// The tensors of a call's arguments and its scale (None: 1 / sqrt of q's last axis).
+bool attention_args(PyObject* const* o, int n, at::Tensor* t, PyObject* scale, double* to) {
+    for (int i = 0; i < n; ++i) {
+        if (!tensor_of(o[i], t + i)) return false;
+        if (i < 4 && !t[i].defined()) {
+            PyErr_SetString(PyExc_TypeError, "linear_attention: tensors are wanted");
+            return false;
+        }
+    }
+    if (scale != Py_None) {
+        *to = PyFloat_AsDouble(scale);
+        return !(*to == -1.0 && PyErr_Occurred());
+    }
+    *to = t[0].dim() && t[0].size(-1) > 0 ? 1.0 / std::sqrt((double)t[0].size(-1)) : 1.0;
+    return true;
+}
+
+// linear_attention(q, k, v, log_decay, state, lengths, scale) -> (out, state)
+PyObject* linear_attention(PyObject*, PyObject* args) {
+    HANDLE_TH_ERRORS
+    PyObject *o[6], *so;
+    if (!PyArg_ParseTuple(args, "OOOOOOO", o, o + 1, o + 2, o + 3, o + 4, o + 5, &so)) return nullptr;
+    at::Tensor t[6];
+    double scale;
+    if (!attention_args(o, 6, t, so, &scale)) return nullptr;
+    no_tangent("linear_attention", {t[0], t[1], t[2], t[3], t[4]});
+    std::pair<at::Tensor, at::Tensor> r;
+    if (wants_grad({t[0], t[1], t[2], t[3], t[4]})) {
+        const auto some = [](const at::Tensor& x) { return x.defined() ? std::optional<at::Tensor>(x) : std::nullopt; };
+        auto both = Attention::apply(t[0], t[1], t[2], t[3], some(t[4]), some(t[5]), scale);
+        r = {both[0], both[1]};
+    } else {
+        r = attention_forward(t[0], t[1], t[2], t[3], t[4], t[5], scale);
+    }
+    return Py_BuildValue("(NN)", THPVariable_Wrap(r.first), THPVariable_Wrap(r.second));
+    END_HANDLE_TH_ERRORS
+}
+
+// linear_attention_step(q, k, v, log_decay, state, scale) -> out; state is updated
+PyObject* linear_attention_step(PyObject*, PyObject* args) {
+    HANDLE_TH_ERRORS
+    PyObject *o[5], *so;
+    if (!PyArg_ParseTuple(args, "OOOOOO", o, o + 1, o + 2, o + 3, o + 4, &so)) return nullptr;
+    at::Tensor t[5];
+    double scale;
+    if (!attention_args(o, 5, t, so, &scale)) return nullptr;
+    const char* const what = "linear_attention_step";
+    at::Tensor &q = t[0], &k = t[1], &v = t[2], &decay = t[3], &state = t[4];
+    TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, what,
+                      ": q and k are (B, Hk, dk), v (B, H, dv)");
+    no_tangent(what, {q, k, v, decay, state});
+    TORCH_CHECK_VALUE(!wants_grad({q, k, v, decay, state}), what, " has no gradient: call linear_attention");
+    at::Tensor out = at::empty(v.sizes(), v.options());
+    const at::Tensor shape = v;
+    q = q.unsqueeze(1), k = k.unsqueeze(1), v = v.unsqueeze(1);
+    if (decay.dim() == 2) decay = decay.unsqueeze(1);
+    const SnAbiLinearAttention a = attention_call(what, q, k, v, decay, nullptr, nullptr, scale);
+    TORCH_CHECK_VALUE(state.defined() && state.scalar_type() == at::kFloat && state.device() == v.device() &&
+                          state.sizes() == at::IntArrayRef({a.B, a.H, a.dk, a.dv}) &&
+                          (!a.B || state.select(0, 0).is_contiguous()),
+                      what, ": state is float32 of (B, H, dk, dv) on the GPU of the others, each sequence's contiguous");
+    TORCH_CHECK_VALUE(a.B < 2 || state.stride(0) >= (int64_t)a.H * a.dk * a.dv, what, ": the states overlap");
+    const int rc = lib.attention_step(&a, static_cast<float*>(address(state)), a.B ? state.stride(0) : 0,
+                                      address(out), stream_of(v));
+    TORCH_CHECK(rc == SN_OK, last_error());
+    state.unsafeGetTensorImpl()->bump_version();  // a graph that saved it must not use it
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// use(addresses of the library's entry points, in the order below)
 PyObject* use(PyObject*, PyObject* args) {
-    unsigned long long p[4];
-    if (!PyArg_ParseTuple(args, "KKKK", p, p + 1, p + 2, p + 3)) return nullptr;
+    unsigned long long p[11];
+    if (!PyArg_ParseTuple(args, "KKKKKKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, p + 7, p + 8, p + 9,
+                          p + 10))
+        return nullptr;
     lib.norm = reinterpret_cast<decltype(lib.norm)>(p[0]);
     lib.norm_bwd = reinterpret_cast<decltype(lib.norm_bwd)>(p[1]);
     lib.norm_bwd_ws = reinterpret_cast<decltype(lib.norm_bwd_ws)>(p[2]);
     lib.last_error = reinterpret_cast<decltype(lib.last_error)>(p[3]);
+    lib.embedding = reinterpret_cast<decltype(lib.embedding)>(p[4]);
+    lib.embedding_bwd = reinterpret_cast<decltype(lib.embedding_bwd)>(p[5]);
+    lib.embedding_bwd_ws = reinterpret_cast<decltype(lib.embedding_bwd_ws)>(p[6]);
+    lib.attention = reinterpret_cast<decltype(lib.attention)>(p[7]);
+    lib.attention_bwd = reinterpret_cast<decltype(lib.attention_bwd)>(p[8]);
+    lib.attention_ws = reinterpret_cast<decltype(lib.attention_ws)>(p[9]);
+    lib.attention_step = reinterpret_cast<decltype(lib.attention_step)>(p[10]);
     Py_RETURN_NONE;
 }
 
@@ -345,6 +637,11 @@ PyMethodDef methods[] = {
     {"read_grads", read_grads, METH_VARARGS,
      "read_grads(list, apart) -> (addresses, sizes, types, index of the GPU)"},
     {"layer_norm", layer_norm, METH_VARARGS, "layer_norm(x, weight, bias, eps) -> y"},
+    {"embedding", embedding, METH_VARARGS, "embedding(tokens, weight, scale) -> rows"},
+    {"linear_attention", linear_attention, METH_VARARGS,
+     "linear_attention(q, k, v, log_decay, state, lengths, scale) -> (out, state)"},
+    {"linear_attention_step", linear_attention_step, METH_VARARGS,
+     "linear_attention_step(q, k, v, log_decay, state, scale) -> out"},
     {"use", use, METH_VARARGS, "use(addresses of the library's entry points)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, methods,

@@ -231,7 +231,9 @@ def _torch_calls():
                                "`python -m sunnynet_b200.build --force`") from e
         m.use(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
             lib.sn_abi_layer_norm, lib.sn_abi_layer_norm_bwd, lib.sn_abi_layer_norm_bwd_ws,
-            lib.sn_abi_last_error)))
+            lib.sn_abi_last_error, lib.sn_abi_embedding, lib.sn_abi_embedding_bwd,
+            lib.sn_abi_embedding_bwd_ws, lib.sn_abi_linear_attention, lib.sn_abi_linear_attention_bwd,
+            lib.sn_abi_linear_attention_ws, lib.sn_abi_linear_attention_step)))
         _TORCH_CALLS = m
     return _TORCH_CALLS
 
@@ -325,76 +327,13 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, bet
     torch.autograd.graph.increment_version(lists[0])  # a graph that saved one must not use it
 
 
-def _embedding_forward(tokens, weight, scale):
-    import torch
-    V, D = weight.shape
-    out = torch.empty(*tokens.shape, D, dtype=weight.dtype, device=weight.device)
-    rc = _lib_loaded().sn_abi_embedding(
-        tokens.data_ptr(), 8 * tokens.element_size(), tokens.numel(), weight.data_ptr(), weight.stride(0), V, D,
-        dtype_code(weight.dtype), scale, out.data_ptr(), current_stream(weight))
-    if rc:
-        check(rc, "embedding")
-    return out
-
-
-_EMBEDDING = None
-
-
-def _embedding_fn():
-    global _EMBEDDING
-    if _EMBEDDING is not None:
-        return _EMBEDDING
-    import torch
-
-    class _Embedding(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, tokens, weight, scale):
-            ctx.save_for_backward(tokens)
-            ctx.weight, ctx.scale = (weight.shape, weight.dtype), scale
-            return _embedding_forward(tokens, weight, scale)
-
-        @staticmethod
-        @torch.autograd.function.once_differentiable
-        def backward(ctx, dout):
-            (tokens,) = ctx.saved_tensors
-            (V, D), dtype = ctx.weight
-            rows = dout.reshape(tokens.numel(), D)  # a view wherever the rows lie at one stride
-            if D > 1 and rows.stride(1) != 1:
-                rows = rows.contiguous()
-            dw = torch.empty(V, D, dtype=dtype, device=dout.device)
-            lib, n = _lib_loaded(), tokens.numel()
-            need = lib.sn_abi_embedding_bwd_ws(n, V, D)
-            ws = torch.empty(need, dtype=torch.uint8, device=dout.device) if need > 0 else None
-            rc = lib.sn_abi_embedding_bwd(
-                tokens.data_ptr(), 8 * tokens.element_size(), n, rows.data_ptr(), rows.stride(0), V, D,
-                dtype_code(dtype), ctx.scale, dw.data_ptr(), None if ws is None else ws.data_ptr(), max(need, 0),
-                current_stream(dout))
-            if rc:
-                check(rc, "embedding_bwd")
-            return None, dw, None
-
-    _EMBEDDING = _Embedding
-    return _EMBEDDING
-
-
 def embedding(tokens, weight, scale: float = 1.0):
     """weight[tokens] * scale: rows (..., D) of weight (V, D) (float32, bfloat16
     or float16, on a GPU; rows may lie at a stride) for int32 or int64 tokens of
     any shape on that GPU. A token outside [0, V) gives a row of NaN, and adds
     nothing to the gradient. Differentiable once in weight: its gradient is dense,
     sums each row's tokens in fp32 in their order, and is the same bits every time."""
-    import torch
-    if weight.dim() != 2 or not weight.is_cuda:
-        raise ValueError("embedding: weight (V, D) on a GPU is wanted")
-    if tokens.dtype not in (torch.int32, torch.int64) or tokens.device != weight.device:
-        raise ValueError(f"embedding: tokens are int32 or int64 on {weight.device}")
-    dtype_code(weight.dtype)
-    tokens = tokens.contiguous()
-    if weight.shape[1] > 1 and weight.stride(1) != 1:
-        weight = weight.contiguous()
-    if torch.is_grad_enabled() and weight.requires_grad:
-        return _embedding_fn().apply(tokens, weight, float(scale))
-    return _embedding_forward(tokens, weight, float(scale))
+    return (_TORCH_CALLS or _torch_calls()).embedding(tokens, weight, scale)
 
 
 def _norm_call(name, grads, max_norm, apart):
@@ -439,117 +378,6 @@ def clip_grads(grads, max_norm):
     return ws[0]
 
 
-_MAX_HEAD = 128  # values of a head of linear_attention
-
-
-def _attention_call(what, q, k, v, log_decay, state, lengths, scale):
-    """The checked arguments of a linear-attention call; q (B, T, Hk, dk)."""
-    import torch
-    if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or v.shape[:2] != q.shape[:2]:
-        raise ValueError(f"{what}: q and k are (B, T, Hk, dk), v (B, T, H, dv)")
-    B, T, Hk, dk = q.shape
-    H, dv = v.shape[2:]
-    if Hk == 0 or H == 0 or H % Hk or not 0 < dk <= _MAX_HEAD or not 0 < dv <= _MAX_HEAD:
-        raise ValueError(f"{what}: heads of 1 to {_MAX_HEAD} values, H a multiple of Hk")
-    code, dev = dtype_code(q.dtype), v.device
-    if not v.is_cuda or k.dtype != q.dtype or v.dtype != q.dtype or q.device != dev or k.device != dev:
-        raise ValueError(f"{what}: q, k and v are of one type, on one GPU")
-    if log_decay.dtype != torch.float32 or log_decay.device != dev or \
-            tuple(log_decay.shape) not in ((H,), (B, T, H)):
-        raise ValueError(f"{what}: log_decay is float32 of ({H},) or ({B}, {T}, {H}) on {dev}")
-    if state is not None and (state.dtype != torch.float32 or state.device != dev or
-                              tuple(state.shape) != (B, H, dk, dv)):
-        raise ValueError(f"{what}: state is float32 of ({B}, {H}, {dk}, {dv}) on {dev}")
-    if lengths is not None and (lengths.dtype != torch.int32 or lengths.device != dev or
-                                tuple(lengths.shape) != (B,)):
-        raise ValueError(f"{what}: lengths are {B} int32 values on {dev}")
-    a = _lib.LinearAttention()
-    a.dtype, a.B, a.T, a.H, a.Hk, a.dk, a.dv = code, B, T, H, Hk, dk, dv
-    a.scale = dk ** -0.5 if scale is None else scale
-    keep = []  # copies that live until the call is made
-    for name, t, d in (("q", q, dk), ("k", k, dk), ("v", v, dv)):
-        if d > 1 and t.stride(3) != 1:
-            t = t.contiguous()
-            keep.append(t)
-        setattr(a, name, t.data_ptr())
-        setattr(a, name + "_stride", t.stride()[:3])
-    a.log_decay = log_decay.data_ptr()
-    a.log_decay_stride = log_decay.stride() if log_decay.dim() == 3 else (0, 0, log_decay.stride(0))
-    for name, t in (("state", state), ("lengths", lengths)):
-        if t is not None:
-            if not t.is_contiguous():
-                t = t.contiguous()
-                keep.append(t)
-            setattr(a, name, t.data_ptr())
-    return a, keep
-
-
-def _attention_forward(q, k, v, log_decay, state, lengths, scale):
-    import torch
-    a, keep = _attention_call("linear_attention", q, k, v, log_decay, state, lengths, scale)
-    lib, ref = _lib_loaded(), ctypes.byref(a)
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    end = torch.empty(a.B, a.H, a.dk, a.dv, dtype=torch.float32, device=v.device)
-    need = lib.sn_abi_linear_attention_ws(ref, 0, 0)
-    ws = torch.empty(need, dtype=torch.uint8, device=v.device) if need > 0 else None
-    rc = lib.sn_abi_linear_attention(ref, out.data_ptr(), end.data_ptr(),
-                                     ws.data_ptr() if need > 0 else None, max(need, 0), current_stream(v))
-    if rc:
-        check(rc, "linear_attention")
-    del keep
-    return out, end
-
-
-_ATTENTION = None
-
-
-def _attention_fn():
-    global _ATTENTION
-    if _ATTENTION is not None:
-        return _ATTENTION
-    import torch
-
-    class _Attention(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, q, k, v, log_decay, state, lengths, scale):
-            ctx.save_for_backward(q, k, v, log_decay, state, lengths)
-            ctx.scale = scale
-            ctx.set_materialize_grads(False)
-            return _attention_forward(q, k, v, log_decay, state, lengths, scale)
-
-        @staticmethod
-        @torch.autograd.function.once_differentiable
-        def backward(ctx, dout, dend):
-            q, k, v, log_decay, state, lengths = ctx.saved_tensors
-            a, keep = _attention_call("linear_attention_bwd", q, k, v, log_decay, state, lengths, ctx.scale)
-            dout = torch.zeros_like(v) if dout is None else dout
-            if a.dv > 1 and dout.stride(3) != 1:
-                dout = dout.contiguous()
-            dend = None if dend is None else dend.contiguous()
-            lib, ref = _lib_loaded(), ctypes.byref(a)
-            new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-            dq, dk, dv = new(q), new(k), new(v)
-            dg = new(log_decay) if ctx.needs_input_grad[3] else None
-            ds = new(state) if ctx.needs_input_grad[4] else None
-            gates = int(dg is not None and log_decay.dim() == 1)
-            if a.B == 0 and dg is not None:
-                dg.zero_()
-            need = lib.sn_abi_linear_attention_ws(ref, 1, gates)
-            ws = torch.empty(need, dtype=torch.uint8, device=v.device) if need > 0 else None
-            to = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-            if a.B:
-                rc = lib.sn_abi_linear_attention_bwd(
-                    ref, to(dout), (_lib.I64 * 3)(*dout.stride()[:3]), to(dend), to(dq), to(dk), to(dv),
-                    to(dg), gates, to(ds), to(ws), max(need, 0), current_stream(v))
-                if rc:
-                    check(rc, "linear_attention_bwd")
-            del keep
-            return dq, dk, dv, dg, ds, None, None
-
-    _ATTENTION = _Attention
-    return _ATTENTION
-
-
 def linear_attention(q, k, v, log_decay, state=None, lengths=None, scale=None):
     """(out, last state) of linear attention with a decay for each head:
     S_t = exp(log_decay_t) S_(t-1) + k_t v_t^T, out_t = scale * S_t^T q_t.
@@ -563,34 +391,11 @@ def linear_attention(q, k, v, log_decay, state=None, lengths=None, scale=None):
     float32. Differentiable once in q, k, v, log_decay and state. Sums and states
     are fp32; products take 16-bit parts of their factors, two of each for
     float16 and float32 (2^-17 of a value). The same call gives the same bits."""
-    import torch
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or
-                                    log_decay.requires_grad or (state is not None and state.requires_grad)):
-        return _attention_fn().apply(q, k, v, log_decay, state, lengths, scale)
-    return _attention_forward(q, k, v, log_decay, state, lengths, scale)
+    return (_TORCH_CALLS or _torch_calls()).linear_attention(q, k, v, log_decay, state, lengths, scale)
 
 
 def linear_attention_step(q, k, v, log_decay, state, scale=None):
     """out (B, H, dv) of one token of each sequence, ``linear_attention`` of T = 1:
     q, k (B, Hk, dk), v (B, H, dv), log_decay (H,) or (B, H); state (B, H, dk,
     dv), in float32, is updated in place (the sequences may lie at a stride)."""
-    import torch
-    if q.dim() != 3 or v.dim() != 3 or k.dim() != 3:
-        raise ValueError("linear_attention_step: q and k are (B, Hk, dk), v (B, H, dv)")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
-        raise ValueError("linear_attention_step has no gradient: call linear_attention")
-    gate = log_decay[:, None] if log_decay.dim() == 2 else log_decay
-    a, keep = _attention_call("linear_attention_step", q[:, None], k[:, None], v[:, None], gate, None, None,
-                              scale)
-    if state.dtype != torch.float32 or state.device != v.device or \
-            tuple(state.shape) != (a.B, a.H, a.dk, a.dv) or (a.B and not state[0].is_contiguous()):
-        raise ValueError(f"linear_attention_step: state is float32 of ({a.B}, {a.H}, {a.dk}, {a.dv}) on "
-                         f"{v.device}, each sequence's contiguous")
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    rc = _lib_loaded().sn_abi_linear_attention_step(ctypes.byref(a), state.data_ptr(), state.stride(0),
-                                                    out.data_ptr(), current_stream(v))
-    if rc:
-        check(rc, "linear_attention_step")
-    torch.autograd.graph.increment_version([state])  # a graph that saved it must not use it
-    del keep
-    return out
+    return (_TORCH_CALLS or _torch_calls()).linear_attention_step(q, k, v, log_decay, state, scale)

@@ -176,10 +176,8 @@ def test_refusals(kernels):
     for tokens, weight in ((t, w[0]), (t.float(), w), (t.cpu(), w), (t, w.cpu()), (t, w.double()), (t, w.long())):
         with pytest.raises((ValueError, TypeError)):
             kernels.embedding(tokens, weight)
-    from sunnynet_b200._lib import SnError
-    with pytest.raises(SnError, match="scale"):
+    with pytest.raises(ValueError, match="scale"):
         kernels.embedding(t, w, float("nan"))
     x = w.requires_grad_()
-    (dw,) = torch.autograd.grad(kernels.embedding(t, x).sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError):
-        torch.autograd.grad(dw.sum(), x)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(kernels.embedding(t, x).sum(), x, create_graph=True)

@@ -347,9 +347,8 @@ def test_only_once_differentiable_and_versions(kernels):
     x = make(1, 10, 2, 2, 8, 8, torch.float32)
     x["q"].requires_grad_()
     out, S = kernels.linear_attention(**x)
-    (dq,) = torch.autograd.grad(out.sum(), x["q"], create_graph=True)
-    with pytest.raises(RuntimeError):
-        torch.autograd.grad(dq.sum(), x["q"])
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(out.sum(), x["q"], create_graph=True)
     state = torch.zeros(1, 2, 8, 8, device="cuda")
     w = torch.ones(1, 2, 8, 8, device="cuda", requires_grad=True)
     y = (w * state).sum()
@@ -372,6 +371,5 @@ def test_refusals_on_the_gpu(kernels):
                   x["state"].clone().requires_grad_()):
         with pytest.raises((ValueError, RuntimeError)):
             kernels.linear_attention_step(**s, state=state)
-    from sunnynet_b200._lib import SnError
-    with pytest.raises(SnError, match="overlap"):
+    with pytest.raises(ValueError, match="overlap"):
         kernels.linear_attention_step(**s, state=x["state"][:1].expand(2, 4, 8, 16))
