@@ -29,7 +29,8 @@ TORCH_CALLS = PKG / "_torch_calls.so"
 SOURCES = ["runtime.cu", "abi.cu", "recur.cu", "quant4.cu", "gemm.cu", "tc_gemm.cu", "sunny.cu",
            "rwkv7.cu", "scan_noalloc.cu", "sunny_fused.cu", "w4a8_tc.cu", "argmax.cu",
            "train.cu", "caller.cu", "norm.cu", "adamw.cu",
-           "sample.cu", "linattn.cu", "embed.cu", "gradnorm.cu"]
+           "sample.cu", "linattn.cu", "linattn_f32.cu", "linattn_bf16.cu", "linattn_f16.cu", "embed.cu",
+           "gradnorm.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O3", "--expt-relaxed-constexpr",
          "-I", str(INCLUDE), "-I", str(CSRC)]

@@ -7,13 +7,16 @@
 // Forward: a copy, bound by HBM. A token outside the vocabulary gives a row of
 // NaN, and no gradient: the device has no other way to tell.
 //
-// Gradient: the tokens are sorted by a stable radix sort of eight bits a pass
-// (two launches each: the counts of every tile, then ranks and places), so that
-// each row's tokens lie side by side in their order and are added in it: the
-// same bits every time, no atomics. Bound by HBM (dout read, dW written once) from some
-// ten thousand tokens on, and by the launches below. While they sort, further
-// CTAs of the same launches fill dW with zeros, which costs nothing then: most
-// rows of a vocabulary occur in no batch, and those that do are overwritten.
+// Gradient: the tokens are sorted by a stable radix sort of eight bits a pass, so
+// that each row's tokens lie side by side in their order and are added in it: the
+// same bits every time, no atomics on values. Up to kNear tokens are sorted by one
+// cluster of eight CTAs in one launch (5003 tokens, two passes: 11 us; four launches
+// of many CTAs took 12, and 10 more of the host's time; 32768 tokens 28 us against
+// 18), more of them by two launches a pass: the counts of every tile, then ranks and places. Bound by HBM
+// (dout read, dW written once) from some ten thousand tokens on, and by latency
+// below. While they sort, further CTAs of the same launches fill dW with zeros,
+// which costs nothing then: most rows of a vocabulary occur in no batch, and those
+// that do are overwritten.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -119,7 +122,7 @@ struct Sorting {
 };
 
 __device__ __forceinline__ uint2 entry(const Sorting& s, int i) {
-    if (s.from) return s.from[i];
+    if (s.from) return __ldcg(s.from + i);  // (written in this launch, or the one before)
     const long long r = row_of(s.tokens, s.wide, i, s.V);
     return make_uint2((unsigned)(r < 0 ? s.V : r), (unsigned)i);  // strangers behind all others
 }
@@ -147,74 +150,121 @@ __global__ void __launch_bounds__(kSort) count_kernel(const Sorting s) {
     for (int i = threadIdx.x; i < kBins; i += blockDim.x) s.counts[blockIdx.x * kBins + i] = count[i];
 }
 
-// A thread for each of the tile's tokens, kSort at a time, in their order.
-__global__ void __launch_bounds__(kSort) place_kernel(const Sorting s) {
-    pdl_trigger();
-    if (blockIdx.x >= (unsigned)s.tiles) return fill_zeros(s);
-    constexpr int WARPS = kSort / 32, PARTS = kSort / kBins;
-    __shared__ int at[kBins], part[PARTS][kBins][2], warp_sum[kBins / 32];
-    __shared__ int seen[WARPS][kBins];  // of a warp, in this round
+// What placing a tile's tokens keeps in shared memory.
+struct Placing {
+    int at[kBins];                      // where the next token of each bin goes
+    int seen[kSort / 32][kBins];        // of a warp, in this round
+    int part[kSort / kBins][kBins][2];  // of the counts: of all tiles, of those before this one
+    int warp_sum[kBins / 32];
+};
+
+// at: behind the tokens of lower bins, and of earlier tiles; count(t, bin) is tile t's.
+template <typename F>
+__device__ __forceinline__ void first_places(Placing& m, int tile, int tiles, F&& count) {
+    constexpr int PARTS = kSort / kBins;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bin = tid % kBins;
-    for (int i = tid; i < WARPS * kBins; i += WARPS * 32) (&seen[0][0])[i] = 0;
-    pdl_wait();
-    // where this tile's tokens of each bin begin: behind those of lower bins, and of earlier tiles
-    {
-        int all = 0, before = 0;
+    int all = 0, before = 0;
 #pragma unroll 16
-        for (int t = tid / kBins; t < s.tiles; t += PARTS) {
-            const int c = s.counts[t * kBins + bin];
-            all += c;
-            before += t < (int)blockIdx.x ? c : 0;
-        }
-        part[tid / kBins][bin][0] = all;
-        part[tid / kBins][bin][1] = before;
-        __syncthreads();
-        int sum = 0;
-        if (tid < kBins) {
-            all = before = 0;
-#pragma unroll
-            for (int p = 0; p < PARTS; ++p) all += part[p][tid][0], before += part[p][tid][1];
-            sum = all;
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const int y = __shfl_up_sync(0xffffffffu, sum, d);
-                if (lane >= d) sum += y;
-            }
-            if (lane == 31) warp_sum[warp] = sum;
-        }
-        __syncthreads();
-        if (tid < kBins) {
-            for (int w = 0; w < warp; ++w) sum += warp_sum[w];
-            at[tid] = sum - all + before;
-        }
-        __syncthreads();
+    for (int t = tid / kBins; t < tiles; t += PARTS) {
+        const int c = count(t, bin);
+        all += c;
+        before += t < tile ? c : 0;
     }
-    const int lo = blockIdx.x * s.per, hi = min(s.n, lo + s.per);
-    for (int base = lo; base < hi; base += WARPS * 32) {
+    m.part[tid / kBins][bin][0] = all;
+    m.part[tid / kBins][bin][1] = before;
+    __syncthreads();
+    int sum = 0;
+    if (tid < kBins) {
+        all = before = 0;
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) all += m.part[p][tid][0], before += m.part[p][tid][1];
+        sum = all;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int y = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += y;
+        }
+        if (lane == 31) m.warp_sum[warp] = sum;
+    }
+    __syncthreads();
+    if (tid < kBins) {
+        for (int w = 0; w < warp; ++w) sum += m.warp_sum[w];
+        m.at[tid] = sum - all + before;
+    }
+    __syncthreads();
+}
+
+// Places tokens [lo, hi): a thread for each, kSort at a time, in their order.
+__device__ __forceinline__ void place_tokens(Placing& m, const Sorting& s, int lo, int hi) {
+    constexpr int WARPS = kSort / 32;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    for (int base = lo; base < hi; base += kSort) {
+        for (int j = tid; j < WARPS * kBins; j += kSort) (&m.seen[0][0])[j] = 0;
+        __syncthreads();
         const int i = base + tid;
         const bool in = i < hi;
         const uint2 e = in ? entry(s, i) : make_uint2(0, 0);
         const unsigned d = e.x >> s.shift & (kBins - 1);
         const unsigned peers = __match_any_sync(0xffffffffu, in ? d : kBins);
         const int rank = __popc(peers & ((1u << lane) - 1));
-        if (in && rank == 0) seen[warp][d] = __popc(peers);
+        if (in && rank == 0) m.seen[warp][d] = __popc(peers);
         __syncthreads();
         if (tid < kBins) {  // counts of the warps become their first places
-            int next = at[tid];
+            int next = m.at[tid];
 #pragma unroll 8
             for (int w = 0; w < WARPS; ++w) {
-                const int c = seen[w][tid];
-                seen[w][tid] = next;
+                const int c = m.seen[w][tid];
+                m.seen[w][tid] = next;
                 next += c;
             }
-            at[tid] = next;
+            m.at[tid] = next;
         }
         __syncthreads();
-        if (in) s.to[seen[warp][d] + rank] = e;
+        if (in) s.to[m.seen[warp][d] + rank] = e;
         __syncthreads();
-        if (base + WARPS * 32 < hi)
-            for (int j = tid; j < WARPS * kBins; j += WARPS * 32) (&seen[0][0])[j] = 0;
+    }
+}
+
+__global__ void __launch_bounds__(kSort) place_kernel(const Sorting s) {
+    pdl_trigger();
+    if (blockIdx.x >= (unsigned)s.tiles) return fill_zeros(s);
+    __shared__ Placing m;
+    pdl_wait();
+    first_places(m, blockIdx.x, s.tiles, [&](int t, int bin) { return s.counts[t * kBins + bin]; });
+    const int lo = blockIdx.x * s.per;
+    place_tokens(m, s, lo, min(s.n, lo + s.per));
+}
+
+// All passes in one launch: the first cluster sorts, each of its CTAs a tile, the
+// others fill zeros.
+constexpr int kCluster = 8, kNear = kCluster * kSort;
+
+__global__ void __launch_bounds__(kSort) __cluster_dims__(kCluster, 1, 1)
+sort_kernel(Sorting s, uint2* list0, uint2* list1, int passes) {
+    pdl_trigger();
+    if (blockIdx.x >= kCluster) return fill_zeros(s);
+    __shared__ Placing m;
+    __shared__ int count[kBins];
+    const int tile = blockIdx.x, lo = min(s.n, tile * s.per), hi = min(s.n, lo + s.per);
+    if (tile == 0 && threadIdx.x == 0) *s.joins = 0;
+    for (int p = 0; p < passes; ++p) {
+        s.shift = 8 * p;
+        s.from = p == 0 ? nullptr : p & 1 ? list0 : list1;
+        s.to = p & 1 ? list1 : list0;
+        for (int i = threadIdx.x; i < kBins; i += kSort) count[i] = 0;
         __syncthreads();
+        for (int i = lo + threadIdx.x; i < hi; i += kSort)
+            atomicAdd(&count[entry(s, i).x >> s.shift & (kBins - 1)], 1);
+        cluster_sync();
+        first_places(m, tile, kCluster, [&](int t, int bin) {
+            int c;
+            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(c) : "r"(dsmem_addr(&count[bin], t)) : "memory");
+            return c;
+        });
+        cluster_sync();  // (the counts are read: they may be overwritten)
+        place_tokens(m, s, lo, hi);
+        __threadfence();
+        cluster_sync();  // every token is in its place
     }
 }
 
@@ -430,7 +480,7 @@ struct Plan {
 Plan plan_of(long long n, long long V, int D) {
     Plan p;
     const auto up = [](long long b) { return (b + 255) / 256 * 256; };
-    p.tiles = (int)std::max(1ll, std::min((long long)kTiles, (n + kSort - 1) / kSort));
+    p.tiles = n <= kNear ? kCluster : (int)std::min((long long)kTiles, (n + kSort - 1) / kSort);
     p.per = (int)((n + p.tiles - 1) / p.tiles);
     p.passes = 1;
     while (V >> 8 * p.passes) ++p.passes;  // (V itself marks strangers)
@@ -512,8 +562,9 @@ sn_status sn_abi_embedding_bwd(const void* tokens, int32_t token_bits, int64_t n
     s.joins = reinterpret_cast<int*>(at + 2 * p.list + p.counts);
     s.n = (int)n, s.tiles = p.tiles, s.per = p.per;
     // the zeros, a part to each launch; where they do not begin at a pack, by one of their own
+    const int launches = n <= kNear ? 1 : 2 * p.passes;
     const bool packed = (uintptr_t)dW % 16 == 0;
-    const long long packs = packed ? bytes / 16 : 0, share = (packs + 2 * p.passes - 1) / (2 * p.passes);
+    const long long packs = packed ? bytes / 16 : 0, share = (packs + launches - 1) / launches;
     if (!packed) SN_TRY(cuda_check(cudaMemsetAsync(dW, 0, bytes, st), "embedding_bwd"));
     long long done = 0;
     const auto zeros = [&] {
@@ -523,20 +574,25 @@ sn_status sn_abi_embedding_bwd(const void* tokens, int32_t token_bits, int64_t n
         s.zero_rest = packed && done == packs ? (int)(bytes % 16) : 0;
         return (unsigned)std::min((s.zero_packs + 4095) / 4096 + (s.zero_rest > 0), 148ll * 4);
     };
-    for (int i = 0; i < p.passes; ++i) {
-        s.shift = 8 * i;
-        s.from = i ? lists[(i - 1) & 1] : nullptr;
-        s.to = lists[i & 1];
-        if (i == 0) {
-            const unsigned more = zeros();
-            count_kernel<<<p.tiles + more, kSort, 0, st>>>(s);
-            SN_TRY(cuda_check(cudaGetLastError(), "embedding launch"));
-        } else {
-            const unsigned more = zeros();
-            SN_TRY(launch_behind(count_kernel, dim3(p.tiles + more), kSort, 0, st, s));
+    if (n <= kNear) {
+        const unsigned more = (zeros() + kCluster - 1) / kCluster * kCluster;
+        sort_kernel<<<kCluster + more, kSort, 0, st>>>(s, lists[0], lists[1], p.passes);
+        SN_TRY(cuda_check(cudaGetLastError(), "embedding launch"));
+    } else {
+        for (int i = 0; i < p.passes; ++i) {
+            s.shift = 8 * i;
+            s.from = i ? lists[(i - 1) & 1] : nullptr;
+            s.to = lists[i & 1];
+            unsigned more = zeros();
+            if (i == 0) {
+                count_kernel<<<p.tiles + more, kSort, 0, st>>>(s);
+                SN_TRY(cuda_check(cudaGetLastError(), "embedding launch"));
+            } else {
+                SN_TRY(launch_behind(count_kernel, dim3(p.tiles + more), kSort, 0, st, s));
+            }
+            more = zeros();
+            SN_TRY(launch_behind(place_kernel, dim3(p.tiles + more), kSort, 0, st, s));
         }
-        const unsigned more = zeros();
-        SN_TRY(launch_behind(place_kernel, dim3(p.tiles + more), kSort, 0, st, s));
     }
     Summing m = {};
     m.sorted = lists[(p.passes - 1) & 1];

@@ -10,9 +10,11 @@
 // to the largest count.
 //
 // Bound by HBM: the norm reads every value once, clipping once more, and writes
-// it. One wave of CTAs takes the tensors' runs of a few thousand values in turn;
-// what the first pass read last is still in L2 when the second begins, so that
-// goes from the last run to the first.
+// it. The tensors are cut into runs of 16 KB of memory, which one wave of CTAs
+// takes in turn (a stretch of neighbouring runs to each CTA was a fifth slower:
+// DRAM pages), with the next run's loads, and the search for its tensor, on their
+// way before the last one's values are used. What the first pass read last is still
+// in L2 when the second begins, so that goes from the last run to the first.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,8 +30,9 @@ namespace sn {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kWave = 148 * 8;     // CTAs at most, each with one part of the sum
-constexpr int kRun = 16384, kShort = 4096;  // values of a run; of a small model's, for more CTAs
+constexpr int kWave = 148 * 4;          // CTAs at most, each with one part of the sum
+constexpr int kPacks = 4;               // 16-byte loads of a thread for a run
+constexpr int kRun = kPacks * kThreads;  // packs of a run
 constexpr int kFew = 32, kMany = 1280;  // tensors of a launch: 30 of the 32 KB of parameters
 
 struct Run {
@@ -42,7 +45,6 @@ struct Run {
 template <int N>
 struct Runs {
     int count, runs;
-    int per;  // values of a run
     Run t[N];
 };
 
@@ -78,13 +80,6 @@ union Pack {
     T v[16 / sizeof(T)];
 };
 
-// Values of a run before its first multiple of 16 bytes.
-template <typename T>
-__device__ __forceinline__ int head_of(const T* p, int n) {
-    const int k = (int)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) % 16 / sizeof(T));
-    return k < n ? k : n;
-}
-
 template <typename T>
 __device__ __forceinline__ double squares(const uint4& w) {
     constexpr int V = 16 / sizeof(T);
@@ -106,53 +101,111 @@ __device__ __forceinline__ double squares(const uint4& w) {
     return d;
 }
 
-constexpr int kAhead = 4;  // loads of a thread on their way
+// A tensor as 16-byte packs of memory: its first and last may be its own in part.
+struct Packs {
+    char* base;
+    int before;       // bytes of the first pack that lie before the tensor
+    long long bytes;  // from the first pack's begin to the tensor's end
+    long long p;      // this thread's first pack of the run
+    int dtype;
+    __device__ __forceinline__ bool has(int k) const { return (p + k * kThreads) * 16 < bytes; }
+    __device__ __forceinline__ bool whole(int k) const {
+        const long long at = (p + k * kThreads) * 16;
+        return at >= before && at + 16 <= bytes;
+    }
+    __device__ __forceinline__ uint4* at(int k) const {
+        return reinterpret_cast<uint4*>(base + (p + k * kThreads) * 16);
+    }
+    // f(16-bit word of the tensor, its place in the pack) for a pack in part
+    template <typename F>
+    __device__ __forceinline__ void words(int k, F&& f) const {
+        const long long at = (p + k * kThreads) * 16;
+        for (int i = 0; i < 8; ++i)
+            if (at + 2 * i >= before && at + 2 * i < bytes) f(reinterpret_cast<uint16_t*>(base + at + 2 * i), i);
+    }
+};
 
-template <typename T>
-__device__ __forceinline__ double square_run(const T* p, int n) {
-    constexpr int V = 16 / sizeof(T);
-    const int head = head_of(p, n), packs = (n - head) / V, tail = head + packs * V;
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < head + (n - tail); i += kThreads) {
-        const double x = (double)to_f(p[i < head ? i : tail + (i - head)]);
-        sum = fma(x, x, sum);
-    }
-    const uint4* at = reinterpret_cast<const uint4*>(p + head);
-    for (int i = threadIdx.x; i < packs; i += kAhead * kThreads) {
-        uint4 w[kAhead];
+template <int N>
+__device__ __forceinline__ Packs packs_of(const Runs<N>& a, int c) {
+    const Run& t = a.t[find(a, c)];
+    Packs x;
+    x.before = (int)(reinterpret_cast<uintptr_t>(t.p) & 15);
+    x.base = static_cast<char*>(t.p) - x.before;
+    x.bytes = x.before + t.n * (t.dtype == SN_F32 ? 4 : 2);
+    x.p = (long long)(c - t.first) * kRun + threadIdx.x;
+    x.dtype = t.dtype;
+    return x;
+}
+
+__device__ __forceinline__ void load(uint4* w, const Packs& x) {
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-            w[k] = i + k * kThreads < packs ? at[i + k * kThreads] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) sum += squares<T>(w[k]);
+    for (int k = 0; k < kPacks; ++k) {
+        w[k] = make_uint4(0, 0, 0, 0);
+        if (x.whole(k)) {
+            w[k] = *x.at(k);
+        } else if (x.has(k)) {
+            uint32_t part[4] = {};
+            x.words(k, [&](const uint16_t* from, int i) { part[i / 2] |= (uint32_t)*from << i % 2 * 16; });
+            w[k] = make_uint4(part[0], part[1], part[2], part[3]);
+        }
     }
-    return sum;
+}
+
+__device__ __forceinline__ void store(const uint4* w, const Packs& x) {
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k) {
+        if (x.whole(k)) {
+            __stcs(x.at(k), w[k]);  // (nothing here reads it again)
+        } else if (x.has(k)) {
+            const uint32_t part[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+            x.words(k, [&](uint16_t* to, int i) { *to = (uint16_t)(part[i / 2] >> i % 2 * 16); });
+        }
+    }
 }
 
 template <typename T>
-__device__ __forceinline__ void scale_run(T* p, int n, float f) {
-    constexpr int V = 16 / sizeof(T);
-    const int head = head_of(p, n), packs = (n - head) / V, tail = head + packs * V;
-    for (int i = threadIdx.x; i < head + (n - tail); i += kThreads) {
-        T* at = p + (i < head ? i : tail + (i - head));
-        *at = from_f<T>(to_f(*at) * f);
-    }
-    uint4* at = reinterpret_cast<uint4*>(p + head);
-    const auto scaled = [&](const uint4& w) {
-        Pack<T> q;
-        q.w = w;
+__device__ __forceinline__ uint4 scaled(const uint4& w, float f) {
+    Pack<T> q;
+    q.w = w;
 #pragma unroll
-        for (int j = 0; j < V; ++j) q.v[j] = from_f<T>(to_f(q.v[j]) * f);
-        return q.w;
-    };
-    for (int i = threadIdx.x; i < packs; i += kAhead * kThreads) {
-        uint4 w[kAhead];
+    for (int j = 0; j < (int)(16 / sizeof(T)); ++j) q.v[j] = from_f<T>(to_f(q.v[j]) * f);
+    return q.w;
+}
+
+// f(a type's zero) for the type of a tensor.
+template <typename F>
+__device__ __forceinline__ void by_type(int dtype, F&& f) {
+    if (dtype == SN_F32)
+        f(0.0f);
+    else if (dtype == SN_BF16)
+        f(__nv_bfloat16());
+    else
+        f(__half());
+}
+
+// f(packs, their values) for this CTA's runs, from the first or (BACK) the last on.
+template <bool BACK, int N, typename F>
+__device__ __forceinline__ void each_run(const Runs<N>& a, F&& f) {
+    const auto run = [&](int i) { return BACK ? a.runs - 1 - i : i; };
+    int i = blockIdx.x;
+    if (i >= a.runs) return;
+    Packs x = packs_of(a, run(i));
+    uint4 w[kPacks];
+    load(w, x);
+    for (;;) {
+        const int next = i + gridDim.x;
+        Packs y = x;
+        uint4 v[kPacks];
+        if (next < a.runs) {
+            y = packs_of(a, run(next));
+            load(v, y);
+        }
+        f(x, w);
+        if (next >= a.runs) break;
+        x = y;
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-            if (i + k * kThreads < packs) w[k] = at[i + k * kThreads];
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-            if (i + k * kThreads < packs) at[i + k * kThreads] = scaled(w[k]);
+        for (int k = 0; k < kPacks; ++k) w[k] = v[k];
+        i = next;
     }
 }
 
@@ -168,28 +221,18 @@ __device__ __forceinline__ double cta_sum(double x) {
     return x;
 }
 
-// f(values, how many) of run c.
-template <int N, typename F>
-__device__ __forceinline__ void with_run(const Runs<N>& a, int c, F&& f) {
-    const Run& t = a.t[find(a, c)];
-    const long long lo = (long long)(c - t.first) * a.per, left = t.n - lo;
-    const int n = left < a.per ? (int)left : a.per;
-    if (t.dtype == SN_F32)
-        f(static_cast<float*>(t.p) + lo, n);
-    else if (t.dtype == SN_BF16)
-        f(static_cast<__nv_bfloat16*>(t.p) + lo, n);
-    else
-        f(static_cast<__half*>(t.p) + lo, n);
-}
-
 template <int N>
-__global__ void __launch_bounds__(kThreads) square_kernel(const __grid_constant__ Runs<N> a, double* parts) {
+__global__ void __launch_bounds__(kThreads, 4) square_kernel(const __grid_constant__ Runs<N> a, double* parts) {
     pdl_trigger();
-    double x = 0.0;
-    for (int c = blockIdx.x; c < a.runs; c += gridDim.x)
-        with_run(a, c, [&](const auto* p, int n) { x += square_run(p, n); });
-    x = cta_sum(x);
-    if (threadIdx.x == 0) parts[blockIdx.x] = x;
+    double sum = 0.0;
+    each_run<false>(a, [&](const Packs& x, const uint4* w) {
+        by_type(x.dtype, [&](auto t) {
+#pragma unroll
+            for (int k = 0; k < kPacks; ++k) sum += squares<decltype(t)>(w[k]);
+        });
+    });
+    sum = cta_sum(sum);
+    if (threadIdx.x == 0) parts[blockIdx.x] = sum;
 }
 
 // The norm and the factor from the parts: in every thread of the CTA.
@@ -219,7 +262,7 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const double* parts, int
 
 // Each CTA sums the parts for itself: a launch between would cost more.
 template <int N>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 scale_kernel(const __grid_constant__ Runs<N> a, const double* parts, int n_parts, double max_norm, float* norm,
              float* factor) {
     pdl_wait();
@@ -229,8 +272,13 @@ scale_kernel(const __grid_constant__ Runs<N> a, const double* parts, int n_parts
         if (factor) *factor = r.y;
     }
     if (r.y == 1.0f) return;
-    for (int c = a.runs - 1 - blockIdx.x; c >= 0; c -= gridDim.x)
-        with_run(a, c, [&](auto* p, int n) { scale_run(p, n, r.y); });
+    each_run<true>(a, [&](const Packs& x, uint4* w) {
+        by_type(x.dtype, [&](auto t) {
+#pragma unroll
+            for (int k = 0; k < kPacks; ++k) w[k] = scaled<decltype(t)>(w[k], r.y);
+        });
+        store(w, x);
+    });
 }
 
 // Launched so that it may start when the kernel before has, and waits for it.
@@ -270,26 +318,27 @@ int check_list(const char* what, const Call& c, double max_norm, long long* tota
     return SN_OK;
 }
 
-// How a list is cut up: launches of up to kMany tensors, each of up to kWave CTAs.
-int run_values(long long total) { return total >= 2ll * kWave * kRun ? kRun : kShort; }
-
-// f(runs, CTAs, parts before them) for each launch; how many parts there are.
+// f(runs, CTAs, parts before them) for each launch of up to kMany tensors and
+// kWave CTAs; how many parts there are. Where an address and type are not at hand
+// yet, the most that they may take.
 template <typename F>
-int each_launch(const Call& c, int per, long long* parts, F&& f) {
+int each_launch(const Call& c, long long* parts, F&& f) {
     *parts = 0;
     for (int i = 0; i < c.count;) {
         Runs<kMany> a;
         a.count = 0;
-        a.per = per;
         long long n = 0;
         for (; i < c.count && a.count < kMany; ++i)
             if (c.sizes[i]) {
-                const long long more = (c.sizes[i] + per - 1) / per;
+                const int type = c.dtypes ? c.dtypes[i] : SN_F32;
+                const long long before = c.grads ? (long long)((uintptr_t)c.grads[i] & 15) : 15;
+                const long long bytes = before + c.sizes[i] * (type == SN_F32 ? 4 : 2);
+                const long long more = (bytes + 16 * kRun - 1) / (16 * kRun);
                 if (n + more > 0x7fffffffll - kWave) {
                     if (a.count) break;
                     return fail(SN_E_INVAL, "grad_norm: a tensor of %lld values", (long long)c.sizes[i]);
                 }
-                a.t[a.count++] = {c.grads ? c.grads[i] : nullptr, c.sizes[i], (int)n, c.dtypes ? c.dtypes[i] : 0};
+                a.t[a.count++] = {c.grads ? c.grads[i] : nullptr, c.sizes[i], (int)n, type};
                 n += more;
             }
         if (!a.count) break;
@@ -297,7 +346,7 @@ int each_launch(const Call& c, int per, long long* parts, F&& f) {
         const unsigned ctas = (unsigned)std::min(n, (long long)kWave);
         if (a.count <= kFew) {
             Runs<kFew> b;
-            b.count = a.count, b.runs = a.runs, b.per = per;
+            b.count = a.count, b.runs = a.runs;
             for (int k = 0; k < a.count; ++k) b.t[k] = a.t[k];
             SN_TRY(f(b, ctas, *parts));
         } else {
@@ -312,9 +361,8 @@ int norm_or_clip(const char* what, const Call& c, double max_norm, bool clip, fl
                  int64_t ws_bytes, void* cuda_stream) {
     long long total;
     SN_TRY(check_list(what, c, max_norm, &total));
-    const int per = run_values(total);
     long long n = 0;
-    SN_TRY(each_launch(c, per, &n, [](const auto&, unsigned, long long) { return SN_OK; }));
+    SN_TRY(each_launch(c, &n, [](const auto&, unsigned, long long) { return SN_OK; }));
     if (n && (!ws || ws_bytes < n * 8)) return fail(SN_E_INVAL, "%s: a workspace of %lld bytes is wanted", what, n * 8);
     CallerDevice dev;
     for (int i = 0; i < c.count; ++i)
@@ -323,14 +371,14 @@ int norm_or_clip(const char* what, const Call& c, double max_norm, bool clip, fl
     SN_TRY(dev.select(what));
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     double* parts = static_cast<double*>(ws);
-    SN_TRY(each_launch(c, per, &n, [&](const auto& a, unsigned ctas, long long before) {
+    SN_TRY(each_launch(c, &n, [&](const auto& a, unsigned ctas, long long before) {
         constexpr int N = sizeof(a.t) / sizeof(a.t[0]);
         square_kernel<N><<<ctas, kThreads, 0, st>>>(a, parts + before);
         return cuda_check(cudaGetLastError(), "grad_norm launch");
     }));
     const int count = (int)n;
     if (!clip || !n) return launch_behind(norm_kernel, 1u, st, (const double*)parts, count, max_norm, norm, factor);
-    return each_launch(c, per, &n, [&](const auto& a, unsigned ctas, long long before) {
+    return each_launch(c, &n, [&](const auto& a, unsigned ctas, long long before) {
         constexpr int N = sizeof(a.t) / sizeof(a.t[0]);
         // (only the first of several may start early: its launch is the one behind the squares)
         if (!before)
@@ -355,8 +403,7 @@ int64_t sn_abi_grad_norm_ws(int32_t count, const int64_t* sizes) {
         total += sizes[i];
     }
     long long n = 0;
-    const int rc = each_launch({count, nullptr, sizes, nullptr}, run_values(total), &n,
-                               [](const auto&, unsigned, long long) { return SN_OK; });
+    const int rc = each_launch({count, nullptr, sizes, nullptr}, &n, [](const auto&, unsigned, long long) { return SN_OK; });
     return rc == SN_OK ? 8 * n : -1;
 }
 

@@ -8,7 +8,9 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "caller.cuh"
 #include "ptx.cuh"
+#include "runtime.cuh"
 
 namespace sn {
 namespace la {
@@ -299,6 +301,42 @@ __device__ __forceinline__ void decays(Decays<C>* to, Weights<C>* weights, const
         to->whole = wrong ? nan : exp2_of(x.x + x.y);
     }
 }
+
+struct Strides {
+    long long b, t, h;
+};
+
+// A call's sizes and arrays.
+struct Job {
+    const void *q, *k, *v;
+    Strides qs, ks, vs, gs;
+    const float* g;
+    const int* lengths;
+    int B, T, H, share, dk, dv;
+    float scale;
+    int whole;  // bit 0: q, 1: k, 2: v, 3: dout come in whole packs
+    int chunks;         // of a sequence
+    bool apart;         // each chunk's sum by a CTA of its own
+};
+
+// The gradients that a call wants, and those it is given.
+struct Wanted {
+    const void* dout;
+    Strides ds;
+    const float* dstate_out;
+    void *dq, *dk, *dv;
+    float *dg, *dstate;
+    bool gates_alike;
+};
+
+// The launches of a call (linattn_kernels.cuh); with `need`, the bytes of workspace
+// alone.
+template <typename T>
+int forward(const Job& j, const float* first, void* out, float* state_out, char* ws, long long ws_bytes,
+            long long* need, cudaStream_t st);
+template <typename T>
+int backward(const Job& j, const float* first, const Wanted& w, char* ws, long long ws_bytes, long long* need,
+             cudaStream_t st);
 
 }  // namespace la
 }  // namespace sn

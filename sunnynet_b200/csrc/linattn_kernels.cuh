@@ -1,0 +1,1195 @@
+// The kernels of linear attention, for one type of values (included by a source
+// file for each, which are compiled side by side).
+#pragma once
+#include <algorithm>
+#include <cmath>
+
+#include "linattn.cuh"
+
+namespace sn {
+namespace la {
+namespace {
+
+// Tokens of a sequence, and its chunks that hold some.
+__device__ __forceinline__ int tokens_of(const Job& j, int b) {
+    return j.lengths ? max(0, min(j.T, j.lengths[b])) : j.T;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* head_of(const void* x, const Strides& s, int b, int h) {
+    return static_cast<const T*>(x) + b * s.b + h * s.h;
+}
+
+// S += sum over the tokens of w_t x_t y_t^T: 16 rows (values `row` on of x), NT
+// column tiles (values `cb` on of y). x w is taken apart as it is formed: the
+// product of the high parts rounded, what that leaves (which bf16 holds exactly),
+// and the products with the low parts: 2^-16 of a value, in three or four
+// instructions for two.
+template <int NP, int NT, int C>
+__device__ __forceinline__ void add_outer(float (*S)[4], const Tile& x, const Tile& y, const uint2* w, int row,
+                                          int cb) {
+    const int q = lane_id() & 3;
+    uint32_t all[C / 16][NP][4];  // all asked for at once
+#pragma unroll
+    for (int kt = 0; kt < C / 16; ++kt)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) x.a_t(all[kt][p], kt * 16, row, p);
+#pragma unroll
+    for (int kt = 0; kt < C / 16; ++kt) {
+        const uint32_t(*xr)[4] = all[kt];
+        uint32_t a[2][4];
+        const uint2 f[2] = {w[kt * 8 + q], w[kt * 8 + 4 + q]};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            a[0][r] = fma2(xr[0][r], f[r / 2].x, 0x80008000u);
+            a[1][r] = fma2(xr[0][r], f[r / 2].x, neg2(a[0][r]));
+            a[1][r] = fma2(xr[0][r], f[r / 2].y, a[1][r]);
+            if constexpr (NP == 2) a[1][r] = fma2(xr[1][r], f[r / 2].x, a[1][r]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT / 2; ++n) {
+            uint32_t b[NP][4];
+#pragma unroll
+            for (int p = 0; p < NP; ++p) y.b_t(b[p], kt * 16, cb + n * 16, p);
+            mma2<2, NP>(S + 2 * n, a, b);
+        }
+    }
+}
+
+// out (16 rows from `ra` of A, columns from `cb` of B) += A B over D: A's rows
+// are tokens, B(k, n) = tile[n][k], or tile[k][n] where TRANS.
+template <int PA, int PB, int D, int NT, bool TRANS>
+__device__ __forceinline__ void product(float (*out)[4], const Tile& A, int ra, const Tile& B, int cb) {
+#pragma unroll
+    for (int kt = 0; kt < D / 16; ++kt) {
+        uint32_t a[PA][4];
+#pragma unroll
+        for (int p = 0; p < PA; ++p) A.a(a[p], ra, kt * 16, p);
+#pragma unroll
+        for (int n = 0; n < NT / 2; ++n) {
+            uint32_t b[PB][4];
+#pragma unroll
+            for (int p = 0; p < PB; ++p) {
+                if constexpr (TRANS)
+                    B.b_t(b[p], kt * 16, cb + n * 16, p);
+                else
+                    B.b(b[p], cb + n * 16, kt * 16, p);
+            }
+            mma2<PA, PB>(out + 2 * n, a, b);
+        }
+    }
+}
+
+// Scores of 16 tokens of A with a strip of NB blocks of 16 tokens of B from
+// block `jb` on, of which [j0, j1) are wanted.
+template <int NP, int D, int NB>
+__device__ __forceinline__ void scores(float (*p)[4], const Tile& A, int ra, const Tile& B, int jb, int j0,
+                                       int j1) {
+#pragma unroll
+    for (int n = 0; n < 2 * NB; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[n][i] = 0.0f;
+#pragma unroll
+    for (int kt = 0; kt < D / 16; ++kt) {
+        uint32_t a[NP][4];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) A.a(a[i], ra, kt * 16, i);
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+            if (jb + j >= j0 && jb + j < j1) {
+                uint32_t b[NP][4];
+#pragma unroll
+                for (int i = 0; i < NP; ++i) B.b(b[i], (jb + j) * 16, kt * 16, i);
+                mma2<NP, NP>(p + 2 * j, a, b);
+            }
+    }
+}
+
+// out += P Y, P such scores as they lie in registers (PP planes of them), Y the
+// tokens' tile.
+template <int PP, int NP, int NB, int NT>
+__device__ __forceinline__ void weighted(float (*out)[4], const float (*p)[4], const Tile& Y, int cb, int jb,
+                                         int j0, int j1) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+        if (jb + j >= j0 && jb + j < j1) {
+            uint32_t a[PP][4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float u = p[2 * j + r / 2][r % 2 * 2], v = p[2 * j + r / 2][r % 2 * 2 + 1];
+                a[0][r] = pack2(u, v);
+                if constexpr (PP == 2) a[1][r] = rest2(u, v, a[0][r]);
+            }
+#pragma unroll
+            for (int n = 0; n < NT / 2; ++n) {
+                uint32_t b[NP][4];
+#pragma unroll
+                for (int i = 0; i < NP; ++i) Y.b_t(b[i], (jb + j) * 16, cb + n * 16, i);
+                mma2<PP, NP>(out + 2 * n, a, b);
+            }
+        }
+}
+
+// The same for one block, whose tokens do not all see each other: a value of Y
+// that is not finite stays away from the rows before its own, which in a matrix
+// product would meet it with a weight of zero.
+template <int NP, int NT>
+__device__ __forceinline__ void weighted_apart(float (*out)[4], const float (*p)[4], const bf16* Y, int ld,
+                                               int step, int cb) {
+    const int l = lane_id();
+#pragma unroll
+    for (int s = 0; s < 16; ++s) {
+        const int from = (l & ~3) | ((s & 7) >> 1);
+        const float p0 = __shfl_sync(0xffffffffu, p[s / 8][s & 1], from);
+        const float p1 = __shfl_sync(0xffffffffu, p[s / 8][2 + (s & 1)], from);
+        const bf16* y = Y + s * ld + cb + (l & 3) * 2;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(y + n * 8);
+            float a = low(w), b = high(w);
+            if constexpr (NP == 2) {
+                const uint32_t w2 = *reinterpret_cast<const uint32_t*>(y + step + n * 8);
+                a += low(w2), b += high(w2);
+            }
+            if (s <= (l >> 2)) out[n][0] += p0 * a, out[n][1] += p0 * b;
+            if (s <= (l >> 2) + 8) out[n][2] += p1 * a, out[n][3] += p1 * b;
+        }
+    }
+}
+
+template <int NT>
+__device__ __forceinline__ void clear(float (*x)[4]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[n][i] = 0.0f;
+}
+template <int NT>
+__device__ __forceinline__ void scale_rows(float (*x)[4], float r0, float r1) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) x[n][0] *= r0, x[n][1] *= r0, x[n][2] *= r1, x[n][3] *= r1;
+}
+// A strip of scores from block jb on, by its columns' factors.
+template <int NB>
+__device__ __forceinline__ void scale_columns(float (*p)[4], const float* column, int jb) {
+#pragma unroll
+    for (int n = 0; n < 2 * NB; ++n) {
+        const float2 f = *reinterpret_cast<const float2*>(column + jb * 16 + n * 8 + (lane_id() & 3) * 2);
+        p[n][0] *= f.x, p[n][1] *= f.y, p[n][2] *= f.x, p[n][3] *= f.y;
+    }
+}
+// The scores of block rb's tokens (rows) with themselves, decayed; later columns are zeros.
+template <int C>
+__device__ __forceinline__ void near_decays(float (*p)[4], const Decays<C>& d, int rb, float scale) {
+    const int l = lane_id();
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = (l >> 2) + (i >> 1) * 8, s = n * 8 + (l & 3) * 2 + (i & 1);
+            p[n][i] = s <= t ? p[n][i] * (d.between(rb * 16 + t, rb * 16 + s) * scale) : 0.0f;
+        }
+}
+
+// 16 rows and NT column tiles of a state in fp32 (dk, dv), from and to registers.
+template <int NT>
+__device__ __forceinline__ void load_state(float (*S)[4], const float* from, int row, int cb, int dk, int dv) {
+    const int l = lane_id();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = row + (l >> 2) + (i >> 1) * 8, c = cb + n * 8 + (l & 3) * 2 + (i & 1);
+            S[n][i] = from && r < dk && c < dv ? from[r * dv + c] : 0.0f;
+        }
+}
+template <int NT>
+__device__ __forceinline__ void store_state(const float (*S)[4], float* to, int row, int cb, int dk, int dv) {
+    const int l = lane_id();
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = row + (l >> 2) + (i >> 1) * 8, c = cb + n * 8 + (l & 3) * 2 + (i & 1);
+            if (r < dk && c < dv) to[r * dv + c] = S[n][i];
+        }
+}
+
+// The same as PN bf16 planes with rows of D values and `plane` values each, by way of 16 rows of shared memory of the
+// warp's own, in packs of 16 bytes.
+template <int PN, int D, int NT>
+__device__ __forceinline__ void state_planes(const float (*S)[4], bf16* to, int plane, int row, int cb, bf16* by) {
+    constexpr int LD = NT * 8 + 8, ROWS = 32 / NT;
+    const int l = lane_id();
+    const uint32_t at = smem_u32(by + (l & 15) * LD + (l >> 4) * 8);
+#pragma unroll
+    for (int p = 0; p < PN; ++p) {
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+            uint32_t r[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float u = S[n + i / 2][i % 2 * 2], v = S[n + i / 2][i % 2 * 2 + 1];
+                r[i] = pack2(u, v);
+                if (p) r[i] = rest2(u, v, r[i]);
+            }
+            stsm4(at + n * 16, r);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 16; i += ROWS)
+            *reinterpret_cast<uint4*>(to + p * plane + (row + l / NT + i) * D + cb + l % NT * 8) =
+                *reinterpret_cast<const uint4*>(by + (l / NT + i) * LD + l % NT * 8);
+        __syncwarp();
+    }
+}
+
+// 16 rows of tokens from t0 on, their columns from `cb`: rows from `end` on are zeros.
+template <typename T, int NT>
+__device__ __forceinline__ void store_rows(const float (*x)[4], T* to, long long stride, int t0, int cb,
+                                           int end, int T_, int d) {
+    const int l = lane_id();
+    const bool pairs = d % 2 == 0 && stride % 2 == 0 && reinterpret_cast<uintptr_t>(to) % (2 * sizeof(T)) == 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int t = t0 + (l >> 2) + i * 8;
+        if (t >= T_) continue;
+        T* row = to + (long long)t * stride;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int c = cb + n * 8 + (l & 3) * 2;
+            const float u = t < end ? x[n][2 * i] : 0.0f, v = t < end ? x[n][2 * i + 1] : 0.0f;
+            if (pairs && c < d) {
+                if constexpr (sizeof(T) == 4) {
+                    *reinterpret_cast<float2*>(row + c) = make_float2(u, v);
+                } else {
+                    T two[2] = {from_f<T>(u), from_f<T>(v)};
+                    uint32_t w;
+                    __builtin_memcpy(&w, two, 4);
+                    *reinterpret_cast<uint32_t*>(row + c) = w;
+                }
+            } else {
+                if (c < d) row[c] = from_f<T>(u);
+                if (c + 1 < d) row[c + 1] = from_f<T>(v);
+            }
+        }
+    }
+}
+
+// The same for 16-bit values by way of 16 rows of shared memory (LD values apart,
+// the warp's own), where the rows come in whole packs of 16 bytes.
+template <typename T, int NT, int LD>
+__device__ __forceinline__ void store_rows_by(bf16* by, const float (*x)[4], T* to, long long stride, int t0,
+                                              int cb, int end, int T_, int d) {
+    if constexpr (sizeof(T) == 2) {
+        if (d % 8 == 0 && stride % 8 == 0 && reinterpret_cast<uintptr_t>(to) % 16 == 0) {
+            const int l = lane_id();
+            const uint32_t at = smem_u32(by + (l & 15) * LD + (l >> 4) * 8);
+#pragma unroll
+            for (int n = 0; n < NT; n += 2) {
+                uint32_t r[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float u = x[n + i / 2][i % 2 * 2], v = x[n + i / 2][i % 2 * 2 + 1];
+                    if constexpr (std::is_same<T, bf16>::value) {
+                        r[i] = pack2(u, v);
+                    } else {
+                        const __half2 h = __floats2half2_rn(u, v);
+                        r[i] = *reinterpret_cast<const uint32_t*>(&h);
+                    }
+                }
+                stsm4(at + n * 16, r);
+            }
+            __syncwarp();
+            constexpr int ROWS = 32 / NT;  // a lane for each pack of a row, rows at once
+            const int row = l / NT, col = cb + l % NT * 8;
+            T* p = to + (long long)(t0 + row) * stride + col;
+            if (col < d) {
+#pragma unroll
+                for (int i = 0; i < 16; i += ROWS) {
+                    const int t = t0 + row + i;
+                    uint4 w = *reinterpret_cast<const uint4*>(by + (row + i) * LD + l % NT * 8);
+                    if (t >= end) w = make_uint4(0, 0, 0, 0);
+                    if (t < T_) *reinterpret_cast<uint4*>(p) = w;
+                    p += ROWS * stride;
+                }
+            }
+            __syncwarp();
+            return;
+        }
+    }
+    store_rows<T, NT>(x, to, stride, t0, cb, end, T_, d);
+}
+
+// Rows [t0, t1) of zeros.
+template <typename T>
+__device__ __forceinline__ void zero_rows(T* to, long long stride, int t0, int t1, int d) {
+    for (long long i = threadIdx.x; i < (long long)max(0, t1 - t0) * d; i += blockDim.x)
+        to[(t0 + i / d) * stride + i % d] = from_f<T>(0.0f);
+}
+
+// The CTA of a kernel: NW warps share a chunk's C / 16 blocks of tokens, and where
+// there are more warps than blocks, a block's columns.
+template <typename T_, int KD_, int VD_, int C_>
+struct Shape {
+    typedef T_ T;
+    static constexpr int NP = planes_of<T_>, C = C_, NW = 8, THREADS = NW * 32;
+    static constexpr int KD = KD_, VD = VD_, LK = KD + 8, LV = VD + 8;  // rows of keys, of values and of states
+    static constexpr int KT = NP * C * LK, VT = NP * C * LV, STATE = KD * LV;
+    static constexpr int RB = C / 16, CG = NW / RB, NK = KD / CG / 8, NV = VD / CG / 8;
+    static_assert(NW % RB == 0 && NK % 2 == 0 && NV % 2 == 0, "whole blocks for the warps");
+    // a states' pass: stages of SUB tokens; eight warps of 16 rows and, of keys up to 64, half of the columns
+    static constexpr int SUB = C < 64 ? C : 64, KS = NP * SUB * LK, VS = NP * SUB * LV;
+    static constexpr int SR = KD / 16, SW = 8, ST = SW * 32, SNT = VD * SR / SW / 8;
+};
+
+__device__ __forceinline__ Tile tile(const bf16* p, int ld, int step) {
+    return {smem_u32(p), (uint32_t)ld * 2, (uint32_t)step * 2};
+}
+
+// ------------------------------------------------------------------ states
+// What a pass over a sequence adds up: x y^T over its tokens, forwards (keys and
+// values) or backwards (queries and the gradient of the outputs).
+struct Pass {
+    const void *x, *y;
+    Strides xs, ys;
+    const float* start;    // the first state, or null
+    float *sums, *factor;  // what each chunk adds to a state of zeros (KD x VD), and its decay
+    bf16* kept;            // the state before (backwards: behind) each chunk, planes of KD x VD
+    float* end;            // the last state, or null
+    bool back;
+};
+
+// The states alone: with KEEP a CTA goes through the chunks of a head; without,
+// each chunk has a CTA, which leaves its sum and factor. The decays of the next
+// chunk are the work of one more warp, and its tiles are on their way meanwhile. PN:
+// planes of the kept states.
+template <class S_, bool KEEP, int PN>
+__global__ void __launch_bounds__(S_::ST + 32, KEEP && S_::SNT > 8 ? 1 : 2)
+state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) {
+    typedef typename S_::T T;
+    constexpr int NP = S_::NP, KD = S_::KD, VD = S_::VD, C = S_::C, NT = S_::SNT, SUB = S_::SUB, PER = C / SUB;
+    constexpr int STAGES = NP == 2 ? 2 : KEEP ? 3 : PER + 1;  // (a single chunk is asked for at once)
+    constexpr int STAGE = S_::KS + S_::VS;
+    extern __shared__ __align__(16) unsigned char smem[];
+    bf16* const tiles = reinterpret_cast<bf16*>(smem);
+    __shared__ Decays<C> dec_[2];
+    __shared__ Weights<C> weights_[2];
+    __shared__ __align__(16) bf16 by_[KEEP ? S_::SW : 1][KEEP ? 16 * (NT * 8 + 8) : 8];
+    const Pass& p = blockIdx.y ? p1 : p0;
+    const long long bh = KEEP ? blockIdx.x : blockIdx.x / j.chunks;
+    const int b = (int)(bh / j.H), h = (int)(bh % j.H), end = tokens_of(j, b);
+    const int c0 = KEEP ? 0 : blockIdx.x % j.chunks;
+    const int live = KEEP ? (end + C - 1) / C : c0 + (c0 * C < end), n = live - c0;
+    const auto chunk = [&](int i) { return p.back ? live - 1 - i : c0 + i; };
+    const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
+
+    if (warp == S_::SW) {  // the decays
+        constexpr int M = C / 32;
+        const float* g = j.g + b * j.gs.b + h * j.gs.h;
+        constexpr int AHEAD = 4;  // chunks whose log decays are on their way
+        float x[AHEAD][M];
+        const auto ask = [&](float* to, int i) {
+#pragma unroll
+            for (int k = 0; k < M; ++k) {
+                const int t = chunk(i) * C + l * M + k;
+                to[k] = i < n && t < end ? g[(long long)t * j.gs.t] : 0.0f;
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) ask(x[i], i);
+        if (n) decays<C>(&dec_[0], &weights_[0], x[0], p.back, j.scale);
+        for (int i = 0; i < n; ++i) {
+            __syncthreads();  // (what is written behind it was read a chunk ago)
+            if (!blockIdx.y) {
+                const float4* from = reinterpret_cast<const float4*>(&dec_[i & 1]);
+                float4* to = reinterpret_cast<float4*>(dec_out + bh * j.chunks + chunk(i));
+                for (int k = l; k < (int)sizeof(Decays<C>) / 16; k += 32) to[k] = from[k];
+            }
+#pragma unroll
+            for (int a = 0; a + 1 < AHEAD; ++a)
+#pragma unroll
+                for (int k = 0; k < M; ++k) x[a][k] = x[a + 1][k];
+            ask(x[AHEAD - 1], i + AHEAD);
+            if (i + 1 < n) decays<C>(&dec_[(i + 1) & 1], &weights_[(i + 1) & 1], x[0], p.back, j.scale);
+#pragma unroll
+            for (int k = 1; k < PER; ++k) __syncthreads();
+        }
+        return;
+    }
+
+    const int row = warp % S_::SR * 16, cb = warp / S_::SR * NT * 8;
+    const T* x = head_of<T>(p.x, p.xs, b, h / j.share);
+    const T* y = head_of<T>(p.y, p.ys, b, h);
+    const bool wx = j.whole >> (p.back ? 0 : 1) & 1, wy = j.whole >> (p.back ? 3 : 2) & 1;
+    Fetch<T, SUB, KD, S_::ST> lx;
+    Fetch<T, SUB, VD, S_::ST> ly;
+    // stage u of the pass: tokens [first(u), first(u) + SUB)
+    const int stages = n * PER;
+    const auto first = [&](int u) { return chunk(u / PER) * C + u % PER * SUB; };
+    const auto fetch = [&](int u, int stage) {
+        if (u < stages) {
+            bf16* to = tiles + stage * STAGE;
+            lx.fetch(to, x, p.xs.t, first(u), end, j.dk, wx);
+            ly.fetch(to + S_::KS, y, p.ys.t, first(u), end, j.dv, wy);
+        }
+        cp_async_commit();
+    };
+    const auto put = [&](int u, int stage) {
+        if (u < stages) {
+            bf16* to = tiles + stage * STAGE;
+            lx.put(to, x, p.xs.t, first(u), end, j.dk, wx);
+            ly.put(to + S_::KS, y, p.ys.t, first(u), end, j.dv, wy);
+        }
+    };
+    for (int u = 0; u < STAGES - 1; ++u) fetch(u, u);
+    put(0, 0);
+    float S[NT][4];
+    load_state<NT>(S, KEEP && p.start ? p.start + bh * j.dk * j.dv : nullptr, row, cb, j.dk, j.dv);
+    int stage = 0;
+    for (int i = 0; i < n; ++i) {
+        const Decays<C>& dec = dec_[i & 1];
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            const int u = i * PER + k;
+            cp_async_wait_group<STAGES - 2>();
+            __syncthreads();
+            fetch(u + STAGES - 1, (stage + STAGES - 1) % STAGES);
+            if (k == 0) {
+                if constexpr (KEEP)
+                    state_planes<PN, VD, NT>(S, p.kept + (bh * j.chunks + chunk(i)) * PN * KD * VD, KD * VD, row, cb,
+                                             by_[warp]);
+                if constexpr (KEEP) {
+                    const float w = dec.whole;
+#pragma unroll
+                    for (int m = 0; m < NT; ++m)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) S[m][e] *= w;
+                }
+            }
+            const bf16* from = tiles + stage * STAGE;
+            add_outer<NP, NT, SUB>(S, tile(from, S_::LK, SUB * S_::LK), tile(from + S_::KS, S_::LV, SUB * S_::LV),
+                                   weights_[i & 1].pair + k * SUB / 2, row, cb);
+            stage = (stage + 1) % STAGES;
+            put(u + 1, stage);
+        }
+    }
+    if constexpr (!KEEP) {
+        if (!n) return;
+        float* const to = p.sums + (bh * j.chunks + c0) * KD * VD;
+#pragma unroll
+        for (int m = 0; m < NT; ++m)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<float2*>(to + (row + (l >> 2) + i * 8) * VD + cb + m * 8 + (l & 3) * 2) =
+                    make_float2(S[m][2 * i], S[m][2 * i + 1]);
+        if (threadIdx.x == 0) p.factor[bh * j.chunks + c0] = dec_[0].whole;
+    } else if (p.end) {
+        store_state<NT>(S, p.end + bh * j.dk * j.dv, row, cb, j.dk, j.dv);
+    }
+}
+
+// The kept states and the last one from the chunks' sums: a thread for four
+// neighbouring values of a state.
+template <int KD, int VD, int C, int PN>
+__global__ void __launch_bounds__(256) scan_kernel(const Job j, const Pass p0, const Pass p1) {
+    const Pass& p = blockIdx.y ? p1 : p0;
+    const long long i = blockIdx.x * 256ll + threadIdx.x, bh = i / (KD * VD / 4);
+    if (bh >= (long long)j.B * j.H) return;
+    const int e = (int)(i % (KD * VD / 4)) * 4, r = e / VD, c = e % VD;
+    const int live = (tokens_of(j, (int)(bh / j.H)) + C - 1) / C;
+    constexpr int SIZE = KD * VD;
+    float S[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        S[k] = p.start && r < j.dk && c + k < j.dv ? p.start[(bh * j.dk + r) * j.dv + c + k] : 0.0f;
+    const float* const sums = p.sums + bh * j.chunks * SIZE + e;
+    const float* const factor = p.factor + bh * j.chunks;
+    bf16* const kept = p.kept + bh * j.chunks * PN * SIZE + e;
+    constexpr int U = 8;  // asked for together
+    for (int k0 = 0; k0 < live; k0 += U) {
+        float4 add[U];
+        float by[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = min(k0 + u, live - 1), k = p.back ? live - 1 - at : at;
+            add[u] = *reinterpret_cast<const float4*>(sums + (long long)k * SIZE);
+            by[u] = factor[k];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (k0 + u < live) {
+                const int k = p.back ? live - 1 - k0 - u : k0 + u;
+                const uint2 hi = {pack2(S[0], S[1]), pack2(S[2], S[3])};
+                *reinterpret_cast<uint2*>(kept + (long long)k * PN * SIZE) = hi;
+                if constexpr (PN == 2)
+                    *reinterpret_cast<uint2*>(kept + (long long)k * PN * SIZE + SIZE) =
+                        make_uint2(rest2(S[0], S[1], hi.x), rest2(S[2], S[3], hi.y));
+                S[0] = by[u] * S[0] + add[u].x, S[1] = by[u] * S[1] + add[u].y;
+                S[2] = by[u] * S[2] + add[u].z, S[3] = by[u] * S[3] + add[u].w;
+            }
+    }
+    if (p.end) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (r < j.dk && c + k < j.dv) p.end[(bh * j.dk + r) * j.dv + c + k] = S[k];
+    }
+}
+
+// ----------------------------------------------------------------- outputs
+// A CTA for each chunk: the states before them are there, so all run at once.
+// Heads go side by side: they lie so in memory.
+struct Chunk {
+    int b, h, c;
+    long long bh;
+    __device__ __forceinline__ explicit Chunk(const Job& j) {
+        const long long n = blockIdx.x / j.H;
+        h = blockIdx.x % j.H;
+        c = (int)(n % j.chunks);
+        b = (int)(n / j.chunks);
+        bh = (long long)b * j.H + h;
+    }
+};
+
+// A tile of kept states (PN planes of KD x VD), and a chunk's decays, by cp.async.
+template <class S_, int PN>
+__device__ __forceinline__ void load_kept(bf16* dst, const bf16* from) {
+    constexpr int PACKS = S_::KD * S_::VD / 8, ROW = S_::VD / 8;
+#pragma unroll
+    for (int n = 0; n < PN * PACKS / S_::THREADS; ++n) {
+        const int i = n * S_::THREADS + threadIdx.x;
+        cp_async16(dst + i / PACKS * S_::STATE + i % PACKS / ROW * S_::LV + i % ROW * 8, from + i * 8, 16);
+    }
+}
+template <int C>
+__device__ __forceinline__ void load_decays(Decays<C>* to, const Decays<C>* from) {
+    if (threadIdx.x < sizeof(Decays<C>) / 16)
+        cp_async16(reinterpret_cast<float4*>(to) + threadIdx.x, reinterpret_cast<const float4*>(from) + threadIdx.x,
+                   16);
+}
+
+template <class S_, int MIN>
+__global__ void __launch_bounds__(S_::THREADS, MIN)
+out_kernel(const Job j, const bf16* kept, const Decays<S_::C>* decs, void* out_) {
+    typedef typename S_::T T;
+    constexpr int NP = S_::NP, KD = S_::KD, C = S_::C, LK = S_::LK, LV = S_::LV, NT = S_::NV, NB = 2;
+    extern __shared__ __align__(16) unsigned char smem[];
+    bf16* const sq = reinterpret_cast<bf16*>(smem);
+    bf16 *const sk = sq + S_::KT, *const sv = sk + S_::KT, *const ss = sv + S_::VT;
+    __shared__ Decays<C> dec;
+    const Chunk at(j);
+    const int end = tokens_of(j, at.b), c0 = at.c * C;
+    const long long ot = (long long)j.H * j.dv;
+    T* out = static_cast<T*>(out_) + (long long)at.b * j.T * ot + (long long)at.h * j.dv;
+    if (c0 >= end) return zero_rows(out, ot, c0, min(c0 + C, j.T), j.dv);
+    const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
+    const int rb = warp % S_::RB, cb = warp / S_::RB * NT * 8;
+    const T* q = head_of<T>(j.q, j.qs, at.b, at.h / j.share);
+    const T* k = head_of<T>(j.k, j.ks, at.b, at.h / j.share);
+    const T* v = head_of<T>(j.v, j.vs, at.b, at.h);
+    Fetch<T, C, KD, S_::THREADS> lq, lk;
+    Fetch<T, C, S_::VD, S_::THREADS> lv;
+    lq.fetch(sq, q, j.qs.t, c0, end, j.dk, j.whole & 1);
+    load_kept<S_, NP>(ss, kept + (at.bh * j.chunks + at.c) * NP * KD * S_::VD);
+    load_decays<C>(&dec, decs + at.bh * j.chunks + at.c);
+    cp_async_commit();
+    lk.fetch(sk, k, j.ks.t, c0, end, j.dk, j.whole >> 1 & 1);
+    lv.fetch(sv, v, j.vs.t, c0, end, j.dv, j.whole >> 2 & 1);
+    cp_async_commit();
+    lq.put(sq, q, j.qs.t, c0, end, j.dk, j.whole & 1);
+    lk.put(sk, k, j.ks.t, c0, end, j.dk, j.whole >> 1 & 1);
+    lv.put(sv, v, j.vs.t, c0, end, j.dv, j.whole >> 2 & 1);
+    cp_async_wait_group<1>();
+    __syncthreads();
+    const Tile tq = tile(sq, LK, C * LK), tk = tile(sk, LK, C * LK), tv = tile(sv, LV, C * LV),
+               ts = tile(ss, LV, S_::STATE);
+
+    // Between the blocks of 16 tokens a decay is 2^(c_t - c_r) 2^(c_r - c_s), r the
+    // last token before the row's block: a factor of the row, which the state's
+    // part shares, and one of the column, which the warp writes down once. Both are
+    // at most 1. Within a block each pair has its own.
+    __shared__ float column_[S_::NW][C];
+    float* const column = column_[warp];
+    for (int s = l; s < rb * 16; s += 32) column[s] = dec.between(rb * 16 - 1, s);
+    __syncwarp();
+    float O[NT][4];
+    const int t = rb * 16 + (l >> 2);
+    const float r0 = (rb ? dec.between(t, rb * 16 - 1) : dec.from_start[t]) * j.scale;
+    const float r1 = (rb ? dec.between(t + 8, rb * 16 - 1) : dec.from_start[t + 8]) * j.scale;
+    const auto before = [&] {
+        clear<NT>(O);
+        product<NP, NP, KD, NT, true>(O, tq, rb * 16, ts, cb);
+        if (rb) {
+            const float begin = dec.from_start[rb * 16 - 1];
+            scale_rows<NT>(O, begin, begin);
+        }
+    };
+    const auto chunk = [&](bool apart) {
+        for (int jb = 0; jb < rb; jb += NB) {
+            float P[2 * NB][4];
+            scores<NP, KD, NB>(P, tq, rb * 16, tk, jb, 0, rb);
+            scale_columns<NB>(P, column, jb);
+            weighted<NP, NP, NB, NT>(O, P, tv, cb, jb, 0, rb);
+        }
+        scale_rows<NT>(O, r0, r1);
+        float P[2][4];
+        scores<NP, KD, 1>(P, tq, rb * 16, tk, rb, rb, rb + 1);
+        near_decays<C>(P, dec, rb, j.scale);
+        if (apart)
+            weighted_apart<NP, NT>(O, P, sv + rb * 16 * LV, LV, C * LV, cb);
+        else
+            weighted<NP, NP, 1, NT>(O, P, tv, cb, rb, rb, rb + 1);
+    };
+    before();
+    cp_async_wait_all();
+    __syncthreads();
+    chunk(false);
+    // a value of v that is not finite reaches every row of its block (times zero, in those before it)
+    float sum = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) sum = fmaf(O[n][0], 0.0f, fmaf(O[n][1], 0.0f, sum));
+    if (__any_sync(0xffffffffu, sum != 0.0f)) {
+        before();
+        chunk(true);
+    }
+    if constexpr (S_::VD <= KD) {  // by way of these rows' queries, which are done with
+        if constexpr (S_::CG > 1) named_bar_sync(rb + 1, S_::CG * 32);
+        store_rows_by<T, NT, LK>(sq + rb * 16 * LK + cb, O, out, ot, c0 + rb * 16, cb, end, j.T, j.dv);
+    } else {
+        store_rows<T, NT>(O, out, ot, c0 + rb * 16, cb, end, j.T, j.dv);
+    }
+}
+
+// ---------------------------------------------------------------- gradients
+struct Grads {
+    const void* dout;
+    Strides ds;
+    const bf16 *before, *behind;  // the states before the chunks, their gradients behind them
+    void *dq, *dk, *dv;
+    float *dq32, *dk32;  // in place of dq, dk: each head's own, where heads share q and k
+    float* dg;           // (B, T, H), or null
+};
+
+// A row of 16-bit pairs (or two planes of them) times a block of products: each
+// lane's part of the sums over the columns, for its rows g and g + 8.
+template <int NP, int NT>
+__device__ __forceinline__ void row_dots(const float (*x)[4], const bf16* tile, int ld, int step, int r,
+                                         int cb, float* sum) {
+    const int l = lane_id();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float s = 0.0f;
+        const bf16* at = tile + (r + (l >> 2) + i * 8) * ld + cb + (l & 3) * 2;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(at + n * 8);
+            float u = low(w), v = high(w);
+            if constexpr (NP == 2) {
+                const uint32_t w2 = *reinterpret_cast<const uint32_t*>(at + step + n * 8);
+                u += low(w2), v += high(w2);
+            }
+            s = fmaf(x[n][2 * i], u, s);
+            s = fmaf(x[n][2 * i + 1], v, s);
+        }
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        sum[i] = s;
+    }
+}
+
+// Sums over the eight lanes that hold the same columns, of N values of each: the
+// lanes share them out, and each ends with one (or, of fewer than eight, with one
+// that others have too). Returns which.
+template <int N>
+__device__ __forceinline__ int column_sums(float* v) {
+    const int l = lane_id();
+    int which = 0;
+#pragma unroll
+    for (int d = 16, n = N; d >= 4; d /= 2) {
+        if (n > 1) {
+            n /= 2;
+            const bool upper = l & d;
+#pragma unroll
+            for (int i = 0; i < n; ++i) {
+                const float keep = upper ? v[n + i] : v[i], give = upper ? v[i] : v[n + i];
+                v[i] = keep + __shfl_xor_sync(0xffffffffu, give, d);
+            }
+            if (upper) which += n;
+        } else {
+            v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
+        }
+    }
+    return which;
+}
+
+template <class S_, int MIN>
+__global__ void __launch_bounds__(S_::THREADS, MIN)
+grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
+    typedef typename S_::T T;
+    constexpr int NP = S_::NP, KD = S_::KD, VD = S_::VD, C = S_::C, LK = S_::LK, LV = S_::LV, NK = S_::NK, NV = S_::NV;
+    constexpr int RB = S_::RB, CG = S_::CG;
+    constexpr int NB = 2;  // blocks of a strip: two accumulators and two strips of scores are held
+    extern __shared__ __align__(16) unsigned char smem[];
+    bf16* const sq = reinterpret_cast<bf16*>(smem);
+    bf16 *const sk = sq + S_::KT, *const sv = sk + S_::KT, *const so = sv + S_::VT;
+    bf16* const ss = so + S_::VT;  // the gradient behind the chunk, then the state before it
+    __shared__ Decays<C> dec;
+    __shared__ float column_[S_::NW][C];
+    // parts of dg: by row block, and by column group where the columns are split
+    __shared__ float col_part[RB][C], row_part[C], dq_part[CG][C], dk_part[CG][C], dot_part[S_::NW];
+    const Chunk at(j);
+    const int end = tokens_of(j, at.b), c0 = at.c * C, c1 = min(c0 + C, j.T);
+    const long long kt = (long long)j.H * j.dk, vt = (long long)j.H * j.dv;
+    const long long k0 = (long long)at.b * j.T * kt + (long long)at.h * j.dk;
+    T* dv = static_cast<T*>(G.dv) + (long long)at.b * j.T * vt + (long long)at.h * j.dv;
+    float* dg = G.dg ? G.dg + (long long)at.b * j.T * j.H + at.h : nullptr;
+    if (c0 >= end) {
+        zero_rows(dv, vt, c0, c1, j.dv);
+        if (G.dq32) {
+            zero_rows(G.dq32 + k0, kt, c0, c1, j.dk);
+            zero_rows(G.dk32 + k0, kt, c0, c1, j.dk);
+        } else {
+            zero_rows(static_cast<T*>(G.dq) + k0, kt, c0, c1, j.dk);
+            zero_rows(static_cast<T*>(G.dk) + k0, kt, c0, c1, j.dk);
+        }
+        if (dg) zero_rows(dg, j.H, c0, c1, 1);
+        return;
+    }
+    const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
+    const int rb = warp % RB, cg = warp / RB, ck = cg * NK * 8, cv = cg * NV * 8;
+    const Tile tq = tile(sq, LK, C * LK), tk = tile(sk, LK, C * LK), tv = tile(sv, LV, C * LV),
+               to = tile(so, LV, C * LV), ts = tile(ss, LV, S_::STATE);
+    const long long kept = (at.bh * j.chunks + at.c) * 2 * KD * VD;
+    {
+        const T* q = head_of<T>(j.q, j.qs, at.b, at.h / j.share);
+        const T* k = head_of<T>(j.k, j.ks, at.b, at.h / j.share);
+        const T* v = head_of<T>(j.v, j.vs, at.b, at.h);
+        const T* dout = head_of<T>(G.dout, G.ds, at.b, at.h);
+        Fetch<T, C, KD, S_::THREADS> lq, lk;
+        Fetch<T, C, VD, S_::THREADS> lv, lo;
+        lk.fetch(sk, k, j.ks.t, c0, end, j.dk, j.whole >> 1 & 1);
+        load_kept<S_, 2>(ss, G.behind + kept);
+        load_decays<C>(&dec, decs + at.bh * j.chunks + at.c);
+        lv.fetch(sv, v, j.vs.t, c0, end, j.dv, j.whole >> 2 & 1);
+        cp_async_commit();
+        lk.put(sk, k, j.ks.t, c0, end, j.dk, j.whole >> 1 & 1);
+        lv.put(sv, v, j.vs.t, c0, end, j.dv, j.whole >> 2 & 1);
+        lq.fetch(sq, q, j.qs.t, c0, end, j.dk, j.whole & 1);
+        lo.fetch(so, dout, G.ds.t, c0, end, j.dv, j.whole >> 3 & 1);
+        cp_async_commit();
+        lq.put(sq, q, j.qs.t, c0, end, j.dk, j.whole & 1);
+        lo.put(so, dout, G.ds.t, c0, end, j.dv, j.whole >> 3 & 1);
+    }
+    cp_async_wait_group<1>();
+    __syncthreads();
+    // (by way of the states' place, a part of it for each warp)
+    constexpr int BK = NK * 8 + 8, BV = NV * 8 + 8, BY = BK > BV ? BK : BV;
+    static_assert(S_::NW * 16 * BY <= 2 * S_::STATE, "room for every warp's rows");
+    bf16* const by = ss + warp * 16 * BY;
+    const auto store_head = [&](const float(*x)[4], void* to16, float* to32) {
+        if (to32)
+            store_rows<float, NK>(x, to32 + k0, kt, c0 + rb * 16, ck, end, j.T, j.dk);
+        else
+            store_rows_by<T, NK, BK>(by, x, static_cast<T*>(to16) + k0, kt, c0 + rb * 16, ck, end, j.T, j.dk);
+    };
+    float* const column = column_[warp];
+    float part[2];
+    const int t = rb * 16 + (l >> 2);  // the lane's tokens: this and 8 behind
+    {
+        // rows s, columns u >= s. Between blocks a decay is 2^(c_u - c_r) 2^(c_r - c_s), r
+        // the last token of the row's block
+        const int r = rb * 16 + 15;
+        for (int u = r + 1 + l; u < C; u += 32) column[u] = dec.between(u, r) * j.scale;
+        const float b0 = dec.between(r, t), b1 = dec.between(r, t + 8), behind = dec.to_end[r];
+        float V[NV][4], K[NK][4], across[2] = {0.0f, 0.0f};
+        clear<NV>(V);
+        product<NP, NP, KD, NV, true>(V, tk, rb * 16, ts, cv);
+        scale_rows<NV>(V, behind, behind);
+        clear<NK>(K);
+        product<NP, 2, VD, NK, false>(K, tv, rb * 16, ts, ck);
+        scale_rows<NK>(K, behind, behind);
+        row_dots<NP, NK>(K, sk, LK, C * LK, rb * 16, ck, part);
+        if ((l & 3) == 0) dk_part[cg][t] = part[0] * b0, dk_part[cg][t + 8] = part[1] * b1;
+        cp_async_wait_all();  // queries and the gradient of the outputs
+        __syncthreads();
+        for (int jb = (rb + 1) / NB * NB; jb < RB; jb += NB) {
+            float P[2 * NB][4], Q[2 * NB][4], down[4 * NB];
+            scores<NP, KD, NB>(P, tk, rb * 16, tq, jb, rb + 1, RB);
+            scores<NP, VD, NB>(Q, tv, rb * 16, to, jb, rb + 1, RB);
+#pragma unroll
+            for (int n = 0; n < 2 * NB; ++n) {
+                const int u = jb * 16 + n * 8 + (l & 3) * 2;
+                const float2 f = *reinterpret_cast<const float2*>(column + u);
+                const bool in = jb + n / 2 > rb;  // (the factors of other blocks are not there)
+                const float x0 = P[n][0] * Q[n][0], x1 = P[n][1] * Q[n][1], x2 = P[n][2] * Q[n][2],
+                            x3 = P[n][3] * Q[n][3];
+                down[2 * n] = in ? (x0 * b0 + x2 * b1) * f.x : 0.0f;
+                down[2 * n + 1] = in ? (x1 * b0 + x3 * b1) * f.y : 0.0f;
+                across[0] += in ? x0 * f.x + x1 * f.y : 0.0f;
+                across[1] += in ? x2 * f.x + x3 * f.y : 0.0f;
+                P[n][0] *= f.x, P[n][1] *= f.y, P[n][2] *= f.x, P[n][3] *= f.y;
+                Q[n][0] *= f.x, Q[n][1] *= f.y, Q[n][2] *= f.x, Q[n][3] *= f.y;
+            }
+            const int which = column_sums<4 * NB>(down);
+            if (cg == 0) col_part[rb][jb * 16 + which / 2 * 8 + (l & 3) * 2 + which % 2] = down[0];
+            weighted<NP, NP, NB, NV>(V, P, to, cv, jb, rb + 1, RB);
+            weighted<NP, NP, NB, NK>(K, Q, tq, ck, jb, rb + 1, RB);
+        }
+        scale_rows<NV>(V, b0, b1);
+        scale_rows<NK>(K, b0, b1);
+        across[0] *= b0, across[1] *= b1;
+        float P[2][4], Q[2][4], down[4] = {};
+        scores<NP, KD, 1>(P, tk, rb * 16, tq, rb, rb, rb + 1);
+        scores<NP, VD, 1>(Q, tv, rb * 16, to, rb, rb, rb + 1);
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int s = t + (i >> 1) * 8, u = rb * 16 + n * 8 + (l & 3) * 2 + (i & 1);
+                const float w = dec.between(u, s) * j.scale, p = P[n][i] * w;
+                const float a = u > s ? p * Q[n][i] : 0.0f;
+                P[n][i] = u >= s ? p : 0.0f;
+                Q[n][i] = u >= s ? Q[n][i] * w : 0.0f;
+                across[i >> 1] += a;
+                down[2 * n + (i & 1)] += a;
+            }
+        const int which = column_sums<4>(down);
+        if (cg == 0) col_part[rb][rb * 16 + which / 2 * 8 + (l & 3) * 2 + which % 2] = down[0];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            across[i] += __shfl_xor_sync(0xffffffffu, across[i], 1);
+            across[i] += __shfl_xor_sync(0xffffffffu, across[i], 2);
+        }
+        if (cg == 0 && (l & 3) == 0) row_part[t] = across[0], row_part[t + 8] = across[1];
+        weighted<NP, NP, 1, NV>(V, P, to, cv, rb, rb, rb + 1);
+        weighted<NP, NP, 1, NK>(K, Q, tq, ck, rb, rb, rb + 1);
+        // <R, S>, and then their place is free
+        float dot = 0.0f;
+        if (dg) {
+            const uint4* from = reinterpret_cast<const uint4*>(G.before + kept);
+            constexpr int PACKS = KD * VD / 8, ROW = VD / 8;
+#pragma unroll 4
+            for (int i = threadIdx.x; i < PACKS; i += S_::THREADS) {
+                const uint4 hi = from[i], lo = from[PACKS + i];
+                const uint4 r = *reinterpret_cast<const uint4*>(ss + i / ROW * LV + i % ROW * 8);
+                const uint4 r2 = *reinterpret_cast<const uint4*>(ss + S_::STATE + i / ROW * LV + i % ROW * 8);
+                const uint32_t a[4] = {r.x, r.y, r.z, r.w}, b[4] = {r2.x, r2.y, r2.z, r2.w};
+                const uint32_t x[4] = {hi.x, hi.y, hi.z, hi.w}, y[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    dot = fmaf(low(a[e]) + low(b[e]), low(x[e]) + low(y[e]), dot);
+                    dot = fmaf(high(a[e]) + high(b[e]), high(x[e]) + high(y[e]), dot);
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 16; d; d /= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+        if (l == 0) dot_part[warp] = dot;
+        __syncthreads();
+        store_rows_by<T, NV, BV>(by, V, dv, vt, c0 + rb * 16, cv, end, j.T, j.dv);
+        store_head(K, G.dk, G.dk32);
+    }
+    __syncthreads();
+    load_kept<S_, 2>(ss, G.before + kept);
+    cp_async_wait_all();
+    for (int s = l; s < rb * 16; s += 32) column[s] = dec.between(rb * 16 - 1, s);
+    __syncthreads();
+    {
+        // rows u, columns s <= u, as the outputs
+        float X[NK][4], P[2][4];
+        clear<NK>(X);
+        product<NP, 2, VD, NK, false>(X, to, rb * 16, ts, ck);
+        const float begin = rb ? dec.from_start[rb * 16 - 1] : 1.0f;
+        scale_rows<NK>(X, begin, begin);
+        const float r0 = (rb ? dec.between(t, rb * 16 - 1) : dec.from_start[t]) * j.scale;
+        const float r1 = (rb ? dec.between(t + 8, rb * 16 - 1) : dec.from_start[t + 8]) * j.scale;
+        row_dots<NP, NK>(X, sq, LK, C * LK, rb * 16, ck, part);
+        if ((l & 3) == 0) dq_part[cg][t] = part[0] * r0, dq_part[cg][t + 8] = part[1] * r1;
+        for (int jb = 0; jb < rb; jb += NB) {
+            float Q[2 * NB][4];
+            scores<NP, VD, NB>(Q, to, rb * 16, tv, jb, 0, rb);
+            scale_columns<NB>(Q, column, jb);
+            weighted<NP, NP, NB, NK>(X, Q, tk, ck, jb, 0, rb);
+        }
+        scale_rows<NK>(X, r0, r1);
+        scores<NP, VD, 1>(P, to, rb * 16, tv, rb, rb, rb + 1);
+        near_decays<C>(P, dec, rb, j.scale);
+        weighted<NP, NP, 1, NK>(X, P, tk, ck, rb, rb, rb + 1);
+        __syncthreads();
+        store_head(X, G.dq, G.dq32);
+    }
+    if (warp == 0 && dg) {
+        // behind: sum over u >= t of (rho_u + r_u) - sum over s >= t of kappa_s; ahead: sum over s < t of l_s
+        constexpr int M = C / 32;
+        float behind[M], ahead[M], all = 0.0f, b = 0.0f, a = 0.0f;
+#pragma unroll
+        for (int i = 0; i < S_::NW; ++i) all += dot_part[i];
+        all *= dec.whole;
+#pragma unroll
+        for (int i = M - 1; i >= 0; --i) {
+            const int u = l * M + i;
+            float x = -row_part[u];
+#pragma unroll
+            for (int r = 0; r < RB; ++r)
+                if (r <= u / 16) x += col_part[r][u];
+#pragma unroll
+            for (int r = 0; r < CG; ++r) x += dq_part[r][u];
+            behind[i] = b += x;
+        }
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            ahead[i] = a;
+#pragma unroll
+            for (int r = 0; r < CG; ++r) a += dk_part[r][l * M + i];
+        }
+        float bs = b, as = a;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const float y = __shfl_down_sync(0xffffffffu, bs, d), z = __shfl_up_sync(0xffffffffu, as, d);
+            if (l + d < 32) bs += y;
+            if (l >= d) as += z;
+        }
+        bs -= b, as -= a;
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            const int u = c0 + l * M + i;
+            if (u < j.T) dg[(long long)u * j.H] = u < end ? all + behind[i] + bs + ahead[i] + as : 0.0f;
+        }
+    }
+}
+
+// Sums over the heads that share one of q and k.
+template <typename T>
+__global__ void __launch_bounds__(256) fold_kernel(const float* x, const float* y, T* to_x, T* to_y,
+                                                   int share, int d, long long n) {
+    const float* from = blockIdx.y ? y : x;
+    T* to = blockIdx.y ? to_y : to_x;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+        const float* at = from + i / d * share * d + i % d;
+        float s = 0.0f;
+        for (int r = 0; r < share; ++r) s += at[(long long)r * d];
+        to[i] = from_f<T>(s);
+    }
+}
+
+// dg (n, H) summed down its rows, in fp64 and always in one order: a CTA for
+// each part of the rows, the parts by a second launch of one.
+__global__ void __launch_bounds__(256) gate_kernel(const float* dg, const double* parts, double* to_parts,
+                                                   float* out, long long n, int H, int count) {
+    __shared__ double s[8];
+    for (int h = blockIdx.y; h < H; h += gridDim.y) {
+        double x = 0.0;
+        if (dg) {
+            for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll)
+                x += (double)dg[i * H + h];
+        } else {
+            for (int i = threadIdx.x; i < count; i += 256) x += parts[(long long)h * count + i];
+        }
+#pragma unroll
+        for (int d = 16; d; d /= 2) x += __shfl_xor_sync(0xffffffffu, x, d);
+        if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = x;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int i = 1; i < 8; ++i) x += s[i];
+            if (dg)
+                to_parts[(long long)h * gridDim.x + blockIdx.x] = x;
+            else
+                out[h] = (float)x;
+        }
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------ launches
+template <class S_>
+struct Sizes {
+    static constexpr int state = (S_::NP == 1 ? 3 : 2) * (S_::KS + S_::VS) * 2, sum = S_::C / S_::SUB * (S_::KS + S_::VS) * 2;
+    static constexpr int out = (2 * S_::KT + S_::VT + S_::NP * S_::STATE) * 2;
+    static constexpr int grad = (2 * S_::KT + 2 * S_::VT + 2 * S_::STATE) * 2;
+};
+
+template <typename K>
+int allow(K* kernel, int bytes, const char* what) {
+    return cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+}
+
+// Whether each chunk's sum gets a CTA: where the heads alone leave SMs idle. (The
+// sums cost a write and a read of a state in fp32 for each chunk; one prompt of 8192
+// tokens and 12 heads of 128 otherwise waits for 128 chunks, one after the other.)
+void cut(Job* j, int C, int passes) {
+    j->chunks = (j->T + C - 1) / C;
+    j->apart = j->chunks > 1 && (long long)j->B * j->H * passes < 148;
+}
+
+constexpr int kGateParts = 64;
+
+// The workspace, in bytes from its start (each a multiple of 256).
+struct Space {
+    long long sums, factor, back, back_factor, decays, kept, kept_back, dq32, dk32, dg, gates, bytes;
+};
+long long up(long long n) { return (n + 255) / 256 * 256; }
+
+template <class S_>
+Space space_of(const Job& j, bool back, bool gates_alike) {
+    Space s = {};
+    const long long bh = (long long)j.B * j.H, plane = bh * j.chunks * S_::KD * S_::VD * 2;
+    long long at = 0;
+    const auto take = [&](long long bytes) {
+        const long long a = at;
+        at += up(bytes);
+        return a;
+    };
+    for (int i = 0; i < 1 + back; ++i)
+        if (j.apart) {
+            (i ? s.back : s.sums) = take(plane * 2);
+            (i ? s.back_factor : s.factor) = take(bh * j.chunks * 4);
+        }
+    s.decays = take(bh * j.chunks * sizeof(Decays<S_::C>));
+    s.kept = take(plane * (back ? 2 : S_::NP));
+    if (back) {
+        s.kept_back = take(plane * 2);
+        if (j.share > 1) {
+            s.dq32 = take(bh * j.T * j.dk * 4);
+            s.dk32 = take(bh * j.T * j.dk * 4);
+        }
+        if (gates_alike) {
+            s.dg = take(bh * j.T * 4);
+            s.gates = take((long long)kGateParts * j.H * 8);
+        }
+    }
+    s.bytes = at;
+    return s;
+}
+
+// The states that the chunks need.
+template <class S_, int PN>
+int states(const Job& j, const Pass& p0, const Pass& p1, bool both, Decays<S_::C>* dec, cudaStream_t st) {
+    const long long bh = (long long)j.B * j.H;
+    constexpr int threads = S_::ST + 32, bytes = Sizes<S_>::state, SIZE = S_::KD * S_::VD;
+    static_assert(bytes <= 180 * 1024, "shared memory of a CTA");
+    if (j.apart) {
+        auto* sum = state_kernel<S_, false, PN>;
+        SN_TRY(allow(sum, Sizes<S_>::sum, "linear_attention"));
+        sum<<<dim3((unsigned)(bh * j.chunks), 1 + both), threads, Sizes<S_>::sum, st>>>(j, p0, p1, dec);
+        scan_kernel<S_::KD, S_::VD, S_::C, PN>
+            <<<dim3((unsigned)((bh * SIZE / 4 + 255) / 256), 1 + both), 256, 0, st>>>(j, p0, p1);
+    } else {
+        auto* keep = state_kernel<S_, true, PN>;
+        SN_TRY(allow(keep, bytes, "linear_attention"));
+        keep<<<dim3((unsigned)bh, 1 + both), threads, bytes, st>>>(j, p0, p1, dec);
+    }
+    return cuda_check(cudaGetLastError(), "linear_attention launch");
+}
+
+int check_space(const Job& j, const Space& s, const char* what, const char* ws, long long ws_bytes) {
+    if (s.bytes > ws_bytes || (s.bytes && !ws))
+        return fail(SN_E_INVAL, "%s: a workspace of %lld bytes is wanted", what, s.bytes);
+    if ((long long)j.B * j.H * j.chunks > 0x7fffffffll)
+        return fail(SN_E_INVAL, "%s: too many chunks", what);
+    return SN_OK;
+}
+
+template <class S_>
+int forward_as(Job j, const float* first, void* out, float* state_out, char* ws, long long ws_bytes, long long* need,
+            cudaStream_t st) {
+    cut(&j, S_::C, 1);
+    const Space s = space_of<S_>(j, false, false);
+    if (need) {
+        *need = s.bytes;
+        return SN_OK;
+    }
+    SN_TRY(check_space(j, s, "linear_attention", ws, ws_bytes));
+    Pass p = {j.k, j.v, j.ks, j.vs};
+    p.start = first;
+    p.sums = reinterpret_cast<float*>(ws + s.sums), p.factor = reinterpret_cast<float*>(ws + s.factor);
+    p.kept = reinterpret_cast<bf16*>(ws + s.kept);
+    p.end = state_out;
+    auto* dec = reinterpret_cast<Decays<S_::C>*>(ws + s.decays);
+    SN_TRY((states<S_, S_::NP>(j, p, p, false, dec, st)));
+    if (!j.chunks) return SN_OK;
+    constexpr int bytes = Sizes<S_>::out;
+    static_assert(bytes <= 220 * 1024, "shared memory of a CTA");
+    auto* kernel = out_kernel<S_, bytes <= 66 * 1024 ? 3 : bytes <= 96 * 1024 ? 2 : 1>;
+    SN_TRY(allow(kernel, bytes, "linear_attention"));
+    kernel<<<(unsigned)((long long)j.B * j.H * j.chunks), S_::THREADS, bytes, st>>>(j, p.kept, dec, out);
+    return cuda_check(cudaGetLastError(), "linear_attention launch");
+}
+
+template <class S_>
+int backward_as(Job j, const float* first, const Wanted& g, char* ws, long long ws_bytes, long long* need,
+             cudaStream_t st) {
+    typedef typename S_::T T;
+    cut(&j, S_::C, 2);
+    const Space s = space_of<S_>(j, true, g.gates_alike);
+    if (need) {
+        *need = s.bytes;
+        return SN_OK;
+    }
+    SN_TRY(check_space(j, s, "linear_attention_bwd", ws, ws_bytes));
+    const auto floats = [&](long long at) { return reinterpret_cast<float*>(ws + at); };
+    Pass p = {j.k, j.v, j.ks, j.vs}, r = {j.q, g.dout, j.qs, g.ds};
+    p.start = first, r.start = g.dstate_out;
+    p.sums = floats(s.sums), p.factor = floats(s.factor);
+    p.kept = reinterpret_cast<bf16*>(ws + s.kept);
+    r.sums = floats(s.back), r.factor = floats(s.back_factor);
+    r.kept = reinterpret_cast<bf16*>(ws + s.kept_back);
+    r.end = g.dstate;
+    r.back = true;
+    auto* dec = reinterpret_cast<Decays<S_::C>*>(ws + s.decays);
+    SN_TRY((states<S_, 2>(j, p, r, true, dec, st)));
+    Grads G = {};
+    G.dout = g.dout, G.ds = g.ds;
+    G.before = p.kept, G.behind = r.kept;
+    G.dq = g.dq, G.dk = g.dk, G.dv = g.dv;
+    if (j.share > 1) G.dq32 = floats(s.dq32), G.dk32 = floats(s.dk32);
+    G.dg = !g.dg ? nullptr : g.gates_alike ? floats(s.dg) : g.dg;
+    constexpr int bytes = Sizes<S_>::grad;
+    static_assert(bytes <= 220 * 1024, "shared memory of a CTA");
+    auto* kernel = grad_kernel<S_, bytes <= 96 * 1024 ? 2 : 1>;
+    SN_TRY(allow(kernel, bytes, "linear_attention_bwd"));
+    if (j.chunks)
+        kernel<<<(unsigned)((long long)j.B * j.H * j.chunks), S_::THREADS, bytes, st>>>(j, G, dec);
+    const long long rows = (long long)j.B * j.T;
+    if (j.share > 1 && rows) {
+        const long long n = rows * (j.H / j.share) * j.dk;
+        fold_kernel<T><<<dim3((unsigned)std::min((n + 255) / 256, 8ll * 148), 2), 256, 0, st>>>(
+            G.dq32, G.dk32, static_cast<T*>(g.dq), static_cast<T*>(g.dk), j.share, j.dk, n);
+    }
+    if (g.dg && g.gates_alike) {
+        double* parts = reinterpret_cast<double*>(ws + s.gates);
+        const unsigned ys = (unsigned)std::min(j.H, 65535);
+        gate_kernel<<<dim3(kGateParts, ys), 256, 0, st>>>(G.dg, nullptr, parts, nullptr, rows, j.H, 0);
+        gate_kernel<<<dim3(1, ys), 256, 0, st>>>(nullptr, parts, nullptr, g.dg, 0, j.H, kGateParts);
+    }
+    return cuda_check(cudaGetLastError(), "linear_attention_bwd launch");
+}
+
+// The widths that the keys and the values are laid out in, and the tokens of a
+// chunk: the longer, the fewer states are kept and read again (in bf16 with heads of
+// up to 64, the states of a chunk of 128 take half of what its keys do), and the more
+// shared memory the tiles take.
+template <typename T, typename F>
+int by_width(const Job& j, F&& f) {
+    constexpr int LONG = planes_of<T> == 1 ? 128 : 64;
+    if (j.dk <= 64) return j.dv <= 64 ? f(Shape<T, 64, 64, LONG>()) : f(Shape<T, 64, 128, 64>());
+    return j.dv <= 64 ? f(Shape<T, 128, 64, 64>()) : f(Shape<T, 128, 128, 64>());
+}
+
+}  // namespace
+
+template <typename T>
+int forward(const Job& j, const float* first, void* out, float* state_out, char* ws, long long ws_bytes,
+            long long* need, cudaStream_t st) {
+    return by_width<T>(j, [&](auto s) {
+        return forward_as<decltype(s)>(j, first, out, state_out, ws, ws_bytes, need, st);
+    });
+}
+
+template <typename T>
+int backward(const Job& j, const float* first, const Wanted& w, char* ws, long long ws_bytes, long long* need,
+             cudaStream_t st) {
+    return by_width<T>(j, [&](auto s) { return backward_as<decltype(s)>(j, first, w, ws, ws_bytes, need, st); });
+}
+
+}  // namespace la
+}  // namespace sn

@@ -10,9 +10,9 @@
 // gradients take 75 us of the host's time (torch's own layer norm 70), as a
 // Function in Python 110; a call without a graph 8 us instead of 11.
 //
-// embedding, linear_attention (calls and nodes alike) and linear_attention_step:
-// with their checks in Python they took 20 to 30 us of the host's time a call,
-// longer than most of their kernels.
+// embedding, linear_attention (calls and nodes alike), linear_attention_step and
+// grad_norm: with their checks in Python they took 20 to 30 us of the host's time
+// a call, longer than most of their kernels.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -51,6 +51,9 @@ struct {
     decltype(&sn_abi_linear_attention_bwd) attention_bwd = nullptr;
     decltype(&sn_abi_linear_attention_ws) attention_ws = nullptr;
     decltype(&sn_abi_linear_attention_step) attention_step = nullptr;
+    decltype(&sn_abi_grad_norm_ws) grad_norm_ws = nullptr;
+    decltype(&sn_abi_grad_norm) grad_norm = nullptr;
+    decltype(&sn_abi_clip_grads) clip_grads = nullptr;
 } lib;
 
 std::string last_error() {
@@ -456,9 +459,9 @@ PyObject* linear_attention_step(PyObject*, PyObject* args) {
 
 // use(addresses of the library's entry points, in the order below)
 PyObject* use(PyObject*, PyObject* args) {
-    unsigned long long p[11];
-    if (!PyArg_ParseTuple(args, "KKKKKKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, p + 7, p + 8, p + 9,
-                          p + 10))
+    unsigned long long p[14];
+    if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, p + 7, p + 8, p + 9,
+                          p + 10, p + 11, p + 12, p + 13))
         return nullptr;
     lib.norm = reinterpret_cast<decltype(lib.norm)>(p[0]);
     lib.norm_bwd = reinterpret_cast<decltype(lib.norm_bwd)>(p[1]);
@@ -471,6 +474,9 @@ PyObject* use(PyObject*, PyObject* args) {
     lib.attention_bwd = reinterpret_cast<decltype(lib.attention_bwd)>(p[8]);
     lib.attention_ws = reinterpret_cast<decltype(lib.attention_ws)>(p[9]);
     lib.attention_step = reinterpret_cast<decltype(lib.attention_step)>(p[10]);
+    lib.grad_norm_ws = reinterpret_cast<decltype(lib.grad_norm_ws)>(p[11]);
+    lib.grad_norm = reinterpret_cast<decltype(lib.grad_norm)>(p[12]);
+    lib.clip_grads = reinterpret_cast<decltype(lib.clip_grads)>(p[13]);
     Py_RETURN_NONE;
 }
 
@@ -570,72 +576,67 @@ PyObject* read(PyObject*, PyObject* args) {
     }
 }
 
-// read_grads(list, apart) -> (addresses, sizes, types, index of the GPU): tensors
-// of float types on one GPU, whose values fill one run of memory in any order;
-// with `apart`, no memory belongs to two of them.
-PyObject* read_grads(PyObject*, PyObject* args) {
+// grad_norm(list, max_norm, clip) -> (norm, factor), with `clip` the norm alone, of the gradients in a list or
+// tuple: tensors of float types on one GPU, each filling one run of memory in any
+// order. With `clip` they are scaled in place; no memory then belongs to two of them.
+PyObject* grad_norm(PyObject*, PyObject* args) {
+    HANDLE_TH_ERRORS
     PyObject* list;
-    int apart;
-    if (!PyArg_ParseTuple(args, "Op", &list, &apart)) return nullptr;
-    try {
-        Py_ssize_t n = 0;
-        PyObject** const of = items(list, &n);
-        if (!of) return nullptr;
-        std::vector<uint64_t> at(n);
-        std::vector<int64_t> sizes(n);
-        std::vector<int32_t> types(n);
-        std::vector<std::pair<uint64_t, uint64_t>> written;
-        c10::Device device(c10::kCPU);
-        for (Py_ssize_t j = 0; j < n; ++j) {
-            if (!THPVariable_Check(of[j])) {
-                PyErr_SetString(PyExc_TypeError, "tensors are wanted");
-                return nullptr;
-            }
-            const at::Tensor& t = THPVariable_Unpack(of[j]);
-            if (t.layout() != at::kStrided) {
-                PyErr_SetString(PyExc_ValueError, "sparse gradients are not supported");
-                return nullptr;
-            }
-            const at::ScalarType type = t.scalar_type();
-            if (type != at::kFloat && type != at::kBFloat16 && type != at::kHalf) {
-                PyErr_SetString(PyExc_TypeError, "gradients are of float32, bfloat16 or float16");
-                return nullptr;
-            }
-            if (j == 0) device = t.device();
-            if (!t.device().is_cuda() || t.device() != device) {
-                PyErr_SetString(PyExc_ValueError, "every gradient must be on one GPU");
-                return nullptr;
-            }
-            if (!t.is_non_overlapping_and_dense()) {
-                PyErr_SetString(PyExc_ValueError, "a gradient's values must fill one run of memory");
-                return nullptr;
-            }
-            sizes[j] = t.numel();
-            types[j] = code(type);
-            at[j] = reinterpret_cast<uint64_t>(sizes[j] ? t.data_ptr() : nullptr);
-            if (apart && sizes[j]) written.emplace_back(at[j], at[j] + sizes[j] * t.element_size());
+    double max_norm;
+    int clip;
+    if (!PyArg_ParseTuple(args, "Odp", &list, &max_norm, &clip)) return nullptr;
+    Py_ssize_t n = 0;
+    PyObject** const of = items(list, &n);
+    if (!of && PyErr_Occurred()) return nullptr;  // (an empty list may have no items at all)
+    const char* const what = clip ? "clip_grads" : "grad_norm";
+    TORCH_CHECK_VALUE(n > 0 && n < 0x7fffffff, what, ": no gradients");
+    TORCH_CHECK_VALUE(max_norm >= 0, what, ": max_norm must not be negative");
+    std::vector<void*> at(n);
+    std::vector<int64_t> sizes(n);
+    std::vector<int32_t> types(n);
+    std::vector<std::pair<uint64_t, uint64_t>> written;
+    for (Py_ssize_t j = 0; j < n; ++j) {
+        TORCH_CHECK_TYPE(THPVariable_Check(of[j]), what, ": tensors are wanted");
+        const at::Tensor& t = THPVariable_Unpack(of[j]);
+        TORCH_CHECK_VALUE(t.layout() == at::kStrided, what, ": sparse gradients are not supported");
+        TORCH_CHECK_TYPE(float_type(t), what, ": gradients are of float32, bfloat16 or float16");
+        TORCH_CHECK_VALUE(t.is_cuda() && t.device() == THPVariable_Unpack(of[0]).device(), what,
+                          ": every gradient must be on one GPU");
+        TORCH_CHECK_VALUE(t.is_non_overlapping_and_dense(), what,
+                          ": a gradient's values must fill one run of memory");
+        sizes[j] = t.numel();
+        types[j] = code(t.scalar_type());
+        at[j] = sizes[j] ? t.data_ptr() : nullptr;
+        if (clip && sizes[j]) {
+            const uint64_t begin = reinterpret_cast<uint64_t>(at[j]);
+            written.emplace_back(begin, begin + sizes[j] * t.element_size());
         }
-        std::sort(written.begin(), written.end());
-        if (std::adjacent_find(written.begin(), written.end(), [](const auto& a, const auto& b) {
-                return b.first < a.second;
-            }) != written.end()) {
-            PyErr_SetString(PyExc_ValueError, "a gradient appears twice, or overlaps another");
-            return nullptr;
-        }
-        return Py_BuildValue("(y#y#y#i)", reinterpret_cast<const char*>(at.data()),
-                             static_cast<Py_ssize_t>(n * 8), reinterpret_cast<const char*>(sizes.data()),
-                             static_cast<Py_ssize_t>(n * 8), reinterpret_cast<const char*>(types.data()),
-                             static_cast<Py_ssize_t>(n * 4), n ? (int)device.index() : -1);
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
-        return nullptr;
     }
+    std::sort(written.begin(), written.end());
+    TORCH_CHECK_VALUE(std::adjacent_find(written.begin(), written.end(),
+                                         [](const auto& a, const auto& b) { return b.first < a.second; }) ==
+                          written.end(),
+                      what, ": a gradient appears twice, or overlaps another");
+    const at::Tensor& first = THPVariable_Unpack(of[0]);
+    const int64_t need = lib.grad_norm_ws((int32_t)n, sizes.data());
+    TORCH_CHECK_VALUE(need >= 0, what, ": too many values");
+    const at::Tensor ws = at::empty({2 + need / 4}, first.options().dtype(at::kFloat));
+    float* const to = ws.data_ptr<float>();
+    const int rc = clip ? lib.clip_grads((int32_t)n, at.data(), sizes.data(), types.data(), max_norm, to, to + 1,
+                                         to + 2, need, stream_of(first))
+                        : lib.grad_norm((int32_t)n, at.data(), sizes.data(), types.data(), max_norm, to, to + 1,
+                                        to + 2, need, stream_of(first));
+    TORCH_CHECK(rc == SN_OK, last_error());
+    if (clip)  // a graph that saved one must not use it
+        for (Py_ssize_t j = 0; j < n; ++j) THPVariable_Unpack(of[j]).unsafeGetTensorImpl()->bump_version();
+    if (clip) return THPVariable_Wrap(ws.select(0, 0));
+    return Py_BuildValue("(NN)", THPVariable_Wrap(ws.select(0, 0)), THPVariable_Wrap(ws.select(0, 1)));
+    END_HANDLE_TH_ERRORS
 }
 
 PyMethodDef methods[] = {
     {"read", read, METH_VARARGS, "read(lists, dtypes, block) -> (addresses, sizes)"},
-    {"read_grads", read_grads, METH_VARARGS,
-     "read_grads(list, apart) -> (addresses, sizes, types, index of the GPU)"},
+    {"grad_norm", grad_norm, METH_VARARGS, "grad_norm(list, max_norm, clip) -> (norm, factor)"},
     {"layer_norm", layer_norm, METH_VARARGS, "layer_norm(x, weight, bias, eps) -> y"},
     {"embedding", embedding, METH_VARARGS, "embedding(tokens, weight, scale) -> rows"},
     {"linear_attention", linear_attention, METH_VARARGS,

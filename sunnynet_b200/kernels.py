@@ -233,7 +233,8 @@ def _torch_calls():
             lib.sn_abi_layer_norm, lib.sn_abi_layer_norm_bwd, lib.sn_abi_layer_norm_bwd_ws,
             lib.sn_abi_last_error, lib.sn_abi_embedding, lib.sn_abi_embedding_bwd,
             lib.sn_abi_embedding_bwd_ws, lib.sn_abi_linear_attention, lib.sn_abi_linear_attention_bwd,
-            lib.sn_abi_linear_attention_ws, lib.sn_abi_linear_attention_step)))
+            lib.sn_abi_linear_attention_ws, lib.sn_abi_linear_attention_step, lib.sn_abi_grad_norm_ws,
+            lib.sn_abi_grad_norm, lib.sn_abi_clip_grads)))
         _TORCH_CALLS = m
     return _TORCH_CALLS
 
@@ -336,46 +337,24 @@ def embedding(tokens, weight, scale: float = 1.0):
     return (_TORCH_CALLS or _torch_calls()).embedding(tokens, weight, scale)
 
 
-def _norm_call(name, grads, max_norm, apart):
-    """The call of a list of gradients: (norm and factor, the list)."""
-    import torch
-    if not isinstance(grads, (list, tuple)):
-        grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    if not grads:
-        raise ValueError(f"{name}: no gradients")
-    max_norm = float(max_norm)
-    if not max_norm >= 0:
-        raise ValueError(f"{name}: max_norm must not be negative")
-    at, sizes, types, _ = _torch_calls().read_grads(grads, apart)
-    lib, n = _lib_loaded(), len(grads)
-    need = lib.sn_abi_grad_norm_ws(n, _address(sizes))
-    ws = torch.empty(2 + need // 4, dtype=torch.float32, device=grads[0].device)
-    to = ws.data_ptr()
-    rc = getattr(lib, "sn_abi_" + name)(n, _address(at), _address(sizes), _address(types), max_norm, to, to + 4,
-                                        to + 8, need, current_stream(ws))
-    if rc:
-        check(rc, name)
-    return ws, grads
-
-
 def grad_norm(grads, max_norm=float("inf")):
     """(norm, factor) of a list of gradients (float32, bfloat16 and float16 mixed
     at will, on one GPU), each one float32 value on the GPU: the square root of
     the sum of all squares, and min(1, max_norm / (norm + 1e-6)), which
     ``adamw_step`` takes as grad_scale. Squares are added in fp32 over a few values
     and in fp64 above; the same bits every time."""
-    ws, _ = _norm_call("grad_norm", grads, max_norm, False)
-    return ws[0], ws[1]
+    if not isinstance(grads, (list, tuple)):
+        grads = list(grads)
+    return (_TORCH_CALLS or _torch_calls()).grad_norm(grads, max_norm, False)
 
 
 def clip_grads(grads, max_norm):
     """The norm of a list of gradients, all of which are scaled in place to a norm
     of max_norm where theirs is larger. (With ``adamw_step`` as the next step,
     ``grad_norm`` and its factor spare the pass that writes them.)"""
-    import torch
-    ws, grads = _norm_call("clip_grads", grads, max_norm, True)
-    torch.autograd.graph.increment_version(grads)
-    return ws[0]
+    if not isinstance(grads, (list, tuple)):
+        grads = list(grads)
+    return (_TORCH_CALLS or _torch_calls()).grad_norm(grads, max_norm, True)
 
 
 def linear_attention(q, k, v, log_decay, state=None, lengths=None, scale=None):

@@ -108,7 +108,7 @@ def near(got, want, most, dtype, rough):
 SIZES = [(1, 1, 1, 1, 1, 1), (2, 3, 2, 1, 5, 7), (1, 64, 2, 2, 64, 64), (2, 65, 3, 3, 64, 48), (1, 63, 1, 1, 33, 17),
          (2, 130, 4, 2, 64, 64), (1, 31, 2, 1, 128, 128), (2, 97, 3, 1, 72, 127), (1, 200, 2, 1, 16, 100),
          (1, 700, 3, 3, 64, 32), (2, 1100, 2, 1, 40, 72), (1, 1000, 2, 2, 128, 128), (1, 515, 1, 1, 9, 3),
-         (5, 70, 100, 50, 8, 8)]
+         (5, 70, 100, 50, 8, 8), (2, 150, 2, 1, 100, 30), (1, 300, 160, 160, 128, 64), (1, 300, 2, 2, 64, 128)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
