@@ -169,12 +169,13 @@ __device__ __forceinline__ void scale_rows(float (*x)[4], float r0, float r1) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) x[n][0] *= r0, x[n][1] *= r0, x[n][2] *= r1, x[n][3] *= r1;
 }
-// A strip of scores from block jb on, by its columns' factors.
-template <int NB>
-__device__ __forceinline__ void scale_columns(float (*p)[4], const float* column, int jb) {
+// A strip of scores from block jb on, by its columns' factors: column(s) is the
+// address of those of s and s + 1.
+template <int NB, typename F>
+__device__ __forceinline__ void scale_columns(float (*p)[4], F&& column, int jb) {
 #pragma unroll
     for (int n = 0; n < 2 * NB; ++n) {
-        const float2 f = *reinterpret_cast<const float2*>(column + jb * 16 + n * 8 + (lane_id() & 3) * 2);
+        const float2 f = *reinterpret_cast<const float2*>(column(jb * 16 + n * 8 + (lane_id() & 3) * 2));
         p[n][0] *= f.x, p[n][1] *= f.y, p[n][2] *= f.x, p[n][3] *= f.y;
     }
 }
@@ -606,11 +607,13 @@ out_kernel(const Job j, const bf16* kept, const Decays<S_::C>* decs, void* out_)
 
     // Between the blocks of 16 tokens a decay is 2^(c_t - c_r) 2^(c_r - c_s), r the
     // last token before the row's block: a factor of the row, which the state's
-    // part shares, and one of the column, which the warp writes down once. Both are
-    // at most 1. Within a block each pair has its own.
-    __shared__ float column_[S_::NW][C];
-    float* const column = column_[warp];
-    for (int s = l; s < rb * 16; s += 32) column[s] = dec.between(rb * 16 - 1, s);
+    // part shares, and one of the column, which the warp writes down once (behind the
+    // rows of the queries and keys of its block, four to a row). Both are at most 1.
+    // Within a block each pair has its own.
+    const auto column = [&](int s) {
+        return reinterpret_cast<float*>((s < 64 ? sq : sk) + (rb * 16 + s % 64 / 4) * LK + KD) + s % 4;
+    };
+    for (int s = l; s < rb * 16; s += 32) *column(s) = dec.between(rb * 16 - 1, s);
     __syncwarp();
     float O[NT][4];
     const int t = rb * 16 + (l >> 2);
@@ -908,7 +911,7 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
         for (int jb = 0; jb < rb; jb += NB) {
             float Q[2 * NB][4];
             scores<NP, VD, NB>(Q, to, rb * 16, tv, jb, 0, rb);
-            scale_columns<NB>(Q, column, jb);
+            scale_columns<NB>(Q, [&](int s) { return column + s; }, jb);
             weighted<NP, NP, NB, NK>(X, Q, tk, ck, jb, 0, rb);
         }
         scale_rows<NK>(X, r0, r1);
@@ -1109,7 +1112,7 @@ int forward_as(Job j, const float* first, void* out, float* state_out, char* ws,
     if (!j.chunks) return SN_OK;
     constexpr int bytes = Sizes<S_>::out;
     static_assert(bytes <= 220 * 1024, "shared memory of a CTA");
-    auto* kernel = out_kernel<S_, bytes <= 66 * 1024 ? 3 : bytes <= 96 * 1024 ? 2 : 1>;
+    auto* kernel = out_kernel<S_, bytes <= 72 * 1024 ? 3 : bytes <= 96 * 1024 ? 2 : 1>;
     SN_TRY(allow(kernel, bytes, "linear_attention"));
     kernel<<<(unsigned)((long long)j.B * j.H * j.chunks), S_::THREADS, bytes, st>>>(j, p.kept, dec, out);
     return cuda_check(cudaGetLastError(), "linear_attention launch");
