@@ -22,15 +22,15 @@
 // q.dq - k.dk from the sequence's end loses all digits over long sequences.)
 //
 // All products are m16n8k16 matrix instructions on bf16 with fp32 sums. bf16
-// values are taken as they are; float16 and float32 ones, and what is computed
-// on the way to an fp32 result (the states, dg), as the sum of two bf16 (2^-17
-// of a value), three products for one. What goes to a 16-bit output alone is
-// rounded to one. The state stays in registers from chunk to chunk, a warp
-// holding 16 rows of it. tcgen05 was not taken: with heads of 64 its products
-// here have 64 columns, and an instruction of 128 x 64 x 16 takes as long as one
-// of 128 x 128 x 16 (90 cycles); the 24 that a chunk of 128 tokens needs would
-// fill three quarters of the time that HBM leaves it, while the decays need the
-// scores in registers and the state rounded anew for each chunk.
+// values are taken as they are, float16 ones as the sum of two bf16 and float32
+// ones of three, which loses nothing; the products of their parts are left out
+// that a result does not hold. What is computed on the way to an fp32 result (the
+// states, dg) is taken apart in three as well, and so keeps fp32's accuracy; what
+// goes to 16-bit outputs alone is rounded to one part (bf16) or two (float16). tcgen05 was
+// not taken: with heads of 64 its products here have 64 columns, and an instruction
+// of 128 x 64 x 16 takes as long as one of 128 x 128 x 16 (90 cycles); the 24 that
+// a chunk of 128 tokens needs would fill three quarters of the time that HBM leaves
+// it, while the decays need the scores in registers and the states anew for each chunk.
 #include <algorithm>
 #include <cmath>
 

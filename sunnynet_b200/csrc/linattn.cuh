@@ -17,10 +17,10 @@ namespace la {
 
 typedef __nv_bfloat16 bf16;
 
-// Planes a type's values take: bf16 is one itself; float16 (exactly) and
-// float32 (to 2^-17 of the value) are the sum of two.
+// Planes a type's values take: bf16 is one itself, float16 the sum of two, float32
+// of three; nothing is lost.
 template <typename T>
-constexpr int planes_of = std::is_same<T, bf16>::value ? 1 : 2;
+constexpr int planes_of = std::is_same<T, bf16>::value ? 1 : std::is_same<T, float>::value ? 3 : 2;
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(bf16 x) { return __bfloat162float(x); }
@@ -68,32 +68,33 @@ __device__ __forceinline__ void mma(float* c, const uint32_t* a, const uint32_t*
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
-// a * b + c of two bf16 each, rounded once.
-__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
-    uint32_t r;
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-    return r;
-}
-__device__ __forceinline__ uint32_t neg2(uint32_t a) {
-    uint32_t r;
-    asm("neg.bf16x2 %0, %1;" : "=r"(r) : "r"(a));
-    return r;
-}
 __device__ __forceinline__ void stsm4(uint32_t at, const uint32_t* r) {
     asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3])
                  : "memory");
 }
 
+// P planes of a pair of values, the first in the low halves.
+template <int P>
+__device__ __forceinline__ void split2(float u, float v, uint32_t (*to)[4], int r) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        to[p][r] = pack2(u, v);
+        if (p + 1 < P) u -= low(to[p][r]), v -= high(to[p][r]);
+    }
+}
+
 // The product of A (PA planes) and B (PB planes) into two neighbouring column
-// tiles of eight: all pairs of planes but the two low ones.
-template <int PA, int PB>
+// tiles of eight. Planes i and j are 2^-8(i + j) of the whole: those products are
+// left out that fp32 (three planes on either side), or a 16-bit result, does not
+// hold.
+template <int PA, int PB, int LIM = (PA > PB ? PA : PB)>
 __device__ __forceinline__ void mma2(float (*c)[4], const uint32_t (*a)[4], const uint32_t (*b)[4]) {
 #pragma unroll
-    for (int i = 0; i < PA; ++i)
+    for (int i = PA - 1; i >= 0; --i)  // the small ones first
 #pragma unroll
-        for (int j = 0; j < PB; ++j)
-            if (i + j < 2) {
+        for (int j = PB - 1; j >= 0; --j)
+            if (i + j < LIM) {
                 mma(c[0], a[i], b[j]);
                 mma(c[1], a[i], b[j] + 2);
             }
@@ -189,19 +190,24 @@ struct Fetch {
                         const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&raw[n].y));
                         x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
                     }
-                    const uint2 hi = {pack2(x[0], x[1]), pack2(x[2], x[3])};
-                    const uint2 lo = {rest2(x[0], x[1], hi.x), rest2(x[2], x[3], hi.y)};
-                    *reinterpret_cast<uint2*>(to) = hi;
-                    *reinterpret_cast<uint2*>(to + PLANE) = lo;
+#pragma unroll
+                    for (int p = 0; p < planes_of<T>; ++p) {
+                        const uint2 part = {pack2(x[0], x[1]), pack2(x[2], x[3])};
+                        *reinterpret_cast<uint2*>(to + p * PLANE) = part;
+                        x[0] -= low(part.x), x[1] -= high(part.x), x[2] -= low(part.y), x[3] -= high(part.y);
+                    }
                 }
             } else {
                 for (int i = threadIdx.x; i < C * D; i += THREADS) {
                     const int row = i / D, col = i % D;
                     const bool in = t0 + row < end && col < d;
-                    const float x = in ? to_f(src[(long long)(t0 + row) * stride + col]) : 0.0f;
-                    const bf16 hi = __float2bfloat16_rn(x);
-                    dst[row * LD + col] = hi;
-                    dst[PLANE + row * LD + col] = __float2bfloat16_rn(x - __bfloat162float(hi));
+                    float x = in ? to_f(src[(long long)(t0 + row) * stride + col]) : 0.0f;
+#pragma unroll
+                    for (int p = 0; p < planes_of<T>; ++p) {
+                        const bf16 part = __float2bfloat16_rn(x);
+                        dst[p * PLANE + row * LD + col] = part;
+                        x -= __bfloat162float(part);
+                    }
                 }
             }
         }
@@ -234,22 +240,13 @@ __device__ __forceinline__ float Decays<C>::between(int t, int s) const {
     return exp2_of(near[t] - near[s] + (far[t] - far[s]));
 }
 
-// What a chunk's tokens weigh in its state, each as the sum of two bf16: pairs of
-// tokens, the high parts in x, the low ones in y.
-template <int C>
-struct alignas(16) Weights {
-    uint2 pair[C / 2];
-};
-
 // By one whole warp, from a lane's C / 32 log decays (zeros behind the end), in
 // the tokens' order. The sums are whole numbers of 2^-40: no rounding, and half
 // the latency of fp64. A log decay beyond 256 (in powers of two) either way leaves
 // nothing, or no finite number, in 32 bits: it is taken as 256, infinities too. A
 // NaN makes every sum from its token on one.
-// The weights are to_end, or (back) scale * from_start.
 template <int C>
-__device__ __forceinline__ void decays(Decays<C>* to, Weights<C>* weights, const float* g, bool back,
-                                       float scale) {
+__device__ __forceinline__ void decays(Decays<C>* to, const float* g) {
     constexpr int N = C / 32;
     constexpr float kLog2e = 1.44269504088896340736f, kRest = 1.92596299e-8f;  // their sum is log2(e) to 2^-50
     const int l = lane_id();
@@ -273,7 +270,6 @@ __device__ __forceinline__ void decays(Decays<C>* to, Weights<C>* weights, const
     const long long all = __shfl_sync(0xffffffffu, before, 31);
     before -= sum;
     const float nan = __int_as_float(0x7fffffff);
-    float w[N];
     const auto value = [](long long x) {  // (the high part is exact)
         const int whole = (int)(x >> 36);
         return make_float2((float)whole * 0.0625f, (float)(x - ((long long)whole << 36)) * 0x1p-40f);
@@ -284,17 +280,8 @@ __device__ __forceinline__ void decays(Decays<C>* to, Weights<C>* weights, const
         const float2 x = value(before + c[i]), y = value(all - before - c[i]);
         to->near[l * N + i] = poor ? nan : x.x;
         to->far[l * N + i] = x.y;
-        const float from_start = poor ? nan : exp2_of(x.x + x.y), to_end = wrong ? nan : exp2_of(y.x + y.y);
-        to->from_start[l * N + i] = from_start;
-        to->to_end[l * N + i] = to_end;
-        w[i] = back ? from_start * scale : to_end;
-    }
-    if constexpr (N > 1) {
-#pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const uint32_t hi = pack2(w[i], w[i + 1]);
-            weights->pair[(l * N + i) / 2] = make_uint2(hi, rest2(w[i], w[i + 1], hi));
-        }
+        to->from_start[l * N + i] = poor ? nan : exp2_of(x.x + x.y);
+        to->to_end[l * N + i] = wrong ? nan : exp2_of(y.x + y.y);
     }
     if (l == 0) {
         const float2 x = value(all);

@@ -20,38 +20,36 @@ __device__ __forceinline__ const T* head_of(const void* x, const Strides& s, int
     return static_cast<const T*>(x) + b * s.b + h * s.h;
 }
 
-// S += sum over the tokens of w_t x_t y_t^T: 16 rows (values `row` on of x), NT
-// column tiles (values `cb` on of y). x w is taken apart as it is formed: the
-// product of the high parts rounded, what that leaves (which bf16 holds exactly),
-// and the products with the low parts: 2^-16 of a value, in three or four
-// instructions for two.
+// S += sum over the tokens of scale w_t x_t y_t^T: 16 rows (values `row` on of x),
+// NT column tiles (values `cb` on of y). x w in fp32, in three planes: what comes of
+// it is an fp32 result. (The planes of a bf16 x formed by packed bf16 instructions,
+// four in place of three, are a third of the work, but the fourth product of each made
+// the whole 8% slower.)
 template <int NP, int NT, int C>
-__device__ __forceinline__ void add_outer(float (*S)[4], const Tile& x, const Tile& y, const uint2* w, int row,
-                                          int cb) {
+__device__ __forceinline__ void add_outer(float (*S)[4], const Tile& x, const Tile& y, const float* w,
+                                          float scale, int row, int cb) {
     const int q = lane_id() & 3;
-    uint32_t all[C / 16][NP][4];  // all asked for at once
-#pragma unroll
-    for (int kt = 0; kt < C / 16; ++kt)
-#pragma unroll
-        for (int p = 0; p < NP; ++p) x.a_t(all[kt][p], kt * 16, row, p);
 #pragma unroll
     for (int kt = 0; kt < C / 16; ++kt) {
-        const uint32_t(*xr)[4] = all[kt];
-        uint32_t a[2][4];
-        const uint2 f[2] = {w[kt * 8 + q], w[kt * 8 + 4 + q]};
+        uint32_t xr[NP][4], a[3][4];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) x.a_t(xr[p], kt * 16, row, p);
+        float2 f[2];
+        f[0] = *reinterpret_cast<const float2*>(w + kt * 16 + 2 * q);
+        f[1] = *reinterpret_cast<const float2*>(w + kt * 16 + 2 * q + 8);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            a[0][r] = fma2(xr[0][r], f[r / 2].x, 0x80008000u);
-            a[1][r] = fma2(xr[0][r], f[r / 2].x, neg2(a[0][r]));
-            a[1][r] = fma2(xr[0][r], f[r / 2].y, a[1][r]);
-            if constexpr (NP == 2) a[1][r] = fma2(xr[1][r], f[r / 2].x, a[1][r]);
+            float u = low(xr[NP - 1][r]), v = high(xr[NP - 1][r]);
+#pragma unroll
+            for (int p = NP - 2; p >= 0; --p) u += low(xr[p][r]), v += high(xr[p][r]);
+            split2<3>(u * (f[r / 2].x * scale), v * (f[r / 2].y * scale), a, r);
         }
 #pragma unroll
         for (int n = 0; n < NT / 2; ++n) {
             uint32_t b[NP][4];
 #pragma unroll
             for (int p = 0; p < NP; ++p) y.b_t(b[p], kt * 16, cb + n * 16, p);
-            mma2<2, NP>(S + 2 * n, a, b);
+            mma2<3, NP>(S + 2 * n, a, b);
         }
     }
 }
@@ -82,7 +80,7 @@ __device__ __forceinline__ void product(float (*out)[4], const Tile& A, int ra, 
 
 // Scores of 16 tokens of A with a strip of NB blocks of 16 tokens of B from
 // block `jb` on, of which [j0, j1) are wanted.
-template <int NP, int D, int NB>
+template <int NP, int D, int NB, int LIM = NP>
 __device__ __forceinline__ void scores(float (*p)[4], const Tile& A, int ra, const Tile& B, int jb, int j0,
                                        int j1) {
 #pragma unroll
@@ -100,7 +98,7 @@ __device__ __forceinline__ void scores(float (*p)[4], const Tile& A, int ra, con
                 uint32_t b[NP][4];
 #pragma unroll
                 for (int i = 0; i < NP; ++i) B.b(b[i], (jb + j) * 16, kt * 16, i);
-                mma2<NP, NP>(p + 2 * j, a, b);
+                mma2<NP, NP, LIM>(p + 2 * j, a, b);
             }
     }
 }
@@ -116,9 +114,7 @@ __device__ __forceinline__ void weighted(float (*out)[4], const float (*p)[4], c
             uint32_t a[PP][4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float u = p[2 * j + r / 2][r % 2 * 2], v = p[2 * j + r / 2][r % 2 * 2 + 1];
-                a[0][r] = pack2(u, v);
-                if constexpr (PP == 2) a[1][r] = rest2(u, v, a[0][r]);
+                split2<PP>(p[2 * j + r / 2][r % 2 * 2], p[2 * j + r / 2][r % 2 * 2 + 1], a, r);
             }
 #pragma unroll
             for (int n = 0; n < NT / 2; ++n) {
@@ -147,8 +143,9 @@ __device__ __forceinline__ void weighted_apart(float (*out)[4], const float (*p)
         for (int n = 0; n < NT; ++n) {
             const uint32_t w = *reinterpret_cast<const uint32_t*>(y + n * 8);
             float a = low(w), b = high(w);
-            if constexpr (NP == 2) {
-                const uint32_t w2 = *reinterpret_cast<const uint32_t*>(y + step + n * 8);
+#pragma unroll
+            for (int p = 1; p < NP; ++p) {
+                const uint32_t w2 = *reinterpret_cast<const uint32_t*>(y + p * step + n * 8);
                 a += low(w2), b += high(w2);
             }
             if (s <= (l >> 2)) out[n][0] += p0 * a, out[n][1] += p0 * b;
@@ -192,26 +189,26 @@ __device__ __forceinline__ void near_decays(float (*p)[4], const Decays<C>& d, i
         }
 }
 
-// 16 rows and NT column tiles of a state in fp32 (dk, dv), from and to registers.
+// 16 rows of a state in fp32 (dk, dv), in NT column tiles, from and to registers.
 template <int NT>
-__device__ __forceinline__ void load_state(float (*S)[4], const float* from, int row, int cb, int dk, int dv) {
+__device__ __forceinline__ void load_state(float (*S)[4], const float* from, int row, int dk, int dv) {
     const int l = lane_id();
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int r = row + (l >> 2) + (i >> 1) * 8, c = cb + n * 8 + (l & 3) * 2 + (i & 1);
+            const int r = row + (l >> 2) + (i >> 1) * 8, c = n * 8 + (l & 3) * 2 + (i & 1);
             S[n][i] = from && r < dk && c < dv ? from[r * dv + c] : 0.0f;
         }
 }
 template <int NT>
-__device__ __forceinline__ void store_state(const float (*S)[4], float* to, int row, int cb, int dk, int dv) {
+__device__ __forceinline__ void store_state(const float (*S)[4], float* to, int row, int dk, int dv) {
     const int l = lane_id();
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int r = row + (l >> 2) + (i >> 1) * 8, c = cb + n * 8 + (l & 3) * 2 + (i & 1);
+            const int r = row + (l >> 2) + (i >> 1) * 8, c = n * 8 + (l & 3) * 2 + (i & 1);
             if (r < dk && c < dv) to[r * dv + c] = S[n][i];
         }
 }
@@ -219,8 +216,8 @@ __device__ __forceinline__ void store_state(const float (*S)[4], float* to, int 
 // The same as PN bf16 planes with rows of D values and `plane` values each, by way of 16 rows of shared memory of the
 // warp's own, in packs of 16 bytes.
 template <int PN, int D, int NT>
-__device__ __forceinline__ void state_planes(const float (*S)[4], bf16* to, int plane, int row, int cb, bf16* by) {
-    constexpr int LD = NT * 8 + 8, ROWS = 32 / NT;
+__device__ __forceinline__ void state_planes(const float (*S)[4], bf16* to, int plane, int row, bf16* by) {
+    constexpr int LD = NT * 8 + 8, ROWS = 32 / NT;  // NT lanes to a row
     const int l = lane_id();
     const uint32_t at = smem_u32(by + (l & 15) * LD + (l >> 4) * 8);
 #pragma unroll
@@ -230,16 +227,19 @@ __device__ __forceinline__ void state_planes(const float (*S)[4], bf16* to, int 
             uint32_t r[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float u = S[n + i / 2][i % 2 * 2], v = S[n + i / 2][i % 2 * 2 + 1];
+                float u = S[n + i / 2][i % 2 * 2], v = S[n + i / 2][i % 2 * 2 + 1];
                 r[i] = pack2(u, v);
-                if (p) r[i] = rest2(u, v, r[i]);
+                for (int q = 0; q < p; ++q) {
+                    u -= low(r[i]), v -= high(r[i]);
+                    r[i] = pack2(u, v);
+                }
             }
             stsm4(at + n * 16, r);
         }
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < 16; i += ROWS)
-            *reinterpret_cast<uint4*>(to + p * plane + (row + l / NT + i) * D + cb + l % NT * 8) =
+            *reinterpret_cast<uint4*>(to + p * plane + (row + l / NT + i) * D + l % NT * 8) =
                 *reinterpret_cast<const uint4*>(by + (l / NT + i) * LD + l % NT * 8);
         __syncwarp();
     }
@@ -339,9 +339,10 @@ struct Shape {
     static constexpr int KT = NP * C * LK, VT = NP * C * LV, STATE = KD * LV;
     static constexpr int RB = C / 16, CG = NW / RB, NK = KD / CG / 8, NV = VD / CG / 8;
     static_assert(NW % RB == 0 && NK % 2 == 0 && NV % 2 == 0, "whole blocks for the warps");
-    // a states' pass: stages of SUB tokens; eight warps of 16 rows and, of keys up to 64, half of the columns
+    // a states' pass: stages of SUB tokens, a warp for every 16 rows (with half of the columns to a warp, the
+    // rows' planes were formed twice: a fifth slower)
     static constexpr int SUB = C < 64 ? C : 64, KS = NP * SUB * LK, VS = NP * SUB * LV;
-    static constexpr int SR = KD / 16, SW = 8, ST = SW * 32, SNT = VD * SR / SW / 8;
+    static constexpr int SW = KD / 16, ST = SW * 32, SNT = VD / 8;
 };
 
 __device__ __forceinline__ Tile tile(const bf16* p, int ld, int step) {
@@ -370,12 +371,14 @@ __global__ void __launch_bounds__(S_::ST + 32, KEEP && S_::SNT > 8 ? 1 : 2)
 state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) {
     typedef typename S_::T T;
     constexpr int NP = S_::NP, KD = S_::KD, VD = S_::VD, C = S_::C, NT = S_::SNT, SUB = S_::SUB, PER = C / SUB;
-    constexpr int STAGES = NP == 2 ? 2 : KEEP ? 3 : PER + 1;  // (a single chunk is asked for at once)
+    // (a single chunk is asked for at once; three planes leave room for one stage, which
+    // is filled when every warp is done with it)
+    constexpr int STAGES = NP == 3 ? 1 : NP == 2 ? 2 : KEEP ? 3 : PER + 1;
+    constexpr int AHEAD = NP == 1 ? STAGES - 1 : 1;  // stages on their way
     constexpr int STAGE = S_::KS + S_::VS;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16* const tiles = reinterpret_cast<bf16*>(smem);
     __shared__ Decays<C> dec_[2];
-    __shared__ Weights<C> weights_[2];
     __shared__ __align__(16) bf16 by_[KEEP ? S_::SW : 1][KEEP ? 16 * (NT * 8 + 8) : 8];
     const Pass& p = blockIdx.y ? p1 : p0;
     const long long bh = KEEP ? blockIdx.x : blockIdx.x / j.chunks;
@@ -388,8 +391,8 @@ state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) 
     if (warp == S_::SW) {  // the decays
         constexpr int M = C / 32;
         const float* g = j.g + b * j.gs.b + h * j.gs.h;
-        constexpr int AHEAD = 4;  // chunks whose log decays are on their way
-        float x[AHEAD][M];
+        constexpr int FAR = 4;  // chunks whose log decays are on their way
+        float x[FAR][M];
         const auto ask = [&](float* to, int i) {
 #pragma unroll
             for (int k = 0; k < M; ++k) {
@@ -398,8 +401,8 @@ state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) 
             }
         };
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) ask(x[i], i);
-        if (n) decays<C>(&dec_[0], &weights_[0], x[0], p.back, j.scale);
+        for (int i = 0; i < FAR; ++i) ask(x[i], i);
+        if (n) decays<C>(&dec_[0], x[0]);
         for (int i = 0; i < n; ++i) {
             __syncthreads();  // (what is written behind it was read a chunk ago)
             if (!blockIdx.y) {
@@ -408,18 +411,18 @@ state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) 
                 for (int k = l; k < (int)sizeof(Decays<C>) / 16; k += 32) to[k] = from[k];
             }
 #pragma unroll
-            for (int a = 0; a + 1 < AHEAD; ++a)
+            for (int a = 0; a + 1 < FAR; ++a)
 #pragma unroll
                 for (int k = 0; k < M; ++k) x[a][k] = x[a + 1][k];
-            ask(x[AHEAD - 1], i + AHEAD);
-            if (i + 1 < n) decays<C>(&dec_[(i + 1) & 1], &weights_[(i + 1) & 1], x[0], p.back, j.scale);
+            ask(x[FAR - 1], i + FAR);
+            if (i + 1 < n) decays<C>(&dec_[(i + 1) & 1], x[0]);
 #pragma unroll
-            for (int k = 1; k < PER; ++k) __syncthreads();
+            for (int k = 1; k < PER * (STAGES == 1 ? 2 : 1); ++k) __syncthreads();
         }
         return;
     }
 
-    const int row = warp % S_::SR * 16, cb = warp / S_::SR * NT * 8;
+    const int row = warp * 16;
     const T* x = head_of<T>(p.x, p.xs, b, h / j.share);
     const T* y = head_of<T>(p.y, p.ys, b, h);
     const bool wx = j.whole >> (p.back ? 0 : 1) & 1, wy = j.whole >> (p.back ? 3 : 2) & 1;
@@ -443,34 +446,39 @@ state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) 
             ly.put(to + S_::KS, y, p.ys.t, first(u), end, j.dv, wy);
         }
     };
-    for (int u = 0; u < STAGES - 1; ++u) fetch(u, u);
+    for (int u = 0; u < AHEAD; ++u) fetch(u, u % STAGES);
     put(0, 0);
     float S[NT][4];
-    load_state<NT>(S, KEEP && p.start ? p.start + bh * j.dk * j.dv : nullptr, row, cb, j.dk, j.dv);
+    if constexpr (KEEP)
+        load_state<NT>(S, p.start ? p.start + bh * j.dk * j.dv : nullptr, row, j.dk, j.dv);
+    else
+        clear<NT>(S);
     int stage = 0;
     for (int i = 0; i < n; ++i) {
         const Decays<C>& dec = dec_[i & 1];
+        float sum[NT][4];
+        clear<NT>(sum);
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
             const int u = i * PER + k;
-            cp_async_wait_group<STAGES - 2>();
+            cp_async_wait_group<AHEAD - 1>();
             __syncthreads();
-            fetch(u + STAGES - 1, (stage + STAGES - 1) % STAGES);
-            if (k == 0) {
-                if constexpr (KEEP)
-                    state_planes<PN, VD, NT>(S, p.kept + (bh * j.chunks + chunk(i)) * PN * KD * VD, KD * VD, row, cb,
-                                             by_[warp]);
-                if constexpr (KEEP) {
-                    const float w = dec.whole;
-#pragma unroll
-                    for (int m = 0; m < NT; ++m)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) S[m][e] *= w;
-                }
-            }
+            fetch(u + AHEAD, (stage + AHEAD) % STAGES);
+            if (KEEP && k == 0)
+                state_planes<PN, VD, NT>(S, p.kept + (bh * j.chunks + chunk(i)) * PN * KD * VD, KD * VD, row, by_[warp]);
             const bf16* from = tiles + stage * STAGE;
-            add_outer<NP, NT, SUB>(S, tile(from, S_::LK, SUB * S_::LK), tile(from + S_::KS, S_::LV, SUB * S_::LV),
-                                   weights_[i & 1].pair + k * SUB / 2, row, cb);
+            add_outer<NP, NT, SUB>(sum, tile(from, S_::LK, SUB * S_::LK), tile(from + S_::KS, S_::LV, SUB * S_::LV),
+                                   (p.back ? dec.from_start : dec.to_end) + k * SUB, p.back ? j.scale : 1.0f, row, 0);
+            // The chunk's sum is added here, not in the matrix instruction, which cuts its sums off: over a
+            // sequence that leaned by 2^-24 of the state a step.
+            if (k + 1 == PER) {
+                const float f = dec.whole;
+#pragma unroll
+                for (int m = 0; m < NT; ++m)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) S[m][e] = fmaf(S[m][e], f, sum[m][e]);
+            }
+            if constexpr (STAGES == 1) __syncthreads();
             stage = (stage + 1) % STAGES;
             put(u + 1, stage);
         }
@@ -482,11 +490,11 @@ state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) 
         for (int m = 0; m < NT; ++m)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                *reinterpret_cast<float2*>(to + (row + (l >> 2) + i * 8) * VD + cb + m * 8 + (l & 3) * 2) =
+                *reinterpret_cast<float2*>(to + (row + (l >> 2) + i * 8) * VD + m * 8 + (l & 3) * 2) =
                     make_float2(S[m][2 * i], S[m][2 * i + 1]);
         if (threadIdx.x == 0) p.factor[bh * j.chunks + c0] = dec_[0].whole;
     } else if (p.end) {
-        store_state<NT>(S, p.end + bh * j.dk * j.dv, row, cb, j.dk, j.dv);
+        store_state<NT>(S, p.end + bh * j.dk * j.dv, row, j.dk, j.dv);
     }
 }
 
@@ -521,11 +529,13 @@ __global__ void __launch_bounds__(256) scan_kernel(const Job j, const Pass p0, c
         for (int u = 0; u < U; ++u)
             if (k0 + u < live) {
                 const int k = p.back ? live - 1 - k0 - u : k0 + u;
-                const uint2 hi = {pack2(S[0], S[1]), pack2(S[2], S[3])};
-                *reinterpret_cast<uint2*>(kept + (long long)k * PN * SIZE) = hi;
-                if constexpr (PN == 2)
-                    *reinterpret_cast<uint2*>(kept + (long long)k * PN * SIZE + SIZE) =
-                        make_uint2(rest2(S[0], S[1], hi.x), rest2(S[2], S[3], hi.y));
+                float part[4] = {S[0], S[1], S[2], S[3]};
+#pragma unroll
+                for (int q = 0; q < PN; ++q) {
+                    const uint2 w = {pack2(part[0], part[1]), pack2(part[2], part[3])};
+                    *reinterpret_cast<uint2*>(kept + ((long long)k * PN + q) * SIZE) = w;
+                    part[0] -= low(w.x), part[1] -= high(w.x), part[2] -= low(w.y), part[3] -= high(w.y);
+                }
                 S[0] = by[u] * S[0] + add[u].x, S[1] = by[u] * S[1] + add[u].y;
                 S[2] = by[u] * S[2] + add[u].z, S[3] = by[u] * S[3] + add[u].w;
             }
@@ -687,8 +697,9 @@ __device__ __forceinline__ void row_dots(const float (*x)[4], const bf16* tile, 
         for (int n = 0; n < NT; ++n) {
             const uint32_t w = *reinterpret_cast<const uint32_t*>(at + n * 8);
             float u = low(w), v = high(w);
-            if constexpr (NP == 2) {
-                const uint32_t w2 = *reinterpret_cast<const uint32_t*>(at + step + n * 8);
+#pragma unroll
+            for (int p = 1; p < NP; ++p) {
+                const uint32_t w2 = *reinterpret_cast<const uint32_t*>(at + p * step + n * 8);
                 u += low(w2), v += high(w2);
             }
             s = fmaf(x[n][2 * i], u, s);
@@ -737,7 +748,6 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
     bf16 *const sk = sq + S_::KT, *const sv = sk + S_::KT, *const so = sv + S_::VT;
     bf16* const ss = so + S_::VT;  // the gradient behind the chunk, then the state before it
     __shared__ Decays<C> dec;
-    __shared__ float column_[S_::NW][C];
     // parts of dg: by row block, and by column group where the columns are split
     __shared__ float col_part[RB][C], row_part[C], dq_part[CG][C], dk_part[CG][C], dot_part[S_::NW];
     const Chunk at(j);
@@ -762,7 +772,7 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
     const int rb = warp % RB, cg = warp / RB, ck = cg * NK * 8, cv = cg * NV * 8;
     const Tile tq = tile(sq, LK, C * LK), tk = tile(sk, LK, C * LK), tv = tile(sv, LV, C * LV),
                to = tile(so, LV, C * LV), ts = tile(ss, LV, S_::STATE);
-    const long long kept = (at.bh * j.chunks + at.c) * 2 * KD * VD;
+    const long long kept = (at.bh * j.chunks + at.c) * 3 * KD * VD;
     {
         const T* q = head_of<T>(j.q, j.qs, at.b, at.h / j.share);
         const T* k = head_of<T>(j.k, j.ks, at.b, at.h / j.share);
@@ -771,7 +781,7 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
         Fetch<T, C, KD, S_::THREADS> lq, lk;
         Fetch<T, C, VD, S_::THREADS> lv, lo;
         lk.fetch(sk, k, j.ks.t, c0, end, j.dk, j.whole >> 1 & 1);
-        load_kept<S_, 2>(ss, G.behind + kept);
+        load_kept<S_, 3>(ss, G.behind + kept);
         load_decays<C>(&dec, decs + at.bh * j.chunks + at.c);
         lv.fetch(sv, v, j.vs.t, c0, end, j.dv, j.whole >> 2 & 1);
         cp_async_commit();
@@ -787,7 +797,7 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
     __syncthreads();
     // (by way of the states' place, a part of it for each warp)
     constexpr int BK = NK * 8 + 8, BV = NV * 8 + 8, BY = BK > BV ? BK : BV;
-    static_assert(S_::NW * 16 * BY <= 2 * S_::STATE, "room for every warp's rows");
+    static_assert(S_::NW * 16 * BY <= 3 * S_::STATE, "room for every warp's rows");
     bf16* const by = ss + warp * 16 * BY;
     const auto store_head = [&](const float(*x)[4], void* to16, float* to32) {
         if (to32)
@@ -795,34 +805,38 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
         else
             store_rows_by<T, NK, BK>(by, x, static_cast<T*>(to16) + k0, kt, c0 + rb * 16, ck, end, j.T, j.dk);
     };
-    float* const column = column_[warp];
+    // factors of columns, as in out_kernel
+    const auto column = [&](int s) {
+        return reinterpret_cast<float*>((s < 64 ? sq : sk) + (rb * 16 + s % 64 / 4) * LK + KD) + s % 4;
+    };
+    constexpr int FINE = NP == 2 ? 3 : NP;  // (the scores' products in full: dg is an fp32 result)
     float part[2];
     const int t = rb * 16 + (l >> 2);  // the lane's tokens: this and 8 behind
     {
         // rows s, columns u >= s. Between blocks a decay is 2^(c_u - c_r) 2^(c_r - c_s), r
         // the last token of the row's block
         const int r = rb * 16 + 15;
-        for (int u = r + 1 + l; u < C; u += 32) column[u] = dec.between(u, r) * j.scale;
-        const float b0 = dec.between(r, t), b1 = dec.between(r, t + 8), behind = dec.to_end[r];
+                const float b0 = dec.between(r, t), b1 = dec.between(r, t + 8), behind = dec.to_end[r];
         float V[NV][4], K[NK][4], across[2] = {0.0f, 0.0f};
         clear<NV>(V);
         product<NP, NP, KD, NV, true>(V, tk, rb * 16, ts, cv);
         scale_rows<NV>(V, behind, behind);
         clear<NK>(K);
-        product<NP, 2, VD, NK, false>(K, tv, rb * 16, ts, ck);
+        product<NP, 3, VD, NK, false>(K, tv, rb * 16, ts, ck);
         scale_rows<NK>(K, behind, behind);
         row_dots<NP, NK>(K, sk, LK, C * LK, rb * 16, ck, part);
         if ((l & 3) == 0) dk_part[cg][t] = part[0] * b0, dk_part[cg][t + 8] = part[1] * b1;
         cp_async_wait_all();  // queries and the gradient of the outputs
+        for (int u = r + 1 + l; u < C; u += 32) *column(u) = dec.between(u, r) * j.scale;
         __syncthreads();
         for (int jb = (rb + 1) / NB * NB; jb < RB; jb += NB) {
             float P[2 * NB][4], Q[2 * NB][4], down[4 * NB];
-            scores<NP, KD, NB>(P, tk, rb * 16, tq, jb, rb + 1, RB);
-            scores<NP, VD, NB>(Q, tv, rb * 16, to, jb, rb + 1, RB);
+            scores<NP, KD, NB, FINE>(P, tk, rb * 16, tq, jb, rb + 1, RB);
+            scores<NP, VD, NB, FINE>(Q, tv, rb * 16, to, jb, rb + 1, RB);
 #pragma unroll
             for (int n = 0; n < 2 * NB; ++n) {
                 const int u = jb * 16 + n * 8 + (l & 3) * 2;
-                const float2 f = *reinterpret_cast<const float2*>(column + u);
+                const float2 f = *reinterpret_cast<const float2*>(column(u));
                 const bool in = jb + n / 2 > rb;  // (the factors of other blocks are not there)
                 const float x0 = P[n][0] * Q[n][0], x1 = P[n][1] * Q[n][1], x2 = P[n][2] * Q[n][2],
                             x3 = P[n][3] * Q[n][3];
@@ -842,8 +856,8 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
         scale_rows<NK>(K, b0, b1);
         across[0] *= b0, across[1] *= b1;
         float P[2][4], Q[2][4], down[4] = {};
-        scores<NP, KD, 1>(P, tk, rb * 16, tq, rb, rb, rb + 1);
-        scores<NP, VD, 1>(Q, tv, rb * 16, to, rb, rb, rb + 1);
+        scores<NP, KD, 1, FINE>(P, tk, rb * 16, tq, rb, rb, rb + 1);
+        scores<NP, VD, 1, FINE>(Q, tv, rb * 16, to, rb, rb, rb + 1);
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -871,18 +885,22 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
         if (dg) {
             const uint4* from = reinterpret_cast<const uint4*>(G.before + kept);
             constexpr int PACKS = KD * VD / 8, ROW = VD / 8;
-#pragma unroll 4
+#pragma unroll 2
             for (int i = threadIdx.x; i < PACKS; i += S_::THREADS) {
-                const uint4 hi = from[i], lo = from[PACKS + i];
-                const uint4 r = *reinterpret_cast<const uint4*>(ss + i / ROW * LV + i % ROW * 8);
-                const uint4 r2 = *reinterpret_cast<const uint4*>(ss + S_::STATE + i / ROW * LV + i % ROW * 8);
-                const uint32_t a[4] = {r.x, r.y, r.z, r.w}, b[4] = {r2.x, r2.y, r2.z, r2.w};
-                const uint32_t x[4] = {hi.x, hi.y, hi.z, hi.w}, y[4] = {lo.x, lo.y, lo.z, lo.w};
+                uint4 x[3], r[3];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    dot = fmaf(low(a[e]) + low(b[e]), low(x[e]) + low(y[e]), dot);
-                    dot = fmaf(high(a[e]) + high(b[e]), high(x[e]) + high(y[e]), dot);
+                for (int p = 0; p < 3; ++p) {
+                    x[p] = from[p * PACKS + i];
+                    r[p] = *reinterpret_cast<const uint4*>(ss + p * S_::STATE + i / ROW * LV + i % ROW * 8);
                 }
+                const auto add = [&](uint32_t a0, uint32_t a1, uint32_t a2, uint32_t b0, uint32_t b1, uint32_t b2) {
+                    dot = fmaf(low(a0) + (low(a1) + low(a2)), low(b0) + (low(b1) + low(b2)), dot);
+                    dot = fmaf(high(a0) + (high(a1) + high(a2)), high(b0) + (high(b1) + high(b2)), dot);
+                };
+                add(x[0].x, x[1].x, x[2].x, r[0].x, r[1].x, r[2].x);
+                add(x[0].y, x[1].y, x[2].y, r[0].y, r[1].y, r[2].y);
+                add(x[0].z, x[1].z, x[2].z, r[0].z, r[1].z, r[2].z);
+                add(x[0].w, x[1].w, x[2].w, r[0].w, r[1].w, r[2].w);
             }
         }
 #pragma unroll
@@ -893,15 +911,15 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
         store_head(K, G.dk, G.dk32);
     }
     __syncthreads();
-    load_kept<S_, 2>(ss, G.before + kept);
+    load_kept<S_, 3>(ss, G.before + kept);
     cp_async_wait_all();
-    for (int s = l; s < rb * 16; s += 32) column[s] = dec.between(rb * 16 - 1, s);
+    for (int s = l; s < rb * 16; s += 32) *column(s) = dec.between(rb * 16 - 1, s);
     __syncthreads();
     {
         // rows u, columns s <= u, as the outputs
         float X[NK][4], P[2][4];
         clear<NK>(X);
-        product<NP, 2, VD, NK, false>(X, to, rb * 16, ts, ck);
+        product<NP, 3, VD, NK, false>(X, to, rb * 16, ts, ck);
         const float begin = rb ? dec.from_start[rb * 16 - 1] : 1.0f;
         scale_rows<NK>(X, begin, begin);
         const float r0 = (rb ? dec.between(t, rb * 16 - 1) : dec.from_start[t]) * j.scale;
@@ -911,7 +929,7 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
         for (int jb = 0; jb < rb; jb += NB) {
             float Q[2 * NB][4];
             scores<NP, VD, NB>(Q, to, rb * 16, tv, jb, 0, rb);
-            scale_columns<NB>(Q, [&](int s) { return column + s; }, jb);
+            scale_columns<NB>(Q, column, jb);
             weighted<NP, NP, NB, NK>(X, Q, tk, ck, jb, 0, rb);
         }
         scale_rows<NK>(X, r0, r1);
@@ -1006,9 +1024,10 @@ __global__ void __launch_bounds__(256) gate_kernel(const float* dg, const double
 // ------------------------------------------------------------------ launches
 template <class S_>
 struct Sizes {
-    static constexpr int state = (S_::NP == 1 ? 3 : 2) * (S_::KS + S_::VS) * 2, sum = S_::C / S_::SUB * (S_::KS + S_::VS) * 2;
+    static constexpr int state = (4 - S_::NP) * (S_::KS + S_::VS) * 2;
+    static constexpr int sum = (S_::NP == 1 ? S_::C / S_::SUB : 4 - S_::NP) * (S_::KS + S_::VS) * 2;
     static constexpr int out = (2 * S_::KT + S_::VT + S_::NP * S_::STATE) * 2;
-    static constexpr int grad = (2 * S_::KT + 2 * S_::VT + 2 * S_::STATE) * 2;
+    static constexpr int grad = (2 * S_::KT + 2 * S_::VT + 3 * S_::STATE) * 2;
 };
 
 template <typename K>
@@ -1048,9 +1067,9 @@ Space space_of(const Job& j, bool back, bool gates_alike) {
             (i ? s.back_factor : s.factor) = take(bh * j.chunks * 4);
         }
     s.decays = take(bh * j.chunks * sizeof(Decays<S_::C>));
-    s.kept = take(plane * (back ? 2 : S_::NP));
+    s.kept = take(plane * (back ? 3 : S_::NP));
     if (back) {
-        s.kept_back = take(plane * 2);
+        s.kept_back = take(plane * 3);
         if (j.share > 1) {
             s.dq32 = take(bh * j.T * j.dk * 4);
             s.dk32 = take(bh * j.T * j.dk * 4);
@@ -1139,7 +1158,7 @@ int backward_as(Job j, const float* first, const Wanted& g, char* ws, long long 
     r.end = g.dstate;
     r.back = true;
     auto* dec = reinterpret_cast<Decays<S_::C>*>(ws + s.decays);
-    SN_TRY((states<S_, 2>(j, p, r, true, dec, st)));
+    SN_TRY((states<S_, 3>(j, p, r, true, dec, st)));
     Grads G = {};
     G.dout = g.dout, G.ds = g.ds;
     G.before = p.kept, G.behind = r.kept;
@@ -1148,7 +1167,7 @@ int backward_as(Job j, const float* first, const Wanted& g, char* ws, long long 
     G.dg = !g.dg ? nullptr : g.gates_alike ? floats(s.dg) : g.dg;
     constexpr int bytes = Sizes<S_>::grad;
     static_assert(bytes <= 220 * 1024, "shared memory of a CTA");
-    auto* kernel = grad_kernel<S_, bytes <= 96 * 1024 ? 2 : 1>;
+    auto* kernel = grad_kernel<S_, bytes <= 102 * 1024 ? 2 : 1>;
     SN_TRY(allow(kernel, bytes, "linear_attention_bwd"));
     if (j.chunks)
         kernel<<<(unsigned)((long long)j.B * j.H * j.chunks), S_::THREADS, bytes, st>>>(j, G, dec);
@@ -1175,7 +1194,7 @@ template <typename T, typename F>
 int by_width(const Job& j, F&& f) {
     constexpr int LONG = planes_of<T> == 1 ? 128 : 64;
     if (j.dk <= 64) return j.dv <= 64 ? f(Shape<T, 64, 64, LONG>()) : f(Shape<T, 64, 128, 64>());
-    return j.dv <= 64 ? f(Shape<T, 128, 64, 64>()) : f(Shape<T, 128, 128, 64>());
+    return j.dv <= 64 ? f(Shape<T, 128, 64, 64>()) : f(Shape<T, 128, 128, planes_of<T> == 1 ? 64 : 32>());
 }
 
 }  // namespace
