@@ -100,6 +100,22 @@ __device__ __forceinline__ void mma2(float (*c)[4], const uint32_t (*a)[4], cons
             }
 }
 
+// The same with the products of the first parts in `c` and the others in `rest`,
+// which the caller adds to it: a matrix instruction cuts its sums off, and six of
+// them into one sum lean by as many times 2^-24.
+template <int PA, int PB, int LIM>
+__device__ __forceinline__ void mma2(float (*c)[4], float (*rest)[4], const uint32_t (*a)[4],
+                                     const uint32_t (*b)[4]) {
+#pragma unroll
+    for (int i = PA - 1; i >= 0; --i)
+#pragma unroll
+        for (int j = PB - 1; j >= 0; --j)
+            if (i + j < LIM) {
+                mma(i + j ? rest[0] : c[0], a[i], b[j]);
+                mma(i + j ? rest[1] : c[1], a[i], b[j] + 2);
+            }
+}
+
 // A tile in shared memory: rows of LD bf16 (8 more than their D values, so that
 // the eight rows that ldmatrix reads at once lie in different banks), its
 // planes `step` values apart. The four ways a 16 x 16 block of it is read, at

@@ -20,6 +20,14 @@ __device__ __forceinline__ const T* head_of(const void* x, const Strides& s, int
     return static_cast<const T*>(x) + b * s.b + h * s.h;
 }
 
+template <int NT>
+__device__ __forceinline__ void clear(float (*x)[4]) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[n][i] = 0.0f;
+}
+
 // S += sum over the tokens of scale w_t x_t y_t^T: 16 rows (values `row` on of x),
 // NT column tiles (values `cb` on of y). x w in fp32, in three planes: what comes of
 // it is an fp32 result. (The planes of a bf16 x formed by packed bf16 instructions,
@@ -54,10 +62,37 @@ __device__ __forceinline__ void add_outer(float (*S)[4], const Tile& x, const Ti
     }
 }
 
+// A second sum for the products of later parts, where fp32 results count on them:
+// add() puts it into the first.
+template <int NP, int NT>
+struct Rest {
+    static constexpr bool ON = NP == 3;
+    float x[ON ? NT : 1][4];
+    __device__ __forceinline__ Rest() {
+        if constexpr (ON) clear<NT>(x);
+    }
+    template <int PA, int PB, int LIM>
+    __device__ __forceinline__ void mma(float (*c)[4], int n, const uint32_t (*a)[4], const uint32_t (*b)[4]) {
+        if constexpr (ON)
+            mma2<PA, PB, LIM>(c + n, x + n, a, b);
+        else
+            mma2<PA, PB, LIM>(c + n, a, b);
+    }
+    __device__ __forceinline__ void add(float (*c)[4]) const {
+        if constexpr (ON) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) c[n][i] += x[n][i];
+        }
+    }
+};
+
 // out (16 rows from `ra` of A, columns from `cb` of B) += A B over D: A's rows
 // are tokens, B(k, n) = tile[n][k], or tile[k][n] where TRANS.
 template <int PA, int PB, int D, int NT, bool TRANS>
 __device__ __forceinline__ void product(float (*out)[4], const Tile& A, int ra, const Tile& B, int cb) {
+    Rest<PA, NT> rest;
 #pragma unroll
     for (int kt = 0; kt < D / 16; ++kt) {
         uint32_t a[PA][4];
@@ -73,9 +108,10 @@ __device__ __forceinline__ void product(float (*out)[4], const Tile& A, int ra, 
                 else
                     B.b(b[p], cb + n * 16, kt * 16, p);
             }
-            mma2<PA, PB>(out + 2 * n, a, b);
+            rest.template mma<PA, PB, (PA > PB ? PA : PB)>(out, 2 * n, a, b);
         }
     }
+    rest.add(out);
 }
 
 // Scores of 16 tokens of A with a strip of NB blocks of 16 tokens of B from
@@ -83,10 +119,8 @@ __device__ __forceinline__ void product(float (*out)[4], const Tile& A, int ra, 
 template <int NP, int D, int NB, int LIM = NP>
 __device__ __forceinline__ void scores(float (*p)[4], const Tile& A, int ra, const Tile& B, int jb, int j0,
                                        int j1) {
-#pragma unroll
-    for (int n = 0; n < 2 * NB; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[n][i] = 0.0f;
+    clear<2 * NB>(p);
+    Rest<NP, 2 * NB> rest;
 #pragma unroll
     for (int kt = 0; kt < D / 16; ++kt) {
         uint32_t a[NP][4];
@@ -98,9 +132,10 @@ __device__ __forceinline__ void scores(float (*p)[4], const Tile& A, int ra, con
                 uint32_t b[NP][4];
 #pragma unroll
                 for (int i = 0; i < NP; ++i) B.b(b[i], (jb + j) * 16, kt * 16, i);
-                mma2<NP, NP, LIM>(p + 2 * j, a, b);
+                rest.template mma<NP, NP, LIM>(p, 2 * j, a, b);
             }
     }
+    rest.add(p);
 }
 
 // out += P Y, P such scores as they lie in registers (PP planes of them), Y the
@@ -108,22 +143,23 @@ __device__ __forceinline__ void scores(float (*p)[4], const Tile& A, int ra, con
 template <int PP, int NP, int NB, int NT>
 __device__ __forceinline__ void weighted(float (*out)[4], const float (*p)[4], const Tile& Y, int cb, int jb,
                                          int j0, int j1) {
+    Rest<PP, NT> rest;
 #pragma unroll
     for (int j = 0; j < NB; ++j)
         if (jb + j >= j0 && jb + j < j1) {
             uint32_t a[PP][4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
+            for (int r = 0; r < 4; ++r)
                 split2<PP>(p[2 * j + r / 2][r % 2 * 2], p[2 * j + r / 2][r % 2 * 2 + 1], a, r);
-            }
 #pragma unroll
             for (int n = 0; n < NT / 2; ++n) {
                 uint32_t b[NP][4];
 #pragma unroll
                 for (int i = 0; i < NP; ++i) Y.b_t(b[i], (jb + j) * 16, cb + n * 16, i);
-                mma2<PP, NP>(out + 2 * n, a, b);
+                rest.template mma<PP, NP, (PP > NP ? PP : NP)>(out, 2 * n, a, b);
             }
         }
+    rest.add(out);
 }
 
 // The same for one block, whose tokens do not all see each other: a value of Y
@@ -154,13 +190,6 @@ __device__ __forceinline__ void weighted_apart(float (*out)[4], const float (*p)
     }
 }
 
-template <int NT>
-__device__ __forceinline__ void clear(float (*x)[4]) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[n][i] = 0.0f;
-}
 template <int NT>
 __device__ __forceinline__ void scale_rows(float (*x)[4], float r0, float r1) {
 #pragma unroll

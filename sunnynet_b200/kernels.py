@@ -11,10 +11,12 @@ reference's ``ScanAVX2``) takes u, p (B,T,N), s0 (B,N) and returns the states;
 on the GPU (then the kernels read them in place, on torch's current stream)
 or on the host (staged through device memory). There is no CPU fallback.
 
-Beside them stand the two other operators of a training step, which the
-reference leaves to torch: ``layer_norm`` (its CenteredScaleNorm with
-eps = s_min^2 + 1e-5) with its gradients, and ``adamw_step``, one AdamW update
-of all of a model's tensors with states in 32 or 8 bits
+Beside them stand the other operators of a training step, which the
+reference leaves to torch: ``embedding`` and ``layer_norm`` (its CenteredScaleNorm
+with eps = s_min^2 + 1e-5) with their gradients, ``linear_attention``, a matrix
+state with a decay for each head (``linear_attention_step`` for single tokens),
+``grad_norm`` and ``clip_grads`` over all gradients, and ``adamw_step``, one AdamW
+update of all of a model's tensors with states in 32 or 8 bits
 (``sunnynet_b200.optim.AdamW`` keeps the states). These only enqueue on
 torch's current stream of their tensors' device, so a training step of them
 can be captured into a CUDA graph.
@@ -367,9 +369,10 @@ def linear_attention(q, k, v, log_decay, state=None, lengths=None, scale=None):
     zeros. lengths (B,) int32: tokens from there on are not read, leave the
     state as it is, and their outputs are zeros. A log decay of minus infinity
     forgets what came before. scale: dk ** -0.5. Out has v's type, states are
-    float32. Differentiable once in q, k, v, log_decay and state. Sums and states
-    are fp32; products take 16-bit parts of their factors, two of each for
-    float16 and float32 (2^-17 of a value). The same call gives the same bits."""
+    float32. Differentiable once in q, k, v, log_decay and state. Results in float32
+    (states and the gradients of decays among them) have float32's accuracy; on the
+    way to outputs of 16 bits, scores and states are rounded to bf16, or to two parts of
+    it for float16. The same call gives the same bits."""
     return (_TORCH_CALLS or _torch_calls()).linear_attention(q, k, v, log_decay, state, lengths, scale)
 
 

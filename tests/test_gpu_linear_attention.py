@@ -3,17 +3,21 @@ single tokens, against the recurrence in 64 bits (its gradients by autograd).
 
 Tolerances. Every output is a sum of products of the inputs, so the same
 recurrence of their absolute values bounds the sum of the magnitudes of its
-terms (M below, one number for each output). A term meets at most
- - float32 and float16: three matrix products, each of two factors in two bf16
-   parts: 2^-17 for each factor and 2^-16 for the product of the low parts that
-   is left out, 2^-15; decays of 2^-20 (ex2.approx: 2^-22, and the sums of the
-   decays, 2^-24 of at most 2^5 where 2^-c is worth anything); fp32 sums of up to
-   64 + 128 terms in a chunk and one more for each chunk of a sequence, 2^-24
-   each: 3 * 2^-15 + 2^-20 + (192 + T / 32) 2^-24 < 2^-13 for T up to 8192;
- - bfloat16: one more rounding to bf16 for what lies between two products (a
-   score, or the state), 2^-8, and the second-order part of both: 2^-8 + 2^-13;
-   the states and the gradient of the decays have none: 2^-13.
-The store adds a half step of the stored type.
+terms (M below, one number for each output). A term of an fp32 result meets at most
+ - three matrix products of factors in three bf16 parts: products of parts that
+   are left out, below 2 * 2^-24 + 2^-32 of a factor's product each, 2^-22 in all;
+ - fp32 sums in matrix instructions, which cut a step's sum off (2^-23): of 128 + 128
+   values by 16, in up to six products each, 96 steps, 2^-16.4;
+ - one sum a chunk of 32 tokens or more, 2^-24 each, 2^-16 for T up to 8192;
+ - three decays: ex2.approx 2^-22, and the argument's rounding, 2^-24 of at most
+   2^5 (what is smaller than 2^-32 is lost beside its neighbours): 3 * 2^-19;
+together below 2^-14.9. The gradient of a token's decay is the difference, within
+its chunk, of two sums that hold the same terms of pairs on one side of the token:
+at most 128 + 7 roundings of 2^-24 of the chunk's terms, whatever is left of them
+(SPREAD: 2^-16 of the sum of |q . dq| over the 128 tokens around). What goes to a 16-bit output is rounded to one bf16 part
+between two products (2^-8, for a score or a state), or, for float16, to two, whose low
+parts' product is left out (2^-16 in each of three products, 2^-14 with the
+parts' own). The store adds a half step of the stored type.
 """
 from __future__ import annotations
 
@@ -23,7 +27,8 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
-FINE = 2.0 ** -13
+FINE = 2.0 ** -14.9
+PARTS = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -14}
 
 
 @pytest.fixture(scope="module")
@@ -88,11 +93,21 @@ def truth(x, scale, ends=None):
     return got
 
 
-def near(got, want, most, dtype, rough):
-    """rough: roundings to bf16 between products."""
+def spread(x, most):
+    """What the gradient of log_decay may be off beside FINE, from the gradients of absolute values."""
+    B, T, H = x["v"].shape[:3]
+    w = (x["q"].double().abs() * most[2]).sum(-1).repeat_interleave(H // x["q"].shape[2], 2)
+    if x["lengths"] is not None:
+        w = torch.where(torch.arange(T, device="cuda")[:, None] < x["lengths"][:, None, None], w, 0.0)
+    w = torch.cat([w, w.new_zeros(B, -T % 128, H)], 1).unflatten(1, (-1, 128)).sum(2, keepdim=True)
+    w = w.expand(-1, -1, 128, -1).flatten(1, 2)[:, :T] * 2.0 ** -16
+    return w.sum((0, 1)) if x["log_decay"].dim() == 1 else w
+
+
+def near(got, want, most, dtype, more=0.0):
     assert got.dtype == dtype and got.shape == want.shape
     e = torch.finfo(dtype).eps / 2
-    bound = ((2.0 ** -8 if rough else 0.0) + FINE) * most
+    bound = (PARTS[dtype] + FINE) * most + more
     tiny = torch.finfo(dtype).smallest_normal * e  # half a step below the normal numbers
     bad = ~((got.double() - want).abs() <= bound + e * (want.abs() + bound) + tiny).flatten()
     if bad.any():
@@ -102,7 +117,7 @@ def near(got, want, most, dtype, rough):
     if want.numel() >= 4096 and want.norm() > 0:
         # as independent roundings (at most 2^-8 / sqrt 3 for each value and each of two stages) add up
         far = float((got.double() - want).norm() / want.norm())
-        assert far <= (2.0 ** -8 if dtype == torch.bfloat16 else e + 2.0 ** -15), far
+        assert far <= {torch.float32: 2.0 ** -18, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype], far
 
 
 SIZES = [(1, 1, 1, 1, 1, 1), (2, 3, 2, 1, 5, 7), (1, 64, 2, 2, 64, 64), (2, 65, 3, 3, 64, 48), (1, 63, 1, 1, 33, 17),
@@ -118,8 +133,8 @@ def test_outputs_and_states(kernels, B, T, H, Hk, dk, dv, dtype):
         x = make(B, T, H, Hk, dk, dv, dtype, decay, state, seed=n)
         got = kernels.linear_attention(**x, scale=0.3)
         (out, S), (mo, ms) = truth(x, 0.3)
-        near(got[0], out, mo, dtype, dtype == torch.bfloat16)
-        near(got[1], S, ms, torch.float32, False)
+        near(got[0], out, mo, dtype)
+        near(got[1], S, ms, torch.float32)
 
 
 def gradients(kernels, x, scale, ends):
@@ -140,10 +155,9 @@ def test_gradients(kernels, B, T, H, Hk, dk, dv, dtype):
                 torch.randn(B, H, dk, dv, device="cuda", generator=gen) if state else None)
         got = gradients(kernels, x, 0.3, ends)
         want, most = truth(x, 0.3, ends)
-        rough = dtype == torch.bfloat16
-        kinds = [(dtype, rough), (torch.float32, False)] + [(dtype, rough)] * 3 + [(torch.float32, False)] * 2
-        for g, w, m, (kind, coarse) in zip(got, want, most, kinds):
-            near(g, w, m, kind, coarse)
+        kinds = [dtype, torch.float32] + [dtype] * 3 + [torch.float32] * 2
+        for n, (g, w, m, kind) in enumerate(zip(got, want, most, kinds)):
+            near(g, w, m, kind, spread(x, most) if n == 5 else 0.0)
 
 
 def test_gradients_against_differences(kernels):
@@ -170,15 +184,14 @@ def test_padded_batches(kernels, T, lengths, dtype):
     x = make(5, T, 2, 1, 64, 32, dtype, lengths=lengths)
     ends = (torch.randn(5, T, 2, 32, device="cuda").to(dtype), torch.randn(5, 2, 64, 32, device="cuda"))
     want, most = truth(x, 0.2, ends)
+    more = spread(x, most)
     behind = torch.arange(T, device="cuda") >= x["lengths"][:, None]
     for n in ("q", "k", "v", "log_decay"):
         x[n][behind] = float("nan")
     ends[0][behind] = float("nan")
     got = gradients(kernels, x, 0.2, ends)
-    rough = dtype == torch.bfloat16
-    for g, w, m, (kind, coarse) in zip(got, want, most, [(dtype, rough), (torch.float32, False)] + [(dtype, rough)] * 3 +
-                                       [(torch.float32, False)] * 2):
-        near(g, w, m, kind, coarse)
+    for n, (g, w, m, kind) in enumerate(zip(got, want, most, [dtype, torch.float32] + [dtype] * 3 + [torch.float32] * 2)):
+        near(g, w, m, kind, more if n == 5 else 0.0)
     for g in (got[0], *got[2:6]):
         assert (g[behind] == 0).all()
 
@@ -199,14 +212,14 @@ def test_decays_that_forget(kernels, T):
         part = {n: x[n][:, a:b] for n in ("q", "k", "v", "log_decay")}
         part["log_decay"] = part["log_decay"].clamp_min(-1e4)
         (o, s), (mo, ms) = truth({**part, "state": None, "lengths": None}, 1.0)
-        near(out[:, a:b], o, mo, torch.float32, False)
-    near(S, s, ms, torch.float32, False)
+        near(out[:, a:b], o, mo, torch.float32)
+    near(S, s, ms, torch.float32)
     # near tokens keep their weight exactly however far the sum of decays is from zero
     x["log_decay"][:] = -40.0
     x["log_decay"][:, 20] = 0.0
     out, _ = kernels.linear_attention(**x, scale=1.0)
     (o, _), (mo, _) = truth(x, 1.0)
-    near(out, o, mo, torch.float32, False)
+    near(out, o, mo, torch.float32)
 
 
 def test_values_without_finite_numbers_stay_in_their_place(kernels):
@@ -303,8 +316,8 @@ def test_a_prompt_in_parts_and_its_next_tokens(kernels, dtype):
         outs.append(out)
     for t in range(690, 700):
         outs.append(kernels.linear_attention_step(*(x[n][:, t] for n in ("q", "k", "v", "log_decay")), S, 0.2)[:, None])
-    near(torch.cat(outs, 1), want[0], most[0], dtype, dtype == torch.bfloat16)
-    near(S, want[1], most[1], torch.float32, False)
+    near(torch.cat(outs, 1), want[0], most[0], dtype)
+    near(S, want[1], most[1], torch.float32)
 
 
 def test_same_bits_captured_and_on_other_streams(kernels):
@@ -373,3 +386,25 @@ def test_refusals_on_the_gpu(kernels):
             kernels.linear_attention_step(**s, state=state)
     with pytest.raises(ValueError, match="overlap"):
         kernels.linear_attention_step(**s, state=x["state"][:1].expand(2, 4, 8, 16))
+
+
+def test_lengths_beyond_the_batch(kernels):
+    """Lengths below zero are none, lengths above T all tokens."""
+    x = make(3, 70, 2, 2, 16, 16, torch.float32, lengths=[-5, 70 + 9, 2 ** 31 - 1])
+    want, most = truth({**x, "lengths": torch.tensor([0, 70, 70], device="cuda")}, 0.3)
+    for g, w, m in zip(kernels.linear_attention(**x, scale=0.3), want, most):
+        near(g, w, m, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_offsets_beyond_32_bits(kernels, dtype):
+    """Tokens, heads and sequences that lie further apart than 2^32 bytes."""
+    x = make(2, 9, 2, 2, 16, 16, dtype, state=False)
+    far = torch.empty((1 << 33) // x["q"].element_size() + (1 << 29), dtype=dtype, device="cuda")
+    T = 1 << 28  # values from one token to the next: nine of them are beyond 2^31
+    wide = far.as_strided((2, 9, 2, 16), ((1 << 31) // 4 + 64, T - (1 << 24), 64, 1))
+    base = [t for t in kernels.linear_attention(**x)]
+    for n in ("q", "k", "v"):
+        wide.copy_(x[n])
+        got = kernels.linear_attention(**{**x, n: wide})
+        assert all(torch.equal(a, b) for a, b in zip(got, base)), n
