@@ -233,6 +233,11 @@ int32_t     sn_abi_rwkv7_dims(const SnAbiRwkv7* m, int32_t* dims8); /* vocab,D,H
 #define SN_BF16  1
 #define SN_F16   2
 
+/* For a caller that knows where its arrays lie (a tensor library): the calling
+ * thread's next call of this section takes every array to be memory of that GPU
+ * and does not ask the driver for each (0.3 us of the host's time). */
+void      sn_abi_arrays_on(int32_t device);
+
 /* Layer norm of `rows` rows of D values (1 to 2^31 - 2^14): y = (x - mean) * rstd * w + b, the
  * variance biased, rstd = 1 / sqrt(var + eps). x has rows at a stride of ldx
  * elements, y is contiguous; both are of `dtype`. w, b (D) are of `wdtype`:

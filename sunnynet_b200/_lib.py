@@ -74,6 +74,7 @@ SIGNATURES = {
     "sn_abi_rwkv7_get_state": (I32, [V, I32, V, V]),
     "sn_abi_rwkv7_dims": (I32, [V, V]),
     # sn_abi.h, enqueue-only operators
+    "sn_abi_arrays_on": (None, [I32]),
     "sn_abi_layer_norm": (I32, [V, I64, V, V, V, V, V, I32, I32, I64, I32, F32, V]),
     "sn_abi_layer_norm_bwd_ws": (I64, [I64, I32, I32]),
     "sn_abi_layer_norm_bwd": (I32, [V, I64, V, I64, V, V, V, V, V, V, V, I64, I32, I32, I64, I32,

@@ -23,15 +23,21 @@ RangeFn range_fn() {
     return fn;
 }
 
+// Where the calling thread's next call finds its arrays, as it says (-1: not said).
+thread_local int t_arrays_on = -1;
+
 constexpr int kMaxDevices = 64;
 std::atomic<int> g_sms[kMaxDevices];  // 0: not asked yet
 
 }  // namespace
 
+CallerDevice::CallerDevice() : device_(t_arrays_on), told_(t_arrays_on >= 0) { t_arrays_on = -1; }
+
 int CallerDevice::add(const char* what, const ArgPtr& a) {
     if (!a.p) return SN_OK;
     if ((uintptr_t)a.p % a.align)
         return fail(SN_E_INVAL, "%s: an array is not aligned to its elements", what);
+    if (told_) return SN_OK;
     if (known((uintptr_t)a.p)) return SN_OK;
     cudaPointerAttributes at;
     if (cudaPointerGetAttributes(&at, a.p) != cudaSuccess) {
@@ -80,3 +86,5 @@ int CallerDevice::select(const char* what) {
 }
 
 }  // namespace sn
+
+extern "C" void sn_abi_arrays_on(int32_t device) { sn::t_arrays_on = device; }

@@ -33,7 +33,7 @@ class CallerDevice {
     int add(const char* what, const ArgPtr& a);
     int select(const char* what);
     int num_sms() const { return sms_; }
-    CallerDevice() = default;
+    CallerDevice();
     CallerDevice(const CallerDevice&) = delete;
     CallerDevice& operator=(const CallerDevice&) = delete;
     ~CallerDevice() {
@@ -54,7 +54,8 @@ class CallerDevice {
     };
     Span spans_[16];
     unsigned next_ = 0, asked_ = 0;
-    int device_ = -1, restore_ = -1, sms_ = 0;
+    int device_, restore_ = -1, sms_ = 0;
+    bool told_;  // the caller vouches for its arrays (sn_abi_arrays_on)
 };
 
 // Bytes of one element of an SN_F32 / SN_BF16 / SN_F16 array, 0 for others.

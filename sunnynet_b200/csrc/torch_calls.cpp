@@ -51,6 +51,7 @@ struct {
     decltype(&sn_abi_linear_attention_bwd) attention_bwd = nullptr;
     decltype(&sn_abi_linear_attention_ws) attention_ws = nullptr;
     decltype(&sn_abi_linear_attention_step) attention_step = nullptr;
+    decltype(&sn_abi_arrays_on) arrays_on = nullptr;
     decltype(&sn_abi_grad_norm_ws) grad_norm_ws = nullptr;
     decltype(&sn_abi_grad_norm) grad_norm = nullptr;
     decltype(&sn_abi_clip_grads) clip_grads = nullptr;
@@ -82,6 +83,14 @@ void* address(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr
 void* stream_of(const at::Tensor& t) {
     return c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
 }
+
+// While it lives, the library's calls take all arrays to be on t's GPU, and do not
+// ask for each.
+struct Known {
+    explicit Known(const at::Tensor& t) { lib.arrays_on(t.get_device()); }
+    ~Known() { lib.arrays_on(-1); }
+    Known(const Known&) = delete;
+};
 
 int32_t weight_code(const at::Tensor& x, const at::Tensor& w, const at::Tensor& b) {
     return code(w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : x.scalar_type());
@@ -216,6 +225,7 @@ at::Tensor embedding_forward(const at::Tensor& tokens, const at::Tensor& w, doub
     std::vector<int64_t> sizes(tokens.sizes().begin(), tokens.sizes().end());
     sizes.push_back(w.size(1));
     at::Tensor out = at::empty(sizes, w.options());
+    const Known known(w);
     const int rc = lib.embedding(address(tokens), 8 * (int32_t)tokens.element_size(), tokens.numel(), address(w),
                                  w.stride(0), w.size(0), (int32_t)w.size(1), code(w.scalar_type()), (float)scale,
                                  address(out), stream_of(w));
@@ -242,6 +252,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
         at::Tensor dw = at::empty({V, D}, dout.options());
         const int64_t need = lib.embedding_bwd_ws(n, V, (int32_t)D);
         const at::Tensor ws = space(need, dout);
+        const Known known(dout);
         const int rc = lib.embedding_bwd(address(tokens), 8 * (int32_t)tokens.element_size(), n, address(rows),
                                          rows.stride(0), V, (int32_t)D, code(dout.scalar_type()),
                                          (float)ctx->saved_data["scale"].toDouble(), address(dw), address(ws),
@@ -334,6 +345,7 @@ std::pair<at::Tensor, at::Tensor> attention_forward(at::Tensor q, at::Tensor k, 
     at::Tensor end = at::empty({a.B, a.H, a.dk, a.dv}, v.options().dtype(at::kFloat));
     const int64_t need = lib.attention_ws(&a, 0, 0);
     const at::Tensor ws = space(need, v);
+    const Known known(v);
     const int rc = lib.attention(&a, address(out), end.data_ptr<float>(), address(ws), need, stream_of(v));
     TORCH_CHECK(rc == SN_OK, "linear_attention: ", last_error());
     return {out, end};
@@ -375,6 +387,7 @@ struct Attention : torch::autograd::Function<Attention> {
             const int64_t need = lib.attention_ws(&a, 1, heads);
             const at::Tensor ws = space(need, v);
             const int64_t stride[3] = {dout.stride(0), dout.stride(1), dout.stride(2)};
+            const Known known(v);
             const int rc = lib.attention_bwd(&a, address(dout), stride, static_cast<float*>(address(dend)),
                                              address(dq), address(dk), address(dv),
                                              static_cast<float*>(address(dg)), heads,
@@ -449,6 +462,7 @@ PyObject* linear_attention_step(PyObject*, PyObject* args) {
                           (!a.B || state.select(0, 0).is_contiguous()),
                       what, ": state is float32 of (B, H, dk, dv) on the GPU of the others, each sequence's contiguous");
     TORCH_CHECK_VALUE(a.B < 2 || state.stride(0) >= (int64_t)a.H * a.dk * a.dv, what, ": the states overlap");
+    const Known known(v);
     const int rc = lib.attention_step(&a, static_cast<float*>(address(state)), a.B ? state.stride(0) : 0,
                                       address(out), stream_of(v));
     TORCH_CHECK(rc == SN_OK, last_error());
@@ -459,9 +473,9 @@ PyObject* linear_attention_step(PyObject*, PyObject* args) {
 
 // use(addresses of the library's entry points, in the order below)
 PyObject* use(PyObject*, PyObject* args) {
-    unsigned long long p[14];
-    if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, p + 7, p + 8, p + 9,
-                          p + 10, p + 11, p + 12, p + 13))
+    unsigned long long p[15];
+    if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKKKK", p, p + 1, p + 2, p + 3, p + 4, p + 5, p + 6, p + 7, p + 8, p + 9,
+                          p + 10, p + 11, p + 12, p + 13, p + 14))
         return nullptr;
     lib.norm = reinterpret_cast<decltype(lib.norm)>(p[0]);
     lib.norm_bwd = reinterpret_cast<decltype(lib.norm_bwd)>(p[1]);
@@ -477,6 +491,7 @@ PyObject* use(PyObject*, PyObject* args) {
     lib.grad_norm_ws = reinterpret_cast<decltype(lib.grad_norm_ws)>(p[11]);
     lib.grad_norm = reinterpret_cast<decltype(lib.grad_norm)>(p[12]);
     lib.clip_grads = reinterpret_cast<decltype(lib.clip_grads)>(p[13]);
+    lib.arrays_on = reinterpret_cast<decltype(lib.arrays_on)>(p[14]);
     Py_RETURN_NONE;
 }
 
@@ -622,6 +637,7 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
     TORCH_CHECK_VALUE(need >= 0, what, ": too many values");
     const at::Tensor ws = at::empty({2 + need / 4}, first.options().dtype(at::kFloat));
     float* const to = ws.data_ptr<float>();
+    const Known known(first);
     const int rc = clip ? lib.clip_grads((int32_t)n, at.data(), sizes.data(), types.data(), max_norm, to, to + 1,
                                          to + 2, need, stream_of(first))
                         : lib.grad_norm((int32_t)n, at.data(), sizes.data(), types.data(), max_norm, to, to + 1,

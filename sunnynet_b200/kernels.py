@@ -236,7 +236,7 @@ def _torch_calls():
             lib.sn_abi_last_error, lib.sn_abi_embedding, lib.sn_abi_embedding_bwd,
             lib.sn_abi_embedding_bwd_ws, lib.sn_abi_linear_attention, lib.sn_abi_linear_attention_bwd,
             lib.sn_abi_linear_attention_ws, lib.sn_abi_linear_attention_step, lib.sn_abi_grad_norm_ws,
-            lib.sn_abi_grad_norm, lib.sn_abi_clip_grads)))
+            lib.sn_abi_grad_norm, lib.sn_abi_clip_grads, lib.sn_abi_arrays_on)))
         _TORCH_CALLS = m
     return _TORCH_CALLS
 
