@@ -359,18 +359,20 @@ __device__ __forceinline__ void zero_rows(T* to, long long stride, int t0, int t
 }
 
 // The CTA of a kernel: NW warps share a chunk's C / 16 blocks of tokens, and where
-// there are more warps than blocks, a block's columns.
+// there are more warps than blocks, a block's columns. In bf16 with heads of up to 64
+// there is a warp to a block: with two, both computed its scores (outputs of 16 x 2048 x
+// 12 heads 69 us instead of 50, gradients 296 instead of 223; chunks of 128 tokens with
+// eight warps 62 and 254); the other forms have too much to do for four warps.
 template <typename T_, int KD_, int VD_, int C_>
 struct Shape {
     typedef T_ T;
-    static constexpr int NP = planes_of<T_>, C = C_, NW = 8, THREADS = NW * 32;
+    static constexpr int NP = planes_of<T_>, C = C_, NW = NP == 1 && KD_ == 64 && VD_ == 64 ? 4 : 8, THREADS = NW * 32;
     static constexpr int KD = KD_, VD = VD_, LK = KD + 8, LV = VD + 8;  // rows of keys, of values and of states
     static constexpr int KT = NP * C * LK, VT = NP * C * LV, STATE = KD * LV;
     static constexpr int RB = C / 16, CG = NW / RB, NK = KD / CG / 8, NV = VD / CG / 8;
     static_assert(NW % RB == 0 && NK % 2 == 0 && NV % 2 == 0, "whole blocks for the warps");
-    // a states' pass: stages of SUB tokens, a warp for every 16 rows (with half of the columns to a warp, the
-    // rows' planes were formed twice: a fifth slower)
-    static constexpr int SUB = C < 64 ? C : 64, KS = NP * SUB * LK, VS = NP * SUB * LV;
+    // a states' pass: a warp for every 16 rows (with half of the columns to a warp, the rows' planes were
+    // formed twice: a fifth slower)
     static constexpr int SW = KD / 16, ST = SW * 32, SNT = VD / 8;
 };
 
@@ -399,12 +401,11 @@ template <class S_, bool KEEP, int PN>
 __global__ void __launch_bounds__(S_::ST + 32, KEEP && S_::SNT > 8 ? 1 : 2)
 state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) {
     typedef typename S_::T T;
-    constexpr int NP = S_::NP, KD = S_::KD, VD = S_::VD, C = S_::C, NT = S_::SNT, SUB = S_::SUB, PER = C / SUB;
-    // (a single chunk is asked for at once; three planes leave room for one stage, which
-    // is filled when every warp is done with it)
-    constexpr int STAGES = NP == 3 ? 1 : NP == 2 ? 2 : KEEP ? 3 : PER + 1;
-    constexpr int AHEAD = NP == 1 ? STAGES - 1 : 1;  // stages on their way
-    constexpr int STAGE = S_::KS + S_::VS;
+    constexpr int NP = S_::NP, KD = S_::KD, VD = S_::VD, C = S_::C, NT = S_::SNT;
+    // (three planes leave room for one stage, which is filled when every warp is done with it)
+    constexpr int STAGES = NP == 3 || !KEEP ? 1 : NP == 2 ? 2 : 3;
+    constexpr int AHEAD = NP == 1 && KEEP ? 2 : 1;  // stages on their way
+    constexpr int STAGE = S_::KT + S_::VT;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16* const tiles = reinterpret_cast<bf16*>(smem);
     __shared__ Decays<C> dec_[2];
@@ -446,7 +447,7 @@ state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) 
             ask(x[FAR - 1], i + FAR);
             if (i + 1 < n) decays<C>(&dec_[(i + 1) & 1], x[0]);
 #pragma unroll
-            for (int k = 1; k < PER * (STAGES == 1 ? 2 : 1); ++k) __syncthreads();
+            for (int k = 1; k < (STAGES == 1 ? 2 : 1); ++k) __syncthreads();
         }
         return;
     }
@@ -455,27 +456,24 @@ state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) 
     const T* x = head_of<T>(p.x, p.xs, b, h / j.share);
     const T* y = head_of<T>(p.y, p.ys, b, h);
     const bool wx = j.whole >> (p.back ? 0 : 1) & 1, wy = j.whole >> (p.back ? 3 : 2) & 1;
-    Fetch<T, SUB, KD, S_::ST> lx;
-    Fetch<T, SUB, VD, S_::ST> ly;
-    // stage u of the pass: tokens [first(u), first(u) + SUB)
-    const int stages = n * PER;
-    const auto first = [&](int u) { return chunk(u / PER) * C + u % PER * SUB; };
-    const auto fetch = [&](int u, int stage) {
-        if (u < stages) {
+    Fetch<T, C, KD, S_::ST> lx;
+    Fetch<T, C, VD, S_::ST> ly;
+    const auto fetch = [&](int i, int stage) {
+        if (i < n) {
             bf16* to = tiles + stage * STAGE;
-            lx.fetch(to, x, p.xs.t, first(u), end, j.dk, wx);
-            ly.fetch(to + S_::KS, y, p.ys.t, first(u), end, j.dv, wy);
+            lx.fetch(to, x, p.xs.t, chunk(i) * C, end, j.dk, wx);
+            ly.fetch(to + S_::KT, y, p.ys.t, chunk(i) * C, end, j.dv, wy);
         }
         cp_async_commit();
     };
-    const auto put = [&](int u, int stage) {
-        if (u < stages) {
+    const auto put = [&](int i, int stage) {
+        if (i < n) {
             bf16* to = tiles + stage * STAGE;
-            lx.put(to, x, p.xs.t, first(u), end, j.dk, wx);
-            ly.put(to + S_::KS, y, p.ys.t, first(u), end, j.dv, wy);
+            lx.put(to, x, p.xs.t, chunk(i) * C, end, j.dk, wx);
+            ly.put(to + S_::KT, y, p.ys.t, chunk(i) * C, end, j.dv, wy);
         }
     };
-    for (int u = 0; u < AHEAD; ++u) fetch(u, u % STAGES);
+    for (int i = 0; i < AHEAD; ++i) fetch(i, i);
     put(0, 0);
     float S[NT][4];
     if constexpr (KEEP)
@@ -485,32 +483,26 @@ state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) 
     int stage = 0;
     for (int i = 0; i < n; ++i) {
         const Decays<C>& dec = dec_[i & 1];
+        cp_async_wait_group<AHEAD - 1>();
+        __syncthreads();
+        fetch(i + AHEAD, (stage + AHEAD) % STAGES);
+        if constexpr (KEEP)
+            state_planes<PN, VD, NT>(S, p.kept + (bh * j.chunks + chunk(i)) * PN * KD * VD, KD * VD, row, by_[warp]);
+        const bf16* from = tiles + stage * STAGE;
         float sum[NT][4];
         clear<NT>(sum);
+        add_outer<NP, NT, C>(sum, tile(from, S_::LK, C * S_::LK), tile(from + S_::KT, S_::LV, C * S_::LV),
+                             p.back ? dec.from_start : dec.to_end, p.back ? j.scale : 1.0f, row, 0);
+        // The chunk's sum is added here, not in the matrix instruction, which cuts its sums off: over a
+        // sequence that leaned by 2^-24 of the state a step.
+        const float f = dec.whole;
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int u = i * PER + k;
-            cp_async_wait_group<AHEAD - 1>();
-            __syncthreads();
-            fetch(u + AHEAD, (stage + AHEAD) % STAGES);
-            if (KEEP && k == 0)
-                state_planes<PN, VD, NT>(S, p.kept + (bh * j.chunks + chunk(i)) * PN * KD * VD, KD * VD, row, by_[warp]);
-            const bf16* from = tiles + stage * STAGE;
-            add_outer<NP, NT, SUB>(sum, tile(from, S_::LK, SUB * S_::LK), tile(from + S_::KS, S_::LV, SUB * S_::LV),
-                                   (p.back ? dec.from_start : dec.to_end) + k * SUB, p.back ? j.scale : 1.0f, row, 0);
-            // The chunk's sum is added here, not in the matrix instruction, which cuts its sums off: over a
-            // sequence that leaned by 2^-24 of the state a step.
-            if (k + 1 == PER) {
-                const float f = dec.whole;
+        for (int m = 0; m < NT; ++m)
 #pragma unroll
-                for (int m = 0; m < NT; ++m)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) S[m][e] = fmaf(S[m][e], f, sum[m][e]);
-            }
-            if constexpr (STAGES == 1) __syncthreads();
-            stage = (stage + 1) % STAGES;
-            put(u + 1, stage);
-        }
+            for (int e = 0; e < 4; ++e) S[m][e] = fmaf(S[m][e], f, sum[m][e]);
+        if constexpr (STAGES == 1) __syncthreads();
+        stage = (stage + 1) % STAGES;
+        put(i + 1, stage);
     }
     if constexpr (!KEEP) {
         if (!n) return;
@@ -647,11 +639,10 @@ out_kernel(const Job j, const bf16* kept, const Decays<S_::C>* decs, void* out_)
     // Between the blocks of 16 tokens a decay is 2^(c_t - c_r) 2^(c_r - c_s), r the
     // last token before the row's block: a factor of the row, which the state's
     // part shares, and one of the column, which the warp writes down once (behind the
-    // rows of the queries and keys of its block, four to a row). Both are at most 1.
-    // Within a block each pair has its own.
-    const auto column = [&](int s) {
-        return reinterpret_cast<float*>((s < 64 ? sq : sk) + (rb * 16 + s % 64 / 4) * LK + KD) + s % 4;
-    };
+    // rows of its block's queries, four to a row). Both are at most 1. Within a block
+    // each pair has its own.
+    static_assert(C <= 64, "room behind the rows");
+    const auto column = [&](int s) { return reinterpret_cast<float*>(sq + (rb * 16 + s / 4) * LK + KD) + s % 4; };
     for (int s = l; s < rb * 16; s += 32) *column(s) = dec.between(rb * 16 - 1, s);
     __syncwarp();
     float O[NT][4];
@@ -835,9 +826,7 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
             store_rows_by<T, NK, BK>(by, x, static_cast<T*>(to16) + k0, kt, c0 + rb * 16, ck, end, j.T, j.dk);
     };
     // factors of columns, as in out_kernel
-    const auto column = [&](int s) {
-        return reinterpret_cast<float*>((s < 64 ? sq : sk) + (rb * 16 + s % 64 / 4) * LK + KD) + s % 4;
-    };
+    const auto column = [&](int s) { return reinterpret_cast<float*>(sq + (rb * 16 + s / 4) * LK + KD) + s % 4; };
     constexpr int FINE = NP == 2 ? 3 : NP;  // (the scores' products in full: dg is an fp32 result)
     float part[2];
     const int t = rb * 16 + (l >> 2);  // the lane's tokens: this and 8 behind
@@ -1053,8 +1042,7 @@ __global__ void __launch_bounds__(256) gate_kernel(const float* dg, const double
 // ------------------------------------------------------------------ launches
 template <class S_>
 struct Sizes {
-    static constexpr int state = (4 - S_::NP) * (S_::KS + S_::VS) * 2;
-    static constexpr int sum = (S_::NP == 1 ? S_::C / S_::SUB : 4 - S_::NP) * (S_::KS + S_::VS) * 2;
+    static constexpr int sum = (S_::KT + S_::VT) * 2, state = (4 - S_::NP) * sum;
     static constexpr int out = (2 * S_::KT + S_::VT + S_::NP * S_::STATE) * 2;
     static constexpr int grad = (2 * S_::KT + 2 * S_::VT + 3 * S_::STATE) * 2;
 };
@@ -1160,7 +1148,7 @@ int forward_as(Job j, const float* first, void* out, float* state_out, char* ws,
     if (!j.chunks) return SN_OK;
     constexpr int bytes = Sizes<S_>::out;
     static_assert(bytes <= 220 * 1024, "shared memory of a CTA");
-    auto* kernel = out_kernel<S_, bytes <= 72 * 1024 ? 3 : bytes <= 96 * 1024 ? 2 : 1>;
+    auto* kernel = out_kernel<S_, bytes <= 40 * 1024 ? 5 : bytes <= 72 * 1024 ? 3 : bytes <= 96 * 1024 ? 2 : 1>;
     SN_TRY(allow(kernel, bytes, "linear_attention"));
     kernel<<<(unsigned)((long long)j.B * j.H * j.chunks), S_::THREADS, bytes, st>>>(j, p.kept, dec, out);
     return cuda_check(cudaGetLastError(), "linear_attention launch");
@@ -1196,7 +1184,7 @@ int backward_as(Job j, const float* first, const Wanted& g, char* ws, long long 
     G.dg = !g.dg ? nullptr : g.gates_alike ? floats(s.dg) : g.dg;
     constexpr int bytes = Sizes<S_>::grad;
     static_assert(bytes <= 220 * 1024, "shared memory of a CTA");
-    auto* kernel = grad_kernel<S_, bytes <= 102 * 1024 ? 2 : 1>;
+    auto* kernel = grad_kernel<S_, bytes <= 66 * 1024 ? 3 : bytes <= 102 * 1024 ? 2 : 1>;
     SN_TRY(allow(kernel, bytes, "linear_attention_bwd"));
     if (j.chunks)
         kernel<<<(unsigned)((long long)j.B * j.H * j.chunks), S_::THREADS, bytes, st>>>(j, G, dec);
@@ -1216,13 +1204,10 @@ int backward_as(Job j, const float* first, const Wanted& g, char* ws, long long 
 }
 
 // The widths that the keys and the values are laid out in, and the tokens of a
-// chunk: the longer, the fewer states are kept and read again (in bf16 with heads of
-// up to 64, the states of a chunk of 128 take half of what its keys do), and the more
-// shared memory the tiles take.
+// chunk: 64, but where the tiles and a state of two or three parts would not fit.
 template <typename T, typename F>
 int by_width(const Job& j, F&& f) {
-    constexpr int LONG = planes_of<T> == 1 ? 128 : 64;
-    if (j.dk <= 64) return j.dv <= 64 ? f(Shape<T, 64, 64, LONG>()) : f(Shape<T, 64, 128, 64>());
+    if (j.dk <= 64) return j.dv <= 64 ? f(Shape<T, 64, 64, 64>()) : f(Shape<T, 64, 128, 64>());
     return j.dv <= 64 ? f(Shape<T, 128, 64, 64>()) : f(Shape<T, 128, 128, planes_of<T> == 1 ? 64 : 32>());
 }
 

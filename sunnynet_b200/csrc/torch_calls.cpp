@@ -288,13 +288,17 @@ PyObject* embedding(PyObject*, PyObject* args) {
 // ----------------------------------------------------------- linear attention
 constexpr int64_t kMaxHead = 128;
 
-// The checked arguments of a call. Tensors are made fit for it in place.
+// The checked arguments of a call. Tensors are made fit for it in place. A single
+// token's have no axis of tokens.
 SnAbiLinearAttention attention_call(const char* what, at::Tensor& q, at::Tensor& k, at::Tensor& v,
                                     at::Tensor& decay, at::Tensor* state, at::Tensor* lengths, double scale) {
-    TORCH_CHECK_VALUE(q.dim() == 4 && v.dim() == 4 && k.sizes() == q.sizes() && v.size(0) == q.size(0) &&
-                          v.size(1) == q.size(1),
-                      what, ": q and k are (B, T, Hk, dk), v (B, T, H, dv)");
-    const int64_t B = q.size(0), T = q.size(1), Hk = q.size(2), dk = q.size(3), H = v.size(2), dv = v.size(3);
+    const int64_t one = v.dim() == 3, n = 4 - one;
+    TORCH_CHECK_VALUE(q.dim() == n && v.dim() == n && k.sizes() == q.sizes() && v.size(0) == q.size(0) &&
+                          (one || v.size(1) == q.size(1)),
+                      what, one ? ": q and k are (B, Hk, dk), v (B, H, dv)"
+                                : ": q and k are (B, T, Hk, dk), v (B, T, H, dv)");
+    const int64_t B = q.size(0), T = one ? 1 : q.size(1), Hk = q.size(n - 2), dk = q.size(n - 1), H = v.size(n - 2),
+                  dv = v.size(n - 1);
     TORCH_CHECK_VALUE(Hk > 0 && H > 0 && H % Hk == 0 && dk > 0 && dk <= kMaxHead && dv > 0 && dv <= kMaxHead, what,
                       ": heads of 1 to 128 values, H a multiple of Hk");
     TORCH_CHECK_VALUE(T < 0x7fffffff - 128 && B * H <= 0x7fffffff, what, ": sizes beyond 31 bits");
@@ -303,8 +307,10 @@ SnAbiLinearAttention attention_call(const char* what, at::Tensor& q, at::Tensor&
                           q.device() == v.device() && k.device() == v.device(),
                       what, ": q, k and v are of one type, on one GPU");
     TORCH_CHECK_VALUE(decay.scalar_type() == at::kFloat && decay.device() == v.device() &&
-                          (decay.sizes() == at::IntArrayRef({H}) || decay.sizes() == at::IntArrayRef({B, T, H})),
-                      what, ": log_decay is float32 of (H) or (B, T, H) on the GPU of the others");
+                          (decay.sizes() == at::IntArrayRef({H}) ||
+                           (one ? decay.sizes() == at::IntArrayRef({B, H}) : decay.sizes() == at::IntArrayRef({B, T, H}))),
+                      what, one ? ": log_decay is float32 of (H) or (B, H) on the GPU of the others"
+                                : ": log_decay is float32 of (H) or (B, T, H) on the GPU of the others");
     TORCH_CHECK_VALUE(std::isfinite(scale), what, ": the scale is not finite");
     SnAbiLinearAttention a = {};
     if (state && state->defined()) {
@@ -321,17 +327,21 @@ SnAbiLinearAttention attention_call(const char* what, at::Tensor& q, at::Tensor&
         *lengths = lengths->contiguous();
         a.lengths = lengths->data_ptr<int32_t>();
     }
-    const auto rows = [](at::Tensor& t, const void** p, int64_t* stride) {
-        if (t.size(3) > 1 && t.stride(3) != 1) t = t.contiguous();
+    const auto rows = [&](at::Tensor& t, const void** p, int64_t* stride) {
+        if (t.size(n - 1) > 1 && t.stride(n - 1) != 1) t = t.contiguous();
         *p = t.data_ptr();
-        for (int i = 0; i < 3; ++i) stride[i] = t.stride(i);
+        stride[0] = t.stride(0);
+        stride[1] = one ? 0 : t.stride(1);
+        stride[2] = t.stride(n - 2);
     };
     rows(q, &a.q, a.q_stride);
     rows(k, &a.k, a.k_stride);
     rows(v, &a.v, a.v_stride);
     a.log_decay = decay.data_ptr<float>();
-    for (int i = 0; i < 3; ++i)
-        a.log_decay_stride[i] = decay.dim() == 3 ? decay.stride(i) : i == 2 ? decay.stride(0) : 0;
+    const bool each = decay.dim() > 1;  // token's
+    a.log_decay_stride[0] = each ? decay.stride(0) : 0;
+    a.log_decay_stride[1] = each && !one ? decay.stride(1) : 0;
+    a.log_decay_stride[2] = decay.stride(decay.dim() - 1);
     a.dtype = code(v.scalar_type());
     a.B = (int32_t)B, a.T = (int32_t)T, a.H = (int32_t)H, a.Hk = (int32_t)Hk, a.dk = (int32_t)dk, a.dv = (int32_t)dv;
     a.scale = (float)scale;
@@ -438,6 +448,16 @@ PyObject* linear_attention(PyObject*, PyObject* args) {
     END_HANDLE_TH_ERRORS
 }
 
+// Whether each sequence's state is contiguous.
+bool rows_of_state(const at::Tensor& s) {
+    int64_t want = 1;
+    for (int i = 3; i > 0; --i) {
+        if (s.size(i) > 1 && s.stride(i) != want) return false;
+        want *= s.size(i);
+    }
+    return true;
+}
+
 // linear_attention_step(q, k, v, log_decay, state, scale) -> out; state is updated
 PyObject* linear_attention_step(PyObject*, PyObject* args) {
     HANDLE_TH_ERRORS
@@ -453,13 +473,10 @@ PyObject* linear_attention_step(PyObject*, PyObject* args) {
     no_tangent(what, {q, k, v, decay, state});
     TORCH_CHECK_VALUE(!wants_grad({q, k, v, decay, state}), what, " has no gradient: call linear_attention");
     at::Tensor out = at::empty(v.sizes(), v.options());
-    const at::Tensor shape = v;
-    q = q.unsqueeze(1), k = k.unsqueeze(1), v = v.unsqueeze(1);
-    if (decay.dim() == 2) decay = decay.unsqueeze(1);
     const SnAbiLinearAttention a = attention_call(what, q, k, v, decay, nullptr, nullptr, scale);
     TORCH_CHECK_VALUE(state.defined() && state.scalar_type() == at::kFloat && state.device() == v.device() &&
                           state.sizes() == at::IntArrayRef({a.B, a.H, a.dk, a.dv}) &&
-                          (!a.B || state.select(0, 0).is_contiguous()),
+                          rows_of_state(state),
                       what, ": state is float32 of (B, H, dk, dv) on the GPU of the others, each sequence's contiguous");
     TORCH_CHECK_VALUE(a.B < 2 || state.stride(0) >= (int64_t)a.H * a.dk * a.dv, what, ": the states overlap");
     const Known known(v);
