@@ -338,7 +338,8 @@ sn_status sn_abi_linear_attention_step(const SnAbiLinearAttention* a, float* sta
 
 /* Rows of an embedding (SN_CAP_TRAIN): out[i] = scale * W[token_i], n rows of D
  * values, contiguous; W (V, D) with rows `ld` values apart, both of `dtype`;
- * tokens int32 or int64 (token_bits). A token outside [0, V) gives a row of NaN.
+ * tokens int32 or int64 (token_bits), fewer than 2^31 - 4096; D at most 2^22. A
+ * token outside [0, V) gives a row of NaN.
  * Its gradient: dW[v] = scale * the sum of dout[i] over token_i = v, in fp32 and
  * in the order of i; dW (V, D) contiguous, overwritten; dout with rows `ld`
  * values apart. The same call gives the same bits. */

@@ -463,9 +463,13 @@ int by_access(int dtype, int width, F&& f) {
     });
 }
 
+// (tokens: their indexes plus a tile's stay in 31 bits; columns: a grid's second axis)
+constexpr long long kMostTokens = 0x7ffff000;
+constexpr int kMostColumns = 1 << 22;
+
 int check_call(const char* what, int64_t n, int64_t V, int32_t D, int64_t ld, int32_t dtype, float scale) {
     if (!dtype_size(dtype)) return fail(SN_E_INVAL, "%s: dtype %d", what, dtype);
-    if (n < 0 || V < 0 || D < 0 || n > 0x7fffffffll || V >= 0x7fffffffll || D > 1 << 30)
+    if (n < 0 || V < 0 || D < 0 || n > kMostTokens || V >= 0x7fffffffll || D > kMostColumns)
         return fail(SN_E_INVAL, "%s: %lld tokens, %lld rows of %d", what, (long long)n, (long long)V, D);
     if (ld < 0 || ld >= 1ll << 44) return fail(SN_E_INVAL, "%s: rows %lld values apart", what, (long long)ld);
     if (!std::isfinite(scale)) return fail(SN_E_INVAL, "%s: the scale is not finite", what);

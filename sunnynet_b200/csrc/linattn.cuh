@@ -1,5 +1,5 @@
 // Pieces of the linear-attention kernels: tiles of tokens in shared memory as
-// one or two bf16 planes, their matrix fragments, and the decays of a chunk.
+// one to three bf16 planes, their matrix fragments, and the decays of a chunk.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -318,8 +318,8 @@ struct Job {
     int B, T, H, share, dk, dv;
     float scale;
     int whole;  // bit 0: q, 1: k, 2: v, 3: dout come in whole packs
-    int chunks;         // of a sequence
-    bool apart;         // each chunk's sum by a CTA of its own
+    int chunks;  // of a sequence
+    bool apart;  // each chunk's sum by a CTA of its own
 };
 
 // The gradients that a call wants, and those it is given.

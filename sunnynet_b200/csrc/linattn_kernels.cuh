@@ -10,7 +10,7 @@ namespace sn {
 namespace la {
 namespace {
 
-// Tokens of a sequence, and its chunks that hold some.
+// Tokens of a sequence.
 __device__ __forceinline__ int tokens_of(const Job& j, int b) {
     return j.lengths ? max(0, min(j.T, j.lengths[b])) : j.T;
 }
@@ -834,7 +834,7 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
         // rows s, columns u >= s. Between blocks a decay is 2^(c_u - c_r) 2^(c_r - c_s), r
         // the last token of the row's block
         const int r = rb * 16 + 15;
-                const float b0 = dec.between(r, t), b1 = dec.between(r, t + 8), behind = dec.to_end[r];
+        const float b0 = dec.between(r, t), b1 = dec.between(r, t + 8), behind = dec.to_end[r];
         float V[NV][4], K[NK][4], across[2] = {0.0f, 0.0f};
         clear<NV>(V);
         product<NP, NP, KD, NV, true>(V, tk, rb * 16, ts, cv);

@@ -270,12 +270,12 @@ PyObject* embedding(PyObject*, PyObject* args) {
     if (!PyArg_ParseTuple(args, "OOd", &to, &wo, &scale)) return nullptr;
     at::Tensor tokens, w;
     if (!tensor_of(to, &tokens) || !tensor_of(wo, &w)) return nullptr;
-    TORCH_CHECK_VALUE(w.defined() && w.dim() == 2 && w.is_cuda() && w.size(1) <= 1 << 30 && w.size(0) < 0x7fffffff,
-                      "embedding: weight (V, D) on a GPU is wanted");
+    TORCH_CHECK_VALUE(w.defined() && w.dim() == 2 && w.is_cuda() && w.size(1) <= 1 << 22 && w.size(0) < 0x7fffffff,
+                      "embedding: weight (V, D) on a GPU is wanted, D at most 2^22");
     TORCH_CHECK_TYPE(float_type(w), "embedding: weight is float32, bfloat16 or float16");
     TORCH_CHECK_VALUE(tokens.defined() && (tokens.scalar_type() == at::kInt || tokens.scalar_type() == at::kLong) &&
-                          tokens.device() == w.device() && tokens.numel() <= 0x7fffffff,
-                      "embedding: tokens are int32 or int64 on the weight's GPU");
+                          tokens.device() == w.device() && tokens.numel() <= 0x7ffff000,
+                      "embedding: tokens are int32 or int64 on the weight's GPU, fewer than 2^31");
     TORCH_CHECK_VALUE(std::isfinite(scale), "embedding: the scale is not finite");
     no_tangent("embedding", {w});
     tokens = tokens.contiguous();
@@ -291,8 +291,9 @@ constexpr int64_t kMaxHead = 128;
 // The checked arguments of a call. Tensors are made fit for it in place. A single
 // token's have no axis of tokens.
 SnAbiLinearAttention attention_call(const char* what, at::Tensor& q, at::Tensor& k, at::Tensor& v,
-                                    at::Tensor& decay, at::Tensor* state, at::Tensor* lengths, double scale) {
-    const int64_t one = v.dim() == 3, n = 4 - one;
+                                    at::Tensor& decay, at::Tensor* state, at::Tensor* lengths, double scale,
+                                    bool one = false) {
+    const int64_t n = 4 - one;
     TORCH_CHECK_VALUE(q.dim() == n && v.dim() == n && k.sizes() == q.sizes() && v.size(0) == q.size(0) &&
                           (one || v.size(1) == q.size(1)),
                       what, one ? ": q and k are (B, Hk, dk), v (B, H, dv)"
@@ -468,22 +469,20 @@ PyObject* linear_attention_step(PyObject*, PyObject* args) {
     if (!attention_args(o, 5, t, so, &scale)) return nullptr;
     const char* const what = "linear_attention_step";
     at::Tensor &q = t[0], &k = t[1], &v = t[2], &decay = t[3], &state = t[4];
-    TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, what,
-                      ": q and k are (B, Hk, dk), v (B, H, dv)");
     no_tangent(what, {q, k, v, decay, state});
     TORCH_CHECK_VALUE(!wants_grad({q, k, v, decay, state}), what, " has no gradient: call linear_attention");
     at::Tensor out = at::empty(v.sizes(), v.options());
-    const SnAbiLinearAttention a = attention_call(what, q, k, v, decay, nullptr, nullptr, scale);
+    const SnAbiLinearAttention a = attention_call(what, q, k, v, decay, nullptr, nullptr, scale, true);
     TORCH_CHECK_VALUE(state.defined() && state.scalar_type() == at::kFloat && state.device() == v.device() &&
                           state.sizes() == at::IntArrayRef({a.B, a.H, a.dk, a.dv}) &&
                           rows_of_state(state),
                       what, ": state is float32 of (B, H, dk, dv) on the GPU of the others, each sequence's contiguous");
     TORCH_CHECK_VALUE(a.B < 2 || state.stride(0) >= (int64_t)a.H * a.dk * a.dv, what, ": the states overlap");
+    state.unsafeGetTensorImpl()->bump_version();  // a graph that saved it must not use it
     const Known known(v);
     const int rc = lib.attention_step(&a, static_cast<float*>(address(state)), a.B ? state.stride(0) : 0,
                                       address(out), stream_of(v));
     TORCH_CHECK(rc == SN_OK, last_error());
-    state.unsafeGetTensorImpl()->bump_version();  // a graph that saved it must not use it
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }
@@ -654,14 +653,14 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
     TORCH_CHECK_VALUE(need >= 0, what, ": too many values");
     const at::Tensor ws = at::empty({2 + need / 4}, first.options().dtype(at::kFloat));
     float* const to = ws.data_ptr<float>();
+    if (clip)  // a graph that saved one must not use it
+        for (Py_ssize_t j = 0; j < n; ++j) THPVariable_Unpack(of[j]).unsafeGetTensorImpl()->bump_version();
     const Known known(first);
     const int rc = clip ? lib.clip_grads((int32_t)n, at.data(), sizes.data(), types.data(), max_norm, to, to + 1,
                                          to + 2, need, stream_of(first))
                         : lib.grad_norm((int32_t)n, at.data(), sizes.data(), types.data(), max_norm, to, to + 1,
                                         to + 2, need, stream_of(first));
     TORCH_CHECK(rc == SN_OK, last_error());
-    if (clip)  // a graph that saved one must not use it
-        for (Py_ssize_t j = 0; j < n; ++j) THPVariable_Unpack(of[j]).unsafeGetTensorImpl()->bump_version();
     if (clip) return THPVariable_Wrap(ws.select(0, 0));
     return Py_BuildValue("(NN)", THPVariable_Wrap(ws.select(0, 0)), THPVariable_Wrap(ws.select(0, 1)));
     END_HANDLE_TH_ERRORS

@@ -21,6 +21,8 @@ class AdamW(torch.optim.Optimizer):
     whose common norm (of all groups) is larger are scaled to it as the step reads
     them, .grad stays as it is; ``grad_norm`` is then the last step's norm, on the GPU."""
 
+    max_norm = grad_norm = None
+
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
                  state_bits=32, max_norm=None):
         if max_norm is not None and not max_norm >= 0:
@@ -31,9 +33,12 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW: lr, eps and weight_decay must not be negative")
         if not all(0 <= b < 1 for b in betas):
             raise ValueError("AdamW: betas are in [0, 1)")
-        self.max_norm, self.grad_norm = max_norm, None
+        self.max_norm = max_norm
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps,
                                       weight_decay=weight_decay, state_bits=state_bits))
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_norm": self.max_norm}
 
     def _state(self, p, bits):
         s = self.state[p]

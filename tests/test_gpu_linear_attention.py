@@ -370,6 +370,30 @@ def test_only_once_differentiable_and_versions(kernels):
         y.backward()
 
 
+def test_inference_mode(kernels):
+    """States of inference mode are updated in it, and outside are refused untouched."""
+    with torch.inference_mode():
+        x = make(2, 1, 2, 2, 8, 8, torch.float32, "head")
+        one = {n: t[:, 0] if n in "qkv" else t for n, t in x.items() if n != "lengths"}
+        (out, end), (mo, me) = truth(x, 8 ** -0.5)
+        near(kernels.linear_attention_step(**one), out[:, 0], mo[:, 0], torch.float32)
+        near(one["state"], end, me, torch.float32)
+    before = one["state"].clone()
+    with torch.no_grad(), pytest.raises(RuntimeError, match="inference"):
+        kernels.linear_attention_step(**one)
+    assert torch.equal(one["state"], before)
+
+
+def test_growing_states(kernels):
+    """Positive log decays, up to e^20 over the sequence."""
+    x = make(1, 200, 2, 1, 24, 40, torch.float32)
+    x["log_decay"] = x["log_decay"].abs().clamp(max=0.1)
+    got = kernels.linear_attention(**x, scale=0.2)
+    (out, S), (mo, ms) = truth(x, 0.2)
+    near(got[0], out, mo, torch.float32)
+    near(got[1], S, ms, torch.float32)
+
+
 def test_refusals_on_the_gpu(kernels):
     x = make(2, 5, 4, 2, 8, 16, torch.float32)
     for change in ({"q": x["q"][:, :4]}, {"k": x["k"][..., :7]}, {"v": x["v"][:, :, :3]}, {"q": x["q"].bfloat16()},

@@ -21,8 +21,8 @@ def test_capability_bit(lib):  # noqa: F811
     assert lib.sn_abi_caps() & (1 << 12)
 
 
-@pytest.mark.parametrize("change", [{"bits": 16}, {"n": -1}, {"n": 1 << 31}, {"V": -1}, {"V": (1 << 31) - 1}, {"D": -1},
-                                    {"D": (1 << 30) + 1}, {"ld": -1}, {"dtype": 3}, {"scale": float("nan")},
+@pytest.mark.parametrize("change", [{"bits": 16}, {"n": -1}, {"n": 1 << 31}, {"n": (1 << 31) - 1}, {"V": -1}, {"V": (1 << 31) - 1}, {"D": -1},
+                                    {"D": (1 << 30) + 1}, {"D": (1 << 22) + 1}, {"ld": -1}, {"dtype": 3}, {"scale": float("nan")},
                                     {"scale": float("inf")}, {"tokens": None}, {"W": None}, {"out": None}])
 def test_embedding(lib, change):  # noqa: F811
     a = dict(tokens=A, bits=64, n=4, W=A, ld=8, V=8, D=8, dtype=0, scale=1.0, out=A, stream=None)
@@ -113,6 +113,8 @@ def test_python_refusals_without_a_gpu(lib):  # noqa: F811
             (lambda: kernels.linear_attention(x, x, None, g), TypeError, "tensors"),
             (lambda: kernels.linear_attention(x, x, v, g, scale="a"), TypeError, None),
             (lambda: kernels.linear_attention_step(x, x, v, g, v), ValueError, "Hk"),
+            (lambda: kernels.linear_attention(x[:, 0], x[:, 0], v[:, 0], g[:, 0]), ValueError, "T, Hk"),
+            (lambda: kernels.linear_attention_step(x[:, 0], x[:, 0], v[:, 0], g[:, 0], v), ValueError, "one GPU"),
             (lambda: kernels.embedding(torch.zeros(3).long(), v[0, 0]), ValueError, "GPU"),
             (lambda: kernels.embedding(3, v[0, 0]), TypeError, "tensors"),
             (lambda: kernels.grad_norm([]), ValueError, "no gradients"),
@@ -142,3 +144,15 @@ def test_optimiser_refuses_a_negative_norm():
     from sunnynet_b200.optim import AdamW
     with pytest.raises(ValueError, match="max_norm"):
         AdamW([torch.nn.Parameter(torch.zeros(3))], max_norm=-1.0)
+
+
+def test_a_copy_of_the_optimiser_keeps_its_bound():
+    import copy
+
+    from sunnynet_b200.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(3))
+    assert copy.deepcopy(AdamW([p], max_norm=2.0)).max_norm == 2.0
+    assert copy.deepcopy(AdamW([p])).max_norm is None
+    old = AdamW.__new__(AdamW)  # as one of before the argument unpickles
+    old.__setstate__({k: v for k, v in AdamW([p]).__getstate__().items() if k != "max_norm"})
+    assert old.max_norm is None and old.grad_norm is None
