@@ -425,17 +425,7 @@ __global__ void __launch_bounds__(kJoin * 32) join_kernel(const Summing s, T* dW
 
 template <typename... P, typename... A>
 int launch_behind(void (*kernel)(P...), dim3 ctas, int threads, int smem, cudaStream_t st, A... args) {
-    cudaLaunchConfig_t c = {};
-    c.gridDim = ctas;
-    c.blockDim = dim3(threads);
-    c.dynamicSmemBytes = smem;
-    c.stream = st;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    c.attrs = &at;
-    c.numAttrs = 1;
-    return cuda_check(cudaLaunchKernelEx(&c, kernel, args...), "embedding launch");
+    return cuda_check(launch_pdl(kernel, ctas, dim3(threads), smem, st, args...), "embedding launch");
 }
 
 // Bytes of the widest access that fits addresses, strides and width.

@@ -284,16 +284,7 @@ scale_kernel(const __grid_constant__ Runs<N> a, const double* parts, int n_parts
 // Launched so that it may start when the kernel before has, and waits for it.
 template <typename... P, typename... A>
 int launch_behind(void (*kernel)(P...), unsigned ctas, cudaStream_t st, A... args) {
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(ctas);
-    c.blockDim = dim3(kThreads);
-    c.stream = st;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    c.attrs = &at;
-    c.numAttrs = 1;
-    return cuda_check(cudaLaunchKernelEx(&c, kernel, args...), "grad_norm launch");
+    return cuda_check(launch_pdl(kernel, dim3(ctas), dim3(kThreads), 0, st, args...), "grad_norm launch");
 }
 
 struct Call {

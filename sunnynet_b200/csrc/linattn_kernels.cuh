@@ -400,6 +400,7 @@ struct Pass {
 template <class S_, bool KEEP, int PN>
 __global__ void __launch_bounds__(S_::ST + 32, KEEP && S_::SNT > 8 ? 1 : 2)
 state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) {
+    pdl_trigger();
     typedef typename S_::T T;
     constexpr int NP = S_::NP, KD = S_::KD, VD = S_::VD, C = S_::C, NT = S_::SNT;
     // (three planes leave room for one stage, which is filled when every warp is done with it)
@@ -523,6 +524,7 @@ state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) 
 // neighbouring values of a state.
 template <int KD, int VD, int C, int PN>
 __global__ void __launch_bounds__(256) scan_kernel(const Job j, const Pass p0, const Pass p1) {
+    pdl_trigger();
     const Pass& p = blockIdx.y ? p1 : p0;
     const long long i = blockIdx.x * 256ll + threadIdx.x, bh = i / (KD * VD / 4);
     if (bh >= (long long)j.B * j.H) return;
@@ -622,6 +624,7 @@ out_kernel(const Job j, const bf16* kept, const Decays<S_::C>* decs, void* out_)
     Fetch<T, C, KD, S_::THREADS> lq, lk;
     Fetch<T, C, S_::VD, S_::THREADS> lv;
     lq.fetch(sq, q, j.qs.t, c0, end, j.dk, j.whole & 1);
+    pdl_wait();  // (the call's inputs were there before its first launch)
     load_kept<S_, NP>(ss, kept + (at.bh * j.chunks + at.c) * NP * KD * S_::VD);
     load_decays<C>(&dec, decs + at.bh * j.chunks + at.c);
     cp_async_commit();
@@ -759,6 +762,7 @@ __device__ __forceinline__ int column_sums(float* v) {
 template <class S_, int MIN>
 __global__ void __launch_bounds__(S_::THREADS, MIN)
 grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
+    pdl_trigger();
     typedef typename S_::T T;
     constexpr int NP = S_::NP, KD = S_::KD, VD = S_::VD, C = S_::C, LK = S_::LK, LV = S_::LV, NK = S_::NK, NV = S_::NV;
     constexpr int RB = S_::RB, CG = S_::CG;
@@ -801,6 +805,7 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
         Fetch<T, C, KD, S_::THREADS> lq, lk;
         Fetch<T, C, VD, S_::THREADS> lv, lo;
         lk.fetch(sk, k, j.ks.t, c0, end, j.dk, j.whole >> 1 & 1);
+        pdl_wait();
         load_kept<S_, 3>(ss, G.behind + kept);
         load_decays<C>(&dec, decs + at.bh * j.chunks + at.c);
         lv.fetch(sv, v, j.vs.t, c0, end, j.dv, j.whole >> 2 & 1);
@@ -1001,6 +1006,8 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
 template <typename T>
 __global__ void __launch_bounds__(256) fold_kernel(const float* x, const float* y, T* to_x, T* to_y,
                                                    int share, int d, long long n) {
+    pdl_trigger();
+    pdl_wait();
     const float* from = blockIdx.y ? y : x;
     T* to = blockIdx.y ? to_y : to_x;
     for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
@@ -1015,6 +1022,8 @@ __global__ void __launch_bounds__(256) fold_kernel(const float* x, const float* 
 // each part of the rows, the parts by a second launch of one.
 __global__ void __launch_bounds__(256) gate_kernel(const float* dg, const double* parts, double* to_parts,
                                                    float* out, long long n, int H, int count) {
+    pdl_trigger();
+    pdl_wait();
     __shared__ double s[8];
     for (int h = blockIdx.y; h < H; h += gridDim.y) {
         double x = 0.0;
@@ -1050,6 +1059,13 @@ struct Sizes {
 template <typename K>
 int allow(K* kernel, int bytes, const char* what) {
     return cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+}
+
+// A launch that may start while the one before ends, whose results it waits for
+// itself. (A call's first launch is an ordinary one: all that came before is done.)
+template <typename... P, typename... A>
+int behind(void (*kernel)(P...), dim3 ctas, int threads, int bytes, cudaStream_t st, A... args) {
+    return cuda_check(launch_pdl(kernel, ctas, dim3(threads), bytes, st, args...), "linear_attention launch");
 }
 
 // Whether each chunk's sum gets a CTA: where the heads alone leave SMs idle. (The
@@ -1110,6 +1126,7 @@ int states(const Job& j, const Pass& p0, const Pass& p1, bool both, Decays<S_::C
         auto* sum = state_kernel<S_, false, PN>;
         SN_TRY(allow(sum, Sizes<S_>::sum, "linear_attention"));
         sum<<<dim3((unsigned)(bh * j.chunks), 1 + both), threads, Sizes<S_>::sum, st>>>(j, p0, p1, dec);
+        // (not launched early: where CTAs of the sums leave first, it would crowd, 10 us instead of 5)
         scan_kernel<S_::KD, S_::VD, S_::C, PN>
             <<<dim3((unsigned)((bh * SIZE / 4 + 255) / 256), 1 + both), 256, 0, st>>>(j, p0, p1);
     } else {
@@ -1150,8 +1167,7 @@ int forward_as(Job j, const float* first, void* out, float* state_out, char* ws,
     static_assert(bytes <= 220 * 1024, "shared memory of a CTA");
     auto* kernel = out_kernel<S_, bytes <= 40 * 1024 ? 5 : bytes <= 72 * 1024 ? 3 : bytes <= 96 * 1024 ? 2 : 1>;
     SN_TRY(allow(kernel, bytes, "linear_attention"));
-    kernel<<<(unsigned)((long long)j.B * j.H * j.chunks), S_::THREADS, bytes, st>>>(j, p.kept, dec, out);
-    return cuda_check(cudaGetLastError(), "linear_attention launch");
+    return behind(kernel, dim3((unsigned)((long long)j.B * j.H * j.chunks)), S_::THREADS, bytes, st, j, p.kept, dec, out);
 }
 
 template <class S_>
@@ -1187,20 +1203,20 @@ int backward_as(Job j, const float* first, const Wanted& g, char* ws, long long 
     auto* kernel = grad_kernel<S_, bytes <= 66 * 1024 ? 3 : bytes <= 102 * 1024 ? 2 : 1>;
     SN_TRY(allow(kernel, bytes, "linear_attention_bwd"));
     if (j.chunks)
-        kernel<<<(unsigned)((long long)j.B * j.H * j.chunks), S_::THREADS, bytes, st>>>(j, G, dec);
+        SN_TRY(behind(kernel, dim3((unsigned)((long long)j.B * j.H * j.chunks)), S_::THREADS, bytes, st, j, G, dec));
     const long long rows = (long long)j.B * j.T;
     if (j.share > 1 && rows) {
         const long long n = rows * (j.H / j.share) * j.dk;
-        fold_kernel<T><<<dim3((unsigned)std::min((n + 255) / 256, 8ll * 148), 2), 256, 0, st>>>(
-            G.dq32, G.dk32, static_cast<T*>(g.dq), static_cast<T*>(g.dk), j.share, j.dk, n);
+        SN_TRY(behind(fold_kernel<T>, dim3((unsigned)std::min((n + 255) / 256, 8ll * 148), 2), 256, 0, st, G.dq32, G.dk32,
+                      static_cast<T*>(g.dq), static_cast<T*>(g.dk), j.share, j.dk, n));
     }
     if (g.dg && g.gates_alike) {
         double* parts = reinterpret_cast<double*>(ws + s.gates);
         const unsigned ys = (unsigned)std::min(j.H, 65535);
-        gate_kernel<<<dim3(kGateParts, ys), 256, 0, st>>>(G.dg, nullptr, parts, nullptr, rows, j.H, 0);
-        gate_kernel<<<dim3(1, ys), 256, 0, st>>>(nullptr, parts, nullptr, g.dg, 0, j.H, kGateParts);
+        SN_TRY(behind(gate_kernel, dim3(kGateParts, ys), 256, 0, st, G.dg, nullptr, parts, nullptr, rows, j.H, 0));
+        SN_TRY(behind(gate_kernel, dim3(1, ys), 256, 0, st, nullptr, parts, nullptr, g.dg, 0, j.H, kGateParts));
     }
-    return cuda_check(cudaGetLastError(), "linear_attention_bwd launch");
+    return SN_OK;
 }
 
 // The widths that the keys and the values are laid out in, and the tokens of a
