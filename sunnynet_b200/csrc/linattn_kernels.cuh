@@ -32,13 +32,12 @@ __device__ __forceinline__ void clear(float (*x)[4]) {
 // NT column tiles (values `cb` on of y). x w in fp32, in three planes: what comes of
 // it is an fp32 result. (The planes of a bf16 x formed by packed bf16 instructions,
 // four in place of three, are a third of the work, but the fourth product of each made
-// the whole 8% slower.)
+// the whole 8% slower.) The chunk has `tokens`; a block of 16 with none is left out.
 template <int NP, int NT, int C>
 __device__ __forceinline__ void add_outer(float (*S)[4], const Tile& x, const Tile& y, const float* w,
-                                          float scale, int row, int cb) {
+                                          float scale, int row, int cb, int tokens) {
     const int q = lane_id() & 3;
-#pragma unroll
-    for (int kt = 0; kt < C / 16; ++kt) {
+    const auto block = [&](int kt) {
         uint32_t xr[NP][4], a[3][4];
 #pragma unroll
         for (int p = 0; p < NP; ++p) x.a_t(xr[p], kt * 16, row, p);
@@ -59,6 +58,13 @@ __device__ __forceinline__ void add_outer(float (*S)[4], const Tile& x, const Ti
             for (int p = 0; p < NP; ++p) y.b_t(b[p], kt * 16, cb + n * 16, p);
             mma2<3, NP>(S + 2 * n, a, b);
         }
+    };
+    if (tokens > C - 16) {
+#pragma unroll
+        for (int kt = 0; kt < C / 16; ++kt) block(kt);
+    } else {
+#pragma unroll 1
+        for (int kt = 0; kt * 16 < tokens; ++kt) block(kt);
     }
 }
 
@@ -493,7 +499,7 @@ state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) 
         float sum[NT][4];
         clear<NT>(sum);
         add_outer<NP, NT, C>(sum, tile(from, S_::LK, C * S_::LK), tile(from + S_::KT, S_::LV, C * S_::LV),
-                             p.back ? dec.from_start : dec.to_end, p.back ? j.scale : 1.0f, row, 0);
+                             p.back ? dec.from_start : dec.to_end, p.back ? j.scale : 1.0f, row, 0, end - chunk(i) * C);
         // The chunk's sum is added here, not in the matrix instruction, which cuts its sums off: over a
         // sequence that leaned by 2^-24 of the state a step.
         const float f = dec.whole;
@@ -618,6 +624,7 @@ out_kernel(const Job j, const bf16* kept, const Decays<S_::C>* decs, void* out_)
     if (c0 >= end) return zero_rows(out, ot, c0, min(c0 + C, j.T), j.dv);
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
     const int rb = warp % S_::RB, cb = warp / S_::RB * NT * 8;
+    const bool on = rb * 16 < end - c0;  // the warp's block holds tokens
     const T* q = head_of<T>(j.q, j.qs, at.b, at.h / j.share);
     const T* k = head_of<T>(j.k, j.ks, at.b, at.h / j.share);
     const T* v = head_of<T>(j.v, j.vs, at.b, at.h);
@@ -653,7 +660,6 @@ out_kernel(const Job j, const bf16* kept, const Decays<S_::C>* decs, void* out_)
     const float r0 = (rb ? dec.between(t, rb * 16 - 1) : dec.from_start[t]) * j.scale;
     const float r1 = (rb ? dec.between(t + 8, rb * 16 - 1) : dec.from_start[t + 8]) * j.scale;
     const auto before = [&] {
-        clear<NT>(O);
         product<NP, NP, KD, NT, true>(O, tq, rb * 16, ts, cb);
         if (rb) {
             const float begin = dec.from_start[rb * 16 - 1];
@@ -676,17 +682,21 @@ out_kernel(const Job j, const bf16* kept, const Decays<S_::C>* decs, void* out_)
         else
             weighted<NP, NP, 1, NT>(O, P, tv, cb, rb, rb, rb + 1);
     };
-    before();
+    clear<NT>(O);
+    if (on) before();
     cp_async_wait_all();
     __syncthreads();
-    chunk(false);
-    // a value of v that is not finite reaches every row of its block (times zero, in those before it)
-    float sum = 0.0f;
+    if (on) {
+        chunk(false);
+        // a value of v that is not finite reaches every row of its block (times zero, in those before it)
+        float sum = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) sum = fmaf(O[n][0], 0.0f, fmaf(O[n][1], 0.0f, sum));
-    if (__any_sync(0xffffffffu, sum != 0.0f)) {
-        before();
-        chunk(true);
+        for (int n = 0; n < NT; ++n) sum = fmaf(O[n][0], 0.0f, fmaf(O[n][1], 0.0f, sum));
+        if (__any_sync(0xffffffffu, sum != 0.0f)) {
+            clear<NT>(O);
+            before();
+            chunk(true);
+        }
     }
     if constexpr (S_::VD <= KD) {  // by way of these rows' queries, which are done with
         if constexpr (S_::CG > 1) named_bar_sync(rb + 1, S_::CG * 32);
@@ -794,6 +804,10 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
     }
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
     const int rb = warp % RB, cg = warp / RB, ck = cg * NK * 8, cv = cg * NV * 8;
+    const int live = min(RB, (end - c0 + 15) / 16);  // blocks that hold tokens
+    const bool on = rb < live;
+    // (in two and three parts the loops run to the chunk's end: with the other bound 6% slower, and 1% faster in one)
+    const int blocks = NP == 1 ? live : RB;
     const Tile tq = tile(sq, LK, C * LK), tk = tile(sk, LK, C * LK), tv = tile(sv, LV, C * LV),
                to = tile(so, LV, C * LV), ts = tile(ss, LV, S_::STATE);
     const long long kept = (at.bh * j.chunks + at.c) * 3 * KD * VD;
@@ -842,67 +856,71 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
         const float b0 = dec.between(r, t), b1 = dec.between(r, t + 8), behind = dec.to_end[r];
         float V[NV][4], K[NK][4], across[2] = {0.0f, 0.0f};
         clear<NV>(V);
-        product<NP, NP, KD, NV, true>(V, tk, rb * 16, ts, cv);
-        scale_rows<NV>(V, behind, behind);
         clear<NK>(K);
-        product<NP, 3, VD, NK, false>(K, tv, rb * 16, ts, ck);
-        scale_rows<NK>(K, behind, behind);
-        row_dots<NP, NK>(K, sk, LK, C * LK, rb * 16, ck, part);
-        if ((l & 3) == 0) dk_part[cg][t] = part[0] * b0, dk_part[cg][t + 8] = part[1] * b1;
+        if (on) {
+            product<NP, NP, KD, NV, true>(V, tk, rb * 16, ts, cv);
+            scale_rows<NV>(V, behind, behind);
+            product<NP, 3, VD, NK, false>(K, tv, rb * 16, ts, ck);
+            scale_rows<NK>(K, behind, behind);
+            row_dots<NP, NK>(K, sk, LK, C * LK, rb * 16, ck, part);
+            if ((l & 3) == 0) dk_part[cg][t] = part[0] * b0, dk_part[cg][t + 8] = part[1] * b1;
+        }
         cp_async_wait_all();  // queries and the gradient of the outputs
         for (int u = r + 1 + l; u < C; u += 32) *column(u) = dec.between(u, r) * j.scale;
         __syncthreads();
-        for (int jb = (rb + 1) / NB * NB; jb < RB; jb += NB) {
-            float P[2 * NB][4], Q[2 * NB][4], down[4 * NB];
-            scores<NP, KD, NB, FINE>(P, tk, rb * 16, tq, jb, rb + 1, RB);
-            scores<NP, VD, NB, FINE>(Q, tv, rb * 16, to, jb, rb + 1, RB);
+        if (on) {
+            for (int jb = (rb + 1) / NB * NB; jb < blocks; jb += NB) {
+                float P[2 * NB][4], Q[2 * NB][4], down[4 * NB];
+                scores<NP, KD, NB, FINE>(P, tk, rb * 16, tq, jb, rb + 1, RB);
+                scores<NP, VD, NB, FINE>(Q, tv, rb * 16, to, jb, rb + 1, RB);
 #pragma unroll
-            for (int n = 0; n < 2 * NB; ++n) {
-                const int u = jb * 16 + n * 8 + (l & 3) * 2;
-                const float2 f = *reinterpret_cast<const float2*>(column(u));
-                const bool in = jb + n / 2 > rb;  // (the factors of other blocks are not there)
-                const float x0 = P[n][0] * Q[n][0], x1 = P[n][1] * Q[n][1], x2 = P[n][2] * Q[n][2],
-                            x3 = P[n][3] * Q[n][3];
-                down[2 * n] = in ? (x0 * b0 + x2 * b1) * f.x : 0.0f;
-                down[2 * n + 1] = in ? (x1 * b0 + x3 * b1) * f.y : 0.0f;
-                across[0] += in ? x0 * f.x + x1 * f.y : 0.0f;
-                across[1] += in ? x2 * f.x + x3 * f.y : 0.0f;
-                P[n][0] *= f.x, P[n][1] *= f.y, P[n][2] *= f.x, P[n][3] *= f.y;
-                Q[n][0] *= f.x, Q[n][1] *= f.y, Q[n][2] *= f.x, Q[n][3] *= f.y;
+                for (int n = 0; n < 2 * NB; ++n) {
+                    const int u = jb * 16 + n * 8 + (l & 3) * 2;
+                    const float2 f = *reinterpret_cast<const float2*>(column(u));
+                    const bool in = jb + n / 2 > rb;  // (the factors of other blocks are not there)
+                    const float x0 = P[n][0] * Q[n][0], x1 = P[n][1] * Q[n][1], x2 = P[n][2] * Q[n][2],
+                                x3 = P[n][3] * Q[n][3];
+                    down[2 * n] = in ? (x0 * b0 + x2 * b1) * f.x : 0.0f;
+                    down[2 * n + 1] = in ? (x1 * b0 + x3 * b1) * f.y : 0.0f;
+                    across[0] += in ? x0 * f.x + x1 * f.y : 0.0f;
+                    across[1] += in ? x2 * f.x + x3 * f.y : 0.0f;
+                    P[n][0] *= f.x, P[n][1] *= f.y, P[n][2] *= f.x, P[n][3] *= f.y;
+                    Q[n][0] *= f.x, Q[n][1] *= f.y, Q[n][2] *= f.x, Q[n][3] *= f.y;
+                }
+                const int which = column_sums<4 * NB>(down);
+                if (cg == 0) col_part[rb][jb * 16 + which / 2 * 8 + (l & 3) * 2 + which % 2] = down[0];
+                weighted<NP, NP, NB, NV>(V, P, to, cv, jb, rb + 1, RB);
+                weighted<NP, NP, NB, NK>(K, Q, tq, ck, jb, rb + 1, RB);
             }
-            const int which = column_sums<4 * NB>(down);
-            if (cg == 0) col_part[rb][jb * 16 + which / 2 * 8 + (l & 3) * 2 + which % 2] = down[0];
-            weighted<NP, NP, NB, NV>(V, P, to, cv, jb, rb + 1, RB);
-            weighted<NP, NP, NB, NK>(K, Q, tq, ck, jb, rb + 1, RB);
-        }
-        scale_rows<NV>(V, b0, b1);
-        scale_rows<NK>(K, b0, b1);
-        across[0] *= b0, across[1] *= b1;
-        float P[2][4], Q[2][4], down[4] = {};
-        scores<NP, KD, 1, FINE>(P, tk, rb * 16, tq, rb, rb, rb + 1);
-        scores<NP, VD, 1, FINE>(Q, tv, rb * 16, to, rb, rb, rb + 1);
+            scale_rows<NV>(V, b0, b1);
+            scale_rows<NK>(K, b0, b1);
+            across[0] *= b0, across[1] *= b1;
+            float P[2][4], Q[2][4], down[4] = {};
+            scores<NP, KD, 1, FINE>(P, tk, rb * 16, tq, rb, rb, rb + 1);
+            scores<NP, VD, 1, FINE>(Q, tv, rb * 16, to, rb, rb, rb + 1);
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int s = t + (i >> 1) * 8, u = rb * 16 + n * 8 + (l & 3) * 2 + (i & 1);
-                const float w = dec.between(u, s) * j.scale, p = P[n][i] * w;
-                const float a = u > s ? p * Q[n][i] : 0.0f;
-                P[n][i] = u >= s ? p : 0.0f;
-                Q[n][i] = u >= s ? Q[n][i] * w : 0.0f;
-                across[i >> 1] += a;
-                down[2 * n + (i & 1)] += a;
+                for (int i = 0; i < 4; ++i) {
+                    const int s = t + (i >> 1) * 8, u = rb * 16 + n * 8 + (l & 3) * 2 + (i & 1);
+                    const float w = dec.between(u, s) * j.scale, p = P[n][i] * w;
+                    const float a = u > s ? p * Q[n][i] : 0.0f;
+                    P[n][i] = u >= s ? p : 0.0f;
+                    Q[n][i] = u >= s ? Q[n][i] * w : 0.0f;
+                    across[i >> 1] += a;
+                    down[2 * n + (i & 1)] += a;
+                }
+            const int which = column_sums<4>(down);
+            if (cg == 0) col_part[rb][rb * 16 + which / 2 * 8 + (l & 3) * 2 + which % 2] = down[0];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                across[i] += __shfl_xor_sync(0xffffffffu, across[i], 1);
+                across[i] += __shfl_xor_sync(0xffffffffu, across[i], 2);
             }
-        const int which = column_sums<4>(down);
-        if (cg == 0) col_part[rb][rb * 16 + which / 2 * 8 + (l & 3) * 2 + which % 2] = down[0];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            across[i] += __shfl_xor_sync(0xffffffffu, across[i], 1);
-            across[i] += __shfl_xor_sync(0xffffffffu, across[i], 2);
+            if (cg == 0 && (l & 3) == 0) row_part[t] = across[0], row_part[t + 8] = across[1];
+            weighted<NP, NP, 1, NV>(V, P, to, cv, rb, rb, rb + 1);
+            weighted<NP, NP, 1, NK>(K, Q, tq, ck, rb, rb, rb + 1);
         }
-        if (cg == 0 && (l & 3) == 0) row_part[t] = across[0], row_part[t + 8] = across[1];
-        weighted<NP, NP, 1, NV>(V, P, to, cv, rb, rb, rb + 1);
-        weighted<NP, NP, 1, NK>(K, Q, tq, ck, rb, rb, rb + 1);
         // <R, S>, and then their place is free
         float dot = 0.0f;
         if (dg) {
@@ -942,23 +960,25 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
         // rows u, columns s <= u, as the outputs
         float X[NK][4], P[2][4];
         clear<NK>(X);
-        product<NP, 3, VD, NK, false>(X, to, rb * 16, ts, ck);
-        const float begin = rb ? dec.from_start[rb * 16 - 1] : 1.0f;
-        scale_rows<NK>(X, begin, begin);
-        const float r0 = (rb ? dec.between(t, rb * 16 - 1) : dec.from_start[t]) * j.scale;
-        const float r1 = (rb ? dec.between(t + 8, rb * 16 - 1) : dec.from_start[t + 8]) * j.scale;
-        row_dots<NP, NK>(X, sq, LK, C * LK, rb * 16, ck, part);
-        if ((l & 3) == 0) dq_part[cg][t] = part[0] * r0, dq_part[cg][t + 8] = part[1] * r1;
-        for (int jb = 0; jb < rb; jb += NB) {
-            float Q[2 * NB][4];
-            scores<NP, VD, NB>(Q, to, rb * 16, tv, jb, 0, rb);
-            scale_columns<NB>(Q, column, jb);
-            weighted<NP, NP, NB, NK>(X, Q, tk, ck, jb, 0, rb);
+        if (on) {
+            product<NP, 3, VD, NK, false>(X, to, rb * 16, ts, ck);
+            const float begin = rb ? dec.from_start[rb * 16 - 1] : 1.0f;
+            scale_rows<NK>(X, begin, begin);
+            const float r0 = (rb ? dec.between(t, rb * 16 - 1) : dec.from_start[t]) * j.scale;
+            const float r1 = (rb ? dec.between(t + 8, rb * 16 - 1) : dec.from_start[t + 8]) * j.scale;
+            row_dots<NP, NK>(X, sq, LK, C * LK, rb * 16, ck, part);
+            if ((l & 3) == 0) dq_part[cg][t] = part[0] * r0, dq_part[cg][t + 8] = part[1] * r1;
+            for (int jb = 0; jb < rb; jb += NB) {
+                float Q[2 * NB][4];
+                scores<NP, VD, NB>(Q, to, rb * 16, tv, jb, 0, rb);
+                scale_columns<NB>(Q, column, jb);
+                weighted<NP, NP, NB, NK>(X, Q, tk, ck, jb, 0, rb);
+            }
+            scale_rows<NK>(X, r0, r1);
+            scores<NP, VD, 1>(P, to, rb * 16, tv, rb, rb, rb + 1);
+            near_decays<C>(P, dec, rb, j.scale);
+            weighted<NP, NP, 1, NK>(X, P, tk, ck, rb, rb, rb + 1);
         }
-        scale_rows<NK>(X, r0, r1);
-        scores<NP, VD, 1>(P, to, rb * 16, tv, rb, rb, rb + 1);
-        near_decays<C>(P, dec, rb, j.scale);
-        weighted<NP, NP, 1, NK>(X, P, tk, ck, rb, rb, rb + 1);
         __syncthreads();
         store_head(X, G.dq, G.dq32);
     }
@@ -972,19 +992,23 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
 #pragma unroll
         for (int i = M - 1; i >= 0; --i) {
             const int u = l * M + i;
-            float x = -row_part[u];
+            if (u / 16 < live) {
+                float x = -row_part[u];
 #pragma unroll
-            for (int r = 0; r < RB; ++r)
-                if (r <= u / 16) x += col_part[r][u];
+                for (int r = 0; r < RB; ++r)
+                    if (r <= u / 16) x += col_part[r][u];
 #pragma unroll
-            for (int r = 0; r < CG; ++r) x += dq_part[r][u];
-            behind[i] = b += x;
+                for (int r = 0; r < CG; ++r) x += dq_part[r][u];
+                b += x;
+            }
+            behind[i] = b;
         }
 #pragma unroll
         for (int i = 0; i < M; ++i) {
             ahead[i] = a;
+            if ((l * M + i) / 16 < live)
 #pragma unroll
-            for (int r = 0; r < CG; ++r) a += dk_part[r][l * M + i];
+                for (int r = 0; r < CG; ++r) a += dk_part[r][l * M + i];
         }
         float bs = b, as = a;
 #pragma unroll
