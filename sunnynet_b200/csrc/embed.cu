@@ -12,11 +12,12 @@
 // same bits every time, no atomics on values. Up to kNear tokens are sorted by one
 // cluster of eight CTAs in one launch (5003 tokens, two passes: 11 us; four launches
 // of many CTAs took 12, and 10 more of the host's time; 32768 tokens 28 us against
-// 18), more of them by two launches a pass: the counts of every tile, then ranks and places. Bound by HBM
-// (dout read, dW written once) from some ten thousand tokens on, and by latency
-// below. While they sort, further CTAs of the same launches fill dW with zeros,
+// 18), more of them by two launches a pass: the counts of every tile, then ranks and
+// places. Bound by HBM (dout read, dW written once) from some ten thousand tokens on,
+// and by latency below. While they sort, further CTAs of the same launches fill dW with zeros,
 // which costs nothing then: most rows of a vocabulary occur in no batch, and those
-// that do are overwritten.
+// that do are overwritten. 32768 tokens of 32000 x 768 in bf16, gradient and rows: 66 us,
+// the sums 19 of them (50 MB in), the rest of the sort's launches and the rows.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -21,7 +21,7 @@
 // (dg sums, of what lies outside a chunk, only what passes token t's gate: the
 // shorter form by differences q.dq - k.dk from the sequence's end loses all digits over
 // long sequences. The chunk's own pairs are summed by rows and columns, u >= t less
-// s >= t: 2^-17 of their sum.)
+// s >= t: 2^-16 of their sum at most.)
 //
 // All products are m16n8k16 matrix instructions on bf16 with fp32 sums. bf16
 // values are taken as they are, float16 ones as the sum of two bf16 and float32
@@ -55,7 +55,8 @@ namespace {
 
 // -------------------------------------------------------------- single token
 // A CTA for each sequence and head: its state goes through once. Lanes stand
-// side by side along a row of the state, so that every access is one run.
+// side by side along a row of the state, so that every access is one run. Bound by HBM: 256
+// sequences x 12 heads of 64 take 15.3 us, 101 MB at 6.6 TB/s.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(128)
 step_kernel(const T* q_, const T* k_, const T* v_, Strides qs, Strides ks, Strides vs, const float* g,
