@@ -16,8 +16,8 @@
 // places. Bound by HBM (dout read, dW written once) from some ten thousand tokens on,
 // and by latency below. While they sort, further CTAs of the same launches fill dW with zeros,
 // which costs nothing then: most rows of a vocabulary occur in no batch, and those
-// that do are overwritten. 32768 tokens of 32000 x 768 in bf16, gradient and rows: 66 us,
-// the sums 19 of them (50 MB in), the rest of the sort's launches and the rows.
+// that do are overwritten. 32768 tokens of 32000 x 768 in bf16, rows 14 us, the sort
+// 18, the sums 17 and the joins of rows of many tokens 7.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -403,10 +403,10 @@ struct Pass {
 // each chunk has a CTA, which leaves its sum and factor. The decays of the next
 // chunk are the work of one more warp, and its tiles are on their way meanwhile. PN:
 // planes of the kept states. A warp has 16 rows of the state in registers, all its columns.
-// 16 x 2048 x 12 of 64 in bf16: 69 us, and both passes of a gradient 116 (3.8 TB/s; matrix
+// 16 x 2048 x 12 of 64 in bf16: 62 us, and both passes of a gradient 116 (3.8 TB/s; matrix
 // instructions 37% of the time): a chunk's sum waits for its weighted values, which take
 // as long to form in three parts as to multiply, and the next chunk waits for it. A state's
-// rows on two CTAs, which would fill the SMs more evenly, took 68 and 164.
+// rows on two CTAs, which would fill the SMs more evenly, gained nothing and took 164.
 template <class S_, bool KEEP, int PN>
 __global__ void __launch_bounds__(S_::ST + 32, KEEP && S_::SNT > 8 ? 1 : 2)
 state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) {
@@ -718,7 +718,7 @@ out_kernel(const Job j, const bf16* kept, const Decays<S_::C>* decs, void* out_)
 // A CTA for each chunk again. First by rows s (dk, dv, with the gradient behind the chunk),
 // then by rows t (dq, with the state before it), so that every product finds its left
 // side in the warp's registers; the scores of do and v are computed for both. 16 x 2048 x
-// 12 of 64 in bf16: 217 us, 643 MB at 2.8 TB/s, matrix instructions 31% of the time: 168
+// 12 of 64 in bf16: 221 us, 643 MB at 2.9 TB/s, matrix instructions 31% of the time: 168
 // registers and 66 KB leave three CTAs of four warps on an SM, which wait for their states,
 // for ldmatrix and for one another. 3 x 1001 x 6 of 40 and 72 in fp32: 75 us, two waves of
 // one CTA an SM.
