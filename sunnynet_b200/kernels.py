@@ -370,8 +370,9 @@ def linear_attention(q, k, v, log_decay, state=None, lengths=None, scale=None):
     state as it is, and their outputs are zeros. A log decay of minus infinity
     forgets what came before; positive ones let a state grow, and sums of them beyond
     88 over a stretch of 64 tokens leave float32's range, whatever follows. What is not
-    finite in v leaves what it reaches not finite, and the outputs before it as they
-    are. scale: dk ** -0.5. Out has v's type, states are
+    finite in q, k or v leaves what it reaches not finite, and the outputs before it as
+    they are (gradients of the 16 tokens around it may not be finite either).
+    scale: dk ** -0.5. Out has v's type, states are
     float32. Differentiable once in q, k, v, log_decay and state. Results in float32
     (states and the gradients of decays among them) have float32's accuracy; on the
     way to outputs of 16 bits, scores and states are rounded to bf16, or to two parts of
