@@ -235,6 +235,25 @@ def test_values_without_finite_numbers_stay_in_their_place(kernels):
     assert not out[0, :130].isnan().any() and not out[0, :, 0].isnan().any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("name", ["q", "k", "v"])
+def test_what_is_not_finite_reaches_nothing_before(kernels, name, dtype):
+    """The outputs of the tokens before are the definition's, what it reaches is not finite."""
+    for value in (float("nan"), float("inf")):
+        x = make(1, 150, 2, 2, 64, 64, dtype, state=False)
+        (want, _), (most, _) = truth(x, 0.3)
+        x[name][0, 73, 1, 5] = value
+        out, S = kernels.linear_attention(**x, scale=0.3)
+        near(out[:, :73], want[:, :73], most[:, :73], dtype)
+        near(out[:, :, 0], want[:, :, 0], most[:, :, 0], dtype)
+        if name == "q":
+            assert not out[0, 73, 1].isfinite().any()
+            near(out[:, 74:], want[:, 74:], most[:, 74:], dtype)
+        else:
+            at = (1, 5) if name == "v" else (1,)
+            assert not (out[0, 73:, *at].isfinite().any() or S[0, 1, 5].isfinite().all())
+
+
 def test_layouts(kernels):
     """Views of one projection, of transposed tensors, at odd addresses, broadcast ones."""
     for dtype in DTYPES:
