@@ -43,10 +43,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 __device__ __forceinline__ float low(uint32_t x) { return __uint_as_float(x << 16); }
 __device__ __forceinline__ float high(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
-// What two values have beyond their bf16 halves.
-__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t hi) {
-    return pack2(a - low(hi), b - high(hi));
-}
 
 __device__ __forceinline__ void ldsm4(uint32_t* r, uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"

@@ -731,7 +731,7 @@ struct Grads {
     float* dg;           // (B, T, H), or null
 };
 
-// A row of 16-bit pairs (or two planes of them) times a block of products: each
+// A row of 16-bit pairs (or more planes of them) times a block of products: each
 // lane's part of the sums over the columns, for its rows g and g + 8.
 template <int NP, int NT>
 __device__ __forceinline__ void row_dots(const float (*x)[4], const bf16* tile, int ld, int step, int r,
