@@ -629,7 +629,11 @@ out_kernel(const Job j, const bf16* kept, const Decays<S_::C>* decs, void* out_)
     const int end = tokens_of(j, at.b), c0 = at.c * C;
     const long long ot = (long long)j.H * j.dv;
     T* out = static_cast<T*>(out_) + (long long)at.b * j.T * ot + (long long)at.h * j.dv;
-    if (c0 >= end) return zero_rows(out, ot, c0, min(c0 + C, j.T), j.dv);
+    if (c0 >= end) {
+        zero_rows(out, ot, c0, min(c0 + C, j.T), j.dv);
+        pdl_wait();  // (where no sequence has a token, all CTAs leave here: not before the states are there)
+        return;
+    }
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;
     const int rb = warp % S_::RB, cb = warp / S_::RB * NT * 8;
     const bool on = rb * 16 < end - c0;  // the warp's block holds tokens
@@ -815,6 +819,7 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
             zero_rows(static_cast<T*>(G.dk) + k0, kt, c0, c1, j.dk);
         }
         if (dg) zero_rows(dg, j.H, c0, c1, 1);
+        pdl_wait();  // (as in out_kernel)
         return;
     }
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31;

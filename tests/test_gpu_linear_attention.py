@@ -451,3 +451,22 @@ def test_offsets_beyond_32_bits(kernels, dtype):
         wide.copy_(x[n])
         got = kernels.linear_attention(**{**x, n: wide})
         assert all(torch.equal(a, b) for a, b in zip(got, base)), n
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,dk,dv", [(64, 16, 128, 128), (2, 3, 64, 64)])
+def test_batches_without_a_token(kernels, B, H, dk, dv, dtype):
+    """Every length zero: outputs and gradients are zeros, the states pass through, and what is enqueued
+    directly behind a call finds them, and may take its workspace."""
+    x = make(B, 130, H, H, dk, dv, dtype, "head", lengths=[0] * B)
+    ends = (torch.ones(B, 130, H, dv, device="cuda", dtype=dtype), torch.randn(B, H, dk, dv, device="cuda"))
+    for _ in range(3):
+        out, S = kernels.linear_attention(**x)
+        after = S.clone()
+        torch.full((1 << 26,), 7.0, device="cuda")
+        assert torch.equal(after, x["state"]) and torch.equal(S, x["state"]) and not out.any()
+        got = gradients(kernels, x, 1.0, ends)
+        after = got[-1].clone()
+        torch.full((1 << 26,), 7.0, device="cuda")
+        assert torch.equal(after, ends[1]) and torch.equal(got[-1], ends[1])
+        assert not any(g.any() for g in got[2:6])
