@@ -78,8 +78,17 @@ step_kernel(const T* q_, const T* k_, const T* v_, Strides qs, Strides ks, Strid
         sq[tid] = to_f(q[tid]) * scale;
         sk[tid] = to_f(k[tid]);
     }
-    const double gate = (double)g[b * gb + h * gh] * 1.4426950408889634074;
-    const float f = exp2_of(gate < -256.0 ? -256.0f : (float)gate);
+    // exp(g) in two parts: a slow decay's factor is the same at every token, and what it is off adds up over
+    // 1 / (1 - f) of them (4096 tokens of decays about 2^-11: 3e-4 by ex2.approx, 8e-6 so: the states' roundings)
+    const float gate = g[b * gb + h * gh];
+    float f, rest = 0.0f;
+    if (fabsf(gate) < 0.5f) {
+        const float e = expm1f(gate);
+        f = 1.0f + e;
+        rest = e - (f - 1.0f);  // (exactly what the sum lost)
+    } else {
+        f = expf(gate);
+    }
     float x[VEC], o[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
@@ -108,7 +117,7 @@ step_kernel(const T* q_, const T* k_, const T* v_, Strides qs, Strides ks, Strid
                     const float kk = sk[r + u * rows], qq = sq[r + u * rows];
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        s[u][i] = fmaf(kk, x[i], f * s[u][i]);
+                        s[u][i] = fmaf(f, s[u][i], fmaf(rest, s[u][i], kk * x[i]));
                         o[i] = fmaf(qq, s[u][i], o[i]);
                     }
                     float* at = S + (r + u * rows) * dv + c * VEC;

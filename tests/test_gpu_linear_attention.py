@@ -21,6 +21,8 @@ parts' own). The store adds a half step of the stored type.
 """
 from __future__ import annotations
 
+import math
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -470,3 +472,43 @@ def test_batches_without_a_token(kernels, B, H, dk, dv, dtype):
         torch.full((1 << 26,), 7.0, device="cuda")
         assert torch.equal(after, ends[1]) and torch.equal(got[-1], ends[1])
         assert not any(g.any() for g in got[2:6])
+
+
+def test_thousands_of_single_tokens(kernels):
+    """Slow decays, one token after the other: an error of the factor, the same each time, would add up. One ulp of
+    exp(g) - 1 (2^-33 for these g) makes 2^-21 of 4096 tokens. Roundings of a state, at most 2^-24 of it each and
+    two a token, fall either way: 2^-24 sqrt(2 / 3) sqrt(4096) as a standard deviation, 2^-15.2 for eight of them."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=gen)  # noqa: E731
+    H, d, n, bound = 64, 16, 4096, 2.0 ** -15.2 + 2.0 ** -21
+    g = -(2.0 ** -11) * (1 + torch.rand(H, device="cuda", generator=gen))
+    f = g.double().exp()[:, None, None]
+    start = r(1, H, d, d)
+    q, k, v = r(n, 1, H, d), r(n, 1, H, d), r(n, 1, H, d)
+    alone, S, want, most = start.clone(), start.clone(), start.double(), start.double().abs()
+    for t in range(n):
+        kernels.linear_attention_step(q[t], torch.zeros_like(k[t]), v[t], g, alone)
+        kernels.linear_attention_step(q[t], k[t], v[t], g, S)
+        want = want * f + k[t].double()[..., None] * v[t].double()[:, :, None]
+        most = torch.maximum(most, want.abs())
+    gone = start.double() * (n * g.double()).exp()[:, None, None]
+    assert float(((alone.double() - gone) / gone).abs().max()) <= bound
+    assert float(((S.double() - want).abs() / most).max()) <= bound
+    # a prompt of the same tokens ends in the same state
+    _, end = kernels.linear_attention(*(x.transpose(0, 1) for x in (q, k, v)), g, start)
+    assert float(((end.double() - want).abs() / most).max()) <= bound
+
+
+@pytest.mark.parametrize("g", [-0.0, -2.0 ** -30, -0.1, -0.49, -0.5, -0.51, -3.0, -20.0, -87.0, 2.0 ** -20, 0.3, 0.5, 0.7, 20.0])
+def test_the_factor_of_a_single_token(kernels, g):
+    """A token that writes nothing leaves exp(g) S: the state's rounding (2^-150 below the normal numbers), and the
+    factor's, by CUDA's bounds of its functions: an ulp of exp(g) - 1 (2^-23 of that at most) near zero, two of
+    exp(g) elsewhere."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    S = torch.randn(1, 2, 64, 64, device="cuda", generator=gen)
+    x = torch.ones(1, 2, 64, device="cuda")
+    decay = torch.full((2,), g, device="cuda")
+    want = S.double() * decay.double().exp()[:, None, None]
+    kernels.linear_attention_step(x, x * 0, x, decay, S)
+    far = 2.0 ** -23 * abs(math.expm1(g)) / math.exp(g) if abs(g) < 0.5 else 2.0 ** -22
+    assert ((S.double() - want).abs() <= (2.0 ** -24 + 2.0 ** -40 + far) * want.abs() + 2.0 ** -150).all()
