@@ -234,8 +234,9 @@ int32_t     sn_abi_rwkv7_dims(const SnAbiRwkv7* m, int32_t* dims8); /* vocab,D,H
 #define SN_F16   2
 
 /* For a caller that knows where its arrays lie (a tensor library): the calling
- * thread's next call of this section takes every array to be memory of that GPU
- * and does not ask the driver for each (0.3 us of the host's time). */
+ * thread's next call of this section that is given arrays takes every one to be
+ * memory of that GPU and does not ask the driver for each (0.3 us of the host's
+ * time). It counts for that call alone, also where it has nothing to do or refuses. */
 void      sn_abi_arrays_on(int32_t device);
 
 /* Layer norm of `rows` rows of D values (1 to 2^31 - 2^14): y = (x - mean) * rstd * w + b, the

@@ -56,6 +56,7 @@ class CallerDevice {
     unsigned next_ = 0, asked_ = 0;
     int device_, restore_ = -1, sms_ = 0;
     bool told_;  // the caller vouches for its arrays (sn_abi_arrays_on)
+    // (that counts for one call: entry points construct this before they return for any reason)
 };
 
 // Bytes of one element of an SN_F32 / SN_BF16 / SN_F16 array, 0 for others.

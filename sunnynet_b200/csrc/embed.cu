@@ -500,12 +500,12 @@ extern "C" {
 
 sn_status sn_abi_embedding(const void* tokens, int32_t token_bits, int64_t n, const void* W, int64_t ld, int64_t V,
                            int32_t D, int32_t dtype, float scale, void* out, void* cuda_stream) {
+    CallerDevice dev;
     SN_TRY(check_call("embedding", n, V, D, ld, dtype, scale));
     if (token_bits != 32 && token_bits != 64) return fail(SN_E_INVAL, "embedding: tokens have 32 or 64 bits");
     if (!n || !D) return SN_OK;
     if (!tokens || !out || (V && !W)) return fail(SN_E_INVAL, "embedding: null pointer");
     const unsigned e = dtype_size(dtype);
-    CallerDevice dev;
     SN_TRY(dev.enter("embedding", {{tokens, (unsigned)token_bits / 8}, {W, e}, {out, e}}));
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     return by_access(dtype, width_of(W, out, ld, D, e), [&](auto t, auto vec) {
@@ -535,12 +535,12 @@ int64_t sn_abi_embedding_bwd_ws(int64_t n, int64_t V, int32_t D) {
 sn_status sn_abi_embedding_bwd(const void* tokens, int32_t token_bits, int64_t n, const void* dout, int64_t ld,
                                int64_t V, int32_t D, int32_t dtype, float scale, void* dW, void* ws,
                                int64_t ws_bytes, void* cuda_stream) {
+    CallerDevice dev;
     SN_TRY(check_call("embedding_bwd", n, V, D, ld, dtype, scale));
     if (token_bits != 32 && token_bits != 64) return fail(SN_E_INVAL, "embedding_bwd: tokens have 32 or 64 bits");
     if (!V || !D) return SN_OK;
     if (!dW || (n && (!tokens || !dout))) return fail(SN_E_INVAL, "embedding_bwd: null pointer");
     const unsigned e = dtype_size(dtype);
-    CallerDevice dev;
     SN_TRY(dev.enter("embedding_bwd",
                      {{tokens, n ? (unsigned)token_bits / 8 : 1}, {dout, n ? e : 1}, {dW, e}, {ws, 16}}));
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);

@@ -351,12 +351,12 @@ int each_launch(const Call& c, long long* parts, F&& f) {
 
 int norm_or_clip(const char* what, const Call& c, double max_norm, bool clip, float* norm, float* factor, void* ws,
                  int64_t ws_bytes, void* cuda_stream) {
+    CallerDevice dev;
     long long total;
     SN_TRY(check_list(what, c, max_norm, &total));
     long long n = 0;
     SN_TRY(each_launch(c, &n, [](const auto&, unsigned, long long) { return SN_OK; }));
     if (n && (!ws || ws_bytes < n * 8)) return fail(SN_E_INVAL, "%s: a workspace of %lld bytes is wanted", what, n * 8);
-    CallerDevice dev;
     for (int i = 0; i < c.count; ++i)
         if (c.sizes[i]) SN_TRY(dev.add(what, {c.grads[i], dtype_size(c.dtypes[i])}));
     for (const ArgPtr& p : {ArgPtr{norm, 4}, {factor, 4}, {ws, 8}}) SN_TRY(dev.add(what, p));

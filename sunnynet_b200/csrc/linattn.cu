@@ -207,13 +207,13 @@ int64_t sn_abi_linear_attention_ws(const SnAbiLinearAttention* a, int32_t backwa
 
 sn_status sn_abi_linear_attention(const SnAbiLinearAttention* a, void* out, float* state_out, void* ws,
                                   int64_t ws_bytes, void* cuda_stream) {
+    CallerDevice dev;
     la::Job j;
     SN_TRY(la::read_job(a, "linear_attention", &j));
     if (!a->B) return SN_OK;
     if (!state_out || (a->T && (!a->log_decay || !a->q || !a->k || !a->v || !out)))
         return fail(SN_E_INVAL, "linear_attention: null pointer");
     const unsigned e = dtype_size(a->dtype);
-    CallerDevice dev;
     SN_TRY(dev.enter("linear_attention", {{a->q, e}, {a->k, e}, {a->v, e}, {a->log_decay, 4}, {a->state, 4},
                                           {a->lengths, 4}, {out, e}, {state_out, 4}, {ws, 16}}));
     return la::by_type(a->dtype, [&](auto t) {
@@ -226,6 +226,7 @@ sn_status sn_abi_linear_attention_bwd(const SnAbiLinearAttention* a, const void*
                                       const int64_t* dout_stride, const float* dstate_out, void* dq, void* dk,
                                       void* dv, float* dlog_decay, int32_t head_gates, float* dstate, void* ws,
                                       int64_t ws_bytes, void* cuda_stream) {
+    CallerDevice dev;
     la::Job j;
     SN_TRY(la::read_job(a, "linear_attention_bwd", &j));
     if (!a->B) {
@@ -236,7 +237,6 @@ sn_status sn_abi_linear_attention_bwd(const SnAbiLinearAttention* a, const void*
         (a->T && (!a->log_decay || !a->q || !a->k || !a->v || !dout || !dq || !dk || !dv)))
         return fail(SN_E_INVAL, "linear_attention_bwd: null pointer");
     const unsigned e = dtype_size(a->dtype);
-    CallerDevice dev;
     SN_TRY(dev.enter("linear_attention_bwd",
                      {{a->q, e}, {a->k, e}, {a->v, e}, {a->log_decay, 4}, {a->state, 4}, {a->lengths, 4},
                       {dout, e}, {dstate_out, 4}, {dq, e}, {dk, e}, {dv, e}, {dlog_decay, 4}, {dstate, 4},
@@ -252,6 +252,7 @@ sn_status sn_abi_linear_attention_bwd(const SnAbiLinearAttention* a, const void*
 
 sn_status sn_abi_linear_attention_step(const SnAbiLinearAttention* a, float* state, int64_t state_stride,
                                        void* out, void* cuda_stream) {
+    CallerDevice dev;
     la::Job j;
     SN_TRY(la::read_job(a, "linear_attention_step", &j));
     if (a->T != 1) return fail(SN_E_INVAL, "linear_attention_step: one token, not %d", a->T);
@@ -262,7 +263,6 @@ sn_status sn_abi_linear_attention_step(const SnAbiLinearAttention* a, float* sta
     if (a->B > 1 && state_stride < size)
         return fail(SN_E_INVAL, "linear_attention_step: states overlap");
     const unsigned e = dtype_size(a->dtype);
-    CallerDevice dev;
     SN_TRY(dev.enter("linear_attention_step",
                      {{a->q, e}, {a->k, e}, {a->v, e}, {a->log_decay, 4}, {state, 4}, {out, e}}));
     const bool four = (uintptr_t)state % 16 == 0 && j.dv % 4 == 0 && (a->B < 2 || state_stride % 4 == 0);

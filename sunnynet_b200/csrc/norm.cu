@@ -1011,6 +1011,7 @@ extern "C" {
 sn_status sn_abi_layer_norm(const void* x, int64_t ldx, const void* w, const void* b, void* y,
                             float* mean, float* rstd, int32_t dtype, int32_t wdtype,
                             int64_t rows, int32_t D, float eps, void* cuda_stream) {
+    CallerDevice dev;
     const unsigned size = dtype_size(dtype), ws = dtype_size(wdtype);
     if (!size || !ws || (wdtype != SN_F32 && wdtype != dtype))
         return fail(SN_E_INVAL, "layer_norm: dtype %d with weights of %d", dtype, wdtype);
@@ -1018,7 +1019,6 @@ sn_status sn_abi_layer_norm(const void* x, int64_t ldx, const void* w, const voi
     if (!(eps >= 0.0f)) return fail(SN_E_INVAL, "layer_norm: eps must not be negative");
     if (rows == 0) return SN_OK;
     if (!x || !y) return fail(SN_E_INVAL, "layer_norm: null pointer");
-    CallerDevice dev;
     SN_TRY(dev.enter("layer_norm", {{x, size}, {w, ws}, {b, ws}, {y, size}, {mean, 4}, {rstd, 4}}));
     const FwdArgs a{x, w, b, y, mean, rstd, rows, ldx, D, wdtype == SN_F32, eps};
     const bool like = alike(x, ldx, y, D, size);
@@ -1052,6 +1052,7 @@ sn_status sn_abi_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int
                                 const void* w, const float* mean, const float* rstd, void* dx,
                                 void* dw, void* db, void* ws, int64_t ws_bytes, int32_t dtype,
                                 int32_t wdtype, int64_t rows, int32_t D, void* cuda_stream) {
+    CallerDevice dev;
     const unsigned size = dtype_size(dtype), wsz = dtype_size(wdtype);
     if (!size || !wsz || (wdtype != SN_F32 && wdtype != dtype))
         return fail(SN_E_INVAL, "layer_norm_bwd: dtype %d with weights of %d", dtype, wdtype);
@@ -1060,7 +1061,6 @@ sn_status sn_abi_layer_norm_bwd(const void* dy, int64_t lddy, const void* x, int
     if (rows && (!dy || !x || !mean || !rstd))
         return fail(SN_E_INVAL, "layer_norm_bwd: null pointer");
     if (!dx && !dw && !db) return SN_OK;
-    CallerDevice dev;
     SN_TRY(dev.enter("layer_norm_bwd", {{dy, size}, {x, size}, {w, wsz}, {mean, 4}, {rstd, 4},
                                         {dx, size}, {dw, wsz}, {db, wsz}, {ws, 4}}));
     const bool sums = dw || db;

@@ -1492,6 +1492,7 @@ extern "C" sn_status sn_abi_sample(const void* logits, int64_t ld, int32_t dtype
                                    const int32_t* top_k, int32_t top_k0, const double* top_p,
                                    double top_p0, const double* min_p, double min_p0, int32_t B,
                                    int32_t V, int32_t* tokens, void* cuda_stream) {
+    CallerDevice dev;
     const unsigned size = dtype_size(dtype);
     if (!size) return fail(SN_E_INVAL, "sample: dtype %d", dtype);
     if (B < 0 || V <= 0 || ld < V) return fail(SN_E_INVAL, "sample: bad dimension");
@@ -1501,7 +1502,6 @@ extern "C" sn_status sn_abi_sample(const void* logits, int64_t ld, int32_t dtype
     if (B == 0) return SN_OK;
     if (!logits || !u || !tokens) return fail(SN_E_INVAL, "sample: null pointer");
     if (B > 0x7fffffff / kMaxCluster) return fail(SN_E_INVAL, "sample: %d rows", B);
-    CallerDevice dev;
     SN_TRY(dev.enter("sample", {{logits, size}, {u, u_f64 ? 8u : 4u}, {temperature, 8},
                                 {top_k, 4}, {top_p, 8}, {min_p, 8}, {tokens, 4}}));
     SampleArgs a{logits, u, top_k, tokens, {temperature, temperature0}, {top_p, top_p0},

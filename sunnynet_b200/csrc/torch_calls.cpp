@@ -84,8 +84,8 @@ void* stream_of(const at::Tensor& t) {
     return c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
 }
 
-// While it lives, the library's calls take all arrays to be on t's GPU, and do not
-// ask for each.
+// The library's next call takes all arrays to be on t's GPU, and does not ask for
+// each. Constructed right before that call.
 struct Known {
     explicit Known(const at::Tensor& t) { lib.arrays_on(t.get_device()); }
     ~Known() { lib.arrays_on(-1); }

@@ -156,3 +156,55 @@ def test_a_copy_of_the_optimiser_keeps_its_bound():
     old = AdamW.__new__(AdamW)  # as one of before the argument unpickles
     old.__setstate__({k: v for k, v in AdamW([p]).__getstate__().items() if k != "max_norm"})
     assert old.max_norm is None and old.grad_norm is None
+
+
+def text(lib):  # noqa: F811
+    buf = ctypes.create_string_buffer(512)
+    lib.sn_abi_last_error(buf, 512)
+    return buf.value
+
+
+def empty_and_refused(lib):  # noqa: F811
+    """Calls that return before they look at an array, with what each returns."""
+    null, stride = ctypes.c_void_p(), (I64 * 3)(1, 1, 1)
+    adamw = lambda count, step: (count, null, null, null, null, null, null, null, 0, 0, 32, step, None, 1e-3, None,  # noqa: E731
+                                 0.9, 0.999, 1e-8, 0.0)
+    norm = lambda dtype, rows: (A, 8, None, None, A, None, None, dtype, 0, rows, 8, 1e-5, None)  # noqa: E731
+    norm_bwd = lambda dtype: (A, 8, A, 8, None, A, A, None, None, None, None, 0, dtype, 0, 4, 8, None)  # noqa: E731
+    draw = lambda B, V_: (A, V_, 0, A, 0, None, 1.0, None, 0, None, 1.0, None, 0.0, B, V_, A, None)  # noqa: E731
+    back = lambda c: lib.sn_abi_linear_attention_bwd(c, A, stride, None, A, A, A, None, 0, None, None, 0, None)  # noqa: E731
+    of = lambda **c: ctypes.byref(call(**c))  # noqa: E731
+    return {
+        "embedding, empty": lambda: lib.sn_abi_embedding(A, 64, 0, A, 8, 8, 8, 0, 1.0, A, None),
+        "embedding, refused": lambda: lib.sn_abi_embedding(A, 64, 4, A, 8, 8, 8, 9, 1.0, A, None),
+        "embedding_bwd, empty": lambda: lib.sn_abi_embedding_bwd(A, 64, 4, A, 8, 0, 8, 0, 1.0, A, None, 0, None),
+        "embedding_bwd, refused": lambda: lib.sn_abi_embedding_bwd(A, 64, 4, A, 8, 8, 8, 9, 1.0, A, None, 0, None),
+        "linear_attention, empty": lambda: lib.sn_abi_linear_attention(of(B=0), A, A, None, 0, None),
+        "linear_attention, refused": lambda: lib.sn_abi_linear_attention(of(dtype=9), A, A, None, 0, None),
+        "linear_attention_bwd, empty": lambda: back(of(B=0)),
+        "linear_attention_bwd, refused": lambda: back(of(dtype=9)),
+        "linear_attention_step, empty": lambda: lib.sn_abi_linear_attention_step(of(B=0, T=1), A, 256, A, None),
+        "linear_attention_step, refused": lambda: lib.sn_abi_linear_attention_step(of(), A, 256, A, None),
+        "grad_norm, refused": lambda: lib.sn_abi_grad_norm(1, None, None, None, 1.0, A, A, A, 8, None),
+        "clip_grads, refused": lambda: lib.sn_abi_clip_grads(1, None, None, None, 1.0, A, A, A, 8, None),
+        "adamw_step, refused": lambda: lib.sn_abi_adamw_step(*adamw(1, 1), None),
+        "adamw_step_scaled, refused": lambda: lib.sn_abi_adamw_step_scaled(*adamw(0, 0), None, None),
+        "layer_norm, empty": lambda: lib.sn_abi_layer_norm(*norm(0, 0)),
+        "layer_norm, refused": lambda: lib.sn_abi_layer_norm(*norm(9, 1)),
+        "layer_norm_bwd, empty": lambda: lib.sn_abi_layer_norm_bwd(*norm_bwd(0)),
+        "layer_norm_bwd, refused": lambda: lib.sn_abi_layer_norm_bwd(*norm_bwd(9)),
+        "sample, empty": lambda: lib.sn_abi_sample(*draw(0, 8)),
+        "sample, refused": lambda: lib.sn_abi_sample(*draw(1, 0)),
+    }
+
+
+def test_what_a_caller_vouches_for_ends_with_its_next_call(lib):  # noqa: F811
+    """sn_abi_arrays_on counts for one call, one that does nothing or is refused too: the call after it asks for
+    its arrays, and refuses these, which lie in host memory."""
+    asks = lambda: lib.sn_abi_embedding(A, 64, 4, A, 8, 8, 8, 0, 1.0, A, None)  # noqa: E731
+    rc, said = asks(), text(lib)
+    assert rc != 0
+    for name, f in empty_and_refused(lib).items():
+        lib.sn_abi_arrays_on(0)
+        assert (f() == 0) == name.endswith("empty"), name
+        assert (asks(), text(lib)) == (rc, said), name
