@@ -165,10 +165,10 @@ struct Norm : torch::autograd::Function<Norm> {
 };
 
 // A tensor or None (an undefined one); false with an error set for others.
-bool tensor_of(PyObject* o, at::Tensor* t) {
+bool tensor_of(const char* what, PyObject* o, at::Tensor* t) {
     if (o == Py_None) return true;
     if (!THPVariable_Check(o)) {
-        PyErr_SetString(PyExc_TypeError, "tensors are wanted");
+        PyErr_Format(PyExc_TypeError, "%s: tensors are wanted", what);
         return false;
     }
     *t = THPVariable_Unpack(o);
@@ -182,7 +182,8 @@ PyObject* layer_norm(PyObject*, PyObject* args) {
     double eps;
     if (!PyArg_ParseTuple(args, "OOOd", &xo, &wo, &bo, &eps)) return nullptr;
     at::Tensor x, w, b;
-    if (!tensor_of(xo, &x) || !tensor_of(wo, &w) || !tensor_of(bo, &b)) return nullptr;
+    const char* const what = "layer_norm";
+    if (!tensor_of(what, xo, &x) || !tensor_of(what, wo, &w) || !tensor_of(what, bo, &b)) return nullptr;
     // (neither path carries a tangent on)
     const auto moves = [](const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); };
     TORCH_CHECK(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() &&
@@ -269,7 +270,7 @@ PyObject* embedding(PyObject*, PyObject* args) {
     double scale;
     if (!PyArg_ParseTuple(args, "OOd", &to, &wo, &scale)) return nullptr;
     at::Tensor tokens, w;
-    if (!tensor_of(to, &tokens) || !tensor_of(wo, &w)) return nullptr;
+    if (!tensor_of("embedding", to, &tokens) || !tensor_of("embedding", wo, &w)) return nullptr;
     TORCH_CHECK_VALUE(w.defined() && w.dim() == 2 && w.is_cuda() && w.size(1) <= 1 << 22 && w.size(0) < 0x7fffffff,
                       "embedding: weight (V, D) on a GPU is wanted, D at most 2^22");
     TORCH_CHECK_TYPE(float_type(w), "embedding: weight is float32, bfloat16 or float16");
@@ -412,11 +413,11 @@ struct Attention : torch::autograd::Function<Attention> {
 };
 
 // The tensors of a call's arguments and its scale (None: 1 / sqrt of q's last axis).
-bool attention_args(PyObject* const* o, int n, at::Tensor* t, PyObject* scale, double* to) {
+bool attention_args(const char* what, PyObject* const* o, int n, at::Tensor* t, PyObject* scale, double* to) {
     for (int i = 0; i < n; ++i) {
-        if (!tensor_of(o[i], t + i)) return false;
+        if (!tensor_of(what, o[i], t + i)) return false;
         if (i < 4 && !t[i].defined()) {
-            PyErr_SetString(PyExc_TypeError, "linear_attention: tensors are wanted");
+            PyErr_Format(PyExc_TypeError, "%s: tensors are wanted", what);
             return false;
         }
     }
@@ -435,8 +436,9 @@ PyObject* linear_attention(PyObject*, PyObject* args) {
     if (!PyArg_ParseTuple(args, "OOOOOOO", o, o + 1, o + 2, o + 3, o + 4, o + 5, &so)) return nullptr;
     at::Tensor t[6];
     double scale;
-    if (!attention_args(o, 6, t, so, &scale)) return nullptr;
-    no_tangent("linear_attention", {t[0], t[1], t[2], t[3], t[4]});
+    const char* const what = "linear_attention";
+    if (!attention_args(what, o, 6, t, so, &scale)) return nullptr;
+    no_tangent(what, {t[0], t[1], t[2], t[3], t[4]});
     std::pair<at::Tensor, at::Tensor> r;
     if (wants_grad({t[0], t[1], t[2], t[3], t[4]})) {
         const auto some = [](const at::Tensor& x) { return x.defined() ? std::optional<at::Tensor>(x) : std::nullopt; };
@@ -466,8 +468,8 @@ PyObject* linear_attention_step(PyObject*, PyObject* args) {
     if (!PyArg_ParseTuple(args, "OOOOOO", o, o + 1, o + 2, o + 3, o + 4, &so)) return nullptr;
     at::Tensor t[5];
     double scale;
-    if (!attention_args(o, 5, t, so, &scale)) return nullptr;
     const char* const what = "linear_attention_step";
+    if (!attention_args(what, o, 5, t, so, &scale)) return nullptr;
     at::Tensor &q = t[0], &k = t[1], &v = t[2], &decay = t[3], &state = t[4];
     no_tangent(what, {q, k, v, decay, state});
     TORCH_CHECK_VALUE(!wants_grad({q, k, v, decay, state}), what, " has no gradient: call linear_attention");

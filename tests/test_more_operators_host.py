@@ -208,3 +208,18 @@ def test_what_a_caller_vouches_for_ends_with_its_next_call(lib):  # noqa: F811
         lib.sn_abi_arrays_on(0)
         assert (f() == 0) == name.endswith("empty"), name
         assert (asks(), text(lib)) == (rc, said), name
+
+
+def test_an_error_names_its_operator(lib):  # noqa: F811
+    from sunnynet_b200 import kernels
+    calls, x = kernels._torch_calls(), torch.zeros(2, 5, 2, 8)
+    for bad, name in ((lambda: calls.layer_norm(3, None, None, 1e-5), "layer_norm"),
+                      (lambda: calls.layer_norm(x, 3, None, 1e-5), "layer_norm"),
+                      (lambda: kernels.embedding(x, 3), "embedding"),
+                      (lambda: kernels.linear_attention(x, 3, x, x), "linear_attention"),
+                      (lambda: kernels.linear_attention(x, None, x, x), "linear_attention"),
+                      (lambda: kernels.linear_attention_step(x, x, x, x, 3), "linear_attention_step"),
+                      (lambda: kernels.linear_attention_step(x, x, None, x, x), "linear_attention_step"),
+                      (lambda: kernels.grad_norm([3]), "grad_norm"), (lambda: kernels.clip_grads([3], 1.0), "clip_grads")):
+        with pytest.raises(TypeError, match="^" + name + ": tensors are wanted"):
+            bad()
