@@ -217,6 +217,12 @@ void no_tangent(const char* what, std::initializer_list<at::Tensor> ts) {
         TORCH_CHECK(!(t.defined() && t._fw_grad(0).defined()), what, " has no forward-mode derivative");
 }
 
+// Views whose sign is not in memory (the imaginary part of a conjugate) become tensors as they read.
+void signed_values(std::initializer_list<at::Tensor*> ts) {
+    for (at::Tensor* t : ts)
+        if (t->defined() && t->is_neg()) *t = t->resolve_neg();
+}
+
 at::Tensor space(int64_t bytes, const at::Tensor& like) {
     return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor();
 }
@@ -246,7 +252,9 @@ struct Embedding : torch::autograd::Function<Embedding> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                    torch::autograd::variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), "embedding can be differentiated once");
-        const at::Tensor tokens = ctx->get_saved_variables()[0], &dout = grads[0];
+        const at::Tensor tokens = ctx->get_saved_variables()[0];
+        at::Tensor& dout = grads[0];
+        signed_values({&dout});
         const int64_t V = ctx->saved_data["rows"].toInt(), D = dout.size(-1), n = tokens.numel();
         at::Tensor rows = dout.reshape({n, D});  // a view wherever the rows lie at one stride
         if (D > 1 && rows.stride(1) != 1) rows = rows.contiguous();
@@ -279,6 +287,7 @@ PyObject* embedding(PyObject*, PyObject* args) {
                       "embedding: tokens are int32 or int64 on the weight's GPU, fewer than 2^31");
     TORCH_CHECK_VALUE(std::isfinite(scale), "embedding: the scale is not finite");
     no_tangent("embedding", {w});
+    signed_values({&w});
     tokens = tokens.contiguous();
     if (w.size(1) > 1 && w.stride(1) != 1) w = w.contiguous();
     if (wants_grad({w})) return THPVariable_Wrap(Embedding::apply(tokens, w, scale));
@@ -387,6 +396,7 @@ struct Attention : torch::autograd::Function<Attention> {
         const SnAbiLinearAttention a = attention_call("linear_attention_bwd", q, k, v, decay, &state, &saved[5],
                                                       ctx->saved_data["scale"].toDouble());
         at::Tensor dout = grads[0], dend = grads[1];
+        signed_values({&dout, &dend});
         if (!dout.defined()) dout = at::zeros(v.sizes(), v.options());
         if (a.dv > 1 && dout.stride(3) != 1) dout = dout.contiguous();
         if (dend.defined()) dend = dend.contiguous();
@@ -439,6 +449,7 @@ PyObject* linear_attention(PyObject*, PyObject* args) {
     const char* const what = "linear_attention";
     if (!attention_args(what, o, 6, t, so, &scale)) return nullptr;
     no_tangent(what, {t[0], t[1], t[2], t[3], t[4]});
+    signed_values({t, t + 1, t + 2, t + 3, t + 4});
     std::pair<at::Tensor, at::Tensor> r;
     if (wants_grad({t[0], t[1], t[2], t[3], t[4]})) {
         const auto some = [](const at::Tensor& x) { return x.defined() ? std::optional<at::Tensor>(x) : std::nullopt; };
@@ -473,11 +484,12 @@ PyObject* linear_attention_step(PyObject*, PyObject* args) {
     at::Tensor &q = t[0], &k = t[1], &v = t[2], &decay = t[3], &state = t[4];
     no_tangent(what, {q, k, v, decay, state});
     TORCH_CHECK_VALUE(!wants_grad({q, k, v, decay, state}), what, " has no gradient: call linear_attention");
+    signed_values({&q, &k, &v, &decay});
     at::Tensor out = at::empty(v.sizes(), v.options());
     const SnAbiLinearAttention a = attention_call(what, q, k, v, decay, nullptr, nullptr, scale, true);
     TORCH_CHECK_VALUE(state.defined() && state.scalar_type() == at::kFloat && state.device() == v.device() &&
                           state.sizes() == at::IntArrayRef({a.B, a.H, a.dk, a.dv}) &&
-                          rows_of_state(state),
+                          rows_of_state(state) && !state.is_neg(),
                       what, ": state is float32 of (B, H, dk, dv) on the GPU of the others, each sequence's contiguous");
     TORCH_CHECK_VALUE(a.B < 2 || state.stride(0) >= (int64_t)a.H * a.dk * a.dv, what, ": the states overlap");
     state.unsafeGetTensorImpl()->bump_version();  // a graph that saved it must not use it

@@ -181,3 +181,13 @@ def test_refusals(kernels):
     x = w.requires_grad_()
     with pytest.raises(RuntimeError, match="once"):
         torch.autograd.grad(kernels.embedding(t, x).sum(), x, create_graph=True)
+
+
+def test_views_with_a_sign(kernels):
+    """The imaginary part of a conjugate is a view whose sign is not in memory: it counts in rows and gradients."""
+    view = lambda t: torch.complex(torch.zeros_like(t), -t).conj().imag  # noqa: E731
+    w, tokens, dout = torch.randn(9, 1, device="cuda"), words(40, 9, "even"), torch.randn(40, 1, device="cuda")
+    assert view(w).is_neg()
+    out, dw = grad(kernels, tokens, w, dout, 1.5)
+    assert torch.equal(kernels.embedding(tokens, view(w), 1.5), out)
+    assert torch.equal(grad(kernels, tokens, w, view(dout), 1.5)[1], dw)

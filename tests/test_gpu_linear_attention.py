@@ -512,3 +512,27 @@ def test_the_factor_of_a_single_token(kernels, g):
     kernels.linear_attention_step(x, x * 0, x, decay, S)
     far = 2.0 ** -23 * abs(math.expm1(g)) / math.exp(g) if abs(g) < 0.5 else 2.0 ** -22
     assert ((S.double() - want).abs() <= (2.0 ** -24 + 2.0 ** -40 + far) * want.abs() + 2.0 ** -150).all()
+
+
+def test_views_with_a_sign(kernels):
+    """The imaginary part of a conjugate is a view whose sign is not in memory: inputs and gradients count with
+    it, and a state that would be written through it is refused."""
+    view = lambda t: torch.complex(torch.zeros_like(t), -t).conj().imag  # noqa: E731
+    x = make(2, 70, 2, 2, 1, 1, torch.float32)
+    assert view(x["log_decay"]).is_neg() and torch.equal(view(x["log_decay"]), x["log_decay"])
+    ends = (torch.randn(2, 70, 2, 1, device="cuda"), torch.randn(2, 2, 1, 1, device="cuda"))
+    want = gradients(kernels, x, 0.3, ends)
+    for n in ("q", "k", "v", "log_decay", "state"):
+        leaf = x[n].detach().clone().requires_grad_()
+        got = kernels.linear_attention(**{**x, n: view(leaf)}, scale=0.3)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), n
+        got = torch.autograd.grad(got, leaf, [view(e) for e in ends])[0]
+        assert torch.equal(got, want[2 + ["q", "k", "v", "log_decay", "state"].index(n)]), n
+    one = {n: x[n][:, 0] for n in ("q", "k", "v", "log_decay")}
+    S = x["state"].clone()
+    want = kernels.linear_attention_step(**one, state=S)
+    for n in one:
+        T = x["state"].clone()
+        assert torch.equal(kernels.linear_attention_step(**{**one, n: view(one[n])}, state=T), want) and torch.equal(S, T), n
+    with pytest.raises(ValueError, match="state"):
+        kernels.linear_attention_step(**{n: t[:1, :1] if t.dim() > 1 else t for n, t in one.items()}, state=view(x["state"][:1, :1]))
