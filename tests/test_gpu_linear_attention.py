@@ -536,3 +536,108 @@ def test_views_with_a_sign(kernels):
         assert torch.equal(kernels.linear_attention_step(**{**one, n: view(one[n])}, state=T), want) and torch.equal(S, T), n
     with pytest.raises(ValueError, match="state"):
         kernels.linear_attention_step(**{n: t[:1, :1] if t.dim() > 1 else t for n, t in one.items()}, state=view(x["state"][:1, :1]))
+
+
+# sequences times heads of 148 or more (74 with gradients): a CTA walks the chunks of a head in turn
+WALKS = [(4, 330, 40, 20, 64, 64), (2, 290, 75, 75, 64, 128), (3, 290, 50, 25, 128, 64), (2, 290, 75, 75, 128, 128)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,H,Hk,dk,dv", WALKS)
+@pytest.mark.parametrize("padded", [False, True])
+def test_many_heads_over_many_chunks(kernels, B, T, H, Hk, dk, dv, dtype, padded):
+    x = make(B, T, H, Hk, dk, dv, dtype, lengths=[T - 1, 129, 0, 257][:B] if padded else None)
+    got = kernels.linear_attention(**x, scale=0.3)
+    (out, S), (mo, ms) = truth(x, 0.3)
+    near(got[0], out, mo, dtype)
+    near(got[1], S, ms, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,H,Hk,dk,dv", [(4, 330, 40, 20, 64, 64), (2, 290, 38, 38, 64, 128), (2, 290, 38, 19, 128, 64),
+                                            (2, 290, 38, 38, 128, 128)])
+@pytest.mark.parametrize("padded", [False, True])
+def test_gradients_of_many_heads_over_many_chunks(kernels, B, T, H, Hk, dk, dv, dtype, padded):
+    x = make(B, T, H, Hk, dk, dv, dtype, "token" if padded else "head", lengths=[T - 1, 129, 0, 257][:B] if padded else None)
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    ends = (torch.randn(B, T, H, dv, device="cuda", generator=gen).to(dtype),
+            torch.randn(B, H, dk, dv, device="cuda", generator=gen))
+    got = gradients(kernels, x, 0.3, ends)
+    want, most = truth(x, 0.3, ends)
+    for n, (g, w, m, kind) in enumerate(zip(got, want, most, [dtype, torch.float32] + [dtype] * 3 + [torch.float32] * 2)):
+        near(g, w, m, kind, spread(x, most) if n == 5 else 0.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,H", [(1, 40, 3), (2, 300, 3), (2, 300, 40)])
+def test_gradients_of_packed_sequences(kernels, B, T, H, dtype):
+    """Minus infinity begins a sequence anew: no gradient crosses it, and its own is zero but for the sums' roundings."""
+    x = make(B, T, H, H, 64, 32, dtype)
+    for c in (0, 1, 7, T // 2, T // 2 + 1, T - 3):
+        x["log_decay"][:, c] = -float("inf")
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    ends = (torch.randn(B, T, H, 32, device="cuda", generator=gen).to(dtype), torch.randn(B, H, 64, 32, device="cuda", generator=gen))
+    got = gradients(kernels, x, 0.3, ends)
+    want, most = truth(x, 0.3, ends)
+    for n, (g, w, m, kind) in enumerate(zip(got, want, most, [dtype, torch.float32] + [dtype] * 3 + [torch.float32] * 2)):
+        near(g, w, m, kind, spread(x, most) if n == 5 else 0.0)
+    assert not got[6].any()  # the first state is forgotten at once
+
+
+def test_gradients_of_growing_states(kernels):
+    """Positive log decays, up to e^20 over the sequence."""
+    x = make(1, 200, 2, 1, 24, 40, torch.float32)
+    x["log_decay"] = x["log_decay"].abs().clamp(max=0.1)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    ends = (torch.randn(1, 200, 2, 40, device="cuda", generator=gen), torch.randn(1, 2, 24, 40, device="cuda", generator=gen))
+    got = gradients(kernels, x, 0.2, ends)
+    want, most = truth(x, 0.2, ends)
+    for n, (g, w, m) in enumerate(zip(got, want, most)):
+        near(g, w, m, torch.float32, spread(x, most) if n == 5 else 0.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("wanted", [("q",), ("k",), ("v",), ("q", "k", "v"), ("log_decay",), ("state",)])
+def test_a_part_of_the_gradients(kernels, dtype, wanted):
+    """What is asked for has the bits that it has beside the others, fixed decays among them; of either result alone."""
+    x = make(2, 150, 4, 2, 64, 64, dtype)
+    ends = (torch.randn(2, 150, 4, 64, device="cuda").to(dtype), torch.randn(2, 4, 64, 64, device="cuda"))
+    for end in (ends, (ends[0], None), (None, ends[1])):
+        if wanted == ("q",) and end[0] is None:
+            continue  # (the last state does not depend on q)
+        all_ = dict(zip(("q", "k", "v", "log_decay", "state"), gradients(kernels, x, 0.3, end)[2:]))
+        leaves = {n: t.detach().clone().requires_grad_(n in wanted) if t is not None and n != "lengths" else t
+                  for n, t in x.items()}
+        outs = [(o, e) for o, e in zip(kernels.linear_attention(**leaves, scale=0.3), end) if e is not None]
+        got = torch.autograd.grad([o for o, _ in outs], [leaves[n] for n in wanted], [e for _, e in outs])
+        assert all(torch.equal(g, all_[n]) for g, n in zip(got, wanted)), end
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_gradient_of_outputs_beyond_32_bits(kernels, dtype):
+    """Its tokens and sequences lie further apart than 2^32 bytes."""
+    x = make(2, 9, 2, 2, 16, 16, dtype, state=False)
+    dout = torch.randn(2, 9, 2, 16, device="cuda").to(dtype)
+    want = gradients(kernels, x, 0.3, (dout, None))
+    far = torch.empty((1 << 33) // dout.element_size() + (1 << 29), dtype=dtype, device="cuda")
+    wide = far.as_strided((2, 9, 2, 16), ((1 << 31) // 4 + 64, (1 << 28) - (1 << 24), 64, 1))
+    wide.copy_(dout)
+    assert all(torch.equal(a, b) for a, b in zip(gradients(kernels, x, 0.3, (wide, None)), want))
+
+
+def test_function_transforms_are_refused(kernels):
+    """torch.func's wrappers have no memory to read: an error, and nothing is launched."""
+    x = make(2, 5, 2, 2, 8, 8, torch.float32)
+    w, tokens = torch.randn(9, 8, device="cuda"), torch.arange(4, device="cuda")
+    rest = {n: x[n] for n in ("k", "v", "log_decay")}
+    one = {n: x[n][:, 0] for n in ("q", "k", "v", "log_decay")}
+    for call in (lambda: torch.func.grad(lambda t: kernels.embedding(tokens, t).sum())(w),
+                 lambda: torch.func.vmap(lambda t: kernels.embedding(t, w))(tokens),
+                 lambda: torch.func.grad(lambda t: kernels.linear_attention(t, **rest)[0].sum())(x["q"]),
+                 lambda: torch.func.jvp(lambda t: kernels.linear_attention(t, **rest)[0], (x["q"],), (x["q"],)),
+                 lambda: torch.func.vmap(lambda t: kernels.linear_attention(t, **rest)[0])(x["q"][None]),
+                 lambda: torch.func.vmap(lambda t: kernels.linear_attention_step(**one, state=t))(x["state"][None]),
+                 lambda: torch.func.vmap(lambda t: kernels.grad_norm([t])[0])(w),
+                 lambda: torch.func.vmap(lambda t: kernels.clip_grads([t], 0.1))(w)):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            call()
