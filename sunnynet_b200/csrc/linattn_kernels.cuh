@@ -1037,7 +1037,10 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
             if (l + d < 32) bs += y;
             if (l >= d) as += z;
         }
-        bs -= b, as -= a;
+        // of the lanes behind and before alone (less the lane's own, large ones would leave nothing of the others)
+        bs = __shfl_down_sync(0xffffffffu, bs, 1), as = __shfl_up_sync(0xffffffffu, as, 1);
+        if (l == 31) bs = 0.0f;
+        if (l == 0) as = 0.0f;
 #pragma unroll
         for (int i = 0; i < M; ++i) {
             const int u = c0 + l * M + i;

@@ -641,3 +641,17 @@ def test_function_transforms_are_refused(kernels):
                  lambda: torch.func.vmap(lambda t: kernels.clip_grads([t], 0.1))(w)):
         with pytest.raises((RuntimeError, NotImplementedError)):
             call()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,T,H,dk,dv", [(2, 4, 2, 11, 1), (2, 5, 90, 118, 3), (2, 128, 3, 64, 64), (1, 349, 21, 4, 3), (2, 70, 80, 128, 128)])
+def test_gradients_of_fast_decays_from_the_last_state(kernels, B, T, H, dk, dv, dtype):
+    """Nothing is subtracted on the way from the last state to a decay's gradient: it is as good as its own terms,
+    however much larger those of later tokens are."""
+    x = make(B, T, H, H, dk, dv, dtype)
+    x["log_decay"] *= 8
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    ends = (None, torch.randn(B, H, dk, dv, device="cuda", generator=gen))
+    got = gradients(kernels, x, 0.3, ends)[5]
+    want, most = truth(x, 0.3, ends)
+    near(got, want[5], most[5], torch.float32, 2.0 ** -116)  # (what an exp2 flushes to zero, times 2^10)
