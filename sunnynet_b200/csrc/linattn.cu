@@ -78,9 +78,25 @@ step_kernel(const T* q_, const T* k_, const T* v_, Strides qs, Strides ks, Strid
         sq[tid] = to_f(q[tid]) * scale;
         sk[tid] = to_f(k[tid]);
     }
+    constexpr int U = 8;  // rows on their way at once; the first are, while the factor is formed
+    float s[U][VEC];
+    const auto fetch = [&](int r) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (in && r + u * rows < dk) {
+                const float* at = S + (r + u * rows) * dv + c * VEC;
+                if constexpr (VEC == 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(at);
+                    s[u][0] = y.x, s[u][1] = y.y, s[u][2] = y.z, s[u][3] = y.w;
+                } else {
+                    s[u][0] = *at;
+                }
+            }
+    };
+    const float gate = g[b * gb + h * gh];
+    fetch(r0);
     // exp(g) in two parts: a slow decay's factor is the same at every token, and what it is off adds up over
     // 1 / (1 - f) of them (4096 tokens of decays about 2^-11: 3e-4 by ex2.approx, 8e-6 so: the states' roundings)
-    const float gate = g[b * gb + h * gh];
     float f, rest = 0.0f;
     if (fabsf(gate) < 0.5f) {
         const float e = expm1f(gate);
@@ -97,20 +113,8 @@ step_kernel(const T* q_, const T* k_, const T* v_, Strides qs, Strides ks, Strid
     }
     __syncthreads();
     if (in) {
-        constexpr int U = 8;
         for (int r = r0; r < dk; r += rows * U) {
-            float s[U][VEC];
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (r + u * rows < dk) {
-                    const float* at = S + (r + u * rows) * dv + c * VEC;
-                    if constexpr (VEC == 4) {
-                        const float4 y = *reinterpret_cast<const float4*>(at);
-                        s[u][0] = y.x, s[u][1] = y.y, s[u][2] = y.z, s[u][3] = y.w;
-                    } else {
-                        s[u][0] = *at;
-                    }
-                }
+            if (r > r0) fetch(r);
 #pragma unroll
             for (int u = 0; u < U; ++u)
                 if (r + u * rows < dk) {
