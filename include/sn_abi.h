@@ -317,7 +317,12 @@ typedef struct {
     float scale;
 } SnAbiLinearAttention;
 /* Bytes of workspace of the calls below (-1 where they would refuse the sizes).
- * head_gates: dlog_decay is (H), else (B, T, H). */
+ * head_gates: dlog_decay is (H), else (B, T, H). For each head and 64 tokens (32
+ * where dk and dv are both above 64 and values are not bf16) a state of dk x dv, each
+ * rounded up to 64 or 128: in 2 bytes for bf16, 4 for float16, 6 for float32, and 12
+ * with `backward`, whatever the type (16 x 2048 tokens of 12 heads of 64: 0.3 GB); 4
+ * or 8 more where B * H is below 148, or 74 with `backward`. With `backward` and Hk
+ * below H also 8 * dk for each token and head. */
 int64_t   sn_abi_linear_attention_ws(const SnAbiLinearAttention* a, int32_t backward,
                                      int32_t head_gates);
 /* out (B, T, H, dv) contiguous, of `dtype`; state_out (B, H, dk, dv) fp32. The
@@ -341,9 +346,9 @@ sn_status sn_abi_linear_attention_step(const SnAbiLinearAttention* a, float* sta
  * values, contiguous; W (V, D) with rows `ld` values apart, both of `dtype`;
  * tokens int32 or int64 (token_bits), fewer than 2^31 - 4096; D at most 2^22. A
  * token outside [0, V) gives a row of NaN.
- * Its gradient: dW[v] = scale * the sum of dout[i] over token_i = v, in fp32 and
- * in the order of i; dW (V, D) contiguous, overwritten; dout with rows `ld`
- * values apart. The same call gives the same bits. */
+ * Its gradient: dW[v] = scale * the sum of dout[i] over token_i = v, in fp32 and in
+ * an order that the call's tokens and sizes decide; dW (V, D) contiguous,
+ * overwritten; dout with rows `ld` values apart. The same call gives the same bits. */
 sn_status sn_abi_embedding(const void* tokens, int32_t token_bits, int64_t n, const void* W,
                            int64_t ld, int64_t V, int32_t D, int32_t dtype, float scale, void* out,
                            void* cuda_stream);
@@ -358,7 +363,8 @@ sn_status sn_abi_embedding_bwd(const void* tokens, int32_t token_bits, int64_t n
  * 1e-6)), each one fp32 value on the GPU or NULL; a NaN among the values makes
  * both NaN. clip_grads also multiplies every value by the factor in place
  * (where it is 1, nothing is written); no tensor may then appear twice or
- * overlap another. The same call gives the same bits. */
+ * overlap another. The same call gives the same bits; the same values at other
+ * addresses modulo 16 may give others. */
 int64_t   sn_abi_grad_norm_ws(int32_t count, const int64_t* sizes);
 sn_status sn_abi_grad_norm(int32_t count, const void* const* grads, const int64_t* sizes,
                            const int32_t* dtypes, double max_norm, float* norm, float* factor,

@@ -8,8 +8,9 @@
 // NaN, and no gradient: the device has no other way to tell.
 //
 // Gradient: the tokens are sorted by a stable radix sort of eight bits a pass, so
-// that each row's tokens lie side by side in their order and are added in it: the
-// same bits every time, no atomics on values. Up to kNear tokens are sorted by one
+// that each row's tokens lie side by side in their order and are added in it, a row
+// of many in pieces, which end where its chunks of sorted tokens do: an order that the
+// call's tokens and sizes decide, the same bits every time, no atomics on values. Up to kNear tokens are sorted by one
 // cluster of eight CTAs in one launch (5003 tokens, two passes: 11 us; four launches
 // of many CTAs took 12, and 10 more of the host's time; 32768 tokens 28 us against
 // 18), more of them by two launches a pass: the counts of every tile, then ranks and

@@ -33,6 +33,8 @@
 // of 128 x 64 x 16 takes as long as one of 128 x 128 x 16 (90 cycles); the 24 that
 // a chunk of 128 tokens needs would fill three quarters of the time that HBM leaves
 // it, while the decays need the scores in registers and the states anew for each chunk.
+// Heads of 128 would fill the instruction; there the traffic of the states is what bounds
+// the calls (see state_kernel), and tcgen05 was not tried.
 #include <algorithm>
 #include <cmath>
 
@@ -56,7 +58,7 @@ namespace {
 // -------------------------------------------------------------- single token
 // A CTA for each sequence and head: its state goes through once. Lanes stand
 // side by side along a row of the state, so that every access is one run. Bound by HBM: 256
-// sequences x 12 heads of 64 take 15.7 us, 102 MB at 6.5 TB/s.
+// sequences x 12 heads of 64 take 17.5 us, one call after the other, 102 MB at 5.8 TB/s.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(128)
 step_kernel(const T* q_, const T* k_, const T* v_, Strides qs, Strides ks, Strides vs, const float* g,

@@ -18,7 +18,8 @@ namespace la {
 typedef __nv_bfloat16 bf16;
 
 // Planes a type's values take: bf16 is one itself, float16 the sum of two, float32
-// of three; nothing is lost.
+// of three; nothing is lost (but that fp32 values from 3.396e38 on, the last 512th of
+// the range, round to infinity in their first part).
 template <typename T>
 constexpr int planes_of = std::is_same<T, bf16>::value ? 1 : std::is_same<T, float>::value ? 3 : 2;
 

@@ -407,6 +407,10 @@ struct Pass {
 // instructions 37% of the time): a chunk's sum waits for its weighted values, which take
 // as long to form in three parts as to multiply, and the next chunk waits for it. A state's
 // rows on two CTAs, which would fill the SMs more evenly, gained nothing and took 164.
+// Where keys are wider than 64 the ninth warp, of the decays, leaves a thread 168 registers
+// (96 where two CTAs share an SM), and the walk spills: up to 256 bytes stored in bf16, 332
+// in fp16, 520 in fp32 (224 there for values wider than 64). 16 x 2048 x 12 of 128 take
+// 0.40 ms in bf16, 1.07 in fp16, 1.67 in fp32, with gradients 1.8, 3.9 and 5.2.
 template <class S_, bool KEEP, int PN>
 __global__ void __launch_bounds__(S_::ST + 32, KEEP && S_::SNT > 8 ? 1 : 2)
 state_kernel(const Job j, const Pass p0, const Pass p1, Decays<S_::C>* dec_out) {
@@ -1117,7 +1121,11 @@ int behind(void (*kernel)(P...), dim3 ctas, int threads, int bytes, cudaStream_t
 
 // Whether each chunk's sum gets a CTA: where the heads alone leave SMs idle. (The
 // sums cost a write and a read of a state in fp32 for each chunk; one prompt of 8192
-// tokens and 12 heads of 128 otherwise waits for 128 chunks, one after the other.)
+// tokens and 12 heads of 128 otherwise waits for 128 chunks, one after the other. 2048 tokens
+// of 64, walked or apart: bf16 48 heads 66 and 43 us, 74 72 and 55, 148 90 and 100, 296 143
+// and 193; fp32 74 heads 244 and 154, 148 340 and 293, 192 422 and 373, 296 557 and 565. Of
+// 128 in bf16: 74 heads 193 and 168, 148 248 and 311. Gradients in bf16, of twice as many
+// walks: 48 heads 185 and 156, 74 220 and 221, 148 340 and 410.)
 void cut(Job* j, int C, int passes) {
     j->chunks = (j->T + C - 1) / C;
     j->apart = j->chunks > 1 && (long long)j->B * j->H * passes < 148;

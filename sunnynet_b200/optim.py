@@ -19,7 +19,8 @@ class AdamW(torch.optim.Optimizer):
     a GPU. The step number lives on the host: to capture a step into a CUDA
     graph, call ``kernels.adamw_step`` with a step tensor. ``max_norm``: gradients
     whose common norm (of all groups) is larger are scaled to it as the step reads
-    them, .grad stays as it is; ``grad_norm`` is then the last step's norm, on the GPU."""
+    them, .grad stays as it is; ``grad_norm`` is then the last step's norm, on the GPU.
+    All gradients are then on one GPU; a state dict does not hold ``max_norm``."""
 
     max_norm = grad_norm = None
 
