@@ -314,8 +314,9 @@ def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr=1e-3, beta1=0.9, bet
                 raise TypeError(f"adamw_step: {name} as a tensor is one {dt} value on "
                                 f"{first.device}")
             on_gpu[name] = v.data_ptr()
-    if grad_scale is not None and (grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or
-                                   grad_scale.device != first.device):
+    if grad_scale is not None and not (
+            isinstance(grad_scale, Tensor) and grad_scale.dtype == torch.float32 and
+            grad_scale.numel() == 1 and grad_scale.device == first.device):
         raise TypeError(f"adamw_step: grad_scale is one float32 value on {first.device}")
     to = [_address(at) + 8 * n * i for i in range(len(lists))]
     rc = _lib_loaded().sn_abi_adamw_step_scaled(

@@ -198,3 +198,11 @@ def test_the_optimiser_takes_the_factor(kernels, bits, dtype):
             kernels.adamw_step([start[0]], [grads[0]], [torch.zeros_like(start[0])], [torch.zeros_like(start[0])], 1, grad_scale=bad)
     with pytest.raises(ValueError):
         AdamW([torch.nn.Parameter(start[0])], max_norm=-1.0)
+
+
+def test_a_factor_that_is_no_tensor(kernels):
+    x = [torch.ones(4, device="cuda") for _ in range(4)]
+    for bad in (0.5, [1.0], "1"):
+        with pytest.raises(TypeError, match="grad_scale"):
+            kernels.adamw_step(*([t] for t in x), 1, grad_scale=bad)
+    assert all(torch.equal(t, torch.ones_like(t)) for t in x)
