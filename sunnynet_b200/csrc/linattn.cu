@@ -18,10 +18,9 @@
 //   dg_t = 2^(c_C) <R, S> + sum over u >= t of q_u . (its dq from S) + sum over s < t of
 //          k_s . (its dk from R) + sum over u >= t > s of scale 2^(c_u - c_s) (q_u . k_s) (do_u . v_s)
 //
-// (dg sums, of what lies outside a chunk, only what passes token t's gate: the
+// (dg sums only what passes token t's gate, so that it is as good as its own terms: the
 // shorter form by differences q.dq - k.dk from the sequence's end loses all digits over
-// long sequences. The chunk's own pairs are summed by rows and columns, u >= t less
-// s >= t: 2^-16 of their sum at most.)
+// long sequences, and differences of the pairs' sums within a chunk those of fast decays.)
 //
 // All products are m16n8k16 matrix instructions on bf16 with fp32 sums. bf16
 // values are taken as they are, float16 ones as the sum of two bf16 and float32

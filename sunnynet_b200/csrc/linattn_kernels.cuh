@@ -792,6 +792,52 @@ __device__ __forceinline__ int column_sums(float* v) {
     return which;
 }
 
+// A 16 x 16 block of products becomes, row by row, its sums from each column on.
+__device__ __forceinline__ void pairs_from(float (*x)[4]) {
+    const int q = lane_id() & 3;
+#pragma unroll
+    for (int h = 0; h < 4; h += 2) {  // rows g and g + 8
+        float after = 0.0f;           // of the later columns
+#pragma unroll
+        for (int n = 1; n >= 0; --n) {
+            float s = x[n][h] + x[n][h + 1];
+#pragma unroll
+            for (int d = 1; d < 4; d *= 2) {
+                const float y = __shfl_down_sync(0xffffffffu, s, d, 4);
+                if (q + d < 4) s += y;
+            }
+            const float y = __shfl_down_sync(0xffffffffu, s, 1, 4), whole = __shfl_sync(0xffffffffu, s, 0, 4);
+            x[n][h + 1] += (q < 3 ? y : 0.0f) + after;
+            x[n][h] += x[n][h + 1];
+            after += whole;
+        }
+    }
+}
+
+// Sums over the lanes before (behind) this one among W neighbours.
+template <int W>
+__device__ __forceinline__ float sum_before(float x) {
+    const int l = lane_id() % W;
+#pragma unroll
+    for (int d = 1; d < W; d *= 2) {
+        const float y = __shfl_up_sync(0xffffffffu, x, d, W);
+        if (l >= d) x += y;
+    }
+    x = __shfl_up_sync(0xffffffffu, x, 1, W);  // (the sum less its own x would lose small others)
+    return l ? x : 0.0f;
+}
+template <int W>
+__device__ __forceinline__ float sum_behind(float x) {
+    const int l = lane_id() % W;
+#pragma unroll
+    for (int d = 1; d < W; d *= 2) {
+        const float y = __shfl_down_sync(0xffffffffu, x, d, W);
+        if (l + d < W) x += y;
+    }
+    x = __shfl_down_sync(0xffffffffu, x, 1, W);
+    return l + 1 < W ? x : 0.0f;
+}
+
 template <class S_, int MIN>
 __global__ void __launch_bounds__(S_::THREADS, MIN)
 grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
@@ -805,7 +851,7 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
     bf16 *const sk = sq + S_::KT, *const sv = sk + S_::KT, *const so = sv + S_::VT;
     bf16* const ss = so + S_::VT;  // the gradient behind the chunk, then the state before it
     __shared__ Decays<C> dec;
-    // parts of dg: by row block, and by column group where the columns are split
+    // parts of dg: by row block (of each block's own pairs: by token), and by column group where the columns are split
     __shared__ float col_part[RB][C], row_part[C], dq_part[CG][C], dk_part[CG][C], dot_part[S_::NW];
     const Chunk at(j);
     const int end = tokens_of(j, at.b), c0 = at.c * C, c1 = min(c0 + C, j.T);
@@ -919,7 +965,7 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
             scale_rows<NV>(V, b0, b1);
             scale_rows<NK>(K, b0, b1);
             across[0] *= b0, across[1] *= b1;
-            float P[2][4], Q[2][4], down[4] = {};
+            float P[2][4], Q[2][4], A[2][4], down[4] = {};
             scores<NP, KD, 1, FINE>(P, tk, rb * 16, tq, rb, rb, rb + 1);
             scores<NP, VD, 1, FINE>(Q, tv, rb * 16, to, rb, rb, rb + 1);
 #pragma unroll
@@ -928,12 +974,17 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
                 for (int i = 0; i < 4; ++i) {
                     const int s = t + (i >> 1) * 8, u = rb * 16 + n * 8 + (l & 3) * 2 + (i & 1);
                     const float w = dec.between(u, s) * j.scale, p = P[n][i] * w;
-                    const float a = u > s ? p * Q[n][i] : 0.0f;
+                    A[n][i] = u > s ? p * Q[n][i] : 0.0f;
                     P[n][i] = u >= s ? p : 0.0f;
                     Q[n][i] = u >= s ? Q[n][i] * w : 0.0f;
-                    across[i >> 1] += a;
-                    down[2 * n + (i & 1)] += a;
                 }
+            // the block's own pairs: of the rows before each column, the sums from it on
+            pairs_from(A);
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if ((l >> 2) + (i >> 1) * 8 < n * 8 + (l & 3) * 2 + (i & 1)) down[2 * n + (i & 1)] += A[n][i];
             const int which = column_sums<4>(down);
             if (cg == 0) col_part[rb][rb * 16 + which / 2 * 8 + (l & 3) * 2 + which % 2] = down[0];
 #pragma unroll
@@ -1007,48 +1058,61 @@ grad_kernel(const Job j, const Grads G, const Decays<S_::C>* decs) {
         store_head(X, G.dq, G.dq32);
     }
     if (warp == 0 && dg) {
-        // behind: sum over u >= t of (rho_u + r_u) - sum over s >= t of kappa_s; ahead: sum over s < t of l_s
-        constexpr int M = C / 32;
-        float behind[M], ahead[M], all = 0.0f, b = 0.0f, a = 0.0f;
+        // A sum for each token t of what passes its gate, and nothing taken away again, so that a
+        // small one is as good as its terms: sums over the chunk from t on of what the outputs have of
+        // the state before it, up to t of what the tokens leave in the one behind; of the pairs those
+        // within t's block, those of its tokens before t with later blocks, of earlier blocks with its
+        // tokens from t on, and of earlier with later blocks.
+        constexpr int M = C / 32, LANES = 16 / M;  // tokens of a lane, lanes of a block
+        const int K = l / LANES;
+        float behind[M], ahead[M], rows[M], cols[M], own[M], all = 0.0f, b = 0.0f, a = 0.0f, r = 0.0f, c = 0.0f;
+        float far[RB + 1] = {};
 #pragma unroll
         for (int i = 0; i < S_::NW; ++i) all += dot_part[i];
         all *= dec.whole;
 #pragma unroll
         for (int i = M - 1; i >= 0; --i) {
             const int u = l * M + i;
-            if (u / 16 < live) {
-                float x = -row_part[u];
+            own[i] = 0.0f;
+            if (K < live) {
 #pragma unroll
-                for (int r = 0; r < RB; ++r)
-                    if (r <= u / 16) x += col_part[r][u];
+                for (int g = 0; g < CG; ++g) b += dq_part[g][u];
+                float x = 0.0f;
 #pragma unroll
-                for (int r = 0; r < CG; ++r) x += dq_part[r][u];
-                b += x;
+                for (int g = 0; g < RB; ++g)
+                    if (g < K) {
+                        x += col_part[g][u];
+                        if (g + 1 < K) far[g + 1] += x;  // of blocks up to g with this one
+                    }
+                c += x;
+                own[i] = col_part[K][u];
             }
-            behind[i] = b;
+            behind[i] = b, cols[i] = c;
         }
 #pragma unroll
         for (int i = 0; i < M; ++i) {
-            ahead[i] = a;
-            if ((l * M + i) / 16 < live)
+            ahead[i] = a, rows[i] = r;
+            if (K < live) {
 #pragma unroll
-                for (int r = 0; r < CG; ++r) a += dk_part[r][l * M + i];
+                for (int g = 0; g < CG; ++g) a += dk_part[g][l * M + i];
+                r += row_part[l * M + i];
+            }
         }
-        float bs = b, as = a;
+        const float outside = sum_behind<32>(b) + sum_before<32>(a);
+        float pairs = sum_before<LANES>(r) + sum_behind<LANES>(c);
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const float y = __shfl_down_sync(0xffffffffu, bs, d), z = __shfl_up_sync(0xffffffffu, as, d);
-            if (l + d < 32) bs += y;
-            if (l >= d) as += z;
+        for (int g = 1; g + 1 < RB; ++g) {
+            float x = far[g];
+#pragma unroll
+            for (int d = 16; d; d /= 2) x += __shfl_xor_sync(0xffffffffu, x, d);
+            if (g == K) pairs += x;
         }
-        // of the lanes behind and before alone (less the lane's own, large ones would leave nothing of the others)
-        bs = __shfl_down_sync(0xffffffffu, bs, 1), as = __shfl_up_sync(0xffffffffu, as, 1);
-        if (l == 31) bs = 0.0f;
-        if (l == 0) as = 0.0f;
 #pragma unroll
         for (int i = 0; i < M; ++i) {
             const int u = c0 + l * M + i;
-            if (u < j.T) dg[(long long)u * j.H] = u < end ? all + behind[i] + bs + ahead[i] + as : 0.0f;
+            if (u < j.T)
+                dg[(long long)u * j.H] =
+                    u < end ? all + (behind[i] + ahead[i] + outside) + (own[i] + rows[i] + cols[i] + pairs) : 0.0f;
         }
     }
 }

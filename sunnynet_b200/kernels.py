@@ -379,9 +379,8 @@ def linear_attention(q, k, v, log_decay, state=None, lengths=None, scale=None):
     they are (gradients of the 16 tokens around it may not be finite either).
     scale: dk ** -0.5. Out has v's type, states are
     float32. Differentiable once in q, k, v, log_decay and state. Results in float32
-    (states and the gradients of decays among them) have float32's accuracy, the gradient
-    of a token's decay beside those of the 64 tokens around it; float32 values from
-    3.396e38 on count as infinite. On the way to outputs of 16 bits, scores and states are rounded to bf16,
+    (states and the gradients of decays among them) have float32's accuracy; float32 values
+    from 3.396e38 on count as infinite. On the way to outputs of 16 bits, scores and states are rounded to bf16,
     or to two parts of it for float16: bf16 outputs are off by 2.4e-3 (root mean square) where
     their own rounding makes 1.7e-3; float32 inputs avoid it. The same call gives the same bits.
 

@@ -655,3 +655,20 @@ def test_gradients_of_fast_decays_from_the_last_state(kernels, B, T, H, dk, dv, 
     got = gradients(kernels, x, 0.3, ends)[5]
     want, most = truth(x, 0.3, ends)
     near(got, want[5], most[5], torch.float32, 2.0 ** -116)  # (what an exp2 flushes to zero, times 2^10)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fast", [1.0, 8.0, 40.0])
+@pytest.mark.parametrize("B,T,H,Hk,dk,dv", [(2, 4, 2, 2, 11, 1), (2, 17, 6, 3, 118, 3), (2, 128, 3, 3, 64, 64), (1, 349, 21, 7, 4, 3),
+                                            (3, 64, 40, 40, 64, 64), (2, 70, 80, 80, 128, 128), (2, 200, 4, 4, 64, 128)])
+def test_gradients_of_decays_are_as_good_as_their_terms(kernels, B, T, H, Hk, dk, dv, dtype, fast):
+    """The same with gradients of the outputs: a decay's own pairs of tokens, however large its neighbours' are.
+    (What goes into them is rounded as in fp32 for every type.)"""
+    x = make(B, T, H, Hk, dk, dv, dtype, lengths=[T, T - 1, T // 3][:B])
+    x["log_decay"] *= fast
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    ends = (torch.randn(B, T, H, dv, device="cuda", generator=gen).to(dtype),
+            torch.randn(B, H, dk, dv, device="cuda", generator=gen))
+    got = gradients(kernels, x, 0.3, ends)[5]
+    want, most = truth(x, 0.3, ends)
+    near(got, want[5], most[5], torch.float32, 2.0 ** -116)
