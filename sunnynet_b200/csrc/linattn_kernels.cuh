@@ -726,9 +726,9 @@ out_kernel(const Job j, const bf16* kept, const Decays<S_::C>* decs, void* out_)
 // A CTA for each chunk again. First by rows s (dk, dv, with the gradient behind the chunk),
 // then by rows t (dq, with the state before it), so that every product finds its left
 // side in the warp's registers; the scores of do and v are computed for both. 16 x 2048 x
-// 12 of 64 in bf16: 221 us, 643 MB at 2.9 TB/s, matrix instructions 31% of the time: 168
+// 12 of 64 in bf16: 223 us, 643 MB at 2.9 TB/s, matrix instructions 30% of the time: 168
 // registers and 66 KB leave three CTAs of four warps on an SM, which wait for their states,
-// for ldmatrix and for one another. 3 x 1001 x 6 of 40 and 72 in fp32: 75 us, two waves of
+// for ldmatrix and for one another. 3 x 1001 x 6 of 40 and 72 in fp32: 77 us, two waves of
 // one CTA an SM.
 struct Grads {
     const void* dout;
